@@ -34,7 +34,7 @@ typedef enum lkv_status {
 #define LKV_HEAD_DIM 128
 #define LKV_BLOCK_TOKENS 32
 #define LKV_BLOCK_ELEMS 4096
-#define LKV_ABI_VERSION 11
+#define LKV_ABI_VERSION 12
 
 /* Version of this ABI (LKV_ABI_VERSION). */
 int32_t lkv_abi_version(void);
@@ -589,6 +589,86 @@ int32_t lkv_rmsnorm(const lkv_rmsnorm_args *args, lkv_stream_t stream);
  * multiple of 8, rows 16-byte aligned, strides in elements. */
 int32_t lkv_silu_mul(const void *gate, int64_t gate_stride, const void *up, int64_t up_stride, void *out,
                      int64_t out_stride, int32_t rows, int32_t width, lkv_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Low-bit projections of the serving path, in the OCP microscaling (MX) formats: blocks of 32 values
+ * along a row share one scale byte e that stands for 2^(e - 127) (255: the block is NaN).  No counterpart
+ * in the reference, whose weights and activations are bf16.
+ *   MX8 rows: e4m3 values, one byte each, and scales [rows, width / 32].
+ *   MX4 weights: e2m1 codes in the kernels' own layout of lkv_mx4_weight_bytes(n, k) bytes (16-byte
+ *     aligned), which lkv_mx4_pack makes of codes [n, k / 2] (column 2 i in the low four bits of byte i) and
+ *     scales [n, k / 32], and lkv_mx4_quantize of bf16 rows; lkv_mx4_unpack gives the values in bf16 (exact
+ *     above bf16's least normal value).
+ * A quantized block's scale is the smallest power of two (at least 2^-127) with max|y| <= 448 * scale (MX4: 6 *
+ * scale), and its values are the nearest ones, ties to even; a block with an infinity or NaN has scale 255.
+ * Strides are in elements (bytes of 8-bit rows).
+ * ------------------------------------------------------------------------------------- */
+
+/* lkv_rmsnorm with an MX8 output: if residual != NULL: residual := bf16(residual + x), and the normalised row is
+ * residual; y = weight * row / sqrt(mean(row^2) + eps), of which the output is the correctly rounded one (no
+ * rounding before it).  hidden is a multiple of 32 up to 16384; bf16 rows are 16-byte aligned, output rows 8. */
+typedef struct lkv_rmsnorm_mx8_args {
+  int32_t struct_size; /* sizeof(lkv_rmsnorm_mx8_args) */
+  int32_t rows;
+  int32_t hidden;
+  int32_t reserved;
+  double eps;
+  const void *x; /* bf16 [rows, hidden] */
+  int64_t x_stride;
+  void *residual; /* optional bf16 [rows, hidden], updated in place */
+  int64_t residual_stride;
+  const void *weight; /* bf16 [hidden] */
+  void *out;          /* e4m3 [rows, hidden] */
+  int64_t out_stride;
+  void *scales; /* e8m0 [rows, hidden / 32] */
+  int64_t scale_stride;
+} lkv_rmsnorm_mx8_args;
+
+int32_t lkv_rmsnorm_mx8(const lkv_rmsnorm_mx8_args *args, lkv_stream_t stream);
+
+/* lkv_silu_mul with an MX8 output: y = gate / (1 + exp(-gate)) * up, rounded once; width is a multiple of 32, bf16
+ * rows are 16-byte aligned, output rows 8. */
+int32_t lkv_silu_mul_mx8(const void *gate, int64_t gate_stride, const void *up, int64_t up_stride, void *out,
+                         int64_t out_stride, void *scales, int64_t scale_stride, int32_t rows, int32_t width,
+                         lkv_stream_t stream);
+
+/* The values of MX8 rows in bf16 (exact inside bf16's normal range). */
+int32_t lkv_mx8_unpack(const void *data, int64_t data_stride, const void *scales, int64_t scale_stride, void *out,
+                       int64_t out_stride, int32_t rows, int32_t width, lkv_stream_t stream);
+
+int64_t lkv_mx4_weight_bytes(int32_t n, int32_t k);
+
+int32_t lkv_mx4_pack(const void *codes, int64_t code_stride, const void *scales, int64_t scale_stride, int32_t n,
+                     int32_t k, void *weight, lkv_stream_t stream);
+
+int32_t lkv_mx4_quantize(const void *src, int64_t src_stride, int32_t n, int32_t k, void *weight, lkv_stream_t stream);
+
+int32_t lkv_mx4_unpack(const void *weight, int32_t n, int32_t k, void *out, int64_t out_stride, lkv_stream_t stream);
+
+/* out[m][n] = bf16(sum_k x[m][k] * weight[n][k] + bias[n]): fp32 sums in a fixed order, rounded once.  bf16 rows: the
+ * products are exact.  MX8 rows: the scaled matrix instruction adds the products of 8 neighbouring columns in fixed
+ * point (bits below 2^-13 of the largest product's exponent are dropped) before it adds to fp32.
+ * in_features is a multiple of 32; x rows are 16-byte aligned. */
+enum { LKV_X_BF16 = 0, LKV_X_MX8 = 1 };
+
+typedef struct lkv_mx4_linear_args {
+  int32_t struct_size; /* sizeof(lkv_mx4_linear_args) */
+  int32_t rows;
+  int32_t out_features;
+  int32_t in_features;
+  int32_t x_format; /* LKV_X_BF16 or LKV_X_MX8 */
+  int32_t reserved;
+  const void *x; /* bf16 or e4m3 [rows, in_features] */
+  int64_t x_stride;
+  const void *x_scales; /* MX8: e8m0 [rows, in_features / 32]; else NULL */
+  int64_t x_scale_stride;
+  const void *weight; /* MX4 layout */
+  const void *bias;   /* optional bf16 [out_features] */
+  void *out;          /* bf16 [rows, out_features] */
+  int64_t out_stride;
+} lkv_mx4_linear_args;
+
+int32_t lkv_mx4_linear(const lkv_mx4_linear_args *args, lkv_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------
  * Achievable-peak probes.  No counterpart in the reference: measurement support for the bench,

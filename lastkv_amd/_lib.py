@@ -11,7 +11,7 @@ import pathlib
 import threading
 
 LIB_PATH = pathlib.Path(__file__).resolve().parent / "liblastkv_amd.so"
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 
 class LastKVNativeError(RuntimeError):
@@ -324,6 +324,48 @@ class NormArgs(ctypes.Structure):
     ]
 
 
+class NormMx8Args(ctypes.Structure):
+    """Mirror of ``lkv_rmsnorm_mx8_args``."""
+
+    _fields_ = [
+        ("struct_size", c_i32),
+        ("rows", c_i32),
+        ("hidden", c_i32),
+        ("reserved", c_i32),
+        ("eps", ctypes.c_double),
+        ("x", c_ptr),
+        ("x_stride", c_i64),
+        ("residual", c_ptr),
+        ("residual_stride", c_i64),
+        ("weight", c_ptr),
+        ("out", c_ptr),
+        ("out_stride", c_i64),
+        ("scales", c_ptr),
+        ("scale_stride", c_i64),
+    ]
+
+
+class Mx4LinearArgs(ctypes.Structure):
+    """Mirror of ``lkv_mx4_linear_args``."""
+
+    _fields_ = [
+        ("struct_size", c_i32),
+        ("rows", c_i32),
+        ("out_features", c_i32),
+        ("in_features", c_i32),
+        ("x_format", c_i32),
+        ("reserved", c_i32),
+        ("x", c_ptr),
+        ("x_stride", c_i64),
+        ("x_scales", c_ptr),
+        ("x_scale_stride", c_i64),
+        ("weight", c_ptr),
+        ("bias", c_ptr),
+        ("out", c_ptr),
+        ("out_stride", c_i64),
+    ]
+
+
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lkv_abi_version": (c_i32, []),
     "lkv_last_error": (ctypes.c_char_p, []),
@@ -348,6 +390,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lkv_blend_chunk": (c_i32, [ctypes.POINTER(BlendArgs), c_ptr]),
     "lkv_rmsnorm": (c_i32, [ctypes.POINTER(NormArgs), c_ptr]),
     "lkv_silu_mul": (c_i32, [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_i32, c_i32, c_ptr]),
+    "lkv_rmsnorm_mx8": (c_i32, [ctypes.POINTER(NormMx8Args), c_ptr]),
+    "lkv_silu_mul_mx8": (c_i32, [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_i32, c_i32, c_ptr]),
+    "lkv_mx8_unpack": (c_i32, [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_i32, c_i32, c_ptr]),
+    "lkv_mx4_weight_bytes": (c_i64, [c_i32, c_i32]),
+    "lkv_mx4_pack": (c_i32, [c_ptr, c_i64, c_ptr, c_i64, c_i32, c_i32, c_ptr, c_ptr]),
+    "lkv_mx4_quantize": (c_i32, [c_ptr, c_i64, c_i32, c_i32, c_ptr, c_ptr]),
+    "lkv_mx4_unpack": (c_i32, [c_ptr, c_i32, c_i32, c_ptr, c_i64, c_ptr]),
+    "lkv_mx4_linear": (c_i32, [ctypes.POINTER(Mx4LinearArgs), c_ptr]),
     "lkv_probe_read": (c_i32, [c_ptr, c_i64, c_ptr, c_i32, c_ptr]),
     "lkv_probe_mfma": (c_i32, [c_ptr, c_i32, c_i32, ctypes.c_uint32, c_ptr]),
 }

@@ -12,6 +12,7 @@ call.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from dataclasses import dataclass
@@ -1004,6 +1005,265 @@ def silu_mul(gate: torch.Tensor, up: torch.Tensor, out: torch.Tensor | None = No
     _require((o_rows, o_width) == (rows, width), "out shape must match gate")
     _lib.check(_lib.load().lkv_silu_mul(gate.data_ptr(), gs, up.data_ptr(), us, out.data_ptr(), os_, rows, width,
                                         _stream(gate.device)), "lkv_silu_mul")
+    return out
+
+
+MX_BLOCK = 32  # values that share one scale
+
+
+def _on_device(device: torch.device):
+    """Launches go to the current device: make it the tensors'."""
+
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+@dataclass
+class MX8Rows:
+    """Rows in 8 bits (OCP MXFP8): ``data`` float8_e4m3fn ``[..., width]`` and one scale byte per 32 values of a
+    row, ``scales`` uint8 ``[..., width / 32]``; byte e stands for 2^(e - 127), 255 for NaN.  ``mx8_unpack`` gives
+    the values in bf16."""
+
+    data: torch.Tensor
+    scales: torch.Tensor
+
+    def __post_init__(self) -> None:
+        d, s = self.data, self.scales
+        _require(isinstance(d, torch.Tensor) and isinstance(s, torch.Tensor), "MX8Rows holds two tensors")
+        _require(d.is_cuda and s.device == d.device, "MX8Rows must be on one GPU (the kernels have no CPU path)")
+        _require(d.dtype == torch.float8_e4m3fn and s.dtype == torch.uint8,
+                 f"MX8Rows holds float8_e4m3fn data and uint8 scales, got {d.dtype} and {s.dtype}")
+        _require(d.dim() >= 1 and d.shape[-1] > 0 and d.shape[-1] % MX_BLOCK == 0, "MX8Rows width must be a multiple of 32")
+        _require(s.shape[:-1] == d.shape[:-1] and s.shape[-1] == d.shape[-1] // MX_BLOCK,
+                 "MX8Rows scales must be [..., width / 32]")
+
+    @classmethod
+    def empty(cls, shape, device: torch.device | str) -> "MX8Rows":
+        shape = tuple(shape)
+        return cls(torch.empty(shape, dtype=torch.float8_e4m3fn, device=device),
+                   torch.empty((*shape[:-1], shape[-1] // MX_BLOCK), dtype=torch.uint8, device=device))
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.data.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+
+@dataclass
+class MX4Weight:
+    """An ``[out_features, in_features]`` weight in 4 bits (OCP MXFP4: e2m1 codes, one scale byte per 32 columns
+    of a row) in the layout that ``mx4_linear`` reads; made by ``mx4_quantize`` or ``mx4_pack``."""
+
+    data: torch.Tensor
+    out_features: int
+    in_features: int
+
+    def __post_init__(self) -> None:
+        d = self.data
+        _require(isinstance(d, torch.Tensor) and d.is_cuda, "MX4Weight must be on a GPU (the kernels have no CPU path)")
+        _require(d.dtype == torch.uint8 and d.is_contiguous(), "MX4Weight data must be contiguous uint8")
+        need = _mx4_bytes(self.out_features, self.in_features)
+        _require(d.numel() == need, f"MX4Weight data holds {d.numel()} bytes, its shape needs {need}")
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+
+def _mx4_bytes(n: int, k: int) -> int:
+    _require(isinstance(n, int) and isinstance(k, int) and 0 < n <= 1 << 24 and 0 < k <= 1 << 24 and k % MX_BLOCK == 0,
+             f"an MX4 weight has 1 to 2^24 rows and a positive multiple of 32 columns up to 2^24, got {n} x {k}")
+    return int(_lib.load().lkv_mx4_weight_bytes(n, k))
+
+
+def _same_device(device: torch.device, **tensors: torch.Tensor | None) -> None:
+    for name, t in tensors.items():
+        _require(t is None or t.device == device, f"{name} must be on {device}")
+
+
+def _mx8_strides(name: str, rows: MX8Rows) -> tuple[int, int, int, int]:
+    """(rows, width, data row stride, scale row stride) of MX8 rows viewed as [rows, width]."""
+
+    d, s = rows.data, rows.scales
+    width = d.shape[-1]
+    if d.dim() == 1:
+        _require(d.stride(0) == 1 and (s.numel() == 1 or s.stride(0) == 1), f"{name} rows must be contiguous")
+        return 1, width, width, width // MX_BLOCK
+    try:
+        d2, s2 = d.view(-1, width), s.view(-1, width // MX_BLOCK)
+    except RuntimeError:
+        d2 = s2 = None
+    _require(d2 is not None, f"{name} must be viewable as [rows, {width}] with one row stride")
+    _require(d2.stride(1) == 1 and (s2.shape[1] == 1 or s2.stride(1) == 1), f"{name} rows must be contiguous")
+    return d2.shape[0], width, d2.stride(0), s2.stride(0)
+
+
+def _mx8_out(x: torch.Tensor, out: MX8Rows | None) -> MX8Rows:
+    _require(x.shape[-1] > 0 and x.shape[-1] % MX_BLOCK == 0, f"rows of 32-value blocks are needed, got a width of {x.shape[-1]}")
+    if out is None:
+        return MX8Rows.empty(x.shape, x.device)
+    _require(isinstance(out, MX8Rows), "out must be MX8Rows")
+    _require(out.shape == x.shape, "out shape must match x")
+    _same_device(x.device, out=out.data)
+    return out
+
+
+def rmsnorm_mx8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: torch.Tensor | None = None,
+                out: MX8Rows | None = None) -> MX8Rows:
+    """``rmsnorm`` with an 8-bit output: the rows of ``x`` (bf16 ``[..., hidden]``, hidden a multiple of 32; with
+    ``residual`` first ``residual += x`` in bf16, in place, and the sum) normalised and multiplied by ``weight``,
+    each block of 32 rounded once, correctly, to e4m3 under the smallest power-of-two scale that holds its largest
+    value.  A block with an infinity or NaN is NaN.  Returns ``out``."""
+
+    _require_bf16_cuda("x", x)
+    _require(x.dim() >= 1, "x must have rows")
+    out = _mx8_out(x, out)
+    _require_bf16_cuda("weight", weight)
+    hidden = x.shape[-1]
+    _require(weight.is_contiguous() and weight.numel() == hidden, "weight must be a contiguous bf16 [hidden] tensor")
+    if residual is not None:
+        _require_bf16_cuda("residual", residual)
+        _require(residual.shape == x.shape, "residual shape must match x")
+    _same_device(x.device, weight=weight, residual=residual)
+    if x.numel() == 0:
+        return out
+    a = _lib.NormMx8Args()
+    a.struct_size = ctypes.sizeof(_lib.NormMx8Args)
+    a.rows, a.hidden, a.x_stride = _rows2d("x", x)
+    a.eps = float(eps)
+    a.x = x.data_ptr()
+    if residual is not None:
+        a.residual, a.residual_stride = residual.data_ptr(), _rows2d("residual", residual)[2]
+    a.weight = weight.data_ptr()
+    _, _, a.out_stride, a.scale_stride = _mx8_strides("out", out)
+    a.out, a.scales = out.data.data_ptr(), out.scales.data_ptr()
+    with _on_device(x.device):
+        _lib.check(_lib.load().lkv_rmsnorm_mx8(ctypes.byref(a), _stream(x.device)), "lkv_rmsnorm_mx8")
+    return out
+
+
+def silu_mul_mx8(gate: torch.Tensor, up: torch.Tensor, out: MX8Rows | None = None) -> MX8Rows:
+    """``F.silu(gate) * up`` of bf16 ``[..., width]`` tensors (width a multiple of 32) with an 8-bit output, each
+    block of 32 rounded once as ``rmsnorm_mx8`` rounds it."""
+
+    _require_bf16_cuda("gate", gate)
+    _require_bf16_cuda("up", up)
+    _require(gate.dim() >= 1 and up.shape == gate.shape, "up shape must match gate")
+    _same_device(gate.device, up=up)
+    out = _mx8_out(gate, out)
+    if gate.numel() == 0:
+        return out
+    rows, width, gs = _rows2d("gate", gate)
+    us = _rows2d("up", up)[2]
+    _, _, os_, ss = _mx8_strides("out", out)
+    with _on_device(gate.device):
+        _lib.check(_lib.load().lkv_silu_mul_mx8(gate.data_ptr(), gs, up.data_ptr(), us, out.data.data_ptr(), os_,
+                                                out.scales.data_ptr(), ss, rows, width, _stream(gate.device)),
+                   "lkv_silu_mul_mx8")
+    return out
+
+
+def mx8_unpack(rows: MX8Rows) -> torch.Tensor:
+    """The values of ``rows`` in bf16."""
+
+    _require(isinstance(rows, MX8Rows), "rows must be MX8Rows")
+    out = torch.empty(rows.shape, dtype=torch.bfloat16, device=rows.device)
+    if out.numel() == 0:
+        return out
+    n, width, ds, ss = _mx8_strides("rows", rows)
+    with _on_device(rows.device):
+        _lib.check(_lib.load().lkv_mx8_unpack(rows.data.data_ptr(), ds, rows.scales.data_ptr(), ss, out.data_ptr(), width,
+                                              n, width, _stream(rows.device)), "lkv_mx8_unpack")
+    return out
+
+
+def mx4_pack(codes: torch.Tensor, scales: torch.Tensor) -> MX4Weight:
+    """An MX4 weight of an MXFP4 checkpoint's tensors: ``codes`` uint8 ``[N, K / 2]`` (column 2 i in the low four
+    bits of byte i) and ``scales`` uint8 ``[N, K / 32]``."""
+
+    for name, t in (("codes", codes), ("scales", scales)):
+        _require(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be on a GPU (the kernels have no CPU path)")
+        _require(t.dtype == torch.uint8 and t.dim() == 2 and (t.shape[1] == 1 or t.stride(1) == 1),
+                 f"{name} must be a uint8 matrix with contiguous rows")
+    n, k = int(codes.shape[0]), 2 * int(codes.shape[1])
+    need = _mx4_bytes(n, k)
+    _require(tuple(scales.shape) == (n, k // MX_BLOCK), f"scales must be [{n}, {k // MX_BLOCK}]")
+    _same_device(codes.device, scales=scales)
+    w = torch.empty(need, dtype=torch.uint8, device=codes.device)
+    with _on_device(w.device):
+        _lib.check(_lib.load().lkv_mx4_pack(codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0), n, k,
+                                            w.data_ptr(), _stream(w.device)), "lkv_mx4_pack")
+    return MX4Weight(w, n, k)
+
+
+def mx4_quantize(weight: torch.Tensor) -> MX4Weight:
+    """``weight`` (bf16 ``[N, K]``, K a multiple of 32) in 4 bits: each block of 32 columns under the smallest
+    power-of-two scale that holds its largest value, rounded to nearest, ties to even."""
+
+    _require_bf16_cuda("weight", weight)
+    _require(weight.dim() == 2 and weight.stride(1) == 1, "weight must be a matrix with contiguous rows")
+    n, k = int(weight.shape[0]), int(weight.shape[1])
+    w = torch.empty(_mx4_bytes(n, k), dtype=torch.uint8, device=weight.device)
+    with _on_device(w.device):
+        _lib.check(_lib.load().lkv_mx4_quantize(weight.data_ptr(), weight.stride(0), n, k, w.data_ptr(),
+                                                _stream(w.device)), "lkv_mx4_quantize")
+    return MX4Weight(w, n, k)
+
+
+def mx4_unpack(weight: MX4Weight) -> torch.Tensor:
+    """The values of ``weight`` as bf16 ``[out_features, in_features]``."""
+
+    _require(isinstance(weight, MX4Weight), "weight must be an MX4Weight")
+    n, k = weight.out_features, weight.in_features
+    out = torch.empty((n, k), dtype=torch.bfloat16, device=weight.device)
+    with _on_device(out.device):
+        _lib.check(_lib.load().lkv_mx4_unpack(weight.data.data_ptr(), n, k, out.data_ptr(), k, _stream(out.device)),
+                   "lkv_mx4_unpack")
+    return out
+
+
+def mx4_linear(x: torch.Tensor | MX8Rows, weight: MX4Weight, bias: torch.Tensor | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """``F.linear`` over a 4-bit weight: ``x`` is bf16 ``[..., in_features]`` or ``MX8Rows`` of that shape, ``bias``
+    bf16 ``[out_features]``; returns bf16 ``[..., out_features]``, fp32 sums in a fixed order rounded once.  Products
+    of bf16 rows are exact; those of 8-bit rows are added eight columns at a time in the matrix instruction's fixed
+    point, which keeps 13 bits below the largest."""
+
+    _require(isinstance(weight, MX4Weight), "weight must be an MX4Weight")
+    n, k = weight.out_features, weight.in_features
+    mx8 = isinstance(x, MX8Rows)
+    if not mx8:
+        _require_bf16_cuda("x", x)
+    _require(len(x.shape) >= 1 and x.shape[-1] == k, f"x must be [..., {k}], got {tuple(x.shape)}")
+    device = x.device
+    if bias is not None:
+        _require_bf16_cuda("bias", bias)
+        _require(bias.is_contiguous() and bias.numel() == n, f"bias must be a contiguous bf16 [{n}] tensor")
+    shape = (*x.shape[:-1], n)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+    _require_bf16_cuda("out", out)
+    _require(tuple(out.shape) == shape, f"out must be {list(shape)}")
+    _same_device(device, weight=weight.data, bias=bias, out=out)
+    if out.numel() == 0:
+        return out
+    a = _lib.Mx4LinearArgs()
+    a.struct_size = ctypes.sizeof(_lib.Mx4LinearArgs)
+    if mx8:
+        a.rows, _, a.x_stride, a.x_scale_stride = _mx8_strides("x", x)
+        a.x, a.x_scales, a.x_format = x.data.data_ptr(), x.scales.data_ptr(), 1
+    else:
+        a.rows, _, a.x_stride = _rows2d("x", x)
+        a.x = x.data_ptr()
+    a.out_features, a.in_features = n, k
+    a.weight, a.bias = weight.data.data_ptr(), _ptr(bias)
+    a.out, a.out_stride = out.data_ptr(), _rows2d("out", out)[2]
+    with _on_device(device):
+        _lib.check(_lib.load().lkv_mx4_linear(ctypes.byref(a), _stream(device)), "lkv_mx4_linear")
     return out
 
 
