@@ -22,12 +22,13 @@ struct LinearParams {
 };
 
 constexpr int kWaves = 8;
+constexpr int kStepTiles = 2;                  // 128-column tiles that a wave loads at once
+constexpr int kStepCols = 128 * kStepTiles;
 
-__device__ inline float e8m0(uint32_t word, int t) {  // the scale's exponent in place (0: read as 2^-127 by the convert)
-  return __uint_as_float(((word >> (8 * t)) & 0xffu) << 23);
-}
+// Byte t of a scale word as the exponent of a float (the converts read no other bits; 0 stands for 2^-127).
+__device__ inline float e8m0(uint32_t word, int t) { return __uint_as_float(((word >> (8 * t)) & 0xffu) << 23); }
 
-// Eight codes of a word as scaled bf16 (exact: 2 significant bits, bf16's exponents).
+// Eight e2m1 codes of a word as scaled bf16 (exact: 2 significant bits, bf16's exponents).
 __device__ inline uint4 e2m1_to_bf16(uint32_t codes, float scale) {
   return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)),
                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1)),
@@ -35,94 +36,202 @@ __device__ inline uint4 e2m1_to_bf16(uint32_t codes, float scale) {
                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3)));
 }
 
-// One workgroup per (NT row tiles of the weight, MT tiles of 16 rows of x); its 8 waves take every eighth unit of 512
-// columns and their sums are added through LDS, in the waves' order.
-template <bool kMx8, int MT, int NT>
-__global__ __launch_bounds__(kWaves * 64) void mx4_rows_kernel(const LinearParams p) {
-  __shared__ f32x4 part[kWaves][MT][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// Eight e4m3 values of two words as scaled bf16 (exact inside bf16's range).
+__device__ inline uint4 e4m3_to_bf16(uint32_t a, uint32_t b, float scale) {
+  return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, false)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, true)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, false)),
+                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, true)));
+}
+
+__device__ inline uint32_t word_of(const uint4& v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
+
+__device__ inline uint4 buffer_load16(__amdgpu_buffer_rsrc_t r, int offset) {
+  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 0));
+}
+
+constexpr int kOutside = 0x7fffffff;  // an offset past every buffer: loads give zeros
+
+// What a wave holds of one step of columns of the weight, and the scales of MX8 rows.
+template <int MT, int NT>
+struct Step {
+  uint4 codes[NT][kStepTiles];
+  uint32_t scale[NT];
+  uint32_t xs[MT];  // lane 16 t + row: the four scale bytes of the row in tile t
+};
+
+// One workgroup per (NT * 8 / KS row tiles of the weight, MT tiles of 16 rows of x).  Its 8 waves form groups of KS that
+// share NT row tiles; wave ks of a group takes steps ks, ks + KS, ... of 256 columns, and the group's sums are added
+// through LDS, in the waves' order.
+// Bound by HBM: the weight's 4.25 bits a value, read once for up to 32 rows of x, converted in registers (one instruction
+// for two values) for bf16 matrix instructions; MX8 rows are converted too (exact products; the scaled matrix instruction
+// would save 64 conversions per 2,048 weights of a wave, not time).  A step's loads are issued one step ahead.
+// us per call with cold weights, bf16 / MX8 rows, beside a plain read of the same bytes: 28672 x 4096 for 1 row 15.3 / 15.0
+// (read 12.3), for 32 20.0 / 20.2; 4096 x 14336 for 1 row 11.2 / 10.6 (read 6.6-8.7), for 32 16.8 / 14.2; 4096 x 4096 for 1 row
+// 4.9 / 4.7 (read 3.5), for 32 6.8 / 6.1; bf16 weights in the library's GEMM: 28672 x 4096 for 32 rows 48.8, 4096 x 4096 13.8.
+// The matrix instruction wants a different row of x in neighbouring lanes, which the L1 would serve 16 bytes a cycle:
+// rows are loaded along their columns (64 bytes a cycle) and turned in a wave's own corner of LDS, its 16-byte chunks
+// swizzled by the row (chunk c of row m at c ^ (m & 7)) so that neither side meets a bank twice (4096 x 4096 for 32 rows
+// 10.6 -> 6.8 us).
+template <bool kMx8, int MT, int NT, int KS>
+__global__ __launch_bounds__(kWaves * 64, MT == 1 && NT <= 2 ? 4 : 2) void mx4_rows_kernel(const LinearParams p) {
+  constexpr int kLoads = kMx8 ? 2 : 4;  // of 1 KiB per tile of 16 rows x 128 columns
+  constexpr int kRowBytes = kMx8 ? 128 : 256;  // of a row in a tile
+  constexpr int kChunks = kRowBytes / 16;
+  constexpr int kStage = MT * 16 * kRowBytes;
+  constexpr int kPart = KS == 1 ? 0 : NT * MT * 64 * sizeof(f32x4);
+  __shared__ __attribute__((aligned(16))) char smem[kWaves * (kStage > kPart ? kStage : kPart)];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
-  const int nt0 = blockIdx.x * NT, m0 = blockIdx.y * (16 * MT);
+  const int ks = wave % KS;
+  const int nt0 = (blockIdx.x * (kWaves / KS) + wave / KS) * NT, m0 = blockIdx.y * (16 * MT);
   const int ntiles = (p.N + 15) >> 4;
   f32x4 acc[NT][MT];
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  int64_t row[MT];
-#pragma unroll
-  for (int j = 0; j < MT; ++j) row[j] = min(m0 + 16 * j + r, p.M - 1);  // (rows past the last repeat it and are not stored)
   const uint8_t* w[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) w[i] = p.w + static_cast<int64_t>(min(nt0 + i, ntiles - 1)) * p.units * kMxUnitBytes;
-  for (int u = wave; u < p.units; u += kWaves) {
-    uint32_t ws[NT];
+  const int valid = min(p.M - m0, 16 * MT);
+  const int stride = static_cast<int>(p.x_stride) * (kMx8 ? 1 : 2), row_bytes = p.K * (kMx8 ? 1 : 2);
+  const __amdgpu_buffer_rsrc_t xb = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<char*>(static_cast<const char*>(p.x) + static_cast<int64_t>(m0) * stride), 0,
+      (valid - 1) * stride + row_bytes, 0x00020000);
+  const int lrow = lane / kChunks, lcol = (lane % kChunks) * 16;  // what this lane loads of a 1 KiB piece
+  const int steps = (p.K + kStepCols - 1) / kStepCols;
+  char* stage = smem + wave * kStage;
+
+  auto load = [&](int h, Step<MT, NT>& st) {
+    const int64_t unit = static_cast<int64_t>(h >> 1) * kMxUnitBytes;
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
-      ws[i] = *reinterpret_cast<const uint32_t*>(w[i] + static_cast<int64_t>(u) * kMxUnitBytes + 4 * kMxTileBytes + lane * 4);
+    for (int i = 0; i < NT; ++i) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int k0 = u * kMxUnitCols + t * 128;
-      if (k0 >= p.K) break;
-      uint4 wv[NT];
+      for (int t = 0; t < kStepTiles; ++t)
+        st.codes[i][t] = load_nt(w[i] + unit + ((h & 1) * kStepTiles + t) * kMxTileBytes + lane * 16);
+      st.scale[i] = reinterpret_cast<const uint32_t*>(w[i] + unit + 4 * kMxTileBytes)[lane];
+    }
+    if constexpr (kMx8) {
+      const int b0 = h * (kStepCols / 32) + 4 * (lane >> 4), blocks = p.K >> 5;
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
-        wv[i] = *reinterpret_cast<const uint4*>(w[i] + static_cast<int64_t>(u) * kMxUnitBytes + t * kMxTileBytes + lane * 16);
-      if constexpr (kMx8) {
-        // x: lane (row, g) takes columns 16 g .. and 64 + 16 g .., scale of block g; past the last column, zeros
-        i32x8 xv[MT];
-        uint32_t xs[MT];
-        const int ka = k0 + 16 * g, kb = ka + 64;
-#pragma unroll
-        for (int j = 0; j < MT; ++j) {
-          const uint8_t* x = static_cast<const uint8_t*>(p.x) + row[j] * p.x_stride;
-          uint4 a = make_uint4(0, 0, 0, 0), b = a;
-          if (ka < p.K) a = *reinterpret_cast<const uint4*>(x + ka);
-          if (kb < p.K) b = *reinterpret_cast<const uint4*>(x + kb);
-          xv[j] = i32x8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
-          xs[j] = k0 + 32 * g < p.K ? p.xs[row[j] * p.xs_stride + (k0 >> 5) + g] : 0u;
-        }
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          const i32x8 a = {(int)wv[i].x, (int)wv[i].y, (int)wv[i].z, (int)wv[i].w, 0, 0, 0, 0};
-#pragma unroll
-          for (int j = 0; j < MT; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, xv[j], acc[i][j], 4, 0, 0,
-                                                                         (ws[i] >> (8 * t)) & 0xffu, 0, xs[j]);
-        }
-      } else {
-        const int k = k0 + 32 * g;
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          uint4 xv[MT];
-#pragma unroll
-          for (int j = 0; j < MT; ++j) {
-            xv[j] = make_uint4(0, 0, 0, 0);
-            if (k < p.K) xv[j] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + row[j] * p.x_stride + k + 8 * s);
-          }
-#pragma unroll
-          for (int i = 0; i < NT; ++i) {
-            const uint32_t c = s == 0 ? wv[i].x : s == 1 ? wv[i].y : s == 2 ? wv[i].z : wv[i].w;
-            const uint4 a = e2m1_to_bf16(c, e8m0(ws[i], t));
-#pragma unroll
-            for (int j = 0; j < MT; ++j) acc[i][j] = mfma_bf16(a, xv[j], acc[i][j]);
+      for (int j = 0; j < MT; ++j) {
+        const uint8_t* s = p.xs + static_cast<int64_t>(m0 + min(16 * j + r, valid - 1)) * p.xs_stride + b0;
+        uint32_t v = 0;
+        if (lane < 16 * kStepTiles) {
+          if (b0 + 4 <= blocks) {
+            __builtin_memcpy(&v, s, 4);
+          } else {
+            for (int q = 0; q < 4; ++q)
+              if (b0 + q < blocks) v |= static_cast<uint32_t>(s[q]) << (8 * q);
           }
         }
+        st.xs[j] = v;
       }
     }
+  };
+  uint4 xr[MT][kLoads];  // the next tile of x, as loaded (16 bytes a lane, neighbouring lanes neighbouring bytes)
+  auto load_x = [&](int tile) {
+    const int col = tile * kRowBytes + lcol;
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int row = 16 * j + i * (64 / kChunks) + lrow;
+        xr[j][i] = buffer_load16(xb, col < row_bytes && row < valid ? row * stride + col : kOutside);
+      }
+  };
+  auto store_x = [&] {
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int row = i * (64 / kChunks) + lrow;
+        *reinterpret_cast<uint4*>(stage + (16 * j + row) * kRowBytes + (lcol ^ ((row & 7) * 16))) = xr[j][i];
+      }
+  };
+  auto compute = [&](int h, int t, const Step<MT, NT>& st) {
+    const int byte = (h & 1) * kStepTiles + t;
+    // lane (row, g) takes block g's 32 columns: step s of the matrix instruction, 8 of them
+    float sx[MT];
+    uint4 lo[MT], hi[MT];
+    if constexpr (kMx8) {
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        sx[j] = e8m0(__shfl(st.xs[j], 16 * t + r) >> (8 * g), 0);
+        const char* at = stage + (16 * j + r) * kRowBytes;
+        lo[j] = *reinterpret_cast<const uint4*>(at + ((32 * g) ^ ((r & 7) * 16)));
+        hi[j] = *reinterpret_cast<const uint4*>(at + ((32 * g + 16) ^ ((r & 7) * 16)));
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      uint4 b[MT];
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        if constexpr (kMx8)
+          b[j] = s == 0   ? e4m3_to_bf16(lo[j].x, lo[j].y, sx[j])
+                 : s == 1 ? e4m3_to_bf16(lo[j].z, lo[j].w, sx[j])
+                 : s == 2 ? e4m3_to_bf16(hi[j].x, hi[j].y, sx[j])
+                          : e4m3_to_bf16(hi[j].z, hi[j].w, sx[j]);
+        else
+          b[j] = *reinterpret_cast<const uint4*>(stage + (16 * j + r) * kRowBytes + ((64 * g + 16 * s) ^ ((r & 7) * 16)));
+      }
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const uint4 a = e2m1_to_bf16(word_of(st.codes[i][t], s), e8m0(st.scale[i], byte));
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[i][j] = mfma_bf16(a, b[j], acc[i][j]);
+      }
+    }
+  };
+
+  // Two steps in turn, so that the next one's loads are not copied (a copy would wait for them).
+  Step<MT, NT> even, odd;
+  auto step = [&](int h, const Step<MT, NT>& now, Step<MT, NT>& then) {
+    const bool more = h + KS < steps;
+    if (more) load(h + KS, then);
+#pragma unroll
+    for (int t = 0; t < kStepTiles; ++t) {
+      store_x();
+      if (t + 1 < kStepTiles)
+        load_x(h * kStepTiles + t + 1);
+      else if (more)
+        load_x((h + KS) * kStepTiles);
+      compute(h, t, now);
+    }
+  };
+  if (ks < steps) {
+    load(ks, even);
+    load_x(ks * kStepTiles);
   }
-#pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    if (i > 0) __syncthreads();
-#pragma unroll
-    for (int j = 0; j < MT; ++j) part[wave][j][lane] = acc[i][j];
+  for (int h = ks; h < steps; h += 2 * KS) {
+    step(h, even, odd);
+    if (h + KS < steps) step(h + KS, odd, even);
+  }
+  f32x4* part = reinterpret_cast<f32x4*>(smem);  // [wave][NT][MT][lane]
+  if constexpr (KS > 1) {
     __syncthreads();
-    const int j = threadIdx.x >> 6;
-    const int n = (nt0 + i) * 16 + 4 * g, m = m0 + 16 * j + r;
-    if (j < MT && m < p.M) {
-      f32x4 s = part[0][j][lane];
 #pragma unroll
-      for (int v = 1; v < kWaves; ++v) s += part[v][j][lane];
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) part[((wave * NT + i) * MT + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+  }
+  // the KS waves of a group of columns take its NT x MT tiles in turn
+#pragma unroll
+  for (int q = 0; q < NT * MT; ++q) {
+    if (q % KS != ks) continue;
+    const int i = q / MT, j = q % MT;
+    const int n = (nt0 + i) * 16 + 4 * g, m = m0 + 16 * j + r;
+    f32x4 s = acc[i][j];
+    if constexpr (KS > 1) {
+      const f32x4* from = part + ((wave / KS) * KS * NT * MT + q) * 64 + lane;
+      s = from[0];
+#pragma unroll
+      for (int v = 1; v < KS; ++v) s += from[v * NT * MT * 64];
+    }
+    if (m < p.M) {
       uint16_t* out = p.out + m * p.out_stride;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -131,29 +240,43 @@ __global__ __launch_bounds__(kWaves * 64) void mx4_rows_kernel(const LinearParam
   }
 }
 
+template <bool kMx8, int MT, int NT, int KS>
+void launch_rows(const LinearParams& p, hipStream_t s) {
+  constexpr int kTiles = NT * kWaves / KS;  // row tiles of a workgroup
+  const dim3 grid(static_cast<unsigned>((p.N + 16 * kTiles - 1) / (16 * kTiles)),
+                  static_cast<unsigned>((p.M + 16 * MT - 1) / (16 * MT)));
+  mx4_rows_kernel<kMx8, MT, NT, KS><<<grid, kWaves * 64, 0, s>>>(p);
+}
+
+// One round of workgroups, one per CU: `per` row tiles of the weight each.  More workgroups read x more often and wait
+// for each other's start and end (4096 x 4096 for 64 rows, us: 10.7 with 512, 7.9 with 256); fewer leave CUs idle (128:
+// 12.0).  For four tiles a workgroup the waves split the columns rather than the rows (14336 x 4096 for 32 rows: 12.3
+// against 14.1 with two tiles and half the columns each).
 template <bool kMx8, int MT>
-void launch_rows(const LinearParams& p, hipStream_t s, int nt) {
-  const int tiles = (p.N + 15) / 16;
-  const dim3 grid(static_cast<unsigned>((tiles + nt - 1) / nt), static_cast<unsigned>((p.M + 16 * MT - 1) / (16 * MT)));
-  if (nt == 4)
-    mx4_rows_kernel<kMx8, MT, 4><<<grid, kWaves * 64, 0, s>>>(p);
-  else if (nt == 2)
-    mx4_rows_kernel<kMx8, MT, 2><<<grid, kWaves * 64, 0, s>>>(p);
+void launch_mt(const LinearParams& p, hipStream_t s) {
+  const int64_t cus = std::max(1, device_cu_count());
+  const int64_t tiles = static_cast<int64_t>((p.N + 15) / 16) * ((p.M + 16 * MT - 1) / (16 * MT));
+  const int64_t per = (tiles + cus - 1) / cus;
+  if (per <= 1)
+    launch_rows<kMx8, MT, 1, 8>(p, s);
+  else if (per <= 2)
+    launch_rows<kMx8, MT, 2, 8>(p, s);
+  else if (per <= 4)
+    launch_rows<kMx8, MT, 4, 8>(p, s);
+  else if (per <= 8)
+    launch_rows<kMx8, MT, 4, 4>(p, s);
+  else if (per <= 16)
+    launch_rows<kMx8, MT, 4, 2>(p, s);
   else
-    mx4_rows_kernel<kMx8, MT, 1><<<grid, kWaves * 64, 0, s>>>(p);
+    launch_rows<kMx8, MT, 4, 1>(p, s);
 }
 
 template <bool kMx8>
 int32_t launch(const LinearParams& p, hipStream_t s) {
-  const int cus = device_cu_count();
-  const int tiles = (p.N + 15) / 16;
-  const int nt = tiles >= 4 * cus ? 4 : tiles >= 2 * cus ? 2 : 1;
-  switch (std::min(4, (p.M + 15) / 16)) {
-    case 1: launch_rows<kMx8, 1>(p, s, nt); break;
-    case 2: launch_rows<kMx8, 2>(p, s, nt); break;
-    case 3: launch_rows<kMx8, 3>(p, s, nt); break;
-    default: launch_rows<kMx8, 4>(p, s, nt);
-  }
+  if (p.M <= 16)
+    launch_mt<kMx8, 1>(p, s);
+  else
+    launch_mt<kMx8, 2>(p, s);
   return check_launch("lkv_mx4_linear");
 }
 
@@ -256,8 +379,8 @@ uintptr_t bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 }  // namespace lkv
 
 #define LKV_REQUIRE_MX4_SHAPE(n, k)                                                                              \
-  LKV_REQUIRE((n) > 0 && (n) <= (1 << 24) && (k) > 0 && (k) <= (1 << 24) && (k) % 32 == 0,                       \
-              "an MX4 weight has 1 to 2^24 rows and a positive multiple of 32 columns up to 2^24, got %d x %d", n, k)
+  LKV_REQUIRE((n) > 0 && (n) <= (1 << 24) && (k) > 0 && (k) <= (1 << 20) && (k) % 32 == 0,                       \
+              "an MX4 weight has 1 to 2^24 rows and a positive multiple of 32 columns up to 2^20, got %d x %d", n, k)
 
 extern "C" int64_t lkv_mx4_weight_bytes(int32_t n, int32_t k) {
   if (n <= 0 || k <= 0) return 0;
@@ -319,6 +442,7 @@ extern "C" int32_t lkv_mx4_linear(const lkv_mx4_linear_args* a, lkv_stream_t str
   LKV_REQUIRE(((bits(a->x) | bits(a->weight)) & 15) == 0 && ((bits(a->out) | bits(a->bias)) & 1) == 0,
               "x and weight must be 16-byte aligned");
   LKV_REQUIRE(a->x_stride % (mx8 ? 16 : 8) == 0, "x rows must be 16-byte aligned");
+  LKV_REQUIRE(a->x_stride >= 0 && a->x_stride <= (1 << 23), "x_stride must be at most 2^23 elements");
   if (a->rows == 0) return LKV_OK;
   LinearParams p;
   p.w = static_cast<const uint8_t*>(a->weight);

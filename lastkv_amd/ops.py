@@ -1075,8 +1075,8 @@ class MX4Weight:
 
 
 def _mx4_bytes(n: int, k: int) -> int:
-    _require(isinstance(n, int) and isinstance(k, int) and 0 < n <= 1 << 24 and 0 < k <= 1 << 24 and k % MX_BLOCK == 0,
-             f"an MX4 weight has 1 to 2^24 rows and a positive multiple of 32 columns up to 2^24, got {n} x {k}")
+    _require(isinstance(n, int) and isinstance(k, int) and 0 < n <= 1 << 24 and 0 < k <= 1 << 20 and k % MX_BLOCK == 0,
+             f"an MX4 weight has 1 to 2^24 rows and a positive multiple of 32 columns up to 2^20, got {n} x {k}")
     return int(_lib.load().lkv_mx4_weight_bytes(n, k))
 
 
