@@ -17,12 +17,14 @@
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
 #include <cstdint>
 #include <cstring>
+#include <vector>
 
 #include "../../include/lastkv_amd.h"
 
@@ -37,14 +39,26 @@ struct Library {
   decltype(&lkv_rmsnorm) rmsnorm;
   decltype(&lkv_silu_mul) silu_mul;
   decltype(&lkv_last_error) last_error;
+  decltype(&lkv_rmsnorm_mx8) rmsnorm_mx8;
+  decltype(&lkv_silu_mul_mx8) silu_mul_mx8;
+  decltype(&lkv_mx8_unpack) mx8_unpack;
+  decltype(&lkv_mx4_linear) mx4_linear;
+  decltype(&lkv_mx4_weight_bytes) mx4_weight_bytes;
 };
 
 Library g_lib;
 PyTypeObject* g_tiled = nullptr;
 PyTypeObject* g_paged = nullptr;
+PyTypeObject* g_mx8 = nullptr;
+PyTypeObject* g_mx4 = nullptr;
 PyObject* g_error = nullptr;  // LastKVNativeError
 PyObject* g_str_k = nullptr;
 PyObject* g_str_v = nullptr;
+PyObject* g_str_data = nullptr;
+PyObject* g_str_scales = nullptr;
+PyObject* g_str_out_features = nullptr;
+PyObject* g_str_in_features = nullptr;
+PyObject* g_no_args = nullptr;  // ()
 constexpr int kMaxDevices = 64;
 int g_cus[kMaxDevices];
 
@@ -673,11 +687,259 @@ PyObject* silu_mul(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
-// bind(addresses: the entry points in Library's order, TiledKV, PagedKV, LastKVNativeError)
+// ---- MX8 rows and MX4 weights ----
+
+// An attribute's tensor as the kernels may address it (empty otherwise).
+at::Tensor tensor_attr(PyObject* o, PyObject* name) {
+  PyObject* a = PyObject_GetAttr(o, name);
+  if (a == nullptr) {
+    PyErr_Clear();
+    return at::Tensor();
+  }
+  const at::Tensor* t = tensor(a);
+  at::Tensor r = t != nullptr ? *t : at::Tensor();
+  Py_DECREF(a);
+  return r;
+}
+
+// Kernels are launched on the current device.
+bool on_current_device(const at::Tensor& t) { return t.device().index() == c10::hip::current_device(); }
+
+// The shape of up to three dims as rows of `width` with one stride (rows2d without the type).
+bool rows_of(const at::Tensor& t, int64_t& n, int64_t& width, int64_t& stride) {
+  if (t.dim() < 2 || t.dim() > 3 || t.numel() == 0) return false;
+  width = t.size(-1);
+  if (width != 1 && t.stride(-1) != 1) return false;
+  if (t.dim() == 2 || t.size(0) == 1) {
+    n = t.size(-2);
+    stride = t.stride(-2);
+  } else {
+    if (t.size(1) != 1 && t.stride(0) != t.size(1) * t.stride(1)) return false;
+    n = t.size(0) * t.size(1);
+    stride = t.size(1) == 1 ? t.stride(0) : t.stride(1);
+  }
+  return n <= INT32_MAX && width <= INT32_MAX;
+}
+
+struct Mx8 {
+  at::Tensor data, scales;
+  int64_t rows = 0, width = 0, stride = 0, scale_stride = 0;
+};
+
+// An MX8Rows object with the forms ops.MX8Rows checks.
+bool mx8_rows(PyObject* o, Mx8& m) {
+  if (Py_TYPE(o) != g_mx8) return false;
+  m.data = tensor_attr(o, g_str_data);
+  m.scales = tensor_attr(o, g_str_scales);
+  int64_t n, blocks;
+  if (!m.data.defined() || !m.scales.defined() || m.data.scalar_type() != at::kFloat8_e4m3fn ||
+      m.scales.scalar_type() != at::kByte || m.scales.device() != m.data.device() || m.data.dim() != m.scales.dim())
+    return false;
+  if (!rows_of(m.data, m.rows, m.width, m.stride) || !rows_of(m.scales, n, blocks, m.scale_stride)) return false;
+  if (m.width % 32 != 0 || blocks * 32 != m.width || n != m.rows) return false;
+  for (int64_t d = 0; d + 1 < m.data.dim(); ++d)
+    if (m.data.size(d) != m.scales.size(d)) return false;
+  return true;
+}
+
+// New MX8 rows of a shape.
+Mx8 new_mx8(at::IntArrayRef shape, const at::Device& dev) {
+  Mx8 m;
+  std::vector<int64_t> blocks(shape.begin(), shape.end());
+  blocks.back() /= 32;
+  m.data = at::empty(shape, at::TensorOptions().dtype(at::kFloat8_e4m3fn).device(dev));
+  m.scales = at::empty(blocks, at::TensorOptions().dtype(at::kByte).device(dev));
+  rows_of(m.data, m.rows, m.width, m.stride);
+  m.scale_stride = m.width / 32;
+  return m;
+}
+
+// The MX8Rows object of tensors that need no check; null with an error set.
+PyObject* wrap_mx8(const Mx8& m) {
+  PyObject* o = g_mx8->tp_new(g_mx8, g_no_args, nullptr);
+  if (o == nullptr) return nullptr;
+  PyObject* d = THPVariable_Wrap(m.data);
+  PyObject* s = d ? THPVariable_Wrap(m.scales) : nullptr;
+  const bool ok = s != nullptr && PyObject_SetAttr(o, g_str_data, d) == 0 && PyObject_SetAttr(o, g_str_scales, s) == 0;
+  Py_XDECREF(d);
+  Py_XDECREF(s);
+  if (ok) return o;
+  Py_DECREF(o);
+  return nullptr;
+}
+
+// As issue(), for an MX8Rows result.
+template <class F>
+PyObject* issue_mx8(const char* what, PyObject* given, const Mx8& out, F&& call) {
+  PyObject* r = given;
+  if (given == Py_None) {
+    r = wrap_mx8(out);
+    if (r == nullptr) return nullptr;
+  } else {
+    Py_INCREF(r);
+  }
+  const int32_t st = without_gil(call);
+  if (st == LKV_OK) return r;
+  Py_DECREF(r);
+  if (st != LKV_ERR_HIP) return not_handled();
+  return PyErr_Format(g_error, "%s failed (status %d): %s", what, static_cast<int>(st), g_lib.last_error());
+}
+
+// The output of an op on bf16 rows t: given MX8Rows of its shape, or new ones.
+bool mx8_out(PyObject* given, const at::Tensor& t, Mx8& m) {
+  if (t.size(-1) % 32 != 0) return false;
+  if (given == Py_None) {
+    m = new_mx8(t.sizes(), t.device());
+    return true;
+  }
+  return mx8_rows(given, m) && m.data.device() == t.device() && m.data.sizes() == t.sizes();
+}
+
+// (x, weight, eps, residual, out)
+PyObject* rmsnorm_mx8(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  if (n != 5 || !plain_mode()) return not_handled();
+  return guarded([&]() -> PyObject* {
+    const at::Tensor *x = tensor(v[0]), *w = tensor(v[1]);
+    lkv_rmsnorm_mx8_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.struct_size = sizeof(a);
+    int64_t nrows, hidden, r2, h2;
+    if (!bf16(x) || !rows_of(*x, nrows, hidden, a.x_stride) || !on_current_device(*x) || !bf16(w) || !w->is_contiguous() ||
+        w->numel() != hidden || w->device() != x->device() || !PyFloat_CheckExact(v[2]))
+      return not_handled();
+    if (v[3] != Py_None) {
+      const at::Tensor* r = tensor(v[3]);
+      if (!bf16(r) || !rows_of(*r, r2, h2, a.residual_stride) || r->sizes() != x->sizes() || r->device() != x->device())
+        return not_handled();
+      a.residual = ptr(*r);
+    }
+    Mx8 out;
+    if (!mx8_out(v[4], *x, out)) return not_handled();
+    a.rows = static_cast<int32_t>(nrows);
+    a.hidden = static_cast<int32_t>(hidden);
+    a.eps = PyFloat_AS_DOUBLE(v[2]);
+    a.x = ptr(*x);
+    a.weight = ptr(*w);
+    a.out = ptr(out.data);
+    a.out_stride = out.stride;
+    a.scales = ptr(out.scales);
+    a.scale_stride = out.scale_stride;
+    const lkv_stream_t s = stream_of(*x);
+    return issue_mx8("lkv_rmsnorm_mx8", v[4], out, [&] { return g_lib.rmsnorm_mx8(&a, s); });
+  });
+}
+
+// (gate, up, out)
+PyObject* silu_mul_mx8(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  if (n != 3 || !plain_mode()) return not_handled();
+  return guarded([&]() -> PyObject* {
+    const at::Tensor *g = tensor(v[0]), *u = tensor(v[1]);
+    int64_t nrows, width, gs, r2, w2, us;
+    if (!bf16(g) || !bf16(u) || !rows_of(*g, nrows, width, gs) || !rows_of(*u, r2, w2, us) || u->sizes() != g->sizes() ||
+        u->device() != g->device() || !on_current_device(*g))
+      return not_handled();
+    Mx8 out;
+    if (!mx8_out(v[2], *g, out)) return not_handled();
+    const lkv_stream_t s = stream_of(*g);
+    return issue_mx8("lkv_silu_mul_mx8", v[2], out, [&] {
+      return g_lib.silu_mul_mx8(ptr(*g), gs, ptr(*u), us, ptr(out.data), out.stride, ptr(out.scales), out.scale_stride,
+                                static_cast<int32_t>(nrows), static_cast<int32_t>(width), s);
+    });
+  });
+}
+
+// (rows,)
+PyObject* mx8_unpack(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  if (n != 1 || !plain_mode()) return not_handled();
+  return guarded([&]() -> PyObject* {
+    Mx8 x;
+    if (!mx8_rows(v[0], x) || !on_current_device(x.data)) return not_handled();
+    const at::Tensor out = new_bf16(x.data.sizes(), x.data.device());
+    const lkv_stream_t s = stream_of(x.data);
+    return issue("lkv_mx8_unpack", Py_None, out, [&] {
+      return g_lib.mx8_unpack(ptr(x.data), x.stride, ptr(x.scales), x.scale_stride, ptr(out), x.width,
+                              static_cast<int32_t>(x.rows), static_cast<int32_t>(x.width), s);
+    });
+  });
+}
+
+bool int_attr(PyObject* o, PyObject* name, int32_t& v) {
+  PyObject* a = PyObject_GetAttr(o, name);
+  const bool ok = a != nullptr && as_i32(a, v);
+  Py_XDECREF(a);
+  PyErr_Clear();
+  return ok;
+}
+
+// (x, weight, bias, out)
+PyObject* mx4_linear(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  if (n != 4 || !plain_mode()) return not_handled();
+  return guarded([&]() -> PyObject* {
+    lkv_mx4_linear_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.struct_size = sizeof(a);
+    if (Py_TYPE(v[1]) != g_mx4 || !int_attr(v[1], g_str_out_features, a.out_features) ||
+        !int_attr(v[1], g_str_in_features, a.in_features) || a.out_features < 1 || a.in_features < 1)
+      return not_handled();
+    const at::Tensor w = tensor_attr(v[1], g_str_data);
+    if (!w.defined() || w.scalar_type() != at::kByte || !w.is_contiguous() ||
+        w.numel() != g_lib.mx4_weight_bytes(a.out_features, a.in_features))
+      return not_handled();
+    at::Tensor x;
+    int64_t nrows, width, r2, w2;
+    if (Py_TYPE(v[0]) == g_mx8) {
+      Mx8 m;
+      if (!mx8_rows(v[0], m)) return not_handled();
+      x = m.data;
+      nrows = m.rows;
+      width = m.width;
+      a.x_format = LKV_X_MX8;
+      a.x_stride = m.stride;
+      a.x_scales = ptr(m.scales);
+      a.x_scale_stride = m.scale_stride;
+    } else {
+      const at::Tensor* t = tensor(v[0]);
+      if (!bf16(t) || !rows_of(*t, nrows, width, a.x_stride)) return not_handled();
+      x = *t;
+    }
+    const at::Device dev = x.device();
+    if (width != a.in_features || w.device() != dev || !on_current_device(x)) return not_handled();
+    const at::Tensor* bias;
+    if (!optional_vector(v[2], at::kBFloat16, a.out_features, dev, bias)) return not_handled();
+    at::Tensor out;
+    if (v[3] != Py_None) {
+      const at::Tensor* o = tensor(v[3]);
+      if (!bf16(o) || o->device() != dev || o->dim() != x.dim() || !rows_of(*o, r2, w2, a.out_stride) || r2 != nrows ||
+          w2 != a.out_features)
+        return not_handled();
+      for (int64_t d = 0; d + 1 < x.dim(); ++d)
+        if (o->size(d) != x.size(d)) return not_handled();
+      const uintptr_t xa = reinterpret_cast<uintptr_t>(x.const_data_ptr()), oa = reinterpret_cast<uintptr_t>(o->const_data_ptr());
+      const uintptr_t xe = xa + ((nrows - 1) * a.x_stride + width) * x.element_size();
+      const uintptr_t oe = oa + ((nrows - 1) * a.out_stride + w2) * 2;
+      if (xa < oe && oa < xe) return not_handled();  // (the Python path refuses an output over its input)
+      out = *o;
+    } else {
+      std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+      shape.back() = a.out_features;
+      out = new_bf16(shape, dev);
+      a.out_stride = a.out_features;
+    }
+    a.rows = static_cast<int32_t>(nrows);
+    a.x = ptr(x);
+    a.weight = ptr(w);
+    a.bias = bias ? ptr(*bias) : nullptr;
+    a.out = ptr(out);
+    const lkv_stream_t s = stream_of(x);
+    return issue("lkv_mx4_linear", v[3], out, [&] { return g_lib.mx4_linear(&a, s); });
+  });
+}
+
+// bind(addresses: the entry points in Library's order, TiledKV, PagedKV, LastKVNativeError, MX8Rows, MX4Weight)
 PyObject* bind(PyObject*, PyObject* args) {
-  PyObject *addresses, *tiled, *paged, *error;
-  if (!PyArg_ParseTuple(args, "O!O!O!O!", &PyTuple_Type, &addresses, &PyType_Type, &tiled, &PyType_Type, &paged, &PyType_Type,
-                        &error))
+  PyObject *addresses, *tiled, *paged, *error, *mx8, *mx4;
+  if (!PyArg_ParseTuple(args, "O!O!O!O!O!O!", &PyTuple_Type, &addresses, &PyType_Type, &tiled, &PyType_Type, &paged,
+                        &PyType_Type, &error, &PyType_Type, &mx8, &PyType_Type, &mx4))
     return nullptr;
   constexpr Py_ssize_t kEntries = sizeof(Library) / sizeof(void*);
   if (PyTuple_GET_SIZE(addresses) != kEntries) {
@@ -696,7 +958,11 @@ PyObject* bind(PyObject*, PyObject* args) {
   Py_INCREF(tiled);
   Py_INCREF(paged);
   Py_INCREF(error);
+  Py_INCREF(mx8);
+  Py_INCREF(mx4);
   g_error = error;
+  g_mx8 = reinterpret_cast<PyTypeObject*>(mx8);
+  g_mx4 = reinterpret_cast<PyTypeObject*>(mx4);
   g_tiled = reinterpret_cast<PyTypeObject*>(tiled);
   g_paged = reinterpret_cast<PyTypeObject*>(paged);
   Py_RETURN_NONE;
@@ -723,6 +989,10 @@ PyMethodDef kMethods[] = {
     {"qkv_epilogue", fast(qkv_epilogue), METH_FASTCALL, nullptr},
     {"rmsnorm", fast(rmsnorm), METH_FASTCALL, nullptr},
     {"silu_mul", fast(silu_mul), METH_FASTCALL, nullptr},
+    {"rmsnorm_mx8", fast(rmsnorm_mx8), METH_FASTCALL, nullptr},
+    {"silu_mul_mx8", fast(silu_mul_mx8), METH_FASTCALL, nullptr},
+    {"mx8_unpack", fast(mx8_unpack), METH_FASTCALL, nullptr},
+    {"mx4_linear", fast(mx4_linear), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 
@@ -734,5 +1004,10 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", "Native launch path of th
 PyMODINIT_FUNC PyInit__host() {
   g_str_k = PyUnicode_InternFromString("k");
   g_str_v = PyUnicode_InternFromString("v");
+  g_str_data = PyUnicode_InternFromString("data");
+  g_str_scales = PyUnicode_InternFromString("scales");
+  g_str_out_features = PyUnicode_InternFromString("out_features");
+  g_str_in_features = PyUnicode_InternFromString("in_features");
+  g_no_args = PyTuple_New(0);
   return PyModule_Create(&kModule);
 }

@@ -176,9 +176,10 @@ def _bind_host() -> bool:
     except _lib.LastKVNativeError:
         return False
     names = ("lkv_decode_attn", "lkv_decode_workspace_bytes", "lkv_prefill_attn", "lkv_prefill_workspace_bytes",
-             "lkv_qkv_epilogue", "lkv_rmsnorm", "lkv_silu_mul", "lkv_last_error")
+             "lkv_qkv_epilogue", "lkv_rmsnorm", "lkv_silu_mul", "lkv_last_error", "lkv_rmsnorm_mx8", "lkv_silu_mul_mx8",
+             "lkv_mx8_unpack", "lkv_mx4_linear", "lkv_mx4_weight_bytes")
     _host.bind(tuple(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names), TiledKV, PagedKV,
-               _lib.LastKVNativeError)
+               _lib.LastKVNativeError, MX8Rows, MX4Weight)
     _host_bound = True
     return True
 
@@ -1085,6 +1086,14 @@ def _same_device(device: torch.device, **tensors: torch.Tensor | None) -> None:
         _require(t is None or t.device == device, f"{name} must be on {device}")
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors meet."""
+
+    span = lambda t: sum((n - 1) * st for n, st in zip(t.shape, t.stride())) * t.element_size() + t.element_size()
+    return (a.numel() > 0 and b.numel() > 0 and a.data_ptr() < b.data_ptr() + span(b)
+            and b.data_ptr() < a.data_ptr() + span(a))
+
+
 def _mx8_strides(name: str, rows: MX8Rows) -> tuple[int, int, int, int]:
     """(rows, width, data row stride, scale row stride) of MX8 rows viewed as [rows, width]."""
 
@@ -1119,6 +1128,10 @@ def rmsnorm_mx8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: 
     each block of 32 rounded once, correctly, to e4m3 under the smallest power-of-two scale that holds its largest
     value.  A block with an infinity or NaN is NaN.  Returns ``out``."""
 
+    if _host_bound or _bind_host():
+        done = _host.rmsnorm_mx8(x, weight, eps, residual, out)
+        if done is not None:
+            return done
     _require_bf16_cuda("x", x)
     _require(x.dim() >= 1, "x must have rows")
     out = _mx8_out(x, out)
@@ -1150,6 +1163,10 @@ def silu_mul_mx8(gate: torch.Tensor, up: torch.Tensor, out: MX8Rows | None = Non
     """``F.silu(gate) * up`` of bf16 ``[..., width]`` tensors (width a multiple of 32) with an 8-bit output, each
     block of 32 rounded once as ``rmsnorm_mx8`` rounds it."""
 
+    if _host_bound or _bind_host():
+        done = _host.silu_mul_mx8(gate, up, out)
+        if done is not None:
+            return done
     _require_bf16_cuda("gate", gate)
     _require_bf16_cuda("up", up)
     _require(gate.dim() >= 1 and up.shape == gate.shape, "up shape must match gate")
@@ -1170,6 +1187,10 @@ def silu_mul_mx8(gate: torch.Tensor, up: torch.Tensor, out: MX8Rows | None = Non
 def mx8_unpack(rows: MX8Rows) -> torch.Tensor:
     """The values of ``rows`` in bf16."""
 
+    if _host_bound or _bind_host():
+        done = _host.mx8_unpack(rows)
+        if done is not None:
+            return done
     _require(isinstance(rows, MX8Rows), "rows must be MX8Rows")
     out = torch.empty(rows.shape, dtype=torch.bfloat16, device=rows.device)
     if out.numel() == 0:
@@ -1233,6 +1254,10 @@ def mx4_linear(x: torch.Tensor | MX8Rows, weight: MX4Weight, bias: torch.Tensor 
     of bf16 rows are exact; those of 8-bit rows are added eight columns at a time in the matrix instruction's fixed
     point, which keeps 13 bits below the largest."""
 
+    if _host_bound or _bind_host():
+        done = _host.mx4_linear(x, weight, bias, out)
+        if done is not None:
+            return done
     _require(isinstance(weight, MX4Weight), "weight must be an MX4Weight")
     n, k = weight.out_features, weight.in_features
     mx8 = isinstance(x, MX8Rows)
@@ -1249,6 +1274,7 @@ def mx4_linear(x: torch.Tensor | MX8Rows, weight: MX4Weight, bias: torch.Tensor 
     _require_bf16_cuda("out", out)
     _require(tuple(out.shape) == shape, f"out must be {list(shape)}")
     _same_device(device, weight=weight.data, bias=bias, out=out)
+    _require(not _overlap(out, x.data if mx8 else x), "out must not overlap x")
     if out.numel() == 0:
         return out
     a = _lib.Mx4LinearArgs()

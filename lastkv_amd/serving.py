@@ -555,6 +555,19 @@ def fuse_linears(mods) -> tuple[torch.Tensor, torch.Tensor | None]:
     return weight, bias
 
 
+def quantize_linears(mods) -> tuple[ops.MX4Weight, torch.Tensor | None]:
+    """One 4-bit weight (and bf16 bias) for ``nn.Linear`` modules that read the same input, their rows one after
+    another as in ``fuse_linears``; the modules keep their own weights."""
+
+    mods = list(mods)
+    with_bias = [m.bias is not None for m in mods]
+    if any(with_bias) and not all(with_bias):
+        raise ValueError("fused projections must all have a bias or none")
+    weight = mods[0].weight.detach() if len(mods) == 1 else torch.cat([m.weight.detach() for m in mods])
+    bias = torch.cat([m.bias.detach() for m in mods]) if all(with_bias) else None
+    return ops.mx4_quantize(weight), bias
+
+
 class LastKVServingModel:
     """Continuous-batching runner of a ``lastkv_amd.llm`` causal LM over a LastKVFastPath: one
     ``step`` runs the decoder over ragged rows (prefill pieces and decode tokens of different
@@ -563,10 +576,23 @@ class LastKVServingModel:
     model's own modules; q / k / v and gate / up run as one GEMM each over weights fused in place
     (``fuse_linears``, the layout of vLLM's ``qkv_proj`` / ``gate_up_proj``): at decode (M = 32 rows)
     hipBLASLt takes ~19 us per projection GEMM whatever its width, so three q / k / v GEMMs cost
-    59 us per layer against 19 us for the fused one."""
+    59 us per layer against 19 us for the fused one.
+
+    ``weights="mxfp4"`` holds the decoder layers' projections in 4 bits (``quantize_linears``: e2m1 with a
+    power-of-two scale per 32 columns; embeddings, norms and lm_head stay bf16) and runs them as ``ops.mx4_linear``.
+    ``activations="mxfp8"`` then also hands q / k / v, gate / up and down 8-bit rows, which the norms and the SwiGLU
+    product write (``ops.rmsnorm_mx8``, ``ops.silu_mul_mx8``); the output projection reads the attention's bf16 rows.
+    The model passed in keeps its bf16 weights."""
 
     def __init__(self, model, *, max_batch: int, max_tokens_per_slot: int, source_pages: int | None = None,
-                 num_splits: int | None = None, device=None, contract: str = "hf"):
+                 num_splits: int | None = None, device=None, contract: str = "hf", weights: str = "bf16",
+                 activations: str = "bf16"):
+        if weights not in ("bf16", "mxfp4"):
+            raise ValueError(f"weights must be 'bf16' or 'mxfp4', got {weights!r}")
+        if activations not in ("bf16", "mxfp8"):
+            raise ValueError(f"activations must be 'bf16' or 'mxfp8', got {activations!r}")
+        if activations == "mxfp8" and weights != "mxfp4":
+            raise ValueError("8-bit activations go with weights='mxfp4'")
         self.model = model
         inner = model.model
         cfg = inner.config
@@ -581,6 +607,13 @@ class LastKVServingModel:
         self.fast = LastKVFastPath.from_model(model, self.pool, max_batch=max_batch, num_splits=num_splits,
                                               contract=contract)
         self.config = cfg
+        self.weights, self.activations = weights, activations
+        if weights == "mxfp4":
+            self._mx4 = [(quantize_linears((l.self_attn.q_proj, l.self_attn.k_proj, l.self_attn.v_proj)),
+                          quantize_linears((l.self_attn.o_proj,)),
+                          quantize_linears((l.mlp.gate_proj, l.mlp.up_proj)), quantize_linears((l.mlp.down_proj,)))
+                         for l in inner.layers]
+            return
         self._qkv = [fuse_linears((l.self_attn.q_proj, l.self_attn.k_proj, l.self_attn.v_proj)) for l in inner.layers]
         self._gate_up = [fuse_linears((l.mlp.gate_proj, l.mlp.up_proj)) for l in inner.layers]
 
@@ -609,6 +642,8 @@ class LastKVServingModel:
         RMSNorms run fused (``lkv_rmsnorm``, LlamaRMSNorm arithmetic) and the MLP's SiLU product as
         ``lkv_silu_mul``, the roles of vLLM's fused_add_rms_norm and silu_and_mul."""
 
+        if self.weights == "mxfp4":
+            return self._layers_mx4(ids)
         inner = self.model.model
         layers = inner.layers
         eps = self.config.rms_norm_eps
@@ -631,6 +666,34 @@ class LastKVServingModel:
             nxt = layers[i + 1].input_layernorm.weight if i + 1 < len(layers) else inner.norm.weight
             h = ops.rmsnorm(m, nxt, eps, residual=hidden)
         return h
+
+    def _layers_mx4(self, ids: torch.Tensor) -> torch.Tensor:
+        """``_layers`` over 4-bit weights."""
+
+        inner = self.model.model
+        layers = inner.layers
+        eps = float(self.config.rms_norm_eps)
+        T = ids.numel()
+        hidden = inner.embed_tokens(ids)  # the residual stream, updated in place
+        Hq = self.config.num_attention_heads
+        out = torch.empty((T, Hq, ops.HEAD_DIM), dtype=hidden.dtype, device=hidden.device)
+        kv = self.config.num_key_value_heads * ops.HEAD_DIM
+        widths = [Hq * ops.HEAD_DIM, kv, kv]
+        inter = self.config.intermediate_size
+        norm, silu_mul = ((ops.rmsnorm_mx8, ops.silu_mul_mx8) if self.activations == "mxfp8" else
+                          (ops.rmsnorm, ops.silu_mul))
+        h = norm(hidden, layers[0].input_layernorm.weight, eps)
+        for i, layer in enumerate(layers):
+            qkv, o, gate_up, down = self._mx4[i]
+            q, k, v = ops.mx4_linear(h, *qkv).split(widths, dim=-1)
+            self.fast.run_layer(i, q, k, v, out)
+            h = norm(ops.mx4_linear(out.view(T, Hq * ops.HEAD_DIM), *o), layer.post_attention_layernorm.weight, eps,
+                     residual=hidden)
+            gu = ops.mx4_linear(h, *gate_up)
+            m = ops.mx4_linear(silu_mul(gu[:, :inter], gu[:, inter:]), *down)
+            if i + 1 < len(layers):
+                h = norm(m, layers[i + 1].input_layernorm.weight, eps, residual=hidden)
+        return ops.rmsnorm(m, inner.norm.weight, eps, residual=hidden)
 
     def decode_graph(self, slots: list[int], num_splits: int | None = None) -> "DecodeGraph":
         """A HIP-graph replay of greedy decode steps for ``slots`` (one token each per step)."""

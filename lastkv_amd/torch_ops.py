@@ -24,7 +24,7 @@ from torch import Tensor
 from . import ops
 
 __all__ = ["decode_attention", "prefill_attention", "merge_states", "qkv_epilogue", "blend_chunk", "rmsnorm",
-           "silu_mul"]
+           "silu_mul", "rmsnorm_mx8", "add_rmsnorm_mx8", "silu_mul_mx8", "mx8_unpack", "mx4_linear", "mx4_linear_mx8"]
 
 
 def _seg(k: Optional[Tensor], v: Optional[Tensor], table: Optional[Tensor]):
@@ -177,3 +177,85 @@ def silu_mul(gate: Tensor, up: Tensor) -> Tensor:
 @silu_mul.register_fake
 def _(gate, up):
     return gate.new_empty(gate.shape)
+
+
+# MX8 rows enter and leave as their two tensors (float8_e4m3fn data, uint8 scales), an MX4 weight as its data and shape.
+def _mx8_like(x: Tensor) -> tuple[Tensor, Tensor]:
+    return (x.new_empty(x.shape, dtype=torch.float8_e4m3fn),
+            x.new_empty((*x.shape[:-1], x.shape[-1] // ops.MX_BLOCK), dtype=torch.uint8))
+
+
+@torch.library.custom_op("lastkv::rmsnorm_mx8", mutates_args=())
+def rmsnorm_mx8(x: Tensor, weight: Tensor, eps: float) -> tuple[Tensor, Tensor]:
+    """``lkv_rmsnorm_mx8`` without a residual: (e4m3 data, e8m0 scales) of the normalised rows."""
+
+    out = ops.rmsnorm_mx8(x, weight, eps)
+    return out.data, out.scales
+
+
+@rmsnorm_mx8.register_fake
+def _(x, weight, eps):
+    return _mx8_like(x)
+
+
+@torch.library.custom_op("lastkv::add_rmsnorm_mx8", mutates_args=("residual",))
+def add_rmsnorm_mx8(x: Tensor, residual: Tensor, weight: Tensor, eps: float) -> tuple[Tensor, Tensor]:
+    """``lkv_rmsnorm_mx8`` with a residual: ``residual += x`` in place, then its normalised rows."""
+
+    out = ops.rmsnorm_mx8(x, weight, eps, residual=residual)
+    return out.data, out.scales
+
+
+@add_rmsnorm_mx8.register_fake
+def _(x, residual, weight, eps):
+    return _mx8_like(x)
+
+
+@torch.library.custom_op("lastkv::silu_mul_mx8", mutates_args=())
+def silu_mul_mx8(gate: Tensor, up: Tensor) -> tuple[Tensor, Tensor]:
+    """``lkv_silu_mul_mx8``: (e4m3 data, e8m0 scales) of ``F.silu(gate) * up``."""
+
+    out = ops.silu_mul_mx8(gate, up)
+    return out.data, out.scales
+
+
+@silu_mul_mx8.register_fake
+def _(gate, up):
+    return _mx8_like(gate)
+
+
+@torch.library.custom_op("lastkv::mx8_unpack", mutates_args=())
+def mx8_unpack(data: Tensor, scales: Tensor) -> Tensor:
+    """``lkv_mx8_unpack``: the values of MX8 rows in bf16."""
+
+    return ops.mx8_unpack(ops.MX8Rows(data, scales))
+
+
+@mx8_unpack.register_fake
+def _(data, scales):
+    return data.new_empty(data.shape, dtype=torch.bfloat16)
+
+
+@torch.library.custom_op("lastkv::mx4_linear", mutates_args=())
+def mx4_linear(x: Tensor, weight: Tensor, out_features: int, bias: Optional[Tensor] = None) -> Tensor:
+    """``lkv_mx4_linear`` of bf16 rows: ``weight`` is an ``ops.MX4Weight``'s data."""
+
+    return ops.mx4_linear(x, ops.MX4Weight(weight, out_features, x.shape[-1]), bias)
+
+
+@mx4_linear.register_fake
+def _(x, weight, out_features, bias=None):
+    return x.new_empty((*x.shape[:-1], out_features))
+
+
+@torch.library.custom_op("lastkv::mx4_linear_mx8", mutates_args=())
+def mx4_linear_mx8(data: Tensor, scales: Tensor, weight: Tensor, out_features: int,
+                   bias: Optional[Tensor] = None) -> Tensor:
+    """``lkv_mx4_linear`` of MX8 rows."""
+
+    return ops.mx4_linear(ops.MX8Rows(data, scales), ops.MX4Weight(weight, out_features, data.shape[-1]), bias)
+
+
+@mx4_linear_mx8.register_fake
+def _(data, scales, weight, out_features, bias=None):
+    return data.new_empty((*data.shape[:-1], out_features), dtype=torch.bfloat16)
