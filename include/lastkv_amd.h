@@ -645,11 +645,15 @@ int32_t lkv_mx4_quantize(const void *src, int64_t src_stride, int32_t n, int32_t
 
 int32_t lkv_mx4_unpack(const void *weight, int32_t n, int32_t k, void *out, int64_t out_stride, lkv_stream_t stream);
 
-/* out[m][n] = bf16(sum_k x[m][k] * weight[n][k] + bias[n]): fp32 sums in a fixed order, rounded once.  bf16 rows: the
- * products are exact.  MX8 rows: the scaled matrix instruction adds the products of 8 neighbouring columns in fixed
- * point (bits below 2^-13 of the largest product's exponent are dropped) before it adds to fp32.
- * in_features is a multiple of 32; x rows are 16-byte aligned. */
+/* out[m][n] = bf16(sum_k x[m][k] * weight[n][k] + bias[n]): exact products, fp32 sums in a fixed order, rounded once.
+ * The tile kernel, which takes calls of many rows (kernel = LKV_MX4_AUTO chooses by sizes), differs for MX8 rows: the
+ * scaled matrix instruction adds the products of 8 neighbouring columns in fixed point (bits below 2^-13 of the largest
+ * power of two of their factors' exponents are dropped) before it adds to fp32.  MX8 values past bf16's range are
+ * infinite for the row kernel.
+ * in_features is a multiple of 32 up to 2^20; x rows are 16-byte aligned, at most 2^21 elements apart; out must not
+ * overlap x. */
 enum { LKV_X_BF16 = 0, LKV_X_MX8 = 1 };
+enum { LKV_MX4_AUTO = 0, LKV_MX4_ROWS = 1, LKV_MX4_TILES = 2 };
 
 typedef struct lkv_mx4_linear_args {
   int32_t struct_size; /* sizeof(lkv_mx4_linear_args) */
@@ -657,7 +661,7 @@ typedef struct lkv_mx4_linear_args {
   int32_t out_features;
   int32_t in_features;
   int32_t x_format; /* LKV_X_BF16 or LKV_X_MX8 */
-  int32_t reserved;
+  int32_t kernel;   /* LKV_MX4_AUTO, or the kernel to take */
   const void *x; /* bf16 or e4m3 [rows, in_features] */
   int64_t x_stride;
   const void *x_scales; /* MX8: e8m0 [rows, in_features / 32]; else NULL */

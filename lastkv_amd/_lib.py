@@ -354,7 +354,7 @@ class Mx4LinearArgs(ctypes.Structure):
         ("out_features", c_i32),
         ("in_features", c_i32),
         ("x_format", c_i32),
-        ("reserved", c_i32),
+        ("kernel", c_i32),
         ("x", c_ptr),
         ("x_stride", c_i64),
         ("x_scales", c_ptr),

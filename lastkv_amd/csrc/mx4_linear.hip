@@ -19,6 +19,8 @@ struct LinearParams {
   int64_t out_stride;
   int32_t M, N, K;
   int32_t units;
+  bool vector_out;  // output rows are 8-byte aligned
+  bool scale_words;  // x scales in whole aligned words: a row's four of a tile
 };
 
 constexpr int kWaves = 8;
@@ -46,11 +48,36 @@ __device__ inline uint4 e4m3_to_bf16(uint32_t a, uint32_t b, float scale) {
 
 __device__ inline uint32_t word_of(const uint4& v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
 
-__device__ inline uint4 buffer_load16(__amdgpu_buffer_rsrc_t r, int offset) {
-  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 0));
+__device__ inline uint4 buffer_load16(__amdgpu_buffer_rsrc_t r, int offset, int scalar_offset = 0) {
+  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, offset, scalar_offset, 0));
 }
 
-constexpr int kOutside = 0x7fffffff;  // an offset past every buffer: loads give zeros
+// 16 bytes of each lane to LDS at `dst` + 16 lane (dst the same for the wave), past the registers.
+__device__ inline void buffer_to_lds16(__amdgpu_buffer_rsrc_t r, char* dst, int offset, int scalar_offset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)dst, 16, offset, scalar_offset, 0, 0);
+}
+
+// Every load of the wave has arrived (those to LDS too).
+__device__ inline void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
+
+// An offset past every buffer (they hold less than 2^30 bytes and a row's columns 2^21): loads give zeros.
+constexpr int kOutside = 0x60000000;
+
+// Four neighbouring outputs of row m.
+__device__ inline void store_out(const LinearParams& p, int m, int n, f32x4 v) {
+  uint16_t* out = p.out + m * p.out_stride;
+  if (p.vector_out && n + 4 <= p.N) {
+    if (p.bias != nullptr) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += bf16_bits_to_f32(p.bias[n + e]);
+    }
+    *reinterpret_cast<uint2*>(out + n) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (n + e < p.N) out[n + e] = f32_to_bf16_bits(v[e] + (p.bias ? bf16_bits_to_f32(p.bias[n + e]) : 0.f));
+}
 
 // What a wave holds of one step of columns of the weight, and the scales of MX8 rows.
 template <int MT, int NT>
@@ -231,13 +258,189 @@ __global__ __launch_bounds__(kWaves * 64, MT == 1 && NT <= 2 ? 4 : 2) void mx4_r
 #pragma unroll
       for (int v = 1; v < KS; ++v) s += from[v * NT * MT * 64];
     }
-    if (m < p.M) {
-      uint16_t* out = p.out + m * p.out_stride;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e < p.N) out[n + e] = f32_to_bf16_bits(s[e] + (p.bias ? bf16_bits_to_f32(p.bias[n + e]) : 0.f));
-    }
+    if (m < p.M) store_out(p, m, n, s);
   }
+}
+
+// Many rows: one workgroup of WN x WM waves per (16 WN TN rows of the weight, 16 WM TM rows of x), each wave TN x TM
+// tiles of 16 x 16.  Tiles of 128 columns of both go to LDS by direct loads, two buffers, one barrier a tile; two workgroups
+// share a CU, so that one's products cover the other's reads of LDS.
+// MX8 rows: both operands and both scales go to the scaled matrix instruction as they are (a code is converted nowhere).
+// Bound by the matrix pipe, of which 4096 rows of 28672 x 4096 reach 2.36 PFLOP/s (407 us; bf16 weights in the library's
+// GEMM 641 us); independent products in registers reach 3.83 PFLOP/s on this card.  With the tile staged through
+// registers 426-447 us, with its LDS writes before the products 454.
+// bf16 rows: the codes are converted in registers as they are used.  1000 rows of 6144 x 4096 take 52 us, 0.97 PFLOP/s, 4096
+// rows 174 us, 1.19 PFLOP/s (library, bf16 weights, 1000 rows: 52 us); bf16 products in registers reach 1.92 PFLOP/s.
+template <bool kMx8, bool kWords, int WN, int WM, int TN, int TM>
+__global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearParams p, int mtiles, int grid) {
+  constexpr int kThreads = WN * WM * 64, kBN = WN * TN, kBM = WM * TM;  // (in tiles of 16)
+  constexpr int kRowBytes = kMx8 ? 128 : 256, kChunks = kRowBytes / 16;
+  constexpr int kXBytes = kBM * 16 * kRowBytes, kWBytes = kBN * kMxTileBytes;
+  constexpr int kBuf = kXBytes + kWBytes + (kMx8 ? kBM * 64 : 0);  // x, codes, one word of scales per row of x
+  constexpr int kXLoads = kBM * 16 * kChunks / kThreads, kWLoads = kBN * 64 / kThreads;
+  __shared__ __attribute__((aligned(16))) char smem[2 * kBuf];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, g = lane >> 4, wn = wave % WN, wm = wave / WN;
+  // an XCD's workgroups in a row share four tiles of x and walk over the weight
+  const int id = xcd_logical_index(blockIdx.x, grid);
+  const int ntiles = (p.N + 15) >> 4, nblocks = (ntiles + kBN - 1) / kBN;
+  const int group = id / (4 * nblocks), in_group = id % (4 * nblocks);
+  const int rows_in_group = min(4, mtiles - 4 * group);
+  const int mb = 4 * group + in_group % rows_in_group, nb = in_group / rows_in_group;
+  const int m0 = mb * kBM * 16, nt0 = nb * kBN;
+
+  const int valid = min(p.M - m0, kBM * 16), blocks = p.K >> 5;
+  const int stride = static_cast<int>(p.x_stride) * (kMx8 ? 1 : 2), row_bytes = p.K * (kMx8 ? 1 : 2);
+  const __amdgpu_buffer_rsrc_t xb = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<char*>(static_cast<const char*>(p.x) + static_cast<int64_t>(m0) * stride), 0,
+      (valid - 1) * stride + row_bytes, 0x00020000);
+  const int tile_stride = p.units * kMxUnitBytes;
+  const __amdgpu_buffer_rsrc_t wb = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(p.w + static_cast<int64_t>(nt0) * tile_stride), 0, min(kBN, ntiles - nt0) * tile_stride, 0x00020000);
+
+  const int xs_stride = static_cast<int>(p.xs_stride);
+  const __amdgpu_buffer_rsrc_t sb = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint8_t*>(p.xs + static_cast<int64_t>(m0) * xs_stride), 0, (valid - 1) * xs_stride + blocks, 0x00020000);
+
+  // what this lane moves: 16 bytes of rows xrow, xrow + kRowStep, ... of x, 16 of a lane's in every code tile.  LDS takes a
+  // wave's bytes in lane order, so the lane picks the chunk that its place in the swizzled row holds.
+  constexpr int kRowStep = kThreads / kChunks;
+  static_assert(kRowStep % 8 == 0, "a lane's rows share their swizzle");
+  const int xrow = tid / kChunks, xcol = ((tid % kChunks) ^ (xrow & 7)) * 16;
+  int xoff[kXLoads];
+#pragma unroll
+  for (int j = 0; j < kXLoads; ++j)
+    xoff[j] = xrow + j * kRowStep < valid ? (xrow + j * kRowStep) * stride + xcol : kOutside;
+  const int soff = tid < valid ? tid * xs_stride : kOutside;
+  char* const wave_dst = smem + wave * 1024;
+  uint32_t sr[4];
+  auto load = [&](int kt, int buf) {
+    const bool in = xcol < row_bytes - kt * kRowBytes;
+#pragma unroll
+    for (int j = 0; j < kXLoads; ++j)
+      buffer_to_lds16(xb, wave_dst + buf * kBuf + j * kThreads * 16, in ? xoff[j] : kOutside, kt * kRowBytes);
+#pragma unroll
+    for (int j = 0; j < kWLoads; ++j)
+      buffer_to_lds16(wb, wave_dst + buf * kBuf + kXBytes + j * kThreads * 16, lane * 16,
+                      (j * (kThreads / 64) + wave) * tile_stride + (kt >> 2) * kMxUnitBytes + (kt & 3) * kMxTileBytes);
+    if constexpr (kMx8) {  // thread t: the four scales of row t
+      if constexpr (kWords) {
+        sr[0] = __builtin_amdgcn_raw_buffer_load_b32(sb, soff, 4 * kt, 0);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          sr[q] = __builtin_amdgcn_raw_buffer_load_b8(sb, 4 * kt + q < blocks ? soff : kOutside, 4 * kt + q, 0);
+      }
+    }
+  };
+  auto store_scales = [&](int buf) {
+    if constexpr (kMx8) {
+      const uint32_t v = kWords ? sr[0] : sr[0] | sr[1] << 8 | sr[2] << 16 | sr[3] << 24;
+      if (tid < kBM * 16) reinterpret_cast<uint32_t*>(smem + buf * kBuf + kXBytes + kWBytes)[tid] = v;
+    }
+  };
+
+  f32x4 acc[TN][TM];
+#pragma unroll
+  for (int i = 0; i < TN; ++i)
+#pragma unroll
+    for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  uint32_t ws[TN], ws_next[TN];  // scale words of this unit and the next
+  auto load_scales = [&](int u) {
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+      ws_next[i] = __builtin_amdgcn_raw_buffer_load_b32(
+          wb, lane * 4, (wn * TN + i) * tile_stride + u * kMxUnitBytes + 4 * kMxTileBytes, 0);
+  };
+
+  const int tiles = (p.K + 127) >> 7;
+  // tile kt = 4 u + t, from buffer t & 1: the fragments are read, then the next tile's loads start, which the products
+  // cover (past the last tile they repeat it)
+  auto step = [&](int kt) {
+    const int t = kt & 3;
+    const char* x = smem + (t & 1) * kBuf + wm * TM * 16 * kRowBytes;
+    const uint4* w = reinterpret_cast<const uint4*>(smem + (t & 1) * kBuf + kXBytes + wn * TN * kMxTileBytes) + lane;
+    uint4 c[TN];
+#pragma unroll
+    for (int i = 0; i < TN; ++i) c[i] = w[i * 64];
+    if constexpr (kMx8) {
+      // x: lane (row, g) takes columns 16 g .. and 64 + 16 g .. of a tile, and the scale of block g
+      const uint32_t* sx = reinterpret_cast<const uint32_t*>(smem + (t & 1) * kBuf + kXBytes + kWBytes) + wm * TM * 16 + r;
+      i32x8 b[TM];
+      uint32_t sb[TM];
+#pragma unroll
+      for (int j = 0; j < TM; ++j) {
+        const char* row = x + (16 * j + r) * kRowBytes;
+        const uint4 lo = *reinterpret_cast<const uint4*>(row + ((g ^ (r & 7)) * 16));
+        const uint4 hi = *reinterpret_cast<const uint4*>(row + (((g + 4) ^ (r & 7)) * 16));
+        b[j] = i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
+        sb[j] = sx[16 * j] >> (8 * g);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      load(min(kt + 1, tiles - 1), (t + 1) & 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < TN; ++i) {
+        const i32x8 a = {(int)c[i].x, (int)c[i].y, (int)c[i].z, (int)c[i].w, 0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < TM; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b[j], acc[i][j], 4, 0, 0, ws[i] >> (8 * t), 0, sb[j]);
+      }
+    } else {
+      uint4 b[4][TM];
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int j = 0; j < TM; ++j)
+          b[s][j] = *reinterpret_cast<const uint4*>(x + (16 * j + r) * kRowBytes + (((4 * g + s) ^ (r & 7)) * 16));
+      __builtin_amdgcn_sched_barrier(0);
+      load(min(kt + 1, tiles - 1), (t + 1) & 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+#pragma unroll
+        for (int i = 0; i < TN; ++i) {
+          const uint4 a = e2m1_to_bf16(word_of(c[i], s), e8m0(ws[i], t));
+#pragma unroll
+          for (int j = 0; j < TM; ++j) acc[i][j] = mfma_bf16(a, b[s][j], acc[i][j]);
+        }
+      }
+    }
+    // the products come before the wait: nothing else orders them, and the compiler would move them behind it
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int j = 0; j < TM; ++j) asm volatile("" : "+v"(acc[i][j]));
+    __builtin_amdgcn_sched_barrier(0);
+    store_scales((t + 1) & 1);
+    wait_loads();
+    __syncthreads();
+  };
+  auto next_unit = [&](int u) {
+#pragma unroll
+    for (int i = 0; i < TN; ++i) ws[i] = ws_next[i];
+    load_scales(min(u + 1, p.units - 1));
+  };
+  load_scales(0);
+  load(0, 0);
+  store_scales(0);
+  wait_loads();
+  __syncthreads();
+  // (one tile per iteration: side by side in one block, the compiler mixes the tiles' products, which nothing orders, and
+  // runs out of registers)
+  for (int u = 0; u < p.units; ++u) {
+    next_unit(u);
+    const int end = min(4 * u + 4, tiles);
+#pragma unroll 1
+    for (int kt = 4 * u; kt < end; ++kt) step(kt);
+  }
+#pragma unroll
+  for (int i = 0; i < TN; ++i)
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      const int n = (nt0 + wn * TN + i) * 16 + 4 * g, m = m0 + (wm * TM + j) * 16 + r;
+      if (m < p.M) store_out(p, m, n, acc[i][j]);
+    }
 }
 
 template <bool kMx8, int MT, int NT, int KS>
@@ -271,12 +474,38 @@ void launch_mt(const LinearParams& p, hipStream_t s) {
     launch_rows<kMx8, MT, 4, 1>(p, s);
 }
 
-template <bool kMx8>
-int32_t launch(const LinearParams& p, hipStream_t s) {
-  if (p.M <= 16)
-    launch_mt<kMx8, 1>(p, s);
+template <bool kMx8, int WN, int WM, int TN, int TM>
+void launch_tile(const LinearParams& p, hipStream_t s) {
+  const int nblocks = (p.N + 16 * WN * TN - 1) / (16 * WN * TN), mtiles = (p.M + 16 * WM * TM - 1) / (16 * WM * TM);
+  const int grid = nblocks * mtiles;
+  if (!kMx8 || p.scale_words)
+    mx4_tile_kernel<kMx8, true, WN, WM, TN, TM><<<grid, WN * WM * 64, 0, s>>>(p, mtiles, grid);
   else
+    mx4_tile_kernel<kMx8, !kMx8, WN, WM, TN, TM><<<grid, WN * WM * 64, 0, s>>>(p, mtiles, grid);
+}
+
+// The tile kernel where the row kernel would give each CU more than 16 tiles of 16 weight rows x 32 rows of x: a round of
+// tiles takes as long whether it fills its CUs or not (us, bf16 / MX8 rows, row kernel against tiles: 28672 x 4096 for 64
+// rows, 14 tiles a CU, 31 / 32 against 38 / 33; for 96 rows, 21, 48 / 50 against 40 / 35; 6144 x 4096 for 256 rows, 12,
+// 25 / 26 against 39 / 34).  Up to 64 rows the row kernel, which HBM bounds, at any width.
+// MX8 rows take 256 x 128 tiles once those fill three quarters of the CUs (4096 rows of 28672 x 4096: 407 us against 478
+// with 128 x 128; 1000 rows of 4096 x 14336, 128 of them: 114 against 98); bf16 rows, which need twice the LDS, always
+// 128 x 128 (757 against 1009).
+template <bool kMx8>
+int32_t launch(const LinearParams& p, hipStream_t s, int kernel) {
+  const int64_t cus = std::max(1, device_cu_count());
+  const int64_t work = static_cast<int64_t>((p.N + 15) / 16) * ((p.M + 31) / 32);
+  if (kernel == LKV_MX4_TILES || (kernel == LKV_MX4_AUTO && p.M > 64 && work > 16 * cus)) {
+    const int64_t wide = static_cast<int64_t>((p.N + 255) / 256) * ((p.M + 127) / 128);
+    if (kMx8 && 4 * wide >= 3 * cus)
+      launch_tile<kMx8, 2, 2, 8, 4>(p, s);
+    else
+      launch_tile<kMx8, 2, 2, 4, 4>(p, s);
+  } else if (p.M <= 16) {
+    launch_mt<kMx8, 1>(p, s);
+  } else {
     launch_mt<kMx8, 2>(p, s);
+  }
   return check_launch("lkv_mx4_linear");
 }
 
@@ -434,6 +663,7 @@ extern "C" int32_t lkv_mx4_linear(const lkv_mx4_linear_args* a, lkv_stream_t str
               static_cast<int32_t>(sizeof(lkv_mx4_linear_args)));
   LKV_REQUIRE(a->x_format == LKV_X_BF16 || a->x_format == LKV_X_MX8, "x_format must be LKV_X_BF16 or LKV_X_MX8, got %d",
               a->x_format);
+  LKV_REQUIRE(a->kernel >= LKV_MX4_AUTO && a->kernel <= LKV_MX4_TILES, "kernel must be one of LKV_MX4_*, got %d", a->kernel);
   const bool mx8 = a->x_format == LKV_X_MX8;
   LKV_REQUIRE(a->rows >= 0 && a->rows <= (1 << 20), "rows must be in [0, 2^20], got %d", a->rows);
   LKV_REQUIRE_MX4_SHAPE(a->out_features, a->in_features);
@@ -442,7 +672,7 @@ extern "C" int32_t lkv_mx4_linear(const lkv_mx4_linear_args* a, lkv_stream_t str
   LKV_REQUIRE(((bits(a->x) | bits(a->weight)) & 15) == 0 && ((bits(a->out) | bits(a->bias)) & 1) == 0,
               "x and weight must be 16-byte aligned");
   LKV_REQUIRE(a->x_stride % (mx8 ? 16 : 8) == 0, "x rows must be 16-byte aligned");
-  LKV_REQUIRE(a->x_stride >= 0 && a->x_stride <= (1 << 23), "x_stride must be at most 2^23 elements");
+  LKV_REQUIRE(a->x_stride >= 0 && a->x_stride <= (1 << 21), "x_stride must be at most 2^21 elements");
   if (a->rows == 0) return LKV_OK;
   LinearParams p;
   p.w = static_cast<const uint8_t*>(a->weight);
@@ -457,5 +687,7 @@ extern "C" int32_t lkv_mx4_linear(const lkv_mx4_linear_args* a, lkv_stream_t str
   p.N = a->out_features;
   p.K = a->in_features;
   p.units = static_cast<int32_t>(mx4_units(a->in_features));
-  return mx8 ? launch<true>(p, as_stream(stream)) : launch<false>(p, as_stream(stream));
+  p.scale_words = (bits(a->x_scales) & 3) == 0 && a->x_scale_stride % 4 == 0 && a->in_features % 128 == 0;
+  p.vector_out = (bits(a->out) & 7) == 0 && a->out_stride % 4 == 0;
+  return mx8 ? launch<true>(p, as_stream(stream), a->kernel) : launch<false>(p, as_stream(stream), a->kernel);
 }

@@ -1250,9 +1250,9 @@ def mx4_unpack(weight: MX4Weight) -> torch.Tensor:
 def mx4_linear(x: torch.Tensor | MX8Rows, weight: MX4Weight, bias: torch.Tensor | None = None,
                out: torch.Tensor | None = None) -> torch.Tensor:
     """``F.linear`` over a 4-bit weight: ``x`` is bf16 ``[..., in_features]`` or ``MX8Rows`` of that shape, ``bias``
-    bf16 ``[out_features]``; returns bf16 ``[..., out_features]``, fp32 sums in a fixed order rounded once.  Products
-    of bf16 rows are exact; those of 8-bit rows are added eight columns at a time in the matrix instruction's fixed
-    point, which keeps 13 bits below the largest."""
+    bf16 ``[out_features]``; returns bf16 ``[..., out_features]``: exact products, fp32 sums in a fixed order, rounded
+    once.  In calls of many 8-bit rows the products are added eight columns at a time in the matrix instruction's fixed
+    point, which keeps 13 bits below the largest, before they are added in fp32.  ``out`` must not overlap ``x``."""
 
     if _host_bound or _bind_host():
         done = _host.mx4_linear(x, weight, bias, out)

@@ -5,20 +5,21 @@
 exact in fp32; K of them and the wave sums are added in fp32, each addition off by at most 2^-24 of the running
 magnitude, which sum |x w| bounds: K * 2^-24 * sum |x w| covers any order; the result is rounded to bf16 once (2^-8
 of a value at most half a step = 2^-9 times its power of two, so 2^-8 relative covers it).
-MX8 rows go through the scaled matrix instruction, which first adds the products of 8 neighbouring columns in fixed
-point: bits below 2^-13 of the largest 2^(ex + ew), the powers of two of a product's factors, are dropped
-(test_mx8_products_keep_13_bits_of_eight pins it), so each of the other 7 products loses less than 2^-13 times the
+The tile kernel's MX8 rows go through the scaled matrix instruction, which first adds the products of 8 neighbouring
+columns in fixed point: bits below 2^-13 of the largest 2^(ex + ew), the powers of two of a product's factors, are dropped
+(test_mx8_products_that_cancel pins it), so each of the other 7 products loses less than 2^-13 times the
 group's largest product, which (largest |x|) * (largest |w|) of the group bounds.
 """
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
 import torch
 
-from lastkv_amd import ops
+from lastkv_amd import _lib, ops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -232,6 +233,24 @@ def group_maxima(v):
     return v.abs().view(v.shape[0], -1, 8).amax(-1)
 
 
+ROWS, TILES = 1, 2
+
+
+@pytest.fixture(params=[ROWS, TILES], ids=["rows", "tiles"])
+def kernel(request, monkeypatch):
+    """Every product of the test on this kernel (the Python body makes the calls)."""
+
+    class Args(_lib.Mx4LinearArgs):
+        def __init__(self):
+            super().__init__()
+            self.kernel = request.param
+
+    monkeypatch.setattr(_lib, "Mx4LinearArgs", Args)
+    monkeypatch.setattr(ops, "_host", None)
+    monkeypatch.setattr(ops, "_host_bound", False)
+    return request.param
+
+
 def check_linear(x, xv, codes, scales, bias=None, out=None):
     w = ops.mx4_pack(codes, scales)
     got = ops.mx4_linear(x, w, bias=bias, out=out)
@@ -252,11 +271,11 @@ def check_linear(x, xv, codes, scales, bias=None, out=None):
 SHAPES = [(1, 1, 32), (1, 16, 512), (1, 4096, 4096), (1, 2050, 14336), (2, 100, 96), (7, 33, 544), (15, 48, 1568), (16, 6144, 512),
           (17, 250, 1024), (31, 1000, 160), (32, 4096, 2048), (33, 17, 4064), (48, 8192, 320), (50, 130, 128), (64, 16400, 256),
           (65, 129, 288), (100, 1000, 1056), (128, 256, 512), (129, 384, 640), (250, 300, 96), (257, 513, 2080),
-          (512, 512, 512), (1000, 6144, 1024)]
+          (512, 512, 512), (1000, 6144, 1024), (1001, 6161, 416), (3000, 2060, 96)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
-def test_linear_bf16_rows(m, n, k):
+def test_linear_bf16_rows(m, n, k, kernel):
     g = _gen(m + n + k)
     codes, scales = random_mx4(g, n, k)
     x = outliers(g, m, k)
@@ -265,7 +284,7 @@ def test_linear_bf16_rows(m, n, k):
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
-def test_linear_mx8_rows(m, n, k):
+def test_linear_mx8_rows(m, n, k, kernel):
     g = _gen(m + n + k + 1)
     codes, scales = random_mx4(g, n, k)
     x = random_mx8(g, m, k)
@@ -274,8 +293,9 @@ def test_linear_mx8_rows(m, n, k):
 
 
 @pytest.mark.parametrize("m", [1, 300])
-def test_mx8_products_that_cancel(m):
-    """256 - 256 + 2^-b: the small product stays (exact products, fp32 sums)."""
+def test_mx8_products_that_cancel(m, kernel):
+    """256 - 256 + 2^-b: the row kernel's products are exact; the tile kernel keeps 2^-5 and more among eight columns
+    and any size in another eight."""
 
     w = ops.mx4_pack(torch.full((16, 256), 0x22, dtype=torch.uint8, device=DEV),
                      torch.full((16, 16), 127, dtype=torch.uint8, device=DEV))
@@ -284,11 +304,32 @@ def test_mx8_products_that_cancel(m):
             x = torch.zeros((m, 512), dtype=torch.float32, device=DEV)
             x[:, 0], x[:, 1], x[:, at] = 256, -256, 2.0 ** -b
             x = ops.MX8Rows(x.to(torch.float8_e4m3fn), torch.full((m, 16), 127, dtype=torch.uint8, device=DEV))
-            assert ops.mx4_linear(x, w).eq(2.0 ** -b).all(), (at, b)
+            want = 0.0 if kernel == TILES and at < 8 and b > 5 else 2.0 ** -b
+            assert ops.mx4_linear(x, w).eq(want).all(), (at, b)
+
+
+@pytest.mark.parametrize("m,n,mx8", [(96, 28672, False), (96, 28672, True), (1000, 6144, True), (1000, 6144, False), (64, 28672, True)])
+def test_linear_kernels_chosen_by_size(m, n, mx8):
+    """Without a fixed kernel the call equals the one whose sizes choose it."""
+
+    g = _gen(m)
+    w = ops.mx4_pack(*random_mx4(g, n, 256))
+    x = random_mx8(g, m, 256) if mx8 else outliers(g, m, 256)
+    a = _lib.Mx4LinearArgs()
+    out = torch.empty((m, n), device=DEV, dtype=BF16)
+    a.struct_size, a.rows, a.out_features, a.in_features = ctypes.sizeof(a), m, n, 256
+    a.kernel = TILES if m > 64 else ROWS
+    data = x.data if mx8 else x
+    a.x, a.x_stride, a.x_format = data.data_ptr(), 256, int(mx8)
+    if mx8:
+        a.x_scales, a.x_scale_stride = x.scales.data_ptr(), 8
+    a.weight, a.out, a.out_stride = w.data.data_ptr(), out.data_ptr(), n
+    _lib.check(_lib.load().lkv_mx4_linear(ctypes.byref(a), torch.cuda.current_stream().cuda_stream), "lkv_mx4_linear")
+    assert torch.equal(out, ops.mx4_linear(x, w))
 
 
 @pytest.mark.parametrize("m", [1, 5, 40, 300])
-def test_linear_bad_values_stay_in_their_row(m):
+def test_linear_bad_values_stay_in_their_row(m, kernel):
     """An infinity or NaN in one row of x: that row is what the products say, every other row is as without it."""
 
     g = _gen(m)
@@ -310,7 +351,7 @@ def test_linear_bad_values_stay_in_their_row(m):
 
 @pytest.mark.parametrize("mx8", [False, True])
 @pytest.mark.parametrize("m", [3, 20, 200])
-def test_linear_strided_rows_and_untouched_neighbours(m, mx8):
+def test_linear_strided_rows_and_untouched_neighbours(m, mx8, kernel):
     g = _gen(m)
     codes, scales = random_mx4(g, 70, 544)
     if mx8:
@@ -328,18 +369,22 @@ def test_linear_strided_rows_and_untouched_neighbours(m, mx8):
         assert y.shape == (1, m, 70) and torch.equal(y[0], out[1:-1, 5:75])
 
 
-def test_linear_past_the_rows_and_columns_reads_nothing_that_counts():
-    """NaN beside the rows of x (the next columns of a wider tensor) does not reach the product."""
+@pytest.mark.parametrize("m", [5, 200])
+def test_linear_past_the_rows_and_columns_reads_nothing_that_counts(m, kernel):
+    """NaN beside the rows of x (the next columns of a wider tensor), and in every place of the columns' tile before, does
+    not reach the product."""
 
     g = _gen(9)
+    nan = torch.full((m, 512), math.nan, device=DEV, dtype=BF16)
+    assert torch.isnan(ops.mx4_linear(nan, ops.mx4_pack(*random_mx4(g, 40, 512)))).all()
     codes, scales = random_mx4(g, 40, 160)
-    wide = torch.full((5, 512), math.nan, device=DEV, dtype=BF16)
-    wide[:, :160] = torch.randn((5, 160), generator=g, device=DEV)
+    wide = nan.clone()
+    wide[:, :160] = torch.randn((m, 160), generator=g, device=DEV)
     check_linear(wide[:, :160], wide[:, :160].double(), codes, scales)
-    x8 = random_mx8(g, 5, 160)
-    data = torch.full((5, 512), 127, device=DEV, dtype=torch.uint8)
+    x8 = random_mx8(g, m, 160)
+    data = torch.full((m, 512), 127, device=DEV, dtype=torch.uint8)
     data[:, :160] = x8.data.view(torch.uint8)
-    s = torch.full((5, 16), 255, device=DEV, dtype=torch.uint8)
+    s = torch.full((m, 16), 255, device=DEV, dtype=torch.uint8)
     s[:, :5] = x8.scales
     x = ops.MX8Rows(data.view(torch.float8_e4m3fn)[:, :160], s[:, :5])
     check_linear(x, mx8_values(x8), codes, scales)
@@ -354,7 +399,9 @@ def test_linear_same_bits_every_time_and_for_every_row_count():
     x = outliers(g, 64, 1024)
     y = ops.mx4_linear(x, w)
     assert torch.equal(y, ops.mx4_linear(x, w))
-    assert torch.equal(y[:16], ops.mx4_linear(x[:16], w))
+    assert torch.equal(y[16:32], ops.mx4_linear(x[16:32].clone(), w))
+    q = ops.rmsnorm_mx8(x, torch.ones(1024, device=DEV, dtype=BF16), 1e-5)  # few rows: the products of their values
+    assert torch.equal(ops.mx4_linear(q, w), ops.mx4_linear(ops.mx8_unpack(q), w))
 
 
 def test_empty_rows():

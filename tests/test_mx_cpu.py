@@ -50,10 +50,10 @@ def _linear(**kw):
 @pytest.mark.parametrize("kw,message", [
     (dict(struct_size=8), b"size mismatch"), (dict(rows=-1), b"rows"), (dict(rows=(1 << 20) + 1), b"rows"),
     (dict(in_features=48), b"multiple of 32"), (dict(in_features=0), b"multiple of 32"), (dict(out_features=0), b"1 to 2^24"),
-    (dict(in_features=(1 << 20) + 32), b"up to 2^20"), (dict(x_format=2), b"x_format"), (dict(x=None), b"null"),
+    (dict(in_features=(1 << 20) + 32), b"up to 2^20"), (dict(x_format=2), b"x_format"), (dict(kernel=3), b"kernel"), (dict(x=None), b"null"),
     (dict(weight=None), b"null"), (dict(out=None), b"null"), (dict(x_format=1), b"x_scales"), (dict(x_scales=16), b"x_scales"),
     (dict(x=24), b"aligned"), (dict(weight=8), b"aligned"), (dict(x_stride=68), b"aligned"),
-    (dict(x_format=1, x_scales=16, x_stride=72), b"aligned"), (dict(x_stride=1 << 24), b"2^23"), (dict(x_stride=-8), b"2^23")])
+    (dict(x_format=1, x_scales=16, x_stride=72), b"aligned"), (dict(x_stride=1 << 24), b"2^21"), (dict(x_stride=-8), b"2^21")])
 def test_linear_refusals(kw, message):
     st, text = _linear(**kw)
     assert st == 1 and message in text, text
