@@ -497,10 +497,13 @@ int32_t launch(const LinearParams& p, hipStream_t s, int kernel) {
   const int64_t work = static_cast<int64_t>((p.N + 15) / 16) * ((p.M + 31) / 32);
   if (kernel == LKV_MX4_TILES || (kernel == LKV_MX4_AUTO && p.M > 64 && work > 16 * cus)) {
     const int64_t wide = static_cast<int64_t>((p.N + 255) / 256) * ((p.M + 127) / 128);
-    if (kMx8 && 4 * wide >= 3 * cus)
-      launch_tile<kMx8, 2, 2, 8, 4>(p, s);
-    else
-      launch_tile<kMx8, 2, 2, 4, 4>(p, s);
+    if constexpr (kMx8) {
+      if (4 * wide >= 3 * cus) {
+        launch_tile<true, 2, 2, 8, 4>(p, s);
+        return check_launch("lkv_mx4_linear");
+      }
+    }
+    launch_tile<kMx8, 2, 2, 4, 4>(p, s);
   } else if (p.M <= 16) {
     launch_mt<kMx8, 1>(p, s);
   } else {

@@ -41,24 +41,11 @@ __device__ inline uint4 pack8(const float (&f)[8]) {
   return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
 }
 
-// Eight values of a lane whose quad holds one block: their bytes, and the block's scale byte.
-__device__ inline uint2 quantize(const double (&y)[8], int& byte) {
-  double amax = fabs(y[0]);
-#pragma unroll
-  for (int j = 1; j < 8; ++j) {
-    const double a = fabs(y[j]);
-    amax = (amax != amax || amax > a) ? amax : a;
-  }
-  byte = e4m3_scale_byte(quad_max(amax));
-  if (byte == 255) return make_uint2(0, 0);
-  const double f = exp2_int(127 - byte);
-  float v[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = to_odd(y[j] * f);
-  return make_uint2(pack_e4m3(v[0], v[1], v[2], v[3]), pack_e4m3(v[4], v[5], v[6], v[7]));
-}
-
-// One workgroup per row, 8 values per thread and chunk.
+// One workgroup per row; thread t owns the 8-element chunks t, t + 256, ... (kChunks of them).  With kAdd the row is
+// residual := bf16(residual + x) first.  y = w * (row * r), r = 1 / sqrt(sum(row^2) / hidden + eps) with the sum and r in 64
+// bits (no order of the sum then shows in a row's output, and no row's squares leave the range).
+// Bound by HBM: every load is issued before the first use, with no branch between them (a chunk past the row rereads the
+// last one); x and the residual are read once and take non-temporal accesses, as in lkv_rmsnorm.
 template <bool kAdd, int kChunks>
 __global__ __launch_bounds__(kThreads) void rmsnorm_mx8_kernel(const NormParams p) {
   __shared__ double part[kThreads / 64];
@@ -67,22 +54,29 @@ __global__ __launch_bounds__(kThreads) void rmsnorm_mx8_kernel(const NormParams 
   const uint4* x = reinterpret_cast<const uint4*>(p.x + row * p.x_stride);
   uint4* res = kAdd ? reinterpret_cast<uint4*>(p.residual + row * p.res_stride) : nullptr;
   const uint4* w = reinterpret_cast<const uint4*>(p.w);
-  uint4 xv[kChunks];
+  uint4 xv[kChunks], rv[kChunks], wv[kChunks];
+#pragma unroll
+  for (int k = 0; k < kChunks; ++k) {
+    const int c = min(static_cast<int>(threadIdx.x) + k * kThreads, chunks - 1);
+    xv[k] = load_nt(x + c);
+    if (kAdd) rv[k] = load_nt(res + c);
+  }
+#pragma unroll
+  for (int k = 0; k < kChunks; ++k) wv[k] = w[min(static_cast<int>(threadIdx.x) + k * kThreads, chunks - 1)];
   double ss = 0.;
 #pragma unroll
   for (int k = 0; k < kChunks; ++k) {
     const int c = threadIdx.x + k * kThreads;
     if (c < chunks) {
       float v[8];
-      xv[k] = x[c];
       unpack8(xv[k], v);
       if (kAdd) {
         float r[8];
-        unpack8(res[c], r);
+        unpack8(rv[k], r);
 #pragma unroll
         for (int j = 0; j < 8; ++j) r[j] += v[j];
         xv[k] = pack8(r);
-        res[c] = xv[k];
+        __builtin_nontemporal_store(__builtin_bit_cast(u32x4, xv[k]), reinterpret_cast<u32x4*>(res + c));
         unpack8(xv[k], v);
       }
 #pragma unroll
@@ -95,24 +89,39 @@ __global__ __launch_bounds__(kThreads) void rmsnorm_mx8_kernel(const NormParams 
   __syncthreads();
   const double total = (part[0] + part[1]) + (part[2] + part[3]);
   const double r = 1. / sqrt(total / p.hidden + p.eps);
+  const float rf = static_cast<float>(r);
 #pragma unroll
   for (int k = 0; k < kChunks; ++k) {
     const int c = threadIdx.x + k * kThreads;
     if (c < chunks) {  // (a block's four chunks are all inside the row or all outside)
-      float h[8], wf[8];
+      float h[8], wf[8], y[8];
       unpack8(xv[k], h);
-      unpack8(w[c], wf);
-      double y[8];
+      unpack8(wv[k], wf);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = static_cast<double>(wf[j]) * (static_cast<double>(h[j]) * r);
+      for (int j = 0; j < 8; ++j) y[j] = wf[j] * (h[j] * rf);  // (three roundings: within 2^-22)
       int byte;
-      const uint2 q = quantize(y, byte);
+      const uint2 q = quantize_e4m3(y, byte, [&](double(&d)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[j] = static_cast<double>(wf[j]) * (static_cast<double>(h[j]) * r);
+      });
       reinterpret_cast<uint2*>(p.out + row * p.out_stride)[c] = q;
       if ((c & 3) == 0) p.scales[row * p.scale_stride + (c >> 2)] = static_cast<uint8_t>(byte);
     }
   }
 }
 
+// g / (1 + e^-g) for -80 <= g within 2^-21.4: v_exp_f32 and v_rcp_f32 are off by one unit in the last place (2^-23), the
+// product with log2(e) is carried in two parts, the reciprocal takes one Newton step.  (Above 80 the sum is 1.)
+__device__ inline float silu(float g) {
+  const float x = -fminf(g, 80.f);
+  const float hi = x * kLog2e, lo = __builtin_fmaf(x, kLog2e, -hi);
+  const float e = fast_exp2(hi);
+  const float d = 1.f + __builtin_fmaf(e, lo * kLn2, e);
+  const float r = __builtin_amdgcn_rcpf(d);
+  return g * __builtin_fmaf(__builtin_fmaf(-d, r, 1.f), r, r);
+}
+
+// y = silu(gate) * up; grid (column groups, rows), one 8-element chunk per thread.
 __global__ __launch_bounds__(256) void silu_mul_mx8_kernel(const uint16_t* gate, int64_t g_stride, const uint16_t* up,
                                                            int64_t u_stride, uint8_t* out, int64_t o_stride,
                                                            uint8_t* scales, int64_t s_stride, int32_t rows,
@@ -120,17 +129,24 @@ __global__ __launch_bounds__(256) void silu_mul_mx8_kernel(const uint16_t* gate,
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= width >> 3) return;
   for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
-    float g[8], u[8];
-    unpack8(reinterpret_cast<const uint4*>(gate + row * g_stride)[c], g);
-    unpack8(reinterpret_cast<const uint4*>(up + row * u_stride)[c], u);
-    double y[8];
+    float g[8], u[8], y[8];
+    unpack8(load_nt(reinterpret_cast<const uint4*>(gate + row * g_stride) + c), g);
+    unpack8(load_nt(reinterpret_cast<const uint4*>(up + row * u_stride) + c), u);
+    float least = g[0];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const double d = g[j];
-      y[j] = d / (1. + exp(-d)) * static_cast<double>(u[j]);
+      y[j] = silu(g[j]) * u[j];
+      least = fminf(least, g[j]);
     }
+    if (least < -80.f) y[0] = __uint_as_float(0x7fc00000u);  // e^-g leaves the range that silu() takes: in 64 bits
     int byte;
-    const uint2 q = quantize(y, byte);
+    const uint2 q = quantize_e4m3(y, byte, [&](double(&d)[8]) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const double x = g[j];
+        d[j] = x / (1. + exp(-x)) * static_cast<double>(u[j]);
+      }
+    });
     reinterpret_cast<uint2*>(out + row * o_stride)[c] = q;
     if ((c & 3) == 0) scales[row * s_stride + (c >> 2)] = static_cast<uint8_t>(byte);
   }
