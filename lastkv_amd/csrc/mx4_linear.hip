@@ -92,7 +92,7 @@ struct Step {
 // through LDS, in the waves' order.
 // Bound by HBM: the weight's 4.25 bits a value, read once for up to 32 rows of x, converted in registers (one instruction
 // for two values) for bf16 matrix instructions; MX8 rows are converted too (exact products; the scaled matrix instruction
-// would save 64 conversions per 2,048 weights of a wave, not time).  A step's loads are issued one step ahead.
+// would save 64 conversions per 2,048 weights of a wave, not time).  The loads of two steps are in flight.
 // us per call with cold weights, bf16 / MX8 rows, beside a plain read of the same bytes: 28672 x 4096 for 1 row 15.3 / 15.0
 // (read 12.3), for 32 20.0 / 20.2; 4096 x 14336 for 1 row 11.2 / 10.6 (read 6.6-8.7), for 32 16.8 / 14.2; 4096 x 4096 for 1 row
 // 4.9 / 4.7 (read 3.5), for 32 6.8 / 6.1; bf16 weights in the library's GEMM: 28672 x 4096 for 32 rows 48.8, 4096 x 4096 13.8.
@@ -101,7 +101,7 @@ struct Step {
 // swizzled by the row (chunk c of row m at c ^ (m & 7)) so that neither side meets a bank twice (4096 x 4096 for 32 rows
 // 10.6 -> 6.8 us).
 template <bool kMx8, int MT, int NT, int KS>
-__global__ __launch_bounds__(kWaves * 64, MT == 1 && NT <= 2 ? 4 : 2) void mx4_rows_kernel(const LinearParams p) {
+__global__ __launch_bounds__(kWaves * 64, MT == 1 && NT == 1 ? 4 : 2) void mx4_rows_kernel(const LinearParams p) {
   constexpr int kLoads = kMx8 ? 2 : 4;  // of 1 KiB per tile of 16 rows x 128 columns
   constexpr int kRowBytes = kMx8 ? 128 : 256;  // of a row in a tile
   constexpr int kChunks = kRowBytes / 16;
@@ -213,28 +213,29 @@ __global__ __launch_bounds__(kWaves * 64, MT == 1 && NT <= 2 ? 4 : 2) void mx4_r
     }
   };
 
-  // Two steps in turn, so that the next one's loads are not copied (a copy would wait for them).
-  Step<MT, NT> even, odd;
+  // The codes of two steps ahead are in flight.  Three steps in turn, so that no loaded one is copied (a copy would wait).
+  Step<MT, NT> s0, s1, s2;
   auto step = [&](int h, const Step<MT, NT>& now, Step<MT, NT>& then) {
-    const bool more = h + KS < steps;
-    if (more) load(h + KS, then);
+    if (h + 2 * KS < steps) load(h + 2 * KS, then);
 #pragma unroll
     for (int t = 0; t < kStepTiles; ++t) {
       store_x();
       if (t + 1 < kStepTiles)
         load_x(h * kStepTiles + t + 1);
-      else if (more)
+      else if (h + KS < steps)
         load_x((h + KS) * kStepTiles);
       compute(h, t, now);
     }
   };
   if (ks < steps) {
-    load(ks, even);
+    load(ks, s0);
     load_x(ks * kStepTiles);
+    if (ks + KS < steps) load(ks + KS, s1);
   }
-  for (int h = ks; h < steps; h += 2 * KS) {
-    step(h, even, odd);
-    if (h + KS < steps) step(h + KS, odd, even);
+  for (int h = ks; h < steps; h += 3 * KS) {
+    step(h, s0, s2);
+    if (h + KS < steps) step(h + KS, s1, s0);
+    if (h + 2 * KS < steps) step(h + 2 * KS, s2, s1);
   }
   f32x4* part = reinterpret_cast<f32x4*>(smem);  // [wave][NT][MT][lane]
   if constexpr (KS > 1) {
