@@ -21,7 +21,10 @@ constexpr int kMxUnitCols = 512;
 constexpr int kMxTileBytes = 1024;
 constexpr int kMxUnitBytes = 4 * kMxTileBytes + 256;
 
-__host__ __device__ inline int64_t mx4_units(int32_t cols) { return (cols + kMxUnitCols - 1) / kMxUnitCols; }
+__host__ __device__ inline int mx4_units(int32_t cols) { return (cols + kMxUnitCols - 1) / kMxUnitCols; }
+
+// Bytes from one row tile to the next: an odd number of 256-byte pieces.
+__host__ __device__ inline int mx4_tile_stride(int units) { return ((units * (kMxUnitBytes / 256)) | 1) * 256; }
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 

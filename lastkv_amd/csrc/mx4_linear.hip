@@ -18,7 +18,7 @@ struct LinearParams {
   uint16_t* out;
   int64_t out_stride;
   int32_t M, N, K;
-  int32_t units;
+  int32_t units, tile_stride;
   bool vector_out;  // output rows are 8-byte aligned
   bool scale_words;  // x scales in whole aligned words: a row's four of a tile
 };
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(kWaves * 64, MT == 1 && NT == 1 ? 4 : 2) void mx4_r
     for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   const uint8_t* w[NT];
 #pragma unroll
-  for (int i = 0; i < NT; ++i) w[i] = p.w + static_cast<int64_t>(min(nt0 + i, ntiles - 1)) * p.units * kMxUnitBytes;
+  for (int i = 0; i < NT; ++i) w[i] = p.w + static_cast<int64_t>(min(nt0 + i, ntiles - 1)) * p.tile_stride;
   const int valid = min(p.M - m0, 16 * MT);
   const int stride = static_cast<int>(p.x_stride) * (kMx8 ? 1 : 2), row_bytes = p.K * (kMx8 ? 1 : 2);
   const __amdgpu_buffer_rsrc_t xb = __builtin_amdgcn_make_buffer_rsrc(
@@ -295,7 +295,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
   const __amdgpu_buffer_rsrc_t xb = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<char*>(static_cast<const char*>(p.x) + static_cast<int64_t>(m0) * stride), 0,
       (valid - 1) * stride + row_bytes, 0x00020000);
-  const int tile_stride = p.units * kMxUnitBytes;
+  const int tile_stride = p.tile_stride;
   const __amdgpu_buffer_rsrc_t wb = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<uint8_t*>(p.w + static_cast<int64_t>(nt0) * tile_stride), 0, min(kBN, ntiles - nt0) * tile_stride, 0x00020000);
 
@@ -517,21 +517,23 @@ int32_t launch(const LinearParams& p, hipStream_t s, int kernel) {
 
 // Lane l of tile t of a unit: its 16 code bytes and its scale byte.  Rows and columns past the matrix: zeros.
 struct PackItem {
-  int64_t unit;
+  int64_t at;  // of the unit's bytes
   int t, lane, n, k;
 };
 
 __device__ inline bool pack_item(int64_t id, int32_t units, int32_t N, int32_t K, PackItem& it) {
   it.lane = id & 63;
   it.t = (id >> 6) & 3;
-  it.unit = id >> 8;
-  it.n = static_cast<int>(it.unit / units) * 16 + (it.lane & 15);
-  it.k = static_cast<int>(it.unit % units) * kMxUnitCols + it.t * 128 + 32 * (it.lane >> 4);
+  const int64_t tile = (id >> 8) / units;
+  const int u = static_cast<int>((id >> 8) % units);
+  it.at = tile * mx4_tile_stride(units) + u * kMxUnitBytes;
+  it.n = static_cast<int>(tile) * 16 + (it.lane & 15);
+  it.k = u * kMxUnitCols + it.t * 128 + 32 * (it.lane >> 4);
   return it.n < N && it.k < K;
 }
 
 __device__ inline void pack_store(uint8_t* out, const PackItem& it, uint4 codes, uint8_t scale) {
-  uint8_t* unit = out + it.unit * kMxUnitBytes;
+  uint8_t* unit = out + it.at;
   *reinterpret_cast<uint4*>(unit + it.t * kMxTileBytes + it.lane * 16) = codes;
   unit[4 * kMxTileBytes + it.lane * 4 + it.t] = scale;
 }
@@ -591,7 +593,7 @@ __global__ __launch_bounds__(256) void mx4_unpack_kernel(const uint8_t* w, uint1
   for (int64_t id = blockIdx.x * int64_t{256} + threadIdx.x; id < items; id += gridDim.x * int64_t{256}) {
     PackItem it;
     if (!pack_item(id, units, N, K, it)) continue;
-    const uint8_t* unit = w + it.unit * kMxUnitBytes;
+    const uint8_t* unit = w + it.at;
     const uint4 c = *reinterpret_cast<const uint4*>(unit + it.t * kMxTileBytes + it.lane * 16);
     const float s = e8m0(unit[4 * kMxTileBytes + it.lane * 4 + it.t], 0);
     uint4* o = reinterpret_cast<uint4*>(out + it.n * o_stride + it.k);
@@ -617,7 +619,7 @@ uintptr_t bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
 
 extern "C" int64_t lkv_mx4_weight_bytes(int32_t n, int32_t k) {
   if (n <= 0 || k <= 0) return 0;
-  return static_cast<int64_t>((n + 15) / 16) * lkv::mx4_units(k) * lkv::kMxUnitBytes;
+  return static_cast<int64_t>((n + 15) / 16) * lkv::mx4_tile_stride(lkv::mx4_units(k));
 }
 
 extern "C" int32_t lkv_mx4_pack(const void* codes, int64_t code_stride, const void* scales, int64_t scale_stride,
@@ -629,7 +631,7 @@ extern "C" int32_t lkv_mx4_pack(const void* codes, int64_t code_stride, const vo
   const int64_t items = pack_items(n, k);
   mx4_pack_kernel<<<pack_grid(items), 256, 0, as_stream(stream)>>>(
       static_cast<const uint8_t*>(codes), code_stride, static_cast<const uint8_t*>(scales), scale_stride,
-      static_cast<uint8_t*>(weight), n, k, static_cast<int32_t>(mx4_units(k)), items);
+      static_cast<uint8_t*>(weight), n, k, mx4_units(k), items);
   return check_launch("lkv_mx4_pack");
 }
 
@@ -642,7 +644,7 @@ extern "C" int32_t lkv_mx4_quantize(const void* src, int64_t src_stride, int32_t
   const int64_t items = pack_items(n, k);
   mx4_quantize_kernel<<<pack_grid(items), 256, 0, as_stream(stream)>>>(static_cast<const uint16_t*>(src), src_stride,
                                                                       static_cast<uint8_t*>(weight), n, k,
-                                                                      static_cast<int32_t>(mx4_units(k)), items);
+                                                                      mx4_units(k), items);
   return check_launch("lkv_mx4_quantize");
 }
 
@@ -655,7 +657,7 @@ extern "C" int32_t lkv_mx4_unpack(const void* weight, int32_t n, int32_t k, void
   const int64_t items = pack_items(n, k);
   mx4_unpack_kernel<<<pack_grid(items), 256, 0, as_stream(stream)>>>(static_cast<const uint8_t*>(weight),
                                                                     static_cast<uint16_t*>(out), out_stride, n, k,
-                                                                    static_cast<int32_t>(mx4_units(k)), items);
+                                                                    mx4_units(k), items);
   return check_launch("lkv_mx4_unpack");
 }
 
@@ -690,7 +692,8 @@ extern "C" int32_t lkv_mx4_linear(const lkv_mx4_linear_args* a, lkv_stream_t str
   p.M = a->rows;
   p.N = a->out_features;
   p.K = a->in_features;
-  p.units = static_cast<int32_t>(mx4_units(a->in_features));
+  p.units = mx4_units(a->in_features);
+  p.tile_stride = mx4_tile_stride(p.units);
   p.scale_words = (bits(a->x_scales) & 3) == 0 && a->x_scale_stride % 4 == 0 && a->in_features % 128 == 0;
   p.vector_out = (bits(a->out) & 7) == 0 && a->out_stride % 4 == 0;
   return mx8 ? launch<true>(p, as_stream(stream), a->kernel) : launch<false>(p, as_stream(stream), a->kernel);

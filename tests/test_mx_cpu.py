@@ -72,7 +72,7 @@ def test_other_refusals_and_sizes():
     for call in (lambda: lib.lkv_mx4_pack(16, 32, 16, 2, 16, 40, 16, None), lambda: lib.lkv_mx4_quantize(16, 64, 0, 64, 16, None),
                  lambda: lib.lkv_mx4_unpack(16, 16, 48, 16, 64, None)):
         assert call() == 1 and b"multiple of 32" in lib.lkv_last_error()
-    assert lib.lkv_mx4_weight_bytes(16, 512) == 4352 and lib.lkv_mx4_weight_bytes(17, 544) == 4 * 4352
+    assert lib.lkv_mx4_weight_bytes(16, 512) == 4352 and lib.lkv_mx4_weight_bytes(17, 544) == 2 * (2 * 4352 + 256)
     assert lib.lkv_mx4_weight_bytes(0, 512) == 0
 
 
