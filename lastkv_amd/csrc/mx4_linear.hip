@@ -19,7 +19,7 @@ struct LinearParams {
   int64_t out_stride;
   int32_t M, N, K;
   int32_t units, tile_stride;
-  bool vector_out;  // output rows are 8-byte aligned
+  bool vector_out;  // output rows are 16-byte aligned
   bool scale_words;  // x scales in whole aligned words: a row's four of a tile
 };
 
@@ -57,8 +57,60 @@ __device__ inline void buffer_to_lds16(__amdgpu_buffer_rsrc_t r, char* dst, int 
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)dst, 16, offset, scalar_offset, 0, 0);
 }
 
-// Every load of the wave has arrived (those to LDS too).
-__device__ inline void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
+__device__ inline void buffer_to_lds4(__amdgpu_buffer_rsrc_t r, char* dst, int offset, int scalar_offset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)dst, 4, offset, scalar_offset, 0, 0);
+}
+
+__device__ inline uint32_t lds_address(const void* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)p));
+}
+
+// A wave's fragments of a tile, read and waited for in one piece of assembly: before an LDS read of its own the compiler
+// waits for every load to LDS in flight, those of later tiles too.
+template <int TN, int kXStep>
+__device__ inline void read_mx8(uint32_t w, uint32_t lo, uint32_t hi, uint32_t sc, uint4 (&c)[TN], uint4 (&l)[4], uint4 (&h)[4],
+                                uint32_t (&s)[4]) {
+  static_assert(TN == 4 || TN == 8, "tiles of a wave");
+  if constexpr (TN == 8) {
+    asm volatile(
+        "ds_read_b128 %0, %20\n ds_read_b128 %8, %21\n ds_read_b128 %12, %22\n"
+        "ds_read_b128 %9, %21 offset:%c24\n ds_read_b128 %13, %22 offset:%c24\n"
+        "ds_read_b128 %10, %21 offset:%c25\n ds_read_b128 %14, %22 offset:%c25\n"
+        "ds_read_b128 %11, %21 offset:%c26\n ds_read_b128 %15, %22 offset:%c26\n"
+        "ds_read_b32 %16, %23\n ds_read_b32 %17, %23 offset:64\n ds_read_b32 %18, %23 offset:128\n ds_read_b32 %19, %23 offset:192\n"
+        "ds_read_b128 %1, %20 offset:1024\n ds_read_b128 %2, %20 offset:2048\n ds_read_b128 %3, %20 offset:3072\n"
+        "ds_read_b128 %4, %20 offset:4096\n ds_read_b128 %5, %20 offset:5120\n ds_read_b128 %6, %20 offset:6144\n"
+        "ds_read_b128 %7, %20 offset:7168\n s_waitcnt lgkmcnt(0)"
+        : "=&v"(c[0]), "=&v"(c[1]), "=&v"(c[2]), "=&v"(c[3]), "=&v"(c[4]), "=&v"(c[5]), "=&v"(c[6]), "=&v"(c[7]), "=&v"(l[0]),
+          "=&v"(l[1]), "=&v"(l[2]), "=&v"(l[3]), "=&v"(h[0]), "=&v"(h[1]), "=&v"(h[2]), "=&v"(h[3]), "=&v"(s[0]), "=&v"(s[1]),
+          "=&v"(s[2]), "=&v"(s[3])
+        : "v"(w), "v"(lo), "v"(hi), "v"(sc), "n"(kXStep), "n"(2 * kXStep), "n"(3 * kXStep)
+        : "memory");
+  } else {
+    asm volatile(
+        "ds_read_b128 %0, %16\n ds_read_b128 %4, %17\n ds_read_b128 %8, %18\n"
+        "ds_read_b128 %5, %17 offset:%c20\n ds_read_b128 %9, %18 offset:%c20\n"
+        "ds_read_b128 %6, %17 offset:%c21\n ds_read_b128 %10, %18 offset:%c21\n"
+        "ds_read_b128 %7, %17 offset:%c22\n ds_read_b128 %11, %18 offset:%c22\n"
+        "ds_read_b32 %12, %19\n ds_read_b32 %13, %19 offset:64\n ds_read_b32 %14, %19 offset:128\n ds_read_b32 %15, %19 offset:192\n"
+        "ds_read_b128 %1, %16 offset:1024\n ds_read_b128 %2, %16 offset:2048\n ds_read_b128 %3, %16 offset:3072\n"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(c[0]), "=&v"(c[1]), "=&v"(c[2]), "=&v"(c[3]), "=&v"(l[0]), "=&v"(l[1]), "=&v"(l[2]), "=&v"(l[3]), "=&v"(h[0]),
+          "=&v"(h[1]), "=&v"(h[2]), "=&v"(h[3]), "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3])
+        : "v"(w), "v"(lo), "v"(hi), "v"(sc), "n"(kXStep), "n"(2 * kXStep), "n"(3 * kXStep)
+        : "memory");
+  }
+}
+
+// All loads of the wave but the last kLeft have arrived (those to LDS too).
+template <int kLeft>
+__device__ inline void wait_and_sync() {
+  static_assert(kLeft < 64, "vmcnt has six bits");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070 | (kLeft & 15) | (kLeft >> 4) << 14);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 // An offset past every buffer (they hold less than 2^30 bytes and a row's columns 2^21): loads give zeros.
 constexpr int kOutside = 0x60000000;
@@ -264,22 +316,24 @@ __global__ __launch_bounds__(kWaves * 64, MT == 1 && NT == 1 ? 4 : 2) void mx4_r
 }
 
 // Many rows: one workgroup of WN x WM waves per (16 WN TN rows of the weight, 16 WM TM rows of x), each wave TN x TM
-// tiles of 16 x 16.  Tiles of 128 columns of both go to LDS by direct loads, two buffers, one barrier a tile; two workgroups
-// share a CU, so that one's products cover the other's reads of LDS.
+// tiles of 16 x 16.  Tiles of 128 columns of both go to LDS by direct loads, kBufs buffers in turn, one barrier a tile; two
+// workgroups share a CU where there are that many, so that one's products cover the other's reads of LDS.
 // MX8 rows: both operands and both scales go to the scaled matrix instruction as they are (a code is converted nowhere).
-// Bound by the matrix pipe, of which 4096 rows of 28672 x 4096 reach 2.36 PFLOP/s (407 us; bf16 weights in the library's
-// GEMM 641 us); independent products in registers reach 3.83 PFLOP/s on this card.  With the tile staged through
-// registers 426-447 us, with its LDS writes before the products 454.
-// bf16 rows: the codes are converted in registers as they are used.  1000 rows of 6144 x 4096 take 52 us, 0.97 PFLOP/s, 4096
-// rows 174 us, 1.19 PFLOP/s (library, bf16 weights, 1000 rows: 52 us); bf16 products in registers reach 1.92 PFLOP/s.
-template <bool kMx8, bool kWords, int WN, int WM, int TN, int TM>
+// Bound by the matrix pipe, of which 4096 rows of 28672 x 4096 reach 2.63 PFLOP/s (366 us; bf16 weights in the library's
+// GEMM 641 us); independent products in registers reach 3.83 PFLOP/s on this card, this loop without its loads 3.4.  With
+// the tile staged through registers the same took 30-50 us more, with the outputs stored from registers 28.
+// bf16 rows: the codes are converted in registers as they are used.  1000 rows of 6144 x 4096 take 49 us, 1.03 PFLOP/s,
+// 4096 rows 158 us, 1.30 PFLOP/s (library, bf16 weights, 1000 rows: 52 us); bf16 products in registers reach 1.92 PFLOP/s.
+template <bool kMx8, bool kWords, int WN, int WM, int TN, int TM, int kBufs>
 __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearParams p, int mtiles, int grid) {
   constexpr int kThreads = WN * WM * 64, kBN = WN * TN, kBM = WM * TM;  // (in tiles of 16)
   constexpr int kRowBytes = kMx8 ? 128 : 256, kChunks = kRowBytes / 16;
   constexpr int kXBytes = kBM * 16 * kRowBytes, kWBytes = kBN * kMxTileBytes;
-  constexpr int kBuf = kXBytes + kWBytes + (kMx8 ? kBM * 64 : 0);  // x, codes, one word of scales per row of x
+  constexpr int kBuf = kXBytes + kWBytes + (kMx8 ? kThreads * 4 : 0);  // x, codes, one word of scales per row of x
   constexpr int kXLoads = kBM * 16 * kChunks / kThreads, kWLoads = kBN * 64 / kThreads;
-  __shared__ __attribute__((aligned(16))) char smem[2 * kBuf];
+  constexpr int kLoads = kXLoads + kWLoads + (kMx8 && kWords);  // of a tile
+  static_assert(kBufs == 2 || kWords, "scales that are not whole words pass through registers");
+  __shared__ __attribute__((aligned(16))) char smem[kBufs * kBuf];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, g = lane >> 4, wn = wave % WN, wm = wave / WN;
   // an XCD's workgroups in a row share four tiles of x and walk over the weight
@@ -313,32 +367,29 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
   for (int j = 0; j < kXLoads; ++j)
     xoff[j] = xrow + j * kRowStep < valid ? (xrow + j * kRowStep) * stride + xcol : kOutside;
   const int soff = tid < valid ? tid * xs_stride : kOutside;
-  char* const wave_dst = smem + wave * 1024;
-  uint32_t sr[4];
-  auto load = [&](int kt, int buf) {
+  auto load = [&](int kt, char* buf) {
     const bool in = xcol < row_bytes - kt * kRowBytes;
 #pragma unroll
     for (int j = 0; j < kXLoads; ++j)
-      buffer_to_lds16(xb, wave_dst + buf * kBuf + j * kThreads * 16, in ? xoff[j] : kOutside, kt * kRowBytes);
+      buffer_to_lds16(xb, buf + wave * 1024 + j * kThreads * 16, in ? xoff[j] : kOutside, kt * kRowBytes);
 #pragma unroll
     for (int j = 0; j < kWLoads; ++j)
-      buffer_to_lds16(wb, wave_dst + buf * kBuf + kXBytes + j * kThreads * 16, lane * 16,
+      buffer_to_lds16(wb, buf + kXBytes + wave * 1024 + j * kThreads * 16, lane * 16,
                       (j * (kThreads / 64) + wave) * tile_stride + (kt >> 2) * kMxUnitBytes + (kt & 3) * kMxTileBytes);
-    if constexpr (kMx8) {  // thread t: the four scales of row t
-      if constexpr (kWords) {
-        sr[0] = __builtin_amdgcn_raw_buffer_load_b32(sb, soff, 4 * kt, 0);
-      } else {
+    if constexpr (kMx8 && kWords)  // thread t: the four scales of row t of x
+      buffer_to_lds4(sb, buf + kXBytes + kWBytes + wave * 256, soff, 4 * kt);
+  };
+  uint32_t sr[4];  // those scales where they are not a whole word, one tile ahead of the loads above
+  auto load_xs = [&](int kt) {
+    if constexpr (kMx8 && !kWords) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          sr[q] = __builtin_amdgcn_raw_buffer_load_b8(sb, 4 * kt + q < blocks ? soff : kOutside, 4 * kt + q, 0);
-      }
+      for (int q = 0; q < 4; ++q)
+        sr[q] = __builtin_amdgcn_raw_buffer_load_b8(sb, 4 * kt + q < blocks ? soff : kOutside, 4 * kt + q, 0);
     }
   };
-  auto store_scales = [&](int buf) {
-    if constexpr (kMx8) {
-      const uint32_t v = kWords ? sr[0] : sr[0] | sr[1] << 8 | sr[2] << 16 | sr[3] << 24;
-      if (tid < kBM * 16) reinterpret_cast<uint32_t*>(smem + buf * kBuf + kXBytes + kWBytes)[tid] = v;
-    }
+  auto store_xs = [&](char* buf) {
+    if constexpr (kMx8 && !kWords)
+      reinterpret_cast<uint32_t*>(buf + kXBytes + kWBytes)[tid] = sr[0] | sr[1] << 8 | sr[2] << 16 | sr[3] << 24;
   };
 
   f32x4 acc[TN][TM];
@@ -355,31 +406,53 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
   };
 
   const int tiles = (p.K + 127) >> 7;
-  // tile kt = 4 u + t, from buffer t & 1: the fragments are read, then the next tile's loads start, which the products
-  // cover (past the last tile they repeat it)
+  // tile kt: the fragments are read, then the loads of tile kt + kBufs - 1 start, which the products cover (past the last
+  // tile they repeat it)
+  char* now = smem;
+  auto after = [&](char* buf, int n) {  // the buffer n further round
+    char* q = buf + n * kBuf;
+    return q < smem + kBufs * kBuf ? q : q - kBufs * kBuf;
+  };
   auto step = [&](int kt) {
     const int t = kt & 3;
-    const char* x = smem + (t & 1) * kBuf + wm * TM * 16 * kRowBytes;
-    const uint4* w = reinterpret_cast<const uint4*>(smem + (t & 1) * kBuf + kXBytes + wn * TN * kMxTileBytes) + lane;
+    auto start_loads = [&] {
+      __builtin_amdgcn_sched_barrier(0);
+      store_xs(after(now, 1));
+      load_xs(min(kt + 2, tiles - 1));
+      load(min(kt + kBufs - 1, tiles - 1), after(now, kBufs - 1));
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    const char* x = now + wm * TM * 16 * kRowBytes;
+    const uint4* w = reinterpret_cast<const uint4*>(now + kXBytes + wn * TN * kMxTileBytes) + lane;
     uint4 c[TN];
+    if constexpr (!(kMx8 && kBufs > 2)) {
 #pragma unroll
-    for (int i = 0; i < TN; ++i) c[i] = w[i * 64];
+      for (int i = 0; i < TN; ++i) c[i] = w[i * 64];
+    }
     if constexpr (kMx8) {
       // x: lane (row, g) takes columns 16 g .. and 64 + 16 g .. of a tile, and the scale of block g
-      const uint32_t* sx = reinterpret_cast<const uint32_t*>(smem + (t & 1) * kBuf + kXBytes + kWBytes) + wm * TM * 16 + r;
-      i32x8 b[TM];
+      const uint32_t* sx = reinterpret_cast<const uint32_t*>(now + kXBytes + kWBytes) + wm * TM * 16 + r;
+      const char* row = x + r * kRowBytes;
+      const char *at_lo = row + ((g ^ (r & 7)) * 16), *at_hi = row + (((g + 4) ^ (r & 7)) * 16);
+      uint4 lo[TM], hi[TM];
       uint32_t sb[TM];
+      if constexpr (kBufs > 2) {
+        read_mx8<TN, 16 * kRowBytes>(lds_address(w), lds_address(at_lo), lds_address(at_hi), lds_address(sx), c, lo, hi, sb);
+      } else {
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+          lo[j] = *reinterpret_cast<const uint4*>(at_lo + j * 16 * kRowBytes);
+          hi[j] = *reinterpret_cast<const uint4*>(at_hi + j * 16 * kRowBytes);
+          sb[j] = sx[16 * j];
+        }
+      }
+      i32x8 b[TM];
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
-        const char* row = x + (16 * j + r) * kRowBytes;
-        const uint4 lo = *reinterpret_cast<const uint4*>(row + ((g ^ (r & 7)) * 16));
-        const uint4 hi = *reinterpret_cast<const uint4*>(row + (((g + 4) ^ (r & 7)) * 16));
-        b[j] = i32x8{(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
-        sb[j] = sx[16 * j] >> (8 * g);
+        b[j] = i32x8{(int)lo[j].x, (int)lo[j].y, (int)lo[j].z, (int)lo[j].w, (int)hi[j].x, (int)hi[j].y, (int)hi[j].z, (int)hi[j].w};
+        sb[j] >>= 8 * g;
       }
-      __builtin_amdgcn_sched_barrier(0);
-      load(min(kt + 1, tiles - 1), (t + 1) & 1);
-      __builtin_amdgcn_sched_barrier(0);
+      start_loads();
 #pragma unroll
       for (int i = 0; i < TN; ++i) {
         const i32x8 a = {(int)c[i].x, (int)c[i].y, (int)c[i].z, (int)c[i].w, 0, 0, 0, 0};
@@ -394,9 +467,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
 #pragma unroll
         for (int j = 0; j < TM; ++j)
           b[s][j] = *reinterpret_cast<const uint4*>(x + (16 * j + r) * kRowBytes + (((4 * g + s) ^ (r & 7)) * 16));
-      __builtin_amdgcn_sched_barrier(0);
-      load(min(kt + 1, tiles - 1), (t + 1) & 1);
-      __builtin_amdgcn_sched_barrier(0);
+      start_loads();
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
 #pragma unroll
@@ -413,9 +484,8 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
 #pragma unroll
       for (int j = 0; j < TM; ++j) asm volatile("" : "+v"(acc[i][j]));
     __builtin_amdgcn_sched_barrier(0);
-    store_scales((t + 1) & 1);
-    wait_loads();
-    __syncthreads();
+    wait_and_sync<(kBufs - 2) * kLoads>();  // tile kt + 1 has arrived
+    now = after(now, 1);
   };
   auto next_unit = [&](int u) {
 #pragma unroll
@@ -423,10 +493,12 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
     load_scales(min(u + 1, p.units - 1));
   };
   load_scales(0);
-  load(0, 0);
-  store_scales(0);
-  wait_loads();
-  __syncthreads();
+  load_xs(0);
+  store_xs(smem);
+  load_xs(min(1, tiles - 1));
+#pragma unroll
+  for (int i = 0; i + 1 < kBufs; ++i) load(min(i, tiles - 1), smem + i * kBuf);
+  wait_and_sync<0>();
   // (one tile per iteration: side by side in one block, the compiler mixes the tiles' products, which nothing orders, and
   // runs out of registers)
   for (int u = 0; u < p.units; ++u) {
@@ -435,13 +507,43 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
 #pragma unroll 1
     for (int kt = 4 * u; kt < end; ++kt) step(kt);
   }
+  if constexpr (kBufs > 2) wait_and_sync<0>();  // (the loads past the last tile still write the buffers)
+  // The outputs go through LDS into whole rows: a lane's four stand 32 bytes wide in 16 rows, which HBM takes at 2 TB/s
+  // (4096 rows of 28672 x 4096: 394 us).
+  constexpr int kOutRow = kBN * 32 + 16;  // bytes of a row of the tile in LDS; the 16 spread the rows over the banks
+  static_assert(kBM * 16 * kOutRow <= kBufs * kBuf, "the tile's outputs take the place of the buffers");
 #pragma unroll
-  for (int i = 0; i < TN; ++i)
+  for (int i = 0; i < TN; ++i) {
+    const int col = (wn * TN + i) * 16 + 4 * g, n = nt0 * 16 + col;
+    float bias[4] = {0.f, 0.f, 0.f, 0.f};
+    if (p.bias != nullptr) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bias[e] = n + e < p.N ? bf16_bits_to_f32(p.bias[n + e]) : 0.f;
+    }
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
-      const int n = (nt0 + wn * TN + i) * 16 + 4 * g, m = m0 + (wm * TM + j) * 16 + r;
-      if (m < p.M) store_out(p, m, n, acc[i][j]);
+      const f32x4 v = acc[i][j];
+      *reinterpret_cast<uint2*>(smem + ((wm * TM + j) * 16 + r) * kOutRow + col * 2) =
+          make_uint2(pack_bf16x2(v[0] + bias[0], v[1] + bias[1]), pack_bf16x2(v[2] + bias[2], v[3] + bias[3]));
     }
+  }
+  __syncthreads();
+  constexpr int kPieces = kBN * 2;  // of 16 bytes in a row
+#pragma unroll 4
+  for (int q = tid; q < kBM * 16 * kPieces; q += kThreads) {
+    const int row = q / kPieces, n = nt0 * 16 + (q % kPieces) * 8;
+    if (row >= valid || n >= p.N) continue;
+    const uint4 v = *reinterpret_cast<const uint4*>(smem + row * kOutRow + (q % kPieces) * 16);
+    uint16_t* out = p.out + static_cast<int64_t>(m0 + row) * p.out_stride + n;
+    if (p.vector_out && n + 8 <= p.N) {
+      *reinterpret_cast<uint4*>(out) = v;
+    } else {
+      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (n + e < p.N) out[e] = static_cast<uint16_t>(u[e >> 1] >> (16 * (e & 1)));
+    }
+  }
 }
 
 template <bool kMx8, int MT, int NT, int KS>
@@ -475,36 +577,44 @@ void launch_mt(const LinearParams& p, hipStream_t s) {
     launch_rows<kMx8, MT, 4, 1>(p, s);
 }
 
-template <bool kMx8, int WN, int WM, int TN, int TM>
+template <bool kMx8, int WN, int WM, int TN, int TM, int kBufs>
 void launch_tile(const LinearParams& p, hipStream_t s) {
   const int nblocks = (p.N + 16 * WN * TN - 1) / (16 * WN * TN), mtiles = (p.M + 16 * WM * TM - 1) / (16 * WM * TM);
   const int grid = nblocks * mtiles;
   if (!kMx8 || p.scale_words)
-    mx4_tile_kernel<kMx8, true, WN, WM, TN, TM><<<grid, WN * WM * 64, 0, s>>>(p, mtiles, grid);
+    mx4_tile_kernel<kMx8, true, WN, WM, TN, TM, kBufs><<<grid, WN * WM * 64, 0, s>>>(p, mtiles, grid);
   else
-    mx4_tile_kernel<kMx8, !kMx8, WN, WM, TN, TM><<<grid, WN * WM * 64, 0, s>>>(p, mtiles, grid);
+    mx4_tile_kernel<kMx8, !kMx8, WN, WM, TN, TM, 2><<<grid, WN * WM * 64, 0, s>>>(p, mtiles, grid);
 }
 
 // The tile kernel where the row kernel would give each CU more than 16 tiles of 16 weight rows x 32 rows of x: a round of
 // tiles takes as long whether it fills its CUs or not (us, bf16 / MX8 rows, row kernel against tiles: 28672 x 4096 for 64
 // rows, 14 tiles a CU, 31 / 32 against 38 / 33; for 96 rows, 21, 48 / 50 against 40 / 35; 6144 x 4096 for 256 rows, 12,
 // 25 / 26 against 39 / 34).  Up to 64 rows the row kernel, which HBM bounds, at any width.
-// MX8 rows take 256 x 128 tiles once those fill three quarters of the CUs (4096 rows of 28672 x 4096: 407 us against 478
-// with 128 x 128; 1000 rows of 4096 x 14336, 128 of them: 114 against 98); bf16 rows, which need twice the LDS, always
-// 128 x 128 (757 against 1009).
+// Tiles of 128 x 128, for MX8 rows with three buffers, whose loads have two tiles' time to arrive: with one workgroup a CU
+// nothing else covers them (1000 rows of 4096 x 14336, 256 workgroups: 74 us, 94 with two).  Once tiles of 256 x 128 give
+// seven eighths of the CUs a workgroup, MX8 rows take those, with two buffers, so that two share a CU (4096 rows of
+// 28672 x 4096: 366 us against 459; 1000 rows of 6144 x 4096, 192 of them: 36.6 against 35.3).
+// bf16 rows take 128 x 64 while 128 x 128 would leave CUs with one workgroup, up to three for two CUs (us: 1000 rows of
+// 4096 x 14336, 256 of 128 x 128: 106 against 118; 6144 x 4096, 384: 48.8 against 49.7; 256 rows of 28672 x 4096, 448: 66
+// against 54).
 template <bool kMx8>
 int32_t launch(const LinearParams& p, hipStream_t s, int kernel) {
   const int64_t cus = std::max(1, device_cu_count());
   const int64_t work = static_cast<int64_t>((p.N + 15) / 16) * ((p.M + 31) / 32);
   if (kernel == LKV_MX4_TILES || (kernel == LKV_MX4_AUTO && p.M > 64 && work > 16 * cus)) {
-    const int64_t wide = static_cast<int64_t>((p.N + 255) / 256) * ((p.M + 127) / 128);
+    const int64_t mtiles = (p.M + 127) / 128;
     if constexpr (kMx8) {
-      if (4 * wide >= 3 * cus) {
-        launch_tile<true, 2, 2, 8, 4>(p, s);
-        return check_launch("lkv_mx4_linear");
-      }
+      if (8 * ((p.N + 255) / 256) * mtiles >= 7 * cus)
+        launch_tile<true, 2, 2, 8, 4, 2>(p, s);
+      else
+        launch_tile<true, 2, 2, 4, 4, 3>(p, s);
+    } else {
+      if (2 * ((p.N + 127) / 128) * mtiles > 3 * cus)
+        launch_tile<false, 2, 2, 4, 4, 2>(p, s);
+      else
+        launch_tile<false, 2, 2, 4, 2, 2>(p, s);
     }
-    launch_tile<kMx8, 2, 2, 4, 4>(p, s);
   } else if (p.M <= 16) {
     launch_mt<kMx8, 1>(p, s);
   } else {
@@ -695,6 +805,6 @@ extern "C" int32_t lkv_mx4_linear(const lkv_mx4_linear_args* a, lkv_stream_t str
   p.units = mx4_units(a->in_features);
   p.tile_stride = mx4_tile_stride(p.units);
   p.scale_words = (bits(a->x_scales) & 3) == 0 && a->x_scale_stride % 4 == 0 && a->in_features % 128 == 0;
-  p.vector_out = (bits(a->out) & 7) == 0 && a->out_stride % 4 == 0;
+  p.vector_out = (bits(a->out) & 15) == 0 && a->out_stride % 8 == 0;
   return mx8 ? launch<true>(p, as_stream(stream), a->kernel) : launch<false>(p, as_stream(stream), a->kernel);
 }

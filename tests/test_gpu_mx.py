@@ -328,6 +328,18 @@ def test_linear_kernels_chosen_by_size(m, n, mx8):
     assert torch.equal(out, ops.mx4_linear(x, w))
 
 
+@pytest.mark.parametrize("mx8", [False, True])
+@pytest.mark.parametrize("m,n,k", [(1030, 8001, 544), (1030, 8001, 640), (129, 28700, 160), (129, 28700, 32), (300, 5000, 1152)])
+def test_linear_large_tiles(m, n, k, mx8):
+    """Sizes that fill the card with tiles: the largest of them, cut at both edges, with scales in whole words and not."""
+
+    g = _gen(m + n + k)
+    codes, scales = random_mx4(g, n, k)
+    bias = torch.randn(n, generator=g, device=DEV).to(BF16) if n % 2 else None
+    x = random_mx8(g, m, k) if mx8 else outliers(g, m, k)
+    check_linear(x, mx8_values(x) if mx8 else x.double(), codes, scales, bias)
+
+
 @pytest.mark.parametrize("m", [1, 5, 40, 300])
 def test_linear_bad_values_stay_in_their_row(m, kernel):
     """An infinity or NaN in one row of x: that row is what the products say, every other row is as without it."""
