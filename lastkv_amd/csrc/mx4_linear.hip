@@ -65,41 +65,20 @@ __device__ inline uint32_t lds_address(const void* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)p));
 }
 
-// A wave's fragments of a tile, read and waited for in one piece of assembly: before an LDS read of its own the compiler
-// waits for every load to LDS in flight, those of later tiles too.
-template <int TN, int kXStep>
-__device__ inline void read_mx8(uint32_t w, uint32_t lo, uint32_t hi, uint32_t sc, uint4 (&c)[TN], uint4 (&l)[4], uint4 (&h)[4],
-                                uint32_t (&s)[4]) {
-  static_assert(TN == 4 || TN == 8, "tiles of a wave");
-  if constexpr (TN == 8) {
-    asm volatile(
-        "ds_read_b128 %0, %20\n ds_read_b128 %8, %21\n ds_read_b128 %12, %22\n"
-        "ds_read_b128 %9, %21 offset:%c24\n ds_read_b128 %13, %22 offset:%c24\n"
-        "ds_read_b128 %10, %21 offset:%c25\n ds_read_b128 %14, %22 offset:%c25\n"
-        "ds_read_b128 %11, %21 offset:%c26\n ds_read_b128 %15, %22 offset:%c26\n"
-        "ds_read_b32 %16, %23\n ds_read_b32 %17, %23 offset:64\n ds_read_b32 %18, %23 offset:128\n ds_read_b32 %19, %23 offset:192\n"
-        "ds_read_b128 %1, %20 offset:1024\n ds_read_b128 %2, %20 offset:2048\n ds_read_b128 %3, %20 offset:3072\n"
-        "ds_read_b128 %4, %20 offset:4096\n ds_read_b128 %5, %20 offset:5120\n ds_read_b128 %6, %20 offset:6144\n"
-        "ds_read_b128 %7, %20 offset:7168\n s_waitcnt lgkmcnt(0)"
-        : "=&v"(c[0]), "=&v"(c[1]), "=&v"(c[2]), "=&v"(c[3]), "=&v"(c[4]), "=&v"(c[5]), "=&v"(c[6]), "=&v"(c[7]), "=&v"(l[0]),
-          "=&v"(l[1]), "=&v"(l[2]), "=&v"(l[3]), "=&v"(h[0]), "=&v"(h[1]), "=&v"(h[2]), "=&v"(h[3]), "=&v"(s[0]), "=&v"(s[1]),
-          "=&v"(s[2]), "=&v"(s[3])
-        : "v"(w), "v"(lo), "v"(hi), "v"(sc), "n"(kXStep), "n"(2 * kXStep), "n"(3 * kXStep)
-        : "memory");
-  } else {
-    asm volatile(
-        "ds_read_b128 %0, %16\n ds_read_b128 %4, %17\n ds_read_b128 %8, %18\n"
-        "ds_read_b128 %5, %17 offset:%c20\n ds_read_b128 %9, %18 offset:%c20\n"
-        "ds_read_b128 %6, %17 offset:%c21\n ds_read_b128 %10, %18 offset:%c21\n"
-        "ds_read_b128 %7, %17 offset:%c22\n ds_read_b128 %11, %18 offset:%c22\n"
-        "ds_read_b32 %12, %19\n ds_read_b32 %13, %19 offset:64\n ds_read_b32 %14, %19 offset:128\n ds_read_b32 %15, %19 offset:192\n"
-        "ds_read_b128 %1, %16 offset:1024\n ds_read_b128 %2, %16 offset:2048\n ds_read_b128 %3, %16 offset:3072\n"
-        "s_waitcnt lgkmcnt(0)"
-        : "=&v"(c[0]), "=&v"(c[1]), "=&v"(c[2]), "=&v"(c[3]), "=&v"(l[0]), "=&v"(l[1]), "=&v"(l[2]), "=&v"(l[3]), "=&v"(h[0]),
-          "=&v"(h[1]), "=&v"(h[2]), "=&v"(h[3]), "=&v"(s[0]), "=&v"(s[1]), "=&v"(s[2]), "=&v"(s[3])
-        : "v"(w), "v"(lo), "v"(hi), "v"(sc), "n"(kXStep), "n"(2 * kXStep), "n"(3 * kXStep)
-        : "memory");
-  }
+// A wave's fragments of a tile (4 of codes, 2 of x), read and waited for in one piece of assembly: before an LDS read of its
+// own the compiler waits for every load to LDS in flight, those of later tiles too.
+template <int kXStep>
+__device__ inline void read_mx8(uint32_t w, uint32_t lo, uint32_t hi, uint32_t sc, uint4 (&c)[4], uint4 (&l)[2], uint4 (&h)[2],
+                                uint32_t (&s)[2]) {
+  asm volatile(
+      "ds_read_b128 %0, %10\n ds_read_b128 %4, %11\n ds_read_b128 %6, %12\n"
+      "ds_read_b128 %5, %11 offset:%c14\n ds_read_b128 %7, %12 offset:%c14\n ds_read_b32 %8, %13\n ds_read_b32 %9, %13 offset:64\n"
+      "ds_read_b128 %1, %10 offset:1024\n ds_read_b128 %2, %10 offset:2048\n ds_read_b128 %3, %10 offset:3072\n"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(c[0]), "=&v"(c[1]), "=&v"(c[2]), "=&v"(c[3]), "=&v"(l[0]), "=&v"(l[1]), "=&v"(h[0]), "=&v"(h[1]), "=&v"(s[0]),
+        "=&v"(s[1])
+      : "v"(w), "v"(lo), "v"(hi), "v"(sc), "n"(kXStep)
+      : "memory");
 }
 
 // All loads of the wave but the last kLeft have arrived (those to LDS too).
@@ -317,9 +296,9 @@ __global__ __launch_bounds__(kWaves * 64, MT == 1 && NT == 1 ? 4 : 2) void mx4_r
 
 // Many rows: one workgroup of WN x WM waves per (16 WN TN rows of the weight, 16 WM TM rows of x), each wave TN x TM
 // tiles of 16 x 16.  Tiles of 128 columns of both go to LDS by direct loads, kBufs buffers in turn, one barrier a tile; two
-// workgroups share a CU where there are that many, so that one's products cover the other's reads of LDS.
+// or three workgroups share a CU where there are that many, so that one's products cover the other's reads of LDS.
 // MX8 rows: both operands and both scales go to the scaled matrix instruction as they are (a code is converted nowhere).
-// Bound by the matrix pipe, of which 4096 rows of 28672 x 4096 reach 2.63 PFLOP/s (366 us; bf16 weights in the library's
+// Bound by the matrix pipe, of which 4096 rows of 28672 x 4096 reach 2.64 PFLOP/s (364 us; bf16 weights in the library's
 // GEMM 641 us); independent products in registers reach 3.83 PFLOP/s on this card, this loop without its loads 3.4.  With
 // the tile staged through registers the same took 30-50 us more, with the outputs stored from registers 28.
 // bf16 rows: the codes are converted in registers as they are used.  1000 rows of 6144 x 4096 take 49 us, 1.03 PFLOP/s,
@@ -332,6 +311,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
   constexpr int kBuf = kXBytes + kWBytes + (kMx8 ? kThreads * 4 : 0);  // x, codes, one word of scales per row of x
   constexpr int kXLoads = kBM * 16 * kChunks / kThreads, kWLoads = kBN * 64 / kThreads;
   constexpr int kLoads = kXLoads + kWLoads + (kMx8 && kWords);  // of a tile
+  static_assert(kBufs == 2 || (kMx8 && TN == 4 && TM == 2), "the tiles of read_mx8");
   static_assert(kBufs == 2 || kWords, "scales that are not whole words pass through registers");
   __shared__ __attribute__((aligned(16))) char smem[kBufs * kBuf];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -413,19 +393,20 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
     char* q = buf + n * kBuf;
     return q < smem + kBufs * kBuf ? q : q - kBufs * kBuf;
   };
-  auto step = [&](int kt) {
-    const int t = kt & 3;
+  auto step = [&](int k0, int t) {
+    const int kt = k0 + t;
     auto start_loads = [&] {
       __builtin_amdgcn_sched_barrier(0);
       store_xs(after(now, 1));
       load_xs(min(kt + 2, tiles - 1));
+      if (t == 0) load_scales(min((kt >> 2) + 1, p.units - 1));
       load(min(kt + kBufs - 1, tiles - 1), after(now, kBufs - 1));
       __builtin_amdgcn_sched_barrier(0);
     };
     const char* x = now + wm * TM * 16 * kRowBytes;
     const uint4* w = reinterpret_cast<const uint4*>(now + kXBytes + wn * TN * kMxTileBytes) + lane;
     uint4 c[TN];
-    if constexpr (!(kMx8 && kBufs > 2)) {
+    if constexpr (kBufs == 2) {
 #pragma unroll
       for (int i = 0; i < TN; ++i) c[i] = w[i * 64];
     }
@@ -437,7 +418,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
       uint4 lo[TM], hi[TM];
       uint32_t sb[TM];
       if constexpr (kBufs > 2) {
-        read_mx8<TN, 16 * kRowBytes>(lds_address(w), lds_address(at_lo), lds_address(at_hi), lds_address(sx), c, lo, hi, sb);
+        read_mx8<16 * kRowBytes>(lds_address(w), lds_address(at_lo), lds_address(at_hi), lds_address(sx), c, lo, hi, sb);
       } else {
 #pragma unroll
         for (int j = 0; j < TM; ++j) {
@@ -487,10 +468,9 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
     wait_and_sync<(kBufs - 2) * kLoads>();  // tile kt + 1 has arrived
     now = after(now, 1);
   };
-  auto next_unit = [&](int u) {
+  auto next_unit = [&] {
 #pragma unroll
     for (int i = 0; i < TN; ++i) ws[i] = ws_next[i];
-    load_scales(min(u + 1, p.units - 1));
   };
   load_scales(0);
   load_xs(0);
@@ -499,13 +479,18 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
 #pragma unroll
   for (int i = 0; i + 1 < kBufs; ++i) load(min(i, tiles - 1), smem + i * kBuf);
   wait_and_sync<0>();
-  // (one tile per iteration: side by side in one block, the compiler mixes the tiles' products, which nothing orders, and
-  // runs out of registers)
-  for (int u = 0; u < p.units; ++u) {
-    next_unit(u);
-    const int end = min(4 * u + 4, tiles);
+  // (the four tiles of a unit without branches, so that the compiler can count the loads since the unit's scale words and
+  // waits for those alone)
+  const int full = tiles >> 2;
+  for (int u = 0; u < full; ++u) {
+    next_unit();
+#pragma unroll
+    for (int t = 0; t < 4; ++t) step(4 * u, t);
+  }
+  if (full < p.units) {
+    next_unit();
 #pragma unroll 1
-    for (int kt = 4 * u; kt < end; ++kt) step(kt);
+    for (int t = 0; t < (tiles & 3); ++t) step(4 * full, t);
   }
   if constexpr (kBufs > 2) wait_and_sync<0>();  // (the loads past the last tile still write the buffers)
   // The outputs go through LDS into whole rows: a lane's four stand 32 bytes wide in 16 rows, which HBM takes at 2 TB/s
@@ -587,33 +572,38 @@ void launch_tile(const LinearParams& p, hipStream_t s) {
     mx4_tile_kernel<kMx8, !kMx8, WN, WM, TN, TM, 2><<<grid, WN * WM * 64, 0, s>>>(p, mtiles, grid);
 }
 
-// The tile kernel where the row kernel would give each CU more than 16 tiles of 16 weight rows x 32 rows of x: a round of
-// tiles takes as long whether it fills its CUs or not (us, bf16 / MX8 rows, row kernel against tiles: 28672 x 4096 for 64
-// rows, 14 tiles a CU, 31 / 32 against 38 / 33; for 96 rows, 21, 48 / 50 against 40 / 35; 6144 x 4096 for 256 rows, 12,
-// 25 / 26 against 39 / 34).  Up to 64 rows the row kernel, which HBM bounds, at any width.
-// Tiles of 128 x 128, for MX8 rows with three buffers, whose loads have two tiles' time to arrive: with one workgroup a CU
-// nothing else covers them (1000 rows of 4096 x 14336, 256 workgroups: 74 us, 94 with two).  Once tiles of 256 x 128 give
-// seven eighths of the CUs a workgroup, MX8 rows take those, with two buffers, so that two share a CU (4096 rows of
-// 28672 x 4096: 366 us against 459; 1000 rows of 6144 x 4096, 192 of them: 36.6 against 35.3).
-// bf16 rows take 128 x 64 while 128 x 128 would leave CUs with one workgroup, up to three for two CUs (us: 1000 rows of
-// 4096 x 14336, 256 of 128 x 128: 106 against 118; 6144 x 4096, 384: 48.8 against 49.7; 256 rows of 28672 x 4096, 448: 66
-// against 54).
+// The tile kernel where the row kernel would give each CU more than 16 tiles of 16 weight rows x 32 rows of x, for MX8 rows
+// more than 6: a round of tiles takes as long whether it fills its CUs or not (us, row kernel against tiles.  bf16 rows:
+// 6144 x 4096 for 256 rows, 12 tiles a CU, 25.3 against 29.5; 28672 x 4096 for 64 rows, 14, 29.0 against 32.7; for 96 rows,
+// 21, 48.9 against 32.9.  MX8 rows: 6144 x 4096 for 128 rows, 6, 15.5 against 16.3; 14336 x 4096 for 64, 7, 16.8 against
+// 17.7; 28672 x 4096 for 32, 7, 19.3 against 17.3; 4096 x 14336 for 256, 8, 43.5 against 44.3; 14336 x 4096 for 96, 10.5,
+// 27.4 against 16.1).  Below that the row kernel, which HBM bounds: at any width up to 32 bf16 rows (128256 x 4096: 62
+// against 97) and up to 16 MX8 rows, whose products it takes exactly.
+// Large tiles where 128 x 64 ones would be more than three a CU (us, MX8 rows: 28672 x 4096 for 4096 rows 364 with
+// 256 x 128, 459 with 128 x 128; 6144 x 4096 for 1000 rows, three a CU, 37.7 against 32.6 with 128 x 64.  bf16 rows, which
+// need twice the LDS, 128 x 128: 28672 x 4096 for 4096 rows 722, 1009 with 256 x 128; 256 rows, 3.5 a CU, 53 against 63 with
+// 128 x 64; 6144 x 4096 for 1000 rows 49.5 against 47.8, 4096 x 14336, two a CU, 123 against 105).
+// Small MX8 tiles take four buffers while that leaves a CU its two workgroups, as few of them wait for memory most of the
+// time, and three for the third (us, two / three / four buffers: 4096 x 14336 for 256 rows, one for two CUs, 84 / 53 / 44;
+// for 1000 rows, two a CU, 85 / 71 / 70; 6144 x 4096 for 1000, three a CU, 31.9 / 32.6 / 36.3).
 template <bool kMx8>
 int32_t launch(const LinearParams& p, hipStream_t s, int kernel) {
   const int64_t cus = std::max(1, device_cu_count());
   const int64_t work = static_cast<int64_t>((p.N + 15) / 16) * ((p.M + 31) / 32);
-  if (kernel == LKV_MX4_TILES || (kernel == LKV_MX4_AUTO && p.M > 64 && work > 16 * cus)) {
-    const int64_t mtiles = (p.M + 127) / 128;
+  if (kernel == LKV_MX4_TILES || (kernel == LKV_MX4_AUTO && p.M > (kMx8 ? 16 : 32) && work > (kMx8 ? 6 : 16) * cus)) {
+    const int64_t small = static_cast<int64_t>((p.N + 127) / 128) * ((p.M + 63) / 64);  // tiles of 128 x 64
     if constexpr (kMx8) {
-      if (8 * ((p.N + 255) / 256) * mtiles >= 7 * cus)
+      if (small <= 2 * cus)
+        launch_tile<true, 2, 2, 4, 2, 4>(p, s);
+      else if (small <= 3 * cus)
+        launch_tile<true, 2, 2, 4, 2, 3>(p, s);
+      else
         launch_tile<true, 2, 2, 8, 4, 2>(p, s);
-      else
-        launch_tile<true, 2, 2, 4, 4, 3>(p, s);
     } else {
-      if (2 * ((p.N + 127) / 128) * mtiles > 3 * cus)
-        launch_tile<false, 2, 2, 4, 4, 2>(p, s);
-      else
+      if (small <= 3 * cus)
         launch_tile<false, 2, 2, 4, 2, 2>(p, s);
+      else
+        launch_tile<false, 2, 2, 4, 4, 2>(p, s);
     }
   } else if (p.M <= 16) {
     launch_mt<kMx8, 1>(p, s);

@@ -308,7 +308,8 @@ def test_mx8_products_that_cancel(m, kernel):
             assert ops.mx4_linear(x, w).eq(want).all(), (at, b)
 
 
-@pytest.mark.parametrize("m,n,mx8", [(96, 28672, False), (96, 28672, True), (1000, 6144, True), (1000, 6144, False), (64, 28672, True)])
+@pytest.mark.parametrize("m,n,mx8", [(96, 28672, False), (96, 28672, True), (1000, 6144, True), (1000, 6144, False),
+                                     (64, 28672, False), (16, 28672, True), (17, 28672, True)])
 def test_linear_kernels_chosen_by_size(m, n, mx8):
     """Without a fixed kernel the call equals the one whose sizes choose it."""
 
@@ -318,7 +319,7 @@ def test_linear_kernels_chosen_by_size(m, n, mx8):
     a = _lib.Mx4LinearArgs()
     out = torch.empty((m, n), device=DEV, dtype=BF16)
     a.struct_size, a.rows, a.out_features, a.in_features = ctypes.sizeof(a), m, n, 256
-    a.kernel = TILES if m > 64 else ROWS
+    a.kernel = TILES if m > (16 if mx8 else 64) else ROWS
     data = x.data if mx8 else x
     a.x, a.x_stride, a.x_format = data.data_ptr(), 256, int(mx8)
     if mx8:
@@ -329,7 +330,7 @@ def test_linear_kernels_chosen_by_size(m, n, mx8):
 
 
 @pytest.mark.parametrize("mx8", [False, True])
-@pytest.mark.parametrize("m,n,k", [(1030, 8001, 544), (1030, 8001, 640), (129, 28700, 160), (129, 28700, 32), (300, 5000, 1152)])
+@pytest.mark.parametrize("m,n,k", [(1030, 8001, 544), (1030, 8001, 640), (129, 28700, 160), (129, 28700, 640), (129, 28700, 32), (300, 5000, 1152)])
 def test_linear_large_tiles(m, n, k, mx8):
     """Sizes that fill the card with tiles: the largest of them, cut at both edges, with scales in whole words and not."""
 
