@@ -20,7 +20,6 @@ struct LinearParams {
   int32_t M, N, K;
   int32_t units, tile_stride;
   bool vector_out;  // output rows are 16-byte aligned
-  bool scale_words;  // x scales in whole aligned words: a row's four of a tile
 };
 
 constexpr int kWaves = 8;
@@ -57,10 +56,6 @@ __device__ inline void buffer_to_lds16(__amdgpu_buffer_rsrc_t r, char* dst, int 
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)dst, 16, offset, scalar_offset, 0, 0);
 }
 
-__device__ inline void buffer_to_lds4(__amdgpu_buffer_rsrc_t r, char* dst, int offset, int scalar_offset) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)dst, 4, offset, scalar_offset, 0, 0);
-}
-
 __device__ inline uint32_t lds_address(const void* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)p));
 }
@@ -68,16 +63,14 @@ __device__ inline uint32_t lds_address(const void* p) {
 // A wave's fragments of a tile (4 of codes, 2 of x), read and waited for in one piece of assembly: before an LDS read of its
 // own the compiler waits for every load to LDS in flight, those of later tiles too.
 template <int kXStep>
-__device__ inline void read_mx8(uint32_t w, uint32_t lo, uint32_t hi, uint32_t sc, uint4 (&c)[4], uint4 (&l)[2], uint4 (&h)[2],
-                                uint32_t (&s)[2]) {
+__device__ inline void read_mx8(uint32_t w, uint32_t lo, uint32_t hi, uint4 (&c)[4], uint4 (&l)[2], uint4 (&h)[2]) {
   asm volatile(
-      "ds_read_b128 %0, %10\n ds_read_b128 %4, %11\n ds_read_b128 %6, %12\n"
-      "ds_read_b128 %5, %11 offset:%c14\n ds_read_b128 %7, %12 offset:%c14\n ds_read_b32 %8, %13\n ds_read_b32 %9, %13 offset:64\n"
-      "ds_read_b128 %1, %10 offset:1024\n ds_read_b128 %2, %10 offset:2048\n ds_read_b128 %3, %10 offset:3072\n"
+      "ds_read_b128 %0, %8\n ds_read_b128 %4, %9\n ds_read_b128 %6, %10\n"
+      "ds_read_b128 %5, %9 offset:%c11\n ds_read_b128 %7, %10 offset:%c11\n"
+      "ds_read_b128 %1, %8 offset:1024\n ds_read_b128 %2, %8 offset:2048\n ds_read_b128 %3, %8 offset:3072\n"
       "s_waitcnt lgkmcnt(0)"
-      : "=&v"(c[0]), "=&v"(c[1]), "=&v"(c[2]), "=&v"(c[3]), "=&v"(l[0]), "=&v"(l[1]), "=&v"(h[0]), "=&v"(h[1]), "=&v"(s[0]),
-        "=&v"(s[1])
-      : "v"(w), "v"(lo), "v"(hi), "v"(sc), "n"(kXStep)
+      : "=&v"(c[0]), "=&v"(c[1]), "=&v"(c[2]), "=&v"(c[3]), "=&v"(l[0]), "=&v"(l[1]), "=&v"(h[0]), "=&v"(h[1])
+      : "v"(w), "v"(lo), "v"(hi), "n"(kXStep)
       : "memory");
 }
 
@@ -298,22 +291,22 @@ __global__ __launch_bounds__(kWaves * 64, MT == 1 && NT == 1 ? 4 : 2) void mx4_r
 // tiles of 16 x 16.  Tiles of 128 columns of both go to LDS by direct loads, kBufs buffers in turn, one barrier a tile; two
 // or three workgroups share a CU where there are that many, so that one's products cover the other's reads of LDS.
 // MX8 rows: both operands and both scales go to the scaled matrix instruction as they are (a code is converted nowhere).
-// Bound by the matrix pipe, of which 4096 rows of 28672 x 4096 reach 2.64 PFLOP/s (364 us; bf16 weights in the library's
+// Bound by the matrix pipe, of which 4096 rows of 28672 x 4096 reach 2.57 PFLOP/s (375 us; bf16 weights in the library's
 // GEMM 641 us); independent products in registers reach 3.83 PFLOP/s on this card, this loop without its loads 3.4.  With
 // the tile staged through registers the same took 30-50 us more, with the outputs stored from registers 28.
-// bf16 rows: the codes are converted in registers as they are used.  1000 rows of 6144 x 4096 take 49 us, 1.03 PFLOP/s,
-// 4096 rows 158 us, 1.30 PFLOP/s (library, bf16 weights, 1000 rows: 52 us); bf16 products in registers reach 1.92 PFLOP/s.
-template <bool kMx8, bool kWords, int WN, int WM, int TN, int TM, int kBufs>
+// bf16 rows: the codes are converted in registers as they are used.  1000 rows of 6144 x 4096 take 46 us, 1.09 PFLOP/s,
+// 4096 rows 160 us, 1.29 PFLOP/s (library, bf16 weights, 1000 rows: 52 us); bf16 products in registers reach 1.92 PFLOP/s.
+template <bool kMx8, int WN, int WM, int TN, int TM, int kBufs>
 __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearParams p, int mtiles, int grid) {
   constexpr int kThreads = WN * WM * 64, kBN = WN * TN, kBM = WM * TM;  // (in tiles of 16)
   constexpr int kRowBytes = kMx8 ? 128 : 256, kChunks = kRowBytes / 16;
   constexpr int kXBytes = kBM * 16 * kRowBytes, kWBytes = kBN * kMxTileBytes;
-  constexpr int kBuf = kXBytes + kWBytes + (kMx8 ? kThreads * 4 : 0);  // x, codes, one word of scales per row of x
+  constexpr int kBuf = kXBytes + kWBytes;
   constexpr int kXLoads = kBM * 16 * kChunks / kThreads, kWLoads = kBN * 64 / kThreads;
-  constexpr int kLoads = kXLoads + kWLoads + (kMx8 && kWords);  // of a tile
+  constexpr int kLoads = kXLoads + kWLoads;  // of a tile
   static_assert(kBufs == 2 || (kMx8 && TN == 4 && TM == 2), "the tiles of read_mx8");
-  static_assert(kBufs == 2 || kWords, "scales that are not whole words pass through registers");
-  __shared__ __attribute__((aligned(16))) char smem[kBufs * kBuf];
+  constexpr int kOutRow = kBN * 32 + 16;  // bytes of an output row in LDS; the 16 spread the rows over the banks
+  __shared__ __attribute__((aligned(16))) char smem[std::max(kBufs * kBuf, kBM * 16 * kOutRow)];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, g = lane >> 4, wn = wave % WN, wm = wave / WN;
   // an XCD's workgroups in a row share four tiles of x and walk over the weight
@@ -333,10 +326,6 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
   const __amdgpu_buffer_rsrc_t wb = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<uint8_t*>(p.w + static_cast<int64_t>(nt0) * tile_stride), 0, min(kBN, ntiles - nt0) * tile_stride, 0x00020000);
 
-  const int xs_stride = static_cast<int>(p.xs_stride);
-  const __amdgpu_buffer_rsrc_t sb = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint8_t*>(p.xs + static_cast<int64_t>(m0) * xs_stride), 0, (valid - 1) * xs_stride + blocks, 0x00020000);
-
   // what this lane moves: 16 bytes of rows xrow, xrow + kRowStep, ... of x, 16 of a lane's in every code tile.  LDS takes a
   // wave's bytes in lane order, so the lane picks the chunk that its place in the swizzled row holds.
   constexpr int kRowStep = kThreads / kChunks;
@@ -346,7 +335,6 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
 #pragma unroll
   for (int j = 0; j < kXLoads; ++j)
     xoff[j] = xrow + j * kRowStep < valid ? (xrow + j * kRowStep) * stride + xcol : kOutside;
-  const int soff = tid < valid ? tid * xs_stride : kOutside;
   auto load = [&](int kt, char* buf) {
     const bool in = xcol < row_bytes - kt * kRowBytes;
 #pragma unroll
@@ -356,20 +344,6 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
     for (int j = 0; j < kWLoads; ++j)
       buffer_to_lds16(wb, buf + kXBytes + wave * 1024 + j * kThreads * 16, lane * 16,
                       (j * (kThreads / 64) + wave) * tile_stride + (kt >> 2) * kMxUnitBytes + (kt & 3) * kMxTileBytes);
-    if constexpr (kMx8 && kWords)  // thread t: the four scales of row t of x
-      buffer_to_lds4(sb, buf + kXBytes + kWBytes + wave * 256, soff, 4 * kt);
-  };
-  uint32_t sr[4];  // those scales where they are not a whole word, one tile ahead of the loads above
-  auto load_xs = [&](int kt) {
-    if constexpr (kMx8 && !kWords) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        sr[q] = __builtin_amdgcn_raw_buffer_load_b8(sb, 4 * kt + q < blocks ? soff : kOutside, 4 * kt + q, 0);
-    }
-  };
-  auto store_xs = [&](char* buf) {
-    if constexpr (kMx8 && !kWords)
-      reinterpret_cast<uint32_t*>(buf + kXBytes + kWBytes)[tid] = sr[0] | sr[1] << 8 | sr[2] << 16 | sr[3] << 24;
   };
 
   f32x4 acc[TN][TM];
@@ -377,12 +351,47 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
   for (int i = 0; i < TN; ++i)
 #pragma unroll
     for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  uint32_t ws[TN], ws_next[TN];  // scale words of this unit and the next
+  // scales of this unit and the next, a byte a tile.  Of x lane (row, g) wants block g of every tile; it loads the four
+  // blocks of tile g, whatever their alignment, and the four lanes of a row turn their bytes into each other's.
+  uint32_t ws[TN], ws_next[TN], xs[TM], xs_next[TM];
+  const uint8_t* const xs_base = p.xs + static_cast<int64_t>(m0) * p.xs_stride;
+  int xs_row[TM];
+  if constexpr (kMx8) {
+#pragma unroll
+    for (int j = 0; j < TM; ++j) xs_row[j] = min((wm * TM + j) * 16 + r, valid - 1) * static_cast<int>(p.xs_stride);
+  }
   auto load_scales = [&](int u) {
 #pragma unroll
     for (int i = 0; i < TN; ++i)
       ws_next[i] = __builtin_amdgcn_raw_buffer_load_b32(
           wb, lane * 4, (wn * TN + i) * tile_stride + u * kMxUnitBytes + 4 * kMxTileBytes, 0);
+    if constexpr (kMx8) {
+      const int b0 = 16 * u + 4 * g;
+      if (16 * u + 16 <= blocks) {
+#pragma unroll
+        for (int j = 0; j < TM; ++j) __builtin_memcpy(&xs_next[j], xs_base + xs_row[j] + b0, 4);
+      } else {  // past the last block its scale: the products there are zero, or its NaN
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+          xs_next[j] = 0;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) xs_next[j] |= static_cast<uint32_t>(xs_base[xs_row[j] + min(b0 + q, blocks - 1)]) << (8 * q);
+        }
+      }
+    }
+  };
+  // (v_perm_b32: bytes 0-3 of the second operand, 4-7 of the first)
+  const uint32_t turn16 = (g & 1) == 0 ? 0x06020400u : 0x03070105u, turn32 = (g & 2) == 0 ? 0x05040100u : 0x03020706u;
+  auto next_unit = [&] {
+#pragma unroll
+    for (int i = 0; i < TN; ++i) ws[i] = ws_next[i];
+    if constexpr (kMx8) {
+#pragma unroll
+      for (int j = 0; j < TM; ++j) {
+        const uint32_t v = __builtin_amdgcn_perm(__shfl_xor(xs_next[j], 16), xs_next[j], turn16);
+        xs[j] = __builtin_amdgcn_perm(__shfl_xor(v, 32), v, turn32);
+      }
+    }
   };
 
   const int tiles = (p.K + 127) >> 7;
@@ -397,8 +406,6 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
     const int kt = k0 + t;
     auto start_loads = [&] {
       __builtin_amdgcn_sched_barrier(0);
-      store_xs(after(now, 1));
-      load_xs(min(kt + 2, tiles - 1));
       if (t == 0) load_scales(min((kt >> 2) + 1, p.units - 1));
       load(min(kt + kBufs - 1, tiles - 1), after(now, kBufs - 1));
       __builtin_amdgcn_sched_barrier(0);
@@ -411,35 +418,30 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
       for (int i = 0; i < TN; ++i) c[i] = w[i * 64];
     }
     if constexpr (kMx8) {
-      // x: lane (row, g) takes columns 16 g .. and 64 + 16 g .. of a tile, and the scale of block g
-      const uint32_t* sx = reinterpret_cast<const uint32_t*>(now + kXBytes + kWBytes) + wm * TM * 16 + r;
+      // x: lane (row, g) takes columns 16 g .. and 64 + 16 g .. of a tile
       const char* row = x + r * kRowBytes;
       const char *at_lo = row + ((g ^ (r & 7)) * 16), *at_hi = row + (((g + 4) ^ (r & 7)) * 16);
       uint4 lo[TM], hi[TM];
-      uint32_t sb[TM];
       if constexpr (kBufs > 2) {
-        read_mx8<16 * kRowBytes>(lds_address(w), lds_address(at_lo), lds_address(at_hi), lds_address(sx), c, lo, hi, sb);
+        read_mx8<16 * kRowBytes>(lds_address(w), lds_address(at_lo), lds_address(at_hi), c, lo, hi);
       } else {
 #pragma unroll
         for (int j = 0; j < TM; ++j) {
           lo[j] = *reinterpret_cast<const uint4*>(at_lo + j * 16 * kRowBytes);
           hi[j] = *reinterpret_cast<const uint4*>(at_hi + j * 16 * kRowBytes);
-          sb[j] = sx[16 * j];
         }
       }
       i32x8 b[TM];
 #pragma unroll
-      for (int j = 0; j < TM; ++j) {
+      for (int j = 0; j < TM; ++j)
         b[j] = i32x8{(int)lo[j].x, (int)lo[j].y, (int)lo[j].z, (int)lo[j].w, (int)hi[j].x, (int)hi[j].y, (int)hi[j].z, (int)hi[j].w};
-        sb[j] >>= 8 * g;
-      }
       start_loads();
 #pragma unroll
       for (int i = 0; i < TN; ++i) {
         const i32x8 a = {(int)c[i].x, (int)c[i].y, (int)c[i].z, (int)c[i].w, 0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < TM; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b[j], acc[i][j], 4, 0, 0, ws[i] >> (8 * t), 0, sb[j]);
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b[j], acc[i][j], 4, 0, 0, ws[i] >> (8 * t), 0, xs[j] >> (8 * t));
       }
     } else {
       uint4 b[4][TM];
@@ -468,14 +470,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
     wait_and_sync<(kBufs - 2) * kLoads>();  // tile kt + 1 has arrived
     now = after(now, 1);
   };
-  auto next_unit = [&] {
-#pragma unroll
-    for (int i = 0; i < TN; ++i) ws[i] = ws_next[i];
-  };
   load_scales(0);
-  load_xs(0);
-  store_xs(smem);
-  load_xs(min(1, tiles - 1));
 #pragma unroll
   for (int i = 0; i + 1 < kBufs; ++i) load(min(i, tiles - 1), smem + i * kBuf);
   wait_and_sync<0>();
@@ -495,8 +490,6 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
   if constexpr (kBufs > 2) wait_and_sync<0>();  // (the loads past the last tile still write the buffers)
   // The outputs go through LDS into whole rows: a lane's four stand 32 bytes wide in 16 rows, which HBM takes at 2 TB/s
   // (4096 rows of 28672 x 4096: 394 us).
-  constexpr int kOutRow = kBN * 32 + 16;  // bytes of a row of the tile in LDS; the 16 spread the rows over the banks
-  static_assert(kBM * 16 * kOutRow <= kBufs * kBuf, "the tile's outputs take the place of the buffers");
 #pragma unroll
   for (int i = 0; i < TN; ++i) {
     const int col = (wn * TN + i) * 16 + 4 * g, n = nt0 * 16 + col;
@@ -566,31 +559,28 @@ template <bool kMx8, int WN, int WM, int TN, int TM, int kBufs>
 void launch_tile(const LinearParams& p, hipStream_t s) {
   const int nblocks = (p.N + 16 * WN * TN - 1) / (16 * WN * TN), mtiles = (p.M + 16 * WM * TM - 1) / (16 * WM * TM);
   const int grid = nblocks * mtiles;
-  if (!kMx8 || p.scale_words)
-    mx4_tile_kernel<kMx8, true, WN, WM, TN, TM, kBufs><<<grid, WN * WM * 64, 0, s>>>(p, mtiles, grid);
-  else
-    mx4_tile_kernel<kMx8, !kMx8, WN, WM, TN, TM, 2><<<grid, WN * WM * 64, 0, s>>>(p, mtiles, grid);
+  mx4_tile_kernel<kMx8, WN, WM, TN, TM, kBufs><<<grid, WN * WM * 64, 0, s>>>(p, mtiles, grid);
 }
 
 // The tile kernel where the row kernel would give each CU more than 16 tiles of 16 weight rows x 32 rows of x, for MX8 rows
-// more than 6: a round of tiles takes as long whether it fills its CUs or not (us, row kernel against tiles.  bf16 rows:
+// more than 4: a round of tiles takes as long whether it fills its CUs or not (us, row kernel against tiles.  bf16 rows:
 // 6144 x 4096 for 256 rows, 12 tiles a CU, 25.3 against 29.5; 28672 x 4096 for 64 rows, 14, 29.0 against 32.7; for 96 rows,
-// 21, 48.9 against 32.9.  MX8 rows: 6144 x 4096 for 128 rows, 6, 15.5 against 16.3; 14336 x 4096 for 64, 7, 16.8 against
-// 17.7; 28672 x 4096 for 32, 7, 19.3 against 17.3; 4096 x 14336 for 256, 8, 43.5 against 44.3; 14336 x 4096 for 96, 10.5,
-// 27.4 against 16.1).  Below that the row kernel, which HBM bounds: at any width up to 32 bf16 rows (128256 x 4096: 62
-// against 97) and up to 16 MX8 rows, whose products it takes exactly.
-// Large tiles where 128 x 64 ones would be more than three a CU (us, MX8 rows: 28672 x 4096 for 4096 rows 364 with
+// 21, 48.9 against 32.9.  MX8 rows: 4096 x 14336 for 128 rows, 4, 25.3 against 46; 2387 x 11744 for 201, 4.1, 48 against 37;
+// 6144 x 4096 for 128, 6, 15.5 against 16.7; 28672 x 4096 for 32, 7, 19.3 against 18.3; 4096 x 14336 for 256, 8, 43.5
+// against 46.6; 14336 x 4096 for 96, 10.5, 27.4 against 16.1).  At any width the row kernel, which HBM bounds, for up to 32
+// bf16 rows (128256 x 4096: 62 against 97) and up to 16 MX8 rows, whose products it takes exactly.
+// Large tiles where 128 x 64 ones would be more than three a CU (us, MX8 rows: 28672 x 4096 for 4096 rows 375 with
 // 256 x 128, 459 with 128 x 128; 6144 x 4096 for 1000 rows, three a CU, 37.7 against 32.6 with 128 x 64.  bf16 rows, which
 // need twice the LDS, 128 x 128: 28672 x 4096 for 4096 rows 722, 1009 with 256 x 128; 256 rows, 3.5 a CU, 53 against 63 with
 // 128 x 64; 6144 x 4096 for 1000 rows 49.5 against 47.8, 4096 x 14336, two a CU, 123 against 105).
 // Small MX8 tiles take four buffers while that leaves a CU its two workgroups, as few of them wait for memory most of the
-// time, and three for the third (us, two / three / four buffers: 4096 x 14336 for 256 rows, one for two CUs, 84 / 53 / 44;
-// for 1000 rows, two a CU, 85 / 71 / 70; 6144 x 4096 for 1000, three a CU, 31.9 / 32.6 / 36.3).
+// time, and three for the third (us, two / three / four buffers: 4096 x 14336 for 256 rows, one for two CUs, 84 / 53 / 46;
+// for 1000 rows, two a CU, 85 / 71 / 67; 6144 x 4096 for 1000, three a CU, 31.9 / 32.6 / 36.3).
 template <bool kMx8>
 int32_t launch(const LinearParams& p, hipStream_t s, int kernel) {
   const int64_t cus = std::max(1, device_cu_count());
   const int64_t work = static_cast<int64_t>((p.N + 15) / 16) * ((p.M + 31) / 32);
-  if (kernel == LKV_MX4_TILES || (kernel == LKV_MX4_AUTO && p.M > (kMx8 ? 16 : 32) && work > (kMx8 ? 6 : 16) * cus)) {
+  if (kernel == LKV_MX4_TILES || (kernel == LKV_MX4_AUTO && p.M > (kMx8 ? 16 : 32) && work > (kMx8 ? 4 : 16) * cus)) {
     const int64_t small = static_cast<int64_t>((p.N + 127) / 128) * ((p.M + 63) / 64);  // tiles of 128 x 64
     if constexpr (kMx8) {
       if (small <= 2 * cus)
@@ -794,7 +784,6 @@ extern "C" int32_t lkv_mx4_linear(const lkv_mx4_linear_args* a, lkv_stream_t str
   p.K = a->in_features;
   p.units = mx4_units(a->in_features);
   p.tile_stride = mx4_tile_stride(p.units);
-  p.scale_words = (bits(a->x_scales) & 3) == 0 && a->x_scale_stride % 4 == 0 && a->in_features % 128 == 0;
   p.vector_out = (bits(a->out) & 15) == 0 && a->out_stride % 8 == 0;
   return mx8 ? launch<true>(p, as_stream(stream), a->kernel) : launch<false>(p, as_stream(stream), a->kernel);
 }
