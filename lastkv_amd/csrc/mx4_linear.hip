@@ -74,6 +74,13 @@ __device__ inline void read_mx8(uint32_t w, uint32_t lo, uint32_t hi, uint4 (&c)
       : "memory");
 }
 
+// Where the 16-byte chunks of row r of a tile of x stand in LDS: chunk c at c ^ this.  One LDS read of 16 bytes serves 16
+// lanes at a time, rows 0-3 and 12-15 of one block of columns with rows 4-11 of the next one's (counted: with r & 7 those
+// meet half of the banks twice, except where the lanes take neighbouring chunks of 128-byte rows), which then lie apart:
+// 256-byte rows, blocks 4 chunks apart; 128-byte rows, blocks 2 apart.
+__device__ inline int swizzle4(int r) { return (r & 3) | ((r & 8) != 0 ? 12 : 0); }
+__device__ inline int swizzle2(int r) { return ((r >> 1) & 1) | ((r >> 1) & 4); }
+
 // All loads of the wave but the last kLeft have arrived (those to LDS too).
 template <int kLeft>
 __device__ inline void wait_and_sync() {
@@ -122,7 +129,7 @@ struct Step {
 // 4.9 / 4.7 (read 3.5), for 32 6.8 / 6.1; bf16 weights in the library's GEMM: 28672 x 4096 for 32 rows 48.8, 4096 x 4096 13.8.
 // The matrix instruction wants a different row of x in neighbouring lanes, which the L1 would serve 16 bytes a cycle:
 // rows are loaded along their columns (64 bytes a cycle) and turned in a wave's own corner of LDS, its 16-byte chunks
-// swizzled by the row (chunk c of row m at c ^ (m & 7)) so that neither side meets a bank twice (4096 x 4096 for 32 rows
+// swizzled by the row so that neither side meets a bank twice (4096 x 4096 for 32 rows
 // 10.6 -> 6.8 us).
 template <bool kMx8, int MT, int NT, int KS>
 __global__ __launch_bounds__(kWaves * 64, MT == 1 && NT == 1 ? 4 : 2) void mx4_rows_kernel(const LinearParams p) {
@@ -198,7 +205,7 @@ __global__ __launch_bounds__(kWaves * 64, MT == 1 && NT == 1 ? 4 : 2) void mx4_r
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int row = i * (64 / kChunks) + lrow;
-        *reinterpret_cast<uint4*>(stage + (16 * j + row) * kRowBytes + (lcol ^ ((row & 7) * 16))) = xr[j][i];
+        *reinterpret_cast<uint4*>(stage + (16 * j + row) * kRowBytes + (lcol ^ ((kMx8 ? swizzle2(row) : swizzle4(row)) * 16))) = xr[j][i];
       }
   };
   auto compute = [&](int h, int t, const Step<MT, NT>& st) {
@@ -211,8 +218,8 @@ __global__ __launch_bounds__(kWaves * 64, MT == 1 && NT == 1 ? 4 : 2) void mx4_r
       for (int j = 0; j < MT; ++j) {
         sx[j] = e8m0(__shfl(st.xs[j], 16 * t + r) >> (8 * g), 0);
         const char* at = stage + (16 * j + r) * kRowBytes;
-        lo[j] = *reinterpret_cast<const uint4*>(at + ((32 * g) ^ ((r & 7) * 16)));
-        hi[j] = *reinterpret_cast<const uint4*>(at + ((32 * g + 16) ^ ((r & 7) * 16)));
+        lo[j] = *reinterpret_cast<const uint4*>(at + ((32 * g) ^ (swizzle2(r) * 16)));
+        hi[j] = *reinterpret_cast<const uint4*>(at + ((32 * g + 16) ^ (swizzle2(r) * 16)));
       }
     }
 #pragma unroll
@@ -226,7 +233,7 @@ __global__ __launch_bounds__(kWaves * 64, MT == 1 && NT == 1 ? 4 : 2) void mx4_r
                  : s == 2 ? e4m3_to_bf16(hi[j].x, hi[j].y, sx[j])
                           : e4m3_to_bf16(hi[j].z, hi[j].w, sx[j]);
         else
-          b[j] = *reinterpret_cast<const uint4*>(stage + (16 * j + r) * kRowBytes + ((64 * g + 16 * s) ^ ((r & 7) * 16)));
+          b[j] = *reinterpret_cast<const uint4*>(stage + (16 * j + r) * kRowBytes + ((64 * g + 16 * s) ^ (swizzle4(r) * 16)));
       }
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
@@ -329,8 +336,8 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
   // what this lane moves: 16 bytes of rows xrow, xrow + kRowStep, ... of x, 16 of a lane's in every code tile.  LDS takes a
   // wave's bytes in lane order, so the lane picks the chunk that its place in the swizzled row holds.
   constexpr int kRowStep = kThreads / kChunks;
-  static_assert(kRowStep % 8 == 0, "a lane's rows share their swizzle");
-  const int xrow = tid / kChunks, xcol = ((tid % kChunks) ^ (xrow & 7)) * 16;
+  static_assert(kRowStep % 16 == 0, "a lane's rows share their swizzle");
+  const int xrow = tid / kChunks, xcol = ((tid % kChunks) ^ (kMx8 ? xrow & 7 : swizzle4(xrow))) * 16;
   int xoff[kXLoads];
 #pragma unroll
   for (int j = 0; j < kXLoads; ++j)
@@ -449,7 +456,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
       for (int s = 0; s < 4; ++s)
 #pragma unroll
         for (int j = 0; j < TM; ++j)
-          b[s][j] = *reinterpret_cast<const uint4*>(x + (16 * j + r) * kRowBytes + (((4 * g + s) ^ (r & 7)) * 16));
+          b[s][j] = *reinterpret_cast<const uint4*>(x + (16 * j + r) * kRowBytes + (((4 * g + s) ^ swizzle4(r)) * 16));
       start_loads();
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
