@@ -601,7 +601,8 @@ int32_t lkv_silu_mul(const void *gate, int64_t gate_stride, const void *up, int6
  *     above bf16's least normal value).
  * A quantized block's scale is the smallest power of two (at least 2^-127) with max|y| <= 448 * scale (MX4: 6 *
  * scale), and its values are the nearest ones, ties to even; a block with an infinity or NaN has scale 255.
- * Strides are in elements (bytes of 8-bit rows).
+ * Strides are in elements (bytes of 8-bit rows); one row's stride is not read by lkv_mx4_linear.  Outputs must not
+ * overlap inputs, except that x may be residual.
  * ------------------------------------------------------------------------------------- */
 
 /* lkv_rmsnorm with an MX8 output: if residual != NULL: residual := bf16(residual + x), and the normalised row is
@@ -650,8 +651,8 @@ int32_t lkv_mx4_unpack(const void *weight, int32_t n, int32_t k, void *out, int6
  * scaled matrix instruction adds the products of 8 neighbouring columns in fixed point (bits below 2^-13 of the largest
  * power of two of their factors' exponents are dropped) before it adds to fp32.  MX8 values past bf16's range are
  * infinite for the row kernel.
- * in_features is a multiple of 32 up to 2^20; x rows are 16-byte aligned, at most 2^21 elements apart; out must not
- * overlap x. */
+ * in_features is a multiple of 32 up to 2^20; x rows are 16-byte aligned, at most 2^21 elements apart (their scales
+ * 2^21 bytes); out must not overlap x. */
 enum { LKV_X_BF16 = 0, LKV_X_MX8 = 1 };
 enum { LKV_MX4_AUTO = 0, LKV_MX4_ROWS = 1, LKV_MX4_TILES = 2 };
 

@@ -785,14 +785,26 @@ PyObject* issue_mx8(const char* what, PyObject* given, const Mx8& out, F&& call)
   return PyErr_Format(g_error, "%s failed (status %d): %s", what, static_cast<int>(st), g_lib.last_error());
 }
 
-// The output of an op on bf16 rows t: given MX8Rows of its shape, or new ones.
-bool mx8_out(PyObject* given, const at::Tensor& t, Mx8& m) {
+// Whether rows (n of `width`, `stride` apart) meet other ones in memory.
+struct Span {
+  uintptr_t from, to;
+  Span(const at::Tensor& t, int64_t n, int64_t width, int64_t stride)
+      : from(reinterpret_cast<uintptr_t>(t.const_data_ptr())), to(from + ((n - 1) * stride + width) * t.element_size()) {}
+  bool meets(const Span& o) const { return from < o.to && o.from < to; }
+};
+
+// The output of an op on bf16 rows t: given MX8Rows of its shape that meet none of the inputs, or new ones.
+bool mx8_out(PyObject* given, const at::Tensor& t, Mx8& m, std::initializer_list<Span> inputs) {
   if (t.size(-1) % 32 != 0) return false;
   if (given == Py_None) {
     m = new_mx8(t.sizes(), t.device());
     return true;
   }
-  return mx8_rows(given, m) && m.data.device() == t.device() && m.data.sizes() == t.sizes();
+  if (!mx8_rows(given, m) || m.data.device() != t.device() || m.data.sizes() != t.sizes()) return false;
+  const Span data(m.data, m.rows, m.width, m.stride), scales(m.scales, m.rows, m.width / 32, m.scale_stride);
+  for (const Span& s : inputs)
+    if (data.meets(s) || scales.meets(s)) return false;
+  return true;
 }
 
 // (x, weight, eps, residual, out)
@@ -807,14 +819,18 @@ PyObject* rmsnorm_mx8(PyObject*, PyObject* const* v, Py_ssize_t n) {
     if (!bf16(x) || !rows_of(*x, nrows, hidden, a.x_stride) || !on_current_device(*x) || !bf16(w) || !w->is_contiguous() ||
         w->numel() != hidden || w->device() != x->device() || !PyFloat_CheckExact(v[2]))
       return not_handled();
+    const Span xspan(*x, nrows, hidden, a.x_stride);
+    Span rspan = xspan;
     if (v[3] != Py_None) {
       const at::Tensor* r = tensor(v[3]);
       if (!bf16(r) || !rows_of(*r, r2, h2, a.residual_stride) || r->sizes() != x->sizes() || r->device() != x->device())
         return not_handled();
+      rspan = Span(*r, r2, h2, a.residual_stride);
+      if (rspan.meets(xspan) && (rspan.from != xspan.from || r->strides() != x->strides())) return not_handled();
       a.residual = ptr(*r);
     }
     Mx8 out;
-    if (!mx8_out(v[4], *x, out)) return not_handled();
+    if (!mx8_out(v[4], *x, out, {xspan, rspan, Span(*w, 1, hidden, 0)})) return not_handled();
     a.rows = static_cast<int32_t>(nrows);
     a.hidden = static_cast<int32_t>(hidden);
     a.eps = PyFloat_AS_DOUBLE(v[2]);
@@ -839,7 +855,7 @@ PyObject* silu_mul_mx8(PyObject*, PyObject* const* v, Py_ssize_t n) {
         u->device() != g->device() || !on_current_device(*g))
       return not_handled();
     Mx8 out;
-    if (!mx8_out(v[2], *g, out)) return not_handled();
+    if (!mx8_out(v[2], *g, out, {Span(*g, nrows, width, gs), Span(*u, r2, w2, us)})) return not_handled();
     const lkv_stream_t s = stream_of(*g);
     return issue_mx8("lkv_silu_mul_mx8", v[2], out, [&] {
       return g_lib.silu_mul_mx8(ptr(*g), gs, ptr(*u), us, ptr(out.data), out.stride, ptr(out.scales), out.scale_stride,
@@ -914,10 +930,7 @@ PyObject* mx4_linear(PyObject*, PyObject* const* v, Py_ssize_t n) {
         return not_handled();
       for (int64_t d = 0; d + 1 < x.dim(); ++d)
         if (o->size(d) != x.size(d)) return not_handled();
-      const uintptr_t xa = reinterpret_cast<uintptr_t>(x.const_data_ptr()), oa = reinterpret_cast<uintptr_t>(o->const_data_ptr());
-      const uintptr_t xe = xa + ((nrows - 1) * a.x_stride + width) * x.element_size();
-      const uintptr_t oe = oa + ((nrows - 1) * a.out_stride + w2) * 2;
-      if (xa < oe && oa < xe) return not_handled();  // (the Python path refuses an output over its input)
+      if (Span(x, nrows, width, a.x_stride).meets(Span(*o, nrows, w2, a.out_stride))) return not_handled();
       out = *o;
     } else {
       std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());

@@ -774,23 +774,27 @@ extern "C" int32_t lkv_mx4_linear(const lkv_mx4_linear_args* a, lkv_stream_t str
   LKV_REQUIRE(mx8 == (a->x_scales != nullptr), "x_scales belong to MX8 rows, and they need them");
   LKV_REQUIRE(((bits(a->x) | bits(a->weight)) & 15) == 0 && ((bits(a->out) | bits(a->bias)) & 1) == 0,
               "x and weight must be 16-byte aligned");
-  LKV_REQUIRE(a->x_stride % (mx8 ? 16 : 8) == 0, "x rows must be 16-byte aligned");
-  LKV_REQUIRE(a->x_stride >= 0 && a->x_stride <= (1 << 21), "x_stride must be at most 2^21 elements");
+  if (a->rows > 1) {  // (one row has no stride)
+    LKV_REQUIRE(a->x_stride % (mx8 ? 16 : 8) == 0, "x rows must be 16-byte aligned");
+    LKV_REQUIRE(a->x_stride >= 0 && a->x_stride <= (1 << 21), "x_stride must be at most 2^21 elements");
+    LKV_REQUIRE(!mx8 || (a->x_scale_stride >= 0 && a->x_scale_stride <= (1 << 21)), "x_scale_stride must be at most 2^21 bytes");
+    LKV_REQUIRE(a->out_stride >= a->out_features, "out rows must not overlap");
+  }
   if (a->rows == 0) return LKV_OK;
   LinearParams p;
   p.w = static_cast<const uint8_t*>(a->weight);
   p.x = a->x;
-  p.x_stride = a->x_stride;
+  p.x_stride = a->rows > 1 ? a->x_stride : 0;
   p.xs = static_cast<const uint8_t*>(a->x_scales);
-  p.xs_stride = a->x_scale_stride;
+  p.xs_stride = a->rows > 1 ? a->x_scale_stride : 0;
   p.bias = static_cast<const uint16_t*>(a->bias);
   p.out = static_cast<uint16_t*>(a->out);
-  p.out_stride = a->out_stride;
+  p.out_stride = a->rows > 1 ? a->out_stride : 0;
   p.M = a->rows;
   p.N = a->out_features;
   p.K = a->in_features;
   p.units = mx4_units(a->in_features);
   p.tile_stride = mx4_tile_stride(p.units);
-  p.vector_out = (bits(a->out) & 15) == 0 && a->out_stride % 8 == 0;
+  p.vector_out = (bits(a->out) & 15) == 0 && p.out_stride % 8 == 0;
   return mx8 ? launch<true>(p, as_stream(stream), a->kernel) : launch<false>(p, as_stream(stream), a->kernel);
 }

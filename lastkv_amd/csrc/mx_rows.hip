@@ -212,6 +212,9 @@ extern "C" int32_t lkv_rmsnorm_mx8(const lkv_rmsnorm_mx8_args* a, lkv_stream_t s
   LKV_REQUIRE(((bits(a->x) | bits(a->weight) | bits(a->residual)) & 15) == 0 && (bits(a->out) & 7) == 0,
               "rows must be 16-byte aligned (8-bit ones 8)");
   LKV_REQUIRE((a->x_stride | a->out_stride | a->residual_stride) % 8 == 0, "row strides must be multiples of 8 elements");
+  LKV_REQUIRE(a->rows <= 1 || (a->out_stride >= a->hidden && a->scale_stride >= a->hidden / kMxBlock &&
+                               (a->residual == nullptr || a->residual_stride >= a->hidden)),
+              "rows of residual, out and scales must not overlap");
   if (a->rows == 0) return LKV_OK;
   NormParams p;
   p.x = static_cast<const uint16_t*>(a->x);
@@ -241,6 +244,7 @@ extern "C" int32_t lkv_silu_mul_mx8(const void* gate, int64_t gate_stride, const
   LKV_REQUIRE(rows >= 0 && width > 0 && width % kMxBlock == 0, "width must be a positive multiple of 32");
   LKV_REQUIRE(((bits(gate) | bits(up)) & 15) == 0 && (bits(out) & 7) == 0, "rows must be 16-byte aligned (8-bit ones 8)");
   LKV_REQUIRE((gate_stride | up_stride | out_stride) % 8 == 0, "row strides must be multiples of 8 elements");
+  LKV_REQUIRE(rows <= 1 || (out_stride >= width && scale_stride >= width / kMxBlock), "rows of out and scales must not overlap");
   if (rows == 0) return LKV_OK;
   silu_mul_mx8_kernel<<<row_grid(rows, width), 256, 0, as_stream(stream)>>>(
       static_cast<const uint16_t*>(gate), gate_stride, static_cast<const uint16_t*>(up), up_stride,
@@ -255,6 +259,7 @@ extern "C" int32_t lkv_mx8_unpack(const void* data, int64_t data_stride, const v
   LKV_REQUIRE(rows >= 0 && width > 0 && width % kMxBlock == 0, "width must be a positive multiple of 32");
   LKV_REQUIRE((bits(out) & 15) == 0 && (bits(data) & 7) == 0, "rows must be 16-byte aligned (8-bit ones 8)");
   LKV_REQUIRE((data_stride | out_stride) % 8 == 0, "row strides must be multiples of 8 elements");
+  LKV_REQUIRE(rows <= 1 || out_stride >= width, "out rows must not overlap");
   if (rows == 0) return LKV_OK;
   mx8_unpack_kernel<<<row_grid(rows, width), 256, 0, as_stream(stream)>>>(
       static_cast<const uint8_t*>(data), data_stride, static_cast<const uint8_t*>(scales), scale_stride,

@@ -1097,6 +1097,7 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 def _mx8_strides(name: str, rows: MX8Rows) -> tuple[int, int, int, int]:
     """(rows, width, data row stride, scale row stride) of MX8 rows viewed as [rows, width]."""
 
+    rows.__post_init__()  # (its fields can be assigned)
     d, s = rows.data, rows.scales
     width = d.shape[-1]
     if d.dim() == 1:
@@ -1111,13 +1112,15 @@ def _mx8_strides(name: str, rows: MX8Rows) -> tuple[int, int, int, int]:
     return d2.shape[0], width, d2.stride(0), s2.stride(0)
 
 
-def _mx8_out(x: torch.Tensor, out: MX8Rows | None) -> MX8Rows:
+def _mx8_out(x: torch.Tensor, out: MX8Rows | None, *inputs: torch.Tensor | None) -> MX8Rows:
     _require(x.shape[-1] > 0 and x.shape[-1] % MX_BLOCK == 0, f"rows of 32-value blocks are needed, got a width of {x.shape[-1]}")
     if out is None:
         return MX8Rows.empty(x.shape, x.device)
     _require(isinstance(out, MX8Rows), "out must be MX8Rows")
     _require(out.shape == x.shape, "out shape must match x")
     _same_device(x.device, out=out.data)
+    for t in (x, *inputs):
+        _require(t is None or not (_overlap(out.data, t) or _overlap(out.scales, t)), "out must not overlap the inputs")
     return out
 
 
@@ -1126,7 +1129,8 @@ def rmsnorm_mx8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: 
     """``rmsnorm`` with an 8-bit output: the rows of ``x`` (bf16 ``[..., hidden]``, hidden a multiple of 32; with
     ``residual`` first ``residual += x`` in bf16, in place, and the sum) normalised and multiplied by ``weight``,
     each block of 32 rounded once, correctly, to e4m3 under the smallest power-of-two scale that holds its largest
-    value.  A block with an infinity or NaN is NaN.  Returns ``out``."""
+    value.  A block with an infinity or NaN is NaN.  Returns ``out``, which must not overlap the inputs; ``residual``
+    may be ``x`` itself."""
 
     if _host_bound or _bind_host():
         done = _host.rmsnorm_mx8(x, weight, eps, residual, out)
@@ -1134,13 +1138,15 @@ def rmsnorm_mx8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: 
             return done
     _require_bf16_cuda("x", x)
     _require(x.dim() >= 1, "x must have rows")
-    out = _mx8_out(x, out)
+    out = _mx8_out(x, out, weight, residual)
     _require_bf16_cuda("weight", weight)
     hidden = x.shape[-1]
     _require(weight.is_contiguous() and weight.numel() == hidden, "weight must be a contiguous bf16 [hidden] tensor")
     if residual is not None:
         _require_bf16_cuda("residual", residual)
         _require(residual.shape == x.shape, "residual shape must match x")
+        _require(not _overlap(residual, x) or (residual.data_ptr() == x.data_ptr() and residual.stride() == x.stride()),
+                 "residual must be x or not overlap it")
     _same_device(x.device, weight=weight, residual=residual)
     if x.numel() == 0:
         return out
@@ -1161,7 +1167,7 @@ def rmsnorm_mx8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: 
 
 def silu_mul_mx8(gate: torch.Tensor, up: torch.Tensor, out: MX8Rows | None = None) -> MX8Rows:
     """``F.silu(gate) * up`` of bf16 ``[..., width]`` tensors (width a multiple of 32) with an 8-bit output, each
-    block of 32 rounded once as ``rmsnorm_mx8`` rounds it."""
+    block of 32 rounded once as ``rmsnorm_mx8`` rounds it.  ``out`` must not overlap the inputs."""
 
     if _host_bound or _bind_host():
         done = _host.silu_mul_mx8(gate, up, out)
@@ -1171,7 +1177,7 @@ def silu_mul_mx8(gate: torch.Tensor, up: torch.Tensor, out: MX8Rows | None = Non
     _require_bf16_cuda("up", up)
     _require(gate.dim() >= 1 and up.shape == gate.shape, "up shape must match gate")
     _same_device(gate.device, up=up)
-    out = _mx8_out(gate, out)
+    out = _mx8_out(gate, out, up)
     if gate.numel() == 0:
         return out
     rows, width, gs = _rows2d("gate", gate)
@@ -1239,6 +1245,7 @@ def mx4_unpack(weight: MX4Weight) -> torch.Tensor:
     """The values of ``weight`` as bf16 ``[out_features, in_features]``."""
 
     _require(isinstance(weight, MX4Weight), "weight must be an MX4Weight")
+    weight.__post_init__()  # (its fields can be assigned)
     n, k = weight.out_features, weight.in_features
     out = torch.empty((n, k), dtype=torch.bfloat16, device=weight.device)
     with _on_device(out.device):
@@ -1252,13 +1259,15 @@ def mx4_linear(x: torch.Tensor | MX8Rows, weight: MX4Weight, bias: torch.Tensor 
     """``F.linear`` over a 4-bit weight: ``x`` is bf16 ``[..., in_features]`` or ``MX8Rows`` of that shape, ``bias``
     bf16 ``[out_features]``; returns bf16 ``[..., out_features]``: exact products, fp32 sums in a fixed order, rounded
     once.  In calls of many 8-bit rows the products are added eight columns at a time in the matrix instruction's fixed
-    point, which keeps 13 bits below the largest, before they are added in fp32.  ``out`` must not overlap ``x``."""
+    point, which keeps 13 bits below the largest, before they are added in fp32.  ``out`` must not reach into the memory from
+    ``x``'s first row to its last."""
 
     if _host_bound or _bind_host():
         done = _host.mx4_linear(x, weight, bias, out)
         if done is not None:
             return done
     _require(isinstance(weight, MX4Weight), "weight must be an MX4Weight")
+    weight.__post_init__()  # (its fields can be assigned)
     n, k = weight.out_features, weight.in_features
     mx8 = isinstance(x, MX8Rows)
     if not mx8:

@@ -382,6 +382,35 @@ def test_linear_strided_rows_and_untouched_neighbours(m, mx8, kernel):
         assert y.shape == (1, m, 70) and torch.equal(y[0], out[1:-1, 5:75])
 
 
+@pytest.mark.parametrize("mx8", [False, True])
+def test_one_row_of_any_stride(mx8, kernel):
+    """The first row of a matrix whose rows are not 16-byte multiples apart."""
+
+    g = _gen(12)
+    codes, scales = random_mx4(g, 40, 96)
+    if mx8:
+        whole = random_mx8(g, 3, 128)
+        data = torch.zeros((3, 101), device=DEV, dtype=torch.uint8).view(torch.float8_e4m3fn)
+        data[:1, :96].view(torch.uint8).copy_(whole.data[:1, :96].view(torch.uint8))
+        x = ops.MX8Rows(data[:1, :96], whole.scales[:1, :3])
+        values = mx8_values(ops.MX8Rows(whole.data[:1, :96].contiguous(), whole.scales[:1, :3].contiguous()))
+    else:
+        x = outliers(g, 3, 101)[:1, :96]
+        values = x.double()
+    check_linear(x, values, codes, scales, None)
+
+
+def test_norm_onto_its_own_residual():
+    """residual = x: the row is doubled in place, then normalised."""
+
+    g = _gen(13)
+    x, w = outliers(g, 9, 2080), (1 + 0.3 * torch.randn(2080, generator=g, device=DEV)).to(BF16)
+    want = (x.float() + x.float()).to(BF16)
+    y = norm_reference(x, w, 1e-5, x)
+    same_mx8(ops.rmsnorm_mx8(x, w, 1e-5, residual=x), y)
+    assert torch.equal(x, want)
+
+
 @pytest.mark.parametrize("m", [5, 200])
 def test_linear_past_the_rows_and_columns_reads_nothing_that_counts(m, kernel):
     """NaN beside the rows of x (the next columns of a wider tensor), and in every place of the columns' tile before, does

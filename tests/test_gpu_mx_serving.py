@@ -201,6 +201,9 @@ def test_refusals_on_the_gpu():
     x, w, n = _randn(1, 4, 64), _weight(2, 16, 64), _randn(3, 64)
     q = _rows8(4, 4, 64)
     wide = _randn(5, 4, 80)
+    over = ops.MX8Rows(x.view(torch.float8_e4m3fn)[:, 64:], _rows8(1, 4, 64).scales)  # x's own bytes
+    mixed, resized = _rows8(4, 4, 64), _weight(2, 16, 64)  # fields assigned later
+    mixed.scales, resized.out_features = mixed.scales[:, :1], 160
     cases = [
         (lambda: ops.rmsnorm_mx8(wide[:, :40], _randn(6, 40), 1e-5), "32-value"),
         (lambda: ops.rmsnorm_mx8(x, n[:32], 1e-5), "weight"),
@@ -209,6 +212,13 @@ def test_refusals_on_the_gpu():
         (lambda: ops.rmsnorm_mx8(x.float(), n, 1e-5), "bfloat16"),
         (lambda: ops.rmsnorm_mx8(_randn(7, 4, 128)[:, ::2], n, 1e-5), "contiguous"),
         (lambda: ops.silu_mul_mx8(x, x[:, :32]), "up shape"),
+        (lambda: ops.silu_mul_mx8(x, x, out=over), "overlap"),
+        (lambda: ops.rmsnorm_mx8(x, n, 1e-5, out=over), "overlap"),
+        (lambda: ops.rmsnorm_mx8(x[:3], n, 1e-5, residual=x[1:]), "overlap"),
+        (lambda: ops.mx8_unpack(mixed), "scales"),
+        (lambda: ops.mx4_linear(mixed, w), "scales"),
+        (lambda: ops.mx4_linear(x, resized), "bytes"),
+        (lambda: ops.mx4_unpack(resized), "bytes"),
         (lambda: ops.MX8Rows(q.data, q.scales[:, :1]), "scales"),
         (lambda: ops.MX8Rows(q.data.view(torch.uint8), q.scales), "float8_e4m3fn"),
         (lambda: ops.MX4Weight(w.data[:-1], 16, 64), "bytes"),
@@ -226,6 +236,8 @@ def test_refusals_on_the_gpu():
         with pytest.raises(ValueError, match=text):
             call()
     from lastkv_amd import _lib
+    with pytest.raises(_lib.LastKVNativeError, match="overlap"):
+        ops.mx4_linear(x, w, out=torch.zeros(16, device=DEV, dtype=BF16).expand(4, 16))
     odd = torch.zeros(4 * 64 + 4, device=DEV, dtype=BF16)[4:].view(4, 64)  # 8 bytes past a 16-byte border
     for call in (lambda: ops.rmsnorm_mx8(odd, n, 1e-5), lambda: ops.silu_mul_mx8(odd, odd), lambda: ops.mx4_linear(odd, w)):
         with pytest.raises(_lib.LastKVNativeError, match="aligned"):

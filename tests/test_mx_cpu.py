@@ -27,7 +27,10 @@ def _norm(**kw):
     (dict(struct_size=8), b"size mismatch"), (dict(rows=-1), b"rows"), (dict(hidden=40), b"multiple of 32"),
     (dict(hidden=0), b"multiple of 32"), (dict(hidden=16416), b"up to 16384"), (dict(x=None), b"null"),
     (dict(scales=None), b"null"), (dict(x=24), b"aligned"), (dict(residual=8), b"aligned"), (dict(out=20), b"aligned"),
-    (dict(x_stride=12), b"multiples of 8"), (dict(out_stride=4), b"multiples of 8")])
+    (dict(x_stride=12), b"multiples of 8"), (dict(out_stride=4), b"multiples of 8"),
+    (dict(rows=2, x_stride=64, out_stride=56, scale_stride=2), b"overlap"),
+    (dict(rows=2, x_stride=64, out_stride=64, scale_stride=1), b"overlap"),
+    (dict(rows=2, x_stride=64, out_stride=64, scale_stride=2, residual=16), b"overlap")])
 def test_norm_refusals(kw, message):
     st, text = _norm(**kw)
     assert st == 1 and message in text, text
@@ -52,8 +55,10 @@ def _linear(**kw):
     (dict(in_features=48), b"multiple of 32"), (dict(in_features=0), b"multiple of 32"), (dict(out_features=0), b"1 to 2^24"),
     (dict(in_features=(1 << 20) + 32), b"up to 2^20"), (dict(x_format=2), b"x_format"), (dict(kernel=3), b"kernel"), (dict(x=None), b"null"),
     (dict(weight=None), b"null"), (dict(out=None), b"null"), (dict(x_format=1), b"x_scales"), (dict(x_scales=16), b"x_scales"),
-    (dict(x=24), b"aligned"), (dict(weight=8), b"aligned"), (dict(x_stride=68), b"aligned"),
-    (dict(x_format=1, x_scales=16, x_stride=72), b"aligned"), (dict(x_stride=1 << 24), b"2^21"), (dict(x_stride=-8), b"2^21")])
+    (dict(x=24), b"aligned"), (dict(weight=8), b"aligned"), (dict(rows=2, x_stride=68), b"aligned"),
+    (dict(rows=2, x_format=1, x_scales=16, x_stride=72), b"aligned"), (dict(rows=2, x_stride=1 << 24), b"2^21"), (dict(rows=2, x_stride=-8), b"2^21"),
+    (dict(rows=2, x_format=1, x_scales=16, x_scale_stride=1 << 32), b"x_scale_stride"),
+    (dict(rows=2, x_format=1, x_scales=16, x_scale_stride=-1), b"x_scale_stride"), (dict(rows=2, out_stride=15), b"overlap")])
 def test_linear_refusals(kw, message):
     st, text = _linear(**kw)
     assert st == 1 and message in text, text
@@ -67,6 +72,8 @@ def test_other_refusals_and_sizes():
     lib = _lib.load()
     assert lib.lkv_silu_mul_mx8(16, 64, 16, 64, 16, 64, 16, 2, 1, 40, None) == 1 and b"multiple of 32" in lib.lkv_last_error()
     assert lib.lkv_silu_mul_mx8(16, 64, 24, 64, 16, 64, 16, 2, 1, 64, None) == 1 and b"aligned" in lib.lkv_last_error()
+    assert lib.lkv_silu_mul_mx8(16, 64, 16, 64, 16, 0, 16, 2, 2, 64, None) == 1 and b"overlap" in lib.lkv_last_error()
+    assert lib.lkv_mx8_unpack(16, 64, 16, 2, 16, 0, 2, 64, None) == 1 and b"overlap" in lib.lkv_last_error()
     assert lib.lkv_mx8_unpack(16, 64, None, 2, 16, 64, 1, 64, None) == 1 and b"null" in lib.lkv_last_error()
     assert lib.lkv_mx8_unpack(16, 60, 16, 2, 16, 64, 1, 64, None) == 1 and b"multiples of 8" in lib.lkv_last_error()
     for call in (lambda: lib.lkv_mx4_pack(16, 32, 16, 2, 16, 40, 16, None), lambda: lib.lkv_mx4_quantize(16, 64, 0, 64, 16, None),
