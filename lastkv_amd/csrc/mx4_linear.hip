@@ -598,9 +598,9 @@ int32_t launch(const LinearParams& p, hipStream_t s, int kernel) {
         launch_tile<true, 2, 2, 8, 4, 2>(p, s);
     } else {
       if (small <= 3 * cus)
-        launch_tile<false, 2, 2, 4, 2, 2>(p, s);
+        launch_tile<false, 4, 1, 2, 4, 2>(p, s);
       else
-        launch_tile<false, 2, 2, 4, 4, 2>(p, s);
+        launch_tile<false, 4, 1, 4, 4, 2>(p, s);
     }
   } else if (p.M <= 16) {
     launch_mt<kMx8, 1>(p, s);
