@@ -81,6 +81,22 @@ __device__ inline void read_mx8(uint32_t w, uint32_t lo, uint32_t hi, uint4 (&c)
 __device__ inline int swizzle4(int r) { return (r & 3) | ((r & 8) != 0 ? 12 : 0); }
 __device__ inline int swizzle2(int r) { return ((r >> 1) & 1) | ((r >> 1) & 4); }
 
+// Likewise the fragments of 4 tiles of bf16 rows, from where their four steps' chunks start.
+template <int kXStep>
+__device__ inline void read_bf16(const uint32_t (&x)[4], uint4 (&b)[4][4]) {
+  asm volatile(
+      "ds_read_b128 %0, %16\n ds_read_b128 %1, %16 offset:%c20\n ds_read_b128 %2, %16 offset:%c21\n ds_read_b128 %3, %16 offset:%c22\n"
+      "ds_read_b128 %4, %17\n ds_read_b128 %5, %17 offset:%c20\n ds_read_b128 %6, %17 offset:%c21\n ds_read_b128 %7, %17 offset:%c22\n"
+      "ds_read_b128 %8, %18\n ds_read_b128 %9, %18 offset:%c20\n ds_read_b128 %10, %18 offset:%c21\n ds_read_b128 %11, %18 offset:%c22\n"
+      "ds_read_b128 %12, %19\n ds_read_b128 %13, %19 offset:%c20\n ds_read_b128 %14, %19 offset:%c21\n"
+      "ds_read_b128 %15, %19 offset:%c22\n s_waitcnt lgkmcnt(0)"
+      : "=&v"(b[0][0]), "=&v"(b[0][1]), "=&v"(b[0][2]), "=&v"(b[0][3]), "=&v"(b[1][0]), "=&v"(b[1][1]), "=&v"(b[1][2]),
+        "=&v"(b[1][3]), "=&v"(b[2][0]), "=&v"(b[2][1]), "=&v"(b[2][2]), "=&v"(b[2][3]), "=&v"(b[3][0]), "=&v"(b[3][1]),
+        "=&v"(b[3][2]), "=&v"(b[3][3])
+      : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "n"(kXStep), "n"(2 * kXStep), "n"(3 * kXStep)
+      : "memory");
+}
+
 // All loads of the wave but the last kLeft have arrived (those to LDS too).
 template <int kLeft>
 __device__ inline void wait_and_sync() {
@@ -295,23 +311,26 @@ __global__ __launch_bounds__(kWaves * 64, MT == 1 && NT == 1 ? 4 : 2) void mx4_r
 }
 
 // Many rows: one workgroup of WN x WM waves per (16 WN TN rows of the weight, 16 WM TM rows of x), each wave TN x TM
-// tiles of 16 x 16.  Tiles of 128 columns of both go to LDS by direct loads, kBufs buffers in turn, one barrier a tile; two
+// tiles of 16 x 16.  Tiles of 128 columns go to LDS by direct loads, kBufs buffers in turn, one barrier a tile; two
 // or three workgroups share a CU where there are that many, so that one's products cover the other's reads of LDS.
 // MX8 rows: both operands and both scales go to the scaled matrix instruction as they are (a code is converted nowhere).
 // Bound by the matrix pipe, of which 4096 rows of 28672 x 4096 reach 2.57 PFLOP/s (375 us; bf16 weights in the library's
 // GEMM 641 us); independent products in registers reach 3.83 PFLOP/s on this card, this loop without its loads 3.4.  With
 // the tile staged through registers the same took 30-50 us more, with the outputs stored from registers 28.
-// bf16 rows: the codes are converted in registers as they are used.  1000 rows of 6144 x 4096 take 46 us, 1.09 PFLOP/s,
-// 4096 rows 160 us, 1.29 PFLOP/s (library, bf16 weights, 1000 rows: 52 us); bf16 products in registers reach 1.92 PFLOP/s.
+// bf16 rows: the codes are converted in registers as they are used, by waves side by side over the weight (WM = 1), so that
+// each is converted once and goes to its wave's registers only.  1000 rows of 6144 x 4096 take 43-45 us, 1.15 PFLOP/s, 4096 rows
+// 151 us, 1.36 PFLOP/s (library, bf16 weights, 1000 rows: 52 us); bf16 products in registers reach 1.92 PFLOP/s.
 template <bool kMx8, int WN, int WM, int TN, int TM, int kBufs>
 __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearParams p, int mtiles, int grid) {
   constexpr int kThreads = WN * WM * 64, kBN = WN * TN, kBM = WM * TM;  // (in tiles of 16)
   constexpr int kRowBytes = kMx8 ? 128 : 256, kChunks = kRowBytes / 16;
-  constexpr int kXBytes = kBM * 16 * kRowBytes, kWBytes = kBN * kMxTileBytes;
+  constexpr bool kOwnCodes = WM == 1;  // a wave's codes are no other's: to registers, the next tile's during the products
+  constexpr int kXBytes = kBM * 16 * kRowBytes, kWBytes = kOwnCodes ? 0 : kBN * kMxTileBytes;
   constexpr int kBuf = kXBytes + kWBytes;
-  constexpr int kXLoads = kBM * 16 * kChunks / kThreads, kWLoads = kBN * 64 / kThreads;
+  constexpr int kXLoads = kBM * 16 * kChunks / kThreads, kWLoads = kOwnCodes ? TN : kBN * 64 / kThreads;
   constexpr int kLoads = kXLoads + kWLoads;  // of a tile
-  static_assert(kBufs == 2 || (kMx8 && TN == 4 && TM == 2), "the tiles of read_mx8");
+  static_assert(!kOwnCodes || 4 % (kBufs - 1) == 0, "tile t of a unit has its codes in place t % (kBufs - 1)");
+  static_assert(kBufs == 2 || (kMx8 ? TN == 4 && TM == 2 : kOwnCodes && TM == 4), "the tiles of read_mx8 and read_bf16");
   constexpr int kOutRow = kBN * 32 + 16;  // bytes of an output row in LDS; the 16 spread the rows over the banks
   __shared__ __attribute__((aligned(16))) char smem[std::max(kBufs * kBuf, kBM * 16 * kOutRow)];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -342,11 +361,18 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
 #pragma unroll
   for (int j = 0; j < kXLoads; ++j)
     xoff[j] = xrow + j * kRowStep < valid ? (xrow + j * kRowStep) * stride + xcol : kOutside;
-  auto load = [&](int kt, char* buf) {
+  uint4 codes[kBufs - 1][TN];  // of the next tiles
+  auto load = [&](int kt, char* buf, int slot) {
     const bool in = xcol < row_bytes - kt * kRowBytes;
 #pragma unroll
     for (int j = 0; j < kXLoads; ++j)
       buffer_to_lds16(xb, buf + wave * 1024 + j * kThreads * 16, in ? xoff[j] : kOutside, kt * kRowBytes);
+    if constexpr (kOwnCodes) {
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+        codes[slot][i] = buffer_load16(wb, lane * 16, (wn * TN + i) * tile_stride + (kt >> 2) * kMxUnitBytes + (kt & 3) * kMxTileBytes);
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < kWLoads; ++j)
       buffer_to_lds16(wb, buf + kXBytes + wave * 1024 + j * kThreads * 16, lane * 16,
@@ -414,13 +440,16 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
     auto start_loads = [&] {
       __builtin_amdgcn_sched_barrier(0);
       if (t == 0) load_scales(min((kt >> 2) + 1, p.units - 1));
-      load(min(kt + kBufs - 1, tiles - 1), after(now, kBufs - 1));
+      load(min(kt + kBufs - 1, tiles - 1), after(now, kBufs - 1), t % (kBufs - 1));
       __builtin_amdgcn_sched_barrier(0);
     };
     const char* x = now + wm * TM * 16 * kRowBytes;
     const uint4* w = reinterpret_cast<const uint4*>(now + kXBytes + wn * TN * kMxTileBytes) + lane;
     uint4 c[TN];
-    if constexpr (kBufs == 2) {
+    if constexpr (kOwnCodes) {
+#pragma unroll
+      for (int i = 0; i < TN; ++i) c[i] = codes[t % (kBufs - 1)][i];
+    } else if constexpr (kBufs == 2) {
 #pragma unroll
       for (int i = 0; i < TN; ++i) c[i] = w[i * 64];
     }
@@ -452,11 +481,18 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
       }
     } else {
       uint4 b[4][TM];
+      const char* at[4];
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
+      for (int s = 0; s < 4; ++s) at[s] = x + r * kRowBytes + (((4 * g + s) ^ swizzle4(r)) * 16);
+      if constexpr (kBufs > 2) {
+        const uint32_t xa[4] = {lds_address(at[0]), lds_address(at[1]), lds_address(at[2]), lds_address(at[3])};
+        read_bf16<16 * kRowBytes>(xa, b);
+      } else {
 #pragma unroll
-        for (int j = 0; j < TM; ++j)
-          b[s][j] = *reinterpret_cast<const uint4*>(x + (16 * j + r) * kRowBytes + (((4 * g + s) ^ swizzle4(r)) * 16));
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+          for (int j = 0; j < TM; ++j) b[s][j] = *reinterpret_cast<const uint4*>(at[s] + j * 16 * kRowBytes);
+      }
       start_loads();
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
@@ -479,7 +515,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
   };
   load_scales(0);
 #pragma unroll
-  for (int i = 0; i + 1 < kBufs; ++i) load(min(i, tiles - 1), smem + i * kBuf);
+  for (int i = 0; i + 1 < kBufs; ++i) load(min(i, tiles - 1), smem + i * kBuf, i);
   wait_and_sync<0>();
   // (the four tiles of a unit without branches, so that the compiler can count the loads since the unit's scale words and
   // waits for those alone)
@@ -491,8 +527,9 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
   }
   if (full < p.units) {
     next_unit();
-#pragma unroll 1
-    for (int t = 0; t < (tiles & 3); ++t) step(4 * full, t);
+#pragma unroll
+    for (int t = 0; t < 3; ++t)
+      if (t < (tiles & 3)) step(4 * full, t);
   }
   if constexpr (kBufs > 2) wait_and_sync<0>();  // (the loads past the last tile still write the buffers)
   // The outputs go through LDS into whole rows: a lane's four stand 32 bytes wide in 16 rows, which HBM takes at 2 TB/s
@@ -569,25 +606,28 @@ void launch_tile(const LinearParams& p, hipStream_t s) {
   mx4_tile_kernel<kMx8, WN, WM, TN, TM, kBufs><<<grid, WN * WM * 64, 0, s>>>(p, mtiles, grid);
 }
 
-// The tile kernel where the row kernel would give each CU more than 16 tiles of 16 weight rows x 32 rows of x, for MX8 rows
+// The tile kernel where the row kernel would give each CU more than 8 tiles of 16 weight rows x 32 rows of x, for MX8 rows
 // more than 4: a round of tiles takes as long whether it fills its CUs or not (us, row kernel against tiles.  bf16 rows:
-// 6144 x 4096 for 256 rows, 12 tiles a CU, 25.3 against 29.5; 28672 x 4096 for 64 rows, 14, 29.0 against 32.7; for 96 rows,
-// 21, 48.9 against 32.9.  MX8 rows: 4096 x 14336 for 128 rows, 4, 25.3 against 46; 2387 x 11744 for 201, 4.1, 48 against 37;
-// 6144 x 4096 for 128, 6, 15.5 against 16.7; 28672 x 4096 for 32, 7, 19.3 against 18.3; 4096 x 14336 for 256, 8, 43.5
-// against 46.6; 14336 x 4096 for 96, 10.5, 27.4 against 16.1).  At any width the row kernel, which HBM bounds, for up to 32
-// bf16 rows (128256 x 4096: 62 against 97) and up to 16 MX8 rows, whose products it takes exactly.
+// 4096 x 14336 for 256 rows, 8 tiles a CU, 44.8 against 68.6; 6968 x 2592 for 143, 8.5, 21.1 against 15.4; 14336 x 4096 for 96,
+// 10.5, 27.0 against 23.2; 6144 x 4096 for 256, 12, 25.1 against 22.9; 28672 x 4096 for 64, 14, 29.0 against 24.2.  MX8 rows:
+// 4096 x 14336 for 128 rows, 4, 25.3 against 46; 2387 x 11744 for 201, 4.1, 48 against 37; 6144 x 4096 for 128, 6, 15.5
+// against 16.7; 28672 x 4096 for 32, 7, 19.3 against 18.3; 14336 x 4096 for 96, 10.5, 27.4 against 16.1).  At any width the
+// row kernel, which HBM bounds, for up to 32 bf16 rows (128256 x 4096: 62 against 97) and up to 16 MX8 rows, whose products it
+// takes exactly.
 // Large tiles where 128 x 64 ones would be more than three a CU (us, MX8 rows: 28672 x 4096 for 4096 rows 375 with
-// 256 x 128, 459 with 128 x 128; 6144 x 4096 for 1000 rows, three a CU, 37.7 against 32.6 with 128 x 64.  bf16 rows, which
-// need twice the LDS, 128 x 128: 28672 x 4096 for 4096 rows 722, 1009 with 256 x 128; 256 rows, 3.5 a CU, 53 against 63 with
-// 128 x 64; 6144 x 4096 for 1000 rows 49.5 against 47.8, 4096 x 14336, two a CU, 123 against 105).
+// 256 x 128, 459 with 128 x 128; 6144 x 4096 for 1000 rows, three a CU, 37.7 against 32.6 with 128 x 64.  bf16 rows: 28672 x
+// 4096 for 4096 rows 690 with 256 x 64, 722 with 128 x 128; for 256 rows, 3.5 a CU, 52 against 61 with 128 x 64; 4096 x 14336 for
+// 1000 rows, two a CU, 110 against 101).
 // Small MX8 tiles take four buffers while that leaves a CU its two workgroups, as few of them wait for memory most of the
 // time, and three for the third (us, two / three / four buffers: 4096 x 14336 for 256 rows, one for two CUs, 84 / 53 / 46;
-// for 1000 rows, two a CU, 85 / 71 / 67; 6144 x 4096 for 1000, three a CU, 31.9 / 32.6 / 36.3).
+// for 1000 rows, two a CU, 85 / 71 / 67; 6144 x 4096 for 1000, three a CU, 31.9 / 32.6 / 36.3).  bf16: three (two / three /
+// five: 4096 x 14336 for 256 rows 93 / 68 / 73; for 1000, 101 / 101 / 110), large tiles two (28672 x 4096 for 4096 rows, two /
+// three, 690 / 709).
 template <bool kMx8>
 int32_t launch(const LinearParams& p, hipStream_t s, int kernel) {
   const int64_t cus = std::max(1, device_cu_count());
   const int64_t work = static_cast<int64_t>((p.N + 15) / 16) * ((p.M + 31) / 32);
-  if (kernel == LKV_MX4_TILES || (kernel == LKV_MX4_AUTO && p.M > (kMx8 ? 16 : 32) && work > (kMx8 ? 4 : 16) * cus)) {
+  if (kernel == LKV_MX4_TILES || (kernel == LKV_MX4_AUTO && p.M > (kMx8 ? 16 : 32) && work > (kMx8 ? 4 : 8) * cus)) {
     const int64_t small = static_cast<int64_t>((p.N + 127) / 128) * ((p.M + 63) / 64);  // tiles of 128 x 64
     if constexpr (kMx8) {
       if (small <= 2 * cus)
@@ -598,7 +638,7 @@ int32_t launch(const LinearParams& p, hipStream_t s, int kernel) {
         launch_tile<true, 2, 2, 8, 4, 2>(p, s);
     } else {
       if (small <= 3 * cus)
-        launch_tile<false, 4, 1, 2, 4, 2>(p, s);
+        launch_tile<false, 4, 1, 2, 4, 3>(p, s);
       else
         launch_tile<false, 4, 1, 4, 4, 2>(p, s);
     }

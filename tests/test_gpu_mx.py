@@ -309,7 +309,7 @@ def test_mx8_products_that_cancel(m, kernel):
 
 
 @pytest.mark.parametrize("m,n,mx8", [(96, 28672, False), (96, 28672, True), (1000, 6144, True), (1000, 6144, False),
-                                     (64, 28672, False), (16, 28672, True), (17, 28672, True)])
+                                     (64, 28672, False), (32, 28672, False), (16, 28672, True), (17, 28672, True)])
 def test_linear_kernels_chosen_by_size(m, n, mx8):
     """Without a fixed kernel the call equals the one whose sizes choose it."""
 
@@ -319,7 +319,7 @@ def test_linear_kernels_chosen_by_size(m, n, mx8):
     a = _lib.Mx4LinearArgs()
     out = torch.empty((m, n), device=DEV, dtype=BF16)
     a.struct_size, a.rows, a.out_features, a.in_features = ctypes.sizeof(a), m, n, 256
-    a.kernel = TILES if m > (16 if mx8 else 64) else ROWS
+    a.kernel = TILES if m > (16 if mx8 else 32) else ROWS
     data = x.data if mx8 else x
     a.x, a.x_stride, a.x_format = data.data_ptr(), 256, int(mx8)
     if mx8:
