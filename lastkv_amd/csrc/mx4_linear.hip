@@ -74,13 +74,6 @@ __device__ inline void read_mx8(uint32_t w, uint32_t lo, uint32_t hi, uint4 (&c)
       : "memory");
 }
 
-// Where the 16-byte chunks of row r of a tile of x stand in LDS: chunk c at c ^ this.  One LDS read of 16 bytes serves 16
-// lanes at a time, rows 0-3 and 12-15 of one block of columns with rows 4-11 of the next one's (counted: with r & 7 those
-// meet half of the banks twice, except where the lanes take neighbouring chunks of 128-byte rows), which then lie apart:
-// 256-byte rows, blocks 4 chunks apart; 128-byte rows, blocks 2 apart.
-__device__ inline int swizzle4(int r) { return (r & 3) | ((r & 8) != 0 ? 12 : 0); }
-__device__ inline int swizzle2(int r) { return ((r >> 1) & 1) | ((r >> 1) & 4); }
-
 // Likewise the fragments of 4 tiles of bf16 rows, from where their four steps' chunks start.
 template <int kXStep>
 __device__ inline void read_bf16(const uint32_t (&x)[4], uint4 (&b)[4][4]) {
@@ -96,6 +89,13 @@ __device__ inline void read_bf16(const uint32_t (&x)[4], uint4 (&b)[4][4]) {
       : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "n"(kXStep), "n"(2 * kXStep), "n"(3 * kXStep)
       : "memory");
 }
+
+// Where the 16-byte chunks of row r of a tile of x stand in LDS: chunk c at c ^ this.  One LDS read of 16 bytes serves 16
+// lanes at a time, rows 0-3 and 12-15 of one block of columns with rows 4-11 of the next one's (counted: with r & 7 those
+// meet half of the banks twice, except where the lanes take neighbouring chunks of 128-byte rows), which then lie apart:
+// 256-byte rows, blocks 4 chunks apart; 128-byte rows, blocks 2 apart.
+__device__ inline int swizzle4(int r) { return (r & 3) | ((r & 8) != 0 ? 12 : 0); }
+__device__ inline int swizzle2(int r) { return ((r >> 1) & 1) | ((r >> 1) & 4); }
 
 // All loads of the wave but the last kLeft have arrived (those to LDS too).
 template <int kLeft>

@@ -383,6 +383,52 @@ def test_linear_strided_rows_and_untouched_neighbours(m, mx8, kernel):
 
 
 @pytest.mark.parametrize("mx8", [False, True])
+@pytest.mark.parametrize("m,n,k", [(70001, 24, 64), (3, 40, 131104), (70, 17, 65568)])
+def test_linear_many_rows_and_long_ones(m, n, k, mx8, kernel):
+    g = _gen(m + k)
+    codes, scales = random_mx4(g, n, k)
+    x = random_mx8(g, m, k) if mx8 else outliers(g, m, k)
+    check_linear(x, mx8_values(x) if mx8 else x.double(), codes, scales, None)
+
+
+def test_offsets_past_32_bits(kernel):
+    """Outputs and rows past 2^31 elements: the last rows are what they are by themselves."""
+
+    g = _gen(15)
+    codes, scales = random_mx4(g, 2064, 32)
+    w = ops.mx4_pack(codes, scales)
+    x = torch.randn((1 << 20, 32), generator=g, device=DEV).to(BF16)
+    assert torch.equal(ops.mx4_linear(x, w)[-100:], ops.mx4_linear(x[-100:].clone(), w))
+    q = ops.silu_mul_mx8(x, x)
+    assert torch.equal(ops.mx4_linear(q, w)[-100:], ops.mx4_linear(ops.MX8Rows(q.data[-100:], q.scales[-100:]), w))
+    n = torch.ones(4096, device=DEV, dtype=BF16)
+    big = torch.randn((1 << 10, 4096), generator=g, device=DEV).to(BF16).repeat(530, 1)  # 2^31 and 50 million
+    for op in (lambda t: ops.rmsnorm_mx8(t, n, 1e-5), lambda t: ops.silu_mul_mx8(t, t)):
+        q = op(big)
+        few = op(big[-100:].clone())
+        assert torch.equal(q.scales[-100:], few.scales)
+        assert torch.equal(q.data[-100:].view(torch.uint8), few.data.view(torch.uint8))
+        assert torch.equal(ops.mx8_unpack(q)[-100:], ops.mx8_unpack(few))
+        del q
+
+
+@pytest.mark.parametrize("mx8", [False, True])
+@pytest.mark.parametrize("m", [1, 20, 200])
+def test_linear_nan_block_of_the_weight(m, mx8, kernel):
+    """Scale byte 255 in one block: NaN in that output feature, the others as without it."""
+
+    g = _gen(14)
+    codes, scales = random_mx4(g, 40, 672)
+    x = random_mx8(g, m, 672) if mx8 else outliers(g, m, 672)
+    want = ops.mx4_linear(x, ops.mx4_pack(codes, scales))
+    scales[13, 20] = 255
+    got = ops.mx4_linear(x, ops.mx4_pack(codes, scales))
+    assert torch.isnan(got[:, 13]).all()
+    got[:, 13] = want[:, 13]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("mx8", [False, True])
 def test_one_row_of_any_stride(mx8, kernel):
     """The first row of a matrix whose rows are not 16-byte multiples apart."""
 
