@@ -67,10 +67,10 @@ __device__ inline void read_mx8(uint32_t w, uint32_t lo, uint32_t hi, uint4 (&c)
   asm volatile(
       "ds_read_b128 %0, %8\n ds_read_b128 %4, %9\n ds_read_b128 %6, %10\n"
       "ds_read_b128 %5, %9 offset:%c11\n ds_read_b128 %7, %10 offset:%c11\n"
-      "ds_read_b128 %1, %8 offset:1024\n ds_read_b128 %2, %8 offset:2048\n ds_read_b128 %3, %8 offset:3072\n"
+      "ds_read_b128 %1, %8 offset:%c12\n ds_read_b128 %2, %8 offset:%c13\n ds_read_b128 %3, %8 offset:%c14\n"
       "s_waitcnt lgkmcnt(0)"
       : "=&v"(c[0]), "=&v"(c[1]), "=&v"(c[2]), "=&v"(c[3]), "=&v"(l[0]), "=&v"(l[1]), "=&v"(h[0]), "=&v"(h[1])
-      : "v"(w), "v"(lo), "v"(hi), "n"(kXStep)
+      : "v"(w), "v"(lo), "v"(hi), "n"(kXStep), "n"(kMxTileBytes), "n"(2 * kMxTileBytes), "n"(3 * kMxTileBytes)
       : "memory");
 }
 
@@ -140,9 +140,9 @@ struct Step {
 // Bound by HBM: the weight's 4.25 bits a value, read once for up to 32 rows of x, converted in registers (one instruction
 // for two values) for bf16 matrix instructions; MX8 rows are converted too (exact products; the scaled matrix instruction
 // would save 64 conversions per 2,048 weights of a wave, not time).  The loads of two steps are in flight.
-// us per call with cold weights, bf16 / MX8 rows, beside a plain read of the same bytes: 28672 x 4096 for 1 row 15.3 / 15.0
-// (read 12.3), for 32 20.0 / 20.2; 4096 x 14336 for 1 row 11.2 / 10.6 (read 6.6-8.7), for 32 16.8 / 14.2; 4096 x 4096 for 1 row
-// 4.9 / 4.7 (read 3.5), for 32 6.8 / 6.1; bf16 weights in the library's GEMM: 28672 x 4096 for 32 rows 48.8, 4096 x 4096 13.8.
+// us per call with cold weights, bf16 / MX8 rows, beside a plain read of the same bytes: 28672 x 4096 for 1 row 15.4 / 14.9
+// (read 12.3), for 32 19.0 / 18.5; 4096 x 14336 for 1 row 11.0 / 10.8 (read 6.6-8.7), for 32 16.8 / 14.2; 4096 x 4096 for 1 row
+// 4.8 / 4.8 (read 3.5), for 32 6.7 / 6.1; bf16 weights in the library's GEMM: 28672 x 4096 for 32 rows 48.8, 4096 x 4096 13.8.
 // The matrix instruction wants a different row of x in neighbouring lanes, which the L1 would serve 16 bytes a cycle:
 // rows are loaded along their columns (64 bytes a cycle) and turned in a wave's own corner of LDS, its 16-byte chunks
 // swizzled by the row so that neither side meets a bank twice (4096 x 4096 for 32 rows
