@@ -45,7 +45,8 @@ __device__ inline uint4 pack8(const float (&f)[8]) {
 // residual := bf16(residual + x) first.  y = w * (row * r), r = 1 / sqrt(sum(row^2) / hidden + eps) with the sum and r in 64
 // bits (no order of the sum then shows in a row's output, and no row's squares leave the range).
 // Bound by HBM: every load is issued before the first use, with no branch between them (a chunk past the row rereads the
-// last one); x and the residual are read once and take non-temporal accesses, as in lkv_rmsnorm.
+// last one); x and the residual are read once and take non-temporal accesses, as in lkv_rmsnorm.  4096 rows of 4096 with a
+// residual: 21.7 us, 5.4 TB/s (lkv_rmsnorm, bf16 out, 22.7; the outputs all in 64 bits 32); one row 3.0.
 template <bool kAdd, int kChunks>
 __global__ __launch_bounds__(kThreads) void rmsnorm_mx8_kernel(const NormParams p) {
   __shared__ double part[kThreads / 64];
@@ -121,7 +122,8 @@ __device__ inline float silu(float g) {
   return g * __builtin_fmaf(__builtin_fmaf(-d, r, 1.f), r, r);
 }
 
-// y = silu(gate) * up; grid (column groups, rows), one 8-element chunk per thread.
+// y = silu(gate) * up; grid (column groups, rows), one 8-element chunk per thread.  Bound by HBM: 4096 rows of 14336 in
+// 50.5 us, 5.9 TB/s (lkv_silu_mul, bf16 out, 52.4; in 64 bits 138); 32 rows 4.3.
 __global__ __launch_bounds__(256) void silu_mul_mx8_kernel(const uint16_t* gate, int64_t g_stride, const uint16_t* up,
                                                            int64_t u_stride, uint8_t* out, int64_t o_stride,
                                                            uint8_t* scales, int64_t s_stride, int32_t rows,
@@ -152,7 +154,8 @@ __global__ __launch_bounds__(256) void silu_mul_mx8_kernel(const uint16_t* gate,
   }
 }
 
-// bf16(e4m3 * 2^(e - 127)), 8 values per thread.  (An output below bf16's normal range rounds, one above it is infinite.)
+// bf16(e4m3 * 2^(e - 127)), 8 values per thread: HBM, 4096 rows of 14336 in 26.8 us, 6.6 TB/s.  (An output below bf16's
+// normal range rounds, one above it is infinite.)
 __global__ __launch_bounds__(256) void mx8_unpack_kernel(const uint8_t* data, int64_t d_stride, const uint8_t* scales,
                                                          int64_t s_stride, uint16_t* out, int64_t o_stride, int32_t rows,
                                                          int32_t width) {
