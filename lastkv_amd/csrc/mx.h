@@ -3,28 +3,13 @@
 //   Scales are e8m0 bytes: byte e stands for 2^(e - 127), 255 for NaN (then the whole block is NaN).
 // A block's scale is the smallest power of two with amax <= top * scale (top: 448 of e4m3, 6 of e2m1), so
 // that no value saturates; its values are rounded to nearest even.
-//
-// MX4 weight layout: 16 rows (output features) x 512 columns form one 4352-byte unit, units ordered
-// [row tile][column unit]; in a unit, 4 tiles of 128 columns of 1024 bytes each, lane l = (row r = l & 15, g = l >> 4)
-// holding 16 bytes at l * 16: the 32 codes of columns 32 g .. 32 g + 31 of the tile (the even one low), one scale
-// block; then 64 words, word l byte t the scale of lane l's block of tile t.  So a wave's operand of a 16 x 128 tile
-// is one contiguous 1 KiB load, both for the scaled 8-bit matrix instruction (lane (r, g) takes columns 32 g ..)
-// and for bf16 ones (step j takes column 32 g + 8 j + i of every g: any order serves that both operands share).
-// Rows and columns past the matrix hold zeros.
 #pragma once
 #include "common.h"
+#include "mx_layout.h"
 
 namespace lkv {
 
 constexpr int kMxBlock = 32;
-constexpr int kMxUnitCols = 512;
-constexpr int kMxTileBytes = 1024;
-constexpr int kMxUnitBytes = 4 * kMxTileBytes + 256;
-
-__host__ __device__ inline int mx4_units(int32_t cols) { return (cols + kMxUnitCols - 1) / kMxUnitCols; }
-
-// Bytes from one row tile to the next: an odd number of 256-byte pieces.
-__host__ __device__ inline int mx4_tile_stride(int units) { return ((units * (kMxUnitBytes / 256)) | 1) * 256; }
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 

@@ -348,9 +348,15 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
   const __amdgpu_buffer_rsrc_t xb = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<char*>(static_cast<const char*>(p.x) + static_cast<int64_t>(m0) * stride), 0,
       (valid - 1) * stride + row_bytes, 0x00020000);
-  const int tile_stride = p.tile_stride;
+  const int wtiles = min(kBN, ntiles - nt0);
   const __amdgpu_buffer_rsrc_t wb = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint8_t*>(p.w + static_cast<int64_t>(nt0) * tile_stride), 0, min(kBN, ntiles - nt0) * tile_stride, 0x00020000);
+      const_cast<uint8_t*>(p.w + static_cast<int64_t>(nt0) * p.tile_stride), 0, wtiles * p.tile_stride, 0x00020000);
+  int wtile[TN], wload[kWLoads];  // starts of the wave's row tiles, and of those that it moves
+#pragma unroll
+  for (int i = 0; i < TN; ++i) wtile[i] = mx4_tile_start(wn * TN + i, wtiles, p.tile_stride);
+#pragma unroll
+  for (int j = 0; j < kWLoads; ++j)
+    wload[j] = mx4_tile_start(kOwnCodes ? wn * TN + j : j * (kThreads / 64) + wave, wtiles, p.tile_stride);
 
   // what this lane moves: 16 bytes of rows xrow, xrow + kRowStep, ... of x, 16 of a lane's in every code tile.  LDS takes a
   // wave's bytes in lane order, so the lane picks the chunk that its place in the swizzled row holds.
@@ -370,13 +376,12 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
     if constexpr (kOwnCodes) {
 #pragma unroll
       for (int i = 0; i < TN; ++i)
-        codes[slot][i] = buffer_load16(wb, lane * 16, (wn * TN + i) * tile_stride + (kt >> 2) * kMxUnitBytes + (kt & 3) * kMxTileBytes);
+        codes[slot][i] = buffer_load16(wb, lane * 16, wload[i] + mx4_codes_at(kt));
       return;
     }
 #pragma unroll
     for (int j = 0; j < kWLoads; ++j)
-      buffer_to_lds16(wb, buf + kXBytes + wave * 1024 + j * kThreads * 16, lane * 16,
-                      (j * (kThreads / 64) + wave) * tile_stride + (kt >> 2) * kMxUnitBytes + (kt & 3) * kMxTileBytes);
+      buffer_to_lds16(wb, buf + kXBytes + wave * 1024 + j * kThreads * 16, lane * 16, wload[j] + mx4_codes_at(kt));
   };
 
   f32x4 acc[TN][TM];
@@ -396,8 +401,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
   auto load_scales = [&](int u) {
 #pragma unroll
     for (int i = 0; i < TN; ++i)
-      ws_next[i] = __builtin_amdgcn_raw_buffer_load_b32(
-          wb, lane * 4, (wn * TN + i) * tile_stride + u * kMxUnitBytes + 4 * kMxTileBytes, 0);
+      ws_next[i] = __builtin_amdgcn_raw_buffer_load_b32(wb, lane * 4, wtile[i] + mx4_scales_at(u), 0);
     if constexpr (kMx8) {
       const int b0 = 16 * u + 4 * g;
       if (16 * u + 16 <= blocks) {
