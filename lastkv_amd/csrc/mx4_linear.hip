@@ -439,7 +439,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
     char* q = buf + n * kBuf;
     return q < smem + kBufs * kBuf ? q : q - kBufs * kBuf;
   };
-  auto step = [&](int k0, int t) {
+  auto step = [&](int k0, int t, bool rest) {
     const int kt = k0 + t;
     auto start_loads = [&] {
       __builtin_amdgcn_sched_barrier(0);
@@ -514,7 +514,12 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
 #pragma unroll
       for (int j = 0; j < TM; ++j) asm volatile("" : "+v"(acc[i][j]));
     __builtin_amdgcn_sched_barrier(0);
-    wait_and_sync<(kBufs - 2) * kLoads>();  // tile kt + 1 has arrived
+    // tile kt + 1 has arrived: all but the last kBufs - 2 steps' loads.  In the rest the compiler drops the codes that no
+    // step reads any more, so that the steps issue fewer than kLoads: there all have arrived.
+    if (kOwnCodes && rest)
+      wait_and_sync<0>();
+    else
+      wait_and_sync<(kBufs - 2) * kLoads>();
     now = after(now, 1);
   };
   load_scales(0);
@@ -527,13 +532,13 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearP
   for (int u = 0; u < full; ++u) {
     next_unit();
 #pragma unroll
-    for (int t = 0; t < 4; ++t) step(4 * u, t);
+    for (int t = 0; t < 4; ++t) step(4 * u, t, false);
   }
   if (full < p.units) {
     next_unit();
 #pragma unroll
     for (int t = 0; t < 3; ++t)
-      if (t < (tiles & 3)) step(4 * full, t);
+      if (t < (tiles & 3)) step(4 * full, t, true);
   }
   if constexpr (kBufs > 2) wait_and_sync<0>();  // (the loads past the last tile still write the buffers)
   // The outputs go through LDS into whole rows: a lane's four stand 32 bytes wide in 16 rows, which HBM takes at 2 TB/s
