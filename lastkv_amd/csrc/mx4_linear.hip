@@ -107,6 +107,14 @@ __device__ inline void wait_and_sync() {
   asm volatile("" ::: "memory");
 }
 
+// A wave's lanes exchange data through LDS: what they wrote before is what they read behind this.  (No instruction: a wave's
+// LDS accesses keep their order; the compiler has to keep it too.)
+__device__ inline void wave_exchange() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
 // An offset past every buffer (they hold less than 2^30 bytes and a row's columns 2^21): loads give zeros.
 constexpr int kOutside = 0x60000000;
 
@@ -266,7 +274,9 @@ __global__ __launch_bounds__(kWaves * 64, MT == 1 && NT == 1 ? 4 : 2) void mx4_r
     if (h + 2 * KS < steps) load(h + 2 * KS, then);
 #pragma unroll
     for (int t = 0; t < kStepTiles; ++t) {
+      wave_exchange();  // (the last tile has been read)
       store_x();
+      wave_exchange();
       if (t + 1 < kStepTiles)
         load_x(h * kStepTiles + t + 1);
       else if (h + KS < steps)
