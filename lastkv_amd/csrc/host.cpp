@@ -802,6 +802,7 @@ bool mx8_out(PyObject* given, const at::Tensor& t, Mx8& m, std::initializer_list
   }
   if (!mx8_rows(given, m) || m.data.device() != t.device() || m.data.sizes() != t.sizes()) return false;
   const Span data(m.data, m.rows, m.width, m.stride), scales(m.scales, m.rows, m.width / 32, m.scale_stride);
+  if (data.meets(scales)) return false;
   for (const Span& s : inputs)
     if (data.meets(s) || scales.meets(s)) return false;
   return true;
@@ -819,7 +820,7 @@ PyObject* rmsnorm_mx8(PyObject*, PyObject* const* v, Py_ssize_t n) {
     if (!bf16(x) || !rows_of(*x, nrows, hidden, a.x_stride) || !on_current_device(*x) || !bf16(w) || !w->is_contiguous() ||
         w->numel() != hidden || w->device() != x->device() || !PyFloat_CheckExact(v[2]))
       return not_handled();
-    const Span xspan(*x, nrows, hidden, a.x_stride);
+    const Span xspan(*x, nrows, hidden, a.x_stride), wspan(*w, 1, hidden, 0);
     Span rspan = xspan;
     if (v[3] != Py_None) {
       const at::Tensor* r = tensor(v[3]);
@@ -827,10 +828,11 @@ PyObject* rmsnorm_mx8(PyObject*, PyObject* const* v, Py_ssize_t n) {
         return not_handled();
       rspan = Span(*r, r2, h2, a.residual_stride);
       if (rspan.meets(xspan) && (rspan.from != xspan.from || r->strides() != x->strides())) return not_handled();
+      if (rspan.meets(wspan)) return not_handled();
       a.residual = ptr(*r);
     }
     Mx8 out;
-    if (!mx8_out(v[4], *x, out, {xspan, rspan, Span(*w, 1, hidden, 0)})) return not_handled();
+    if (!mx8_out(v[4], *x, out, {xspan, rspan, wspan})) return not_handled();
     a.rows = static_cast<int32_t>(nrows);
     a.hidden = static_cast<int32_t>(hidden);
     a.eps = PyFloat_AS_DOUBLE(v[2]);
@@ -902,9 +904,9 @@ PyObject* mx4_linear(PyObject*, PyObject* const* v, Py_ssize_t n) {
         w.numel() != g_lib.mx4_weight_bytes(a.out_features, a.in_features))
       return not_handled();
     at::Tensor x;
+    Mx8 m;
     int64_t nrows, width, r2, w2;
     if (Py_TYPE(v[0]) == g_mx8) {
-      Mx8 m;
       if (!mx8_rows(v[0], m)) return not_handled();
       x = m.data;
       nrows = m.rows;
@@ -930,7 +932,11 @@ PyObject* mx4_linear(PyObject*, PyObject* const* v, Py_ssize_t n) {
         return not_handled();
       for (int64_t d = 0; d + 1 < x.dim(); ++d)
         if (o->size(d) != x.size(d)) return not_handled();
-      if (Span(x, nrows, width, a.x_stride).meets(Span(*o, nrows, w2, a.out_stride))) return not_handled();
+      const Span ospan(*o, nrows, w2, a.out_stride);
+      if (ospan.meets(Span(x, nrows, width, a.x_stride)) || ospan.meets(Span(w, 1, w.numel(), 0)) ||
+          (m.scales.defined() && ospan.meets(Span(m.scales, nrows, width / 32, m.scale_stride))) ||
+          (bias != nullptr && ospan.meets(Span(*bias, 1, w2, 0))))
+        return not_handled();
       out = *o;
     } else {
       std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());

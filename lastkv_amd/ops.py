@@ -1094,6 +1094,20 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
             and b.data_ptr() < a.data_ptr() + span(a))
 
 
+def _beside(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of matching rows, the same distance apart, keep to columns of their own."""
+
+    try:
+        a, b = (t.view(-1, t.shape[-1]) for t in (a, b))
+    except RuntimeError:
+        return False
+    step = a.stride(0) * a.element_size()
+    if a.shape[0] < 2 or step <= 0 or a.stride(1) != 1 or b.stride(1) != 1 or step != b.stride(0) * b.element_size():
+        return False
+    gap = (b.data_ptr() - a.data_ptr()) % step
+    return a.shape[1] * a.element_size() <= gap <= step - b.shape[1] * b.element_size()
+
+
 def _mx8_strides(name: str, rows: MX8Rows) -> tuple[int, int, int, int]:
     """(rows, width, data row stride, scale row stride) of MX8 rows viewed as [rows, width]."""
 
@@ -1119,6 +1133,7 @@ def _mx8_out(x: torch.Tensor, out: MX8Rows | None, *inputs: torch.Tensor | None)
     _require(isinstance(out, MX8Rows), "out must be MX8Rows")
     _require(out.shape == x.shape, "out shape must match x")
     _same_device(x.device, out=out.data)
+    _require(not _overlap(out.data, out.scales) or _beside(out.data, out.scales), "out's data and scales must not overlap")
     for t in (x, *inputs):
         _require(t is None or not (_overlap(out.data, t) or _overlap(out.scales, t)), "out must not overlap the inputs")
     return out
@@ -1147,6 +1162,7 @@ def rmsnorm_mx8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: 
         _require(residual.shape == x.shape, "residual shape must match x")
         _require(not _overlap(residual, x) or (residual.data_ptr() == x.data_ptr() and residual.stride() == x.stride()),
                  "residual must be x or not overlap it")
+        _require(not _overlap(residual, weight), "residual must not overlap weight")
     _same_device(x.device, weight=weight, residual=residual)
     if x.numel() == 0:
         return out
@@ -1260,7 +1276,7 @@ def mx4_linear(x: torch.Tensor | MX8Rows, weight: MX4Weight, bias: torch.Tensor 
     bf16 ``[out_features]``; returns bf16 ``[..., out_features]``: exact products, fp32 sums in a fixed order, rounded
     once.  In calls of many 8-bit rows the products are added eight columns at a time in the matrix instruction's fixed
     point, which keeps 13 bits below the largest, before they are added in fp32.  ``out`` must not reach into the memory from
-    ``x``'s first row to its last."""
+    ``x``'s first row to its last, that of its scales, the weight or ``bias``."""
 
     if _host_bound or _bind_host():
         done = _host.mx4_linear(x, weight, bias, out)
@@ -1284,6 +1300,8 @@ def mx4_linear(x: torch.Tensor | MX8Rows, weight: MX4Weight, bias: torch.Tensor 
     _require(tuple(out.shape) == shape, f"out must be {list(shape)}")
     _same_device(device, weight=weight.data, bias=bias, out=out)
     _require(not _overlap(out, x.data if mx8 else x), "out must not overlap x")
+    for name, t in (("x's scales", x.scales if mx8 else None), ("the weight", weight.data), ("bias", bias)):
+        _require(t is None or not _overlap(out, t), f"out must not overlap {name}")
     if out.numel() == 0:
         return out
     a = _lib.Mx4LinearArgs()
