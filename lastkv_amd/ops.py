@@ -1135,7 +1135,8 @@ def _mx8_out(x: torch.Tensor, out: MX8Rows | None, *inputs: torch.Tensor | None)
     _same_device(x.device, out=out.data)
     _require(not _overlap(out.data, out.scales) or _beside(out.data, out.scales), "out's data and scales must not overlap")
     for t in (x, *inputs):
-        _require(t is None or not (_overlap(out.data, t) or _overlap(out.scales, t)), "out must not overlap the inputs")
+        for o in (out.data, out.scales):
+            _require(t is None or not _overlap(o, t) or _beside(o, t), "out must not overlap the inputs")
     return out
 
 
@@ -1145,7 +1146,7 @@ def rmsnorm_mx8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: 
     ``residual`` first ``residual += x`` in bf16, in place, and the sum) normalised and multiplied by ``weight``,
     each block of 32 rounded once, correctly, to e4m3 under the smallest power-of-two scale that holds its largest
     value.  A block with an infinity or NaN is NaN.  Returns ``out``, which must not overlap the inputs; ``residual``
-    may be ``x`` itself."""
+    may be ``x`` itself, or columns beside it in one tensor."""
 
     if _host_bound or _bind_host():
         done = _host.rmsnorm_mx8(x, weight, eps, residual, out)
@@ -1160,7 +1161,8 @@ def rmsnorm_mx8(x: torch.Tensor, weight: torch.Tensor, eps: float, *, residual: 
     if residual is not None:
         _require_bf16_cuda("residual", residual)
         _require(residual.shape == x.shape, "residual shape must match x")
-        _require(not _overlap(residual, x) or (residual.data_ptr() == x.data_ptr() and residual.stride() == x.stride()),
+        _require(not _overlap(residual, x) or _beside(residual, x) or
+                 (residual.data_ptr() == x.data_ptr() and residual.stride() == x.stride()),
                  "residual must be x or not overlap it")
         _require(not _overlap(residual, weight), "residual must not overlap weight")
     _same_device(x.device, weight=weight, residual=residual)

@@ -73,3 +73,27 @@ def test_residual_over_the_weight(path):
         ops.rmsnorm_mx8(x, r[3], 1e-5, residual=r[:4])
     assert torch.equal(r, before)
     same_mx8(ops.rmsnorm_mx8(x, r[4], 1e-5, residual=r[:4]), norm_reference(x, before[4], 1e-5, before[:4]))
+
+
+def test_columns_of_one_tensor_side_by_side(path):
+    """x, the residual and the output in rows of one tensor: none reaches into another's columns."""
+
+    g = _gen(4)
+    rows, k = 5, 96
+    pool = torch.zeros((rows, 640), dtype=torch.uint8, device=DEV)
+    x, r = pool[:, :192].view(BF16), pool[:, 192:384].view(BF16)
+    x.copy_(outliers(g, rows, k))
+    r.copy_(outliers(g, rows, k))
+    out = ops.MX8Rows(pool[:, 384:480].view(torch.float8_e4m3fn), pool[:, 480:483])
+    w = (1 + 0.3 * torch.randn(k, generator=g, device=DEV)).to(BF16)
+    keep, want_r = x.clone(), (r.float() + x.float()).to(BF16)
+    want = norm_reference(x, w, 1e-5, r.clone())
+    same_mx8(ops.rmsnorm_mx8(x, w, 1e-5, residual=r, out=out), want)
+    assert torch.equal(r, want_r) and torch.equal(x, keep) and not pool[:, 483:].any()
+    want = x.double() / (1 + torch.exp(-x.double())) * r.double()
+    same_mx8(ops.silu_mul_mx8(x, r, out=out), want)
+    half = pool[:, 96:288].view(BF16)  # the second half of x and the first of r
+    for call in (lambda: ops.rmsnorm_mx8(x, w, 1e-5, residual=half),
+                 lambda: ops.silu_mul_mx8(x, r, out=ops.MX8Rows(pool[:, 352:448].view(torch.float8_e4m3fn), pool[:, 480:483]))):
+        with pytest.raises(ValueError, match="overlap"):
+            call()
