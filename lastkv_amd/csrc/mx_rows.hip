@@ -100,6 +100,11 @@ __global__ __launch_bounds__(kThreads) void rmsnorm_mx8_kernel(const NormParams 
       unpack8(wv[k], wf);
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] = wf[j] * (h[j] * rf);  // (three roundings: within 2^-22)
+      // ... where h rf stays in fp32's normal range.  Below it another 2^-150 |w| are missing, up to 2^-43 of a block's
+      // maximum for |w| <= 2^10 (that is at least 2^-97), 2^-24 of what does not round to zero; larger weights take 64 bits.
+      const float wmax = fmax_nan(fmax3_nan(fmax3_nan(fmax3_nan(fabsf(wf[0]), fabsf(wf[1]), fabsf(wf[2])), fabsf(wf[3]), fabsf(wf[4])),
+                                            fabsf(wf[5]), fabsf(wf[6])), fabsf(wf[7]));
+      if (wmax > 0x1p10f) y[0] = __uint_as_float(0x7fc00000u);
       int byte;
       const uint2 q = quantize_e4m3(y, byte, [&](double(&d)[8]) {
 #pragma unroll
