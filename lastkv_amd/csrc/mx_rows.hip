@@ -184,17 +184,27 @@ __global__ __launch_bounds__(256) void mx8_unpack_kernel(const uint8_t* data, in
   }
 }
 
+constexpr int32_t kMaxNormRows = 1 << 23;  // of a launch: a grid has fewer than 2^32 threads
+
 template <bool kAdd>
-void launch_norm(const NormParams& p, int32_t rows, hipStream_t s) {
+void launch_norm(NormParams p, int32_t rows, hipStream_t s) {
   const int chunks = (p.hidden + kThreads * 8 - 1) / (kThreads * 8);
-  if (chunks <= 1)
-    rmsnorm_mx8_kernel<kAdd, 1><<<rows, kThreads, 0, s>>>(p);
-  else if (chunks <= 2)
-    rmsnorm_mx8_kernel<kAdd, 2><<<rows, kThreads, 0, s>>>(p);
-  else if (chunks <= 4)
-    rmsnorm_mx8_kernel<kAdd, 4><<<rows, kThreads, 0, s>>>(p);
-  else
-    rmsnorm_mx8_kernel<kAdd, kMaxChunks><<<rows, kThreads, 0, s>>>(p);
+  while (rows > 0) {
+    const int32_t n = std::min(rows, kMaxNormRows);
+    if (chunks <= 1)
+      rmsnorm_mx8_kernel<kAdd, 1><<<n, kThreads, 0, s>>>(p);
+    else if (chunks <= 2)
+      rmsnorm_mx8_kernel<kAdd, 2><<<n, kThreads, 0, s>>>(p);
+    else if (chunks <= 4)
+      rmsnorm_mx8_kernel<kAdd, 4><<<n, kThreads, 0, s>>>(p);
+    else
+      rmsnorm_mx8_kernel<kAdd, kMaxChunks><<<n, kThreads, 0, s>>>(p);
+    rows -= n;
+    p.x += n * p.x_stride;
+    if (kAdd) p.residual += n * p.res_stride;
+    p.out += n * p.out_stride;
+    p.scales += n * p.scale_stride;
+  }
 }
 
 dim3 row_grid(int32_t rows, int32_t width) {

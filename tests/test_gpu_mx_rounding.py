@@ -29,3 +29,19 @@ def test_rmsnorm_mx8_of_tiny_values_under_large_weights(low, row):
     w[:32] = 1
     assert (x[:, 32:] != 0).any() and torch.isfinite(w).all()
     same_mx8(ops.rmsnorm_mx8(x, w, 1e-5), norm_reference(x, w, 1e-5))
+
+
+@pytest.mark.parametrize("add", [False, True])
+def test_rmsnorm_mx8_of_more_rows_than_a_grid_has(add):
+    """2^24 + 3 rows: a workgroup of 256 threads each would be 2^32 threads and more."""
+
+    rows = (1 << 24) + 3
+    x = torch.randn((1 << 12, 32), generator=_gen(5), device=DEV).to(BF16).repeat((rows >> 12) + 1, 1)[:rows]
+    w = torch.ones(32, device=DEV, dtype=BF16)
+    residual = x.flip(0) if add else None
+    at = torch.tensor([0, 1, (1 << 23) - 1, 1 << 23, (1 << 23) + 1, (1 << 24) - 1, 1 << 24, rows - 1], device=DEV)
+    want = norm_reference(x[at], w, 1e-5, residual[at] if add else None)
+    sums = (residual[at].float() + x[at].float()).to(BF16) if add else None
+    q = ops.rmsnorm_mx8(x, w, 1e-5, residual=residual)
+    same_mx8(ops.MX8Rows(q.data[at], q.scales[at]), want)
+    assert not add or torch.equal(residual[at], sums)
