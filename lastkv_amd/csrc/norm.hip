@@ -150,18 +150,27 @@ __global__ __launch_bounds__(256) void silu_mul_kernel(const uint16_t* gate, int
   }
 }
 
+constexpr int32_t kNormMaxRows = 1 << 23;  // of a launch: a grid has fewer than 2^32 threads
+
 // The RMSNorm instance that holds a row of `hidden` elements.
 template <bool kAdd>
-void launch_rmsnorm(const NormParams& p, int32_t rows, hipStream_t s) {
+void launch_rmsnorm(NormParams p, int32_t rows, hipStream_t s) {
   const int chunks = (p.hidden + kNormThreads * 8 - 1) / (kNormThreads * 8);
-  if (chunks <= 1)
-    rmsnorm_kernel<kAdd, 1><<<rows, kNormThreads, 0, s>>>(p);
-  else if (chunks <= 2)
-    rmsnorm_kernel<kAdd, 2><<<rows, kNormThreads, 0, s>>>(p);
-  else if (chunks <= 4)
-    rmsnorm_kernel<kAdd, 4><<<rows, kNormThreads, 0, s>>>(p);
-  else
-    rmsnorm_kernel<kAdd, kNormMaxChunks><<<rows, kNormThreads, 0, s>>>(p);
+  while (rows > 0) {
+    const int32_t n = std::min(rows, kNormMaxRows);
+    if (chunks <= 1)
+      rmsnorm_kernel<kAdd, 1><<<n, kNormThreads, 0, s>>>(p);
+    else if (chunks <= 2)
+      rmsnorm_kernel<kAdd, 2><<<n, kNormThreads, 0, s>>>(p);
+    else if (chunks <= 4)
+      rmsnorm_kernel<kAdd, 4><<<n, kNormThreads, 0, s>>>(p);
+    else
+      rmsnorm_kernel<kAdd, kNormMaxChunks><<<n, kNormThreads, 0, s>>>(p);
+    rows -= n;
+    p.x += n * p.x_stride;
+    if (kAdd) p.residual += n * p.res_stride;
+    p.out += n * p.out_stride;
+  }
 }
 
 }  // namespace
