@@ -1273,13 +1273,22 @@ def mx4_unpack(weight: MX4Weight) -> torch.Tensor:
 
 
 def mx4_linear(x: torch.Tensor | MX8Rows, weight: MX4Weight, bias: torch.Tensor | None = None,
-               out: torch.Tensor | None = None) -> torch.Tensor:
+               out: torch.Tensor | None = None, *, exact: bool = False) -> torch.Tensor:
     """``F.linear`` over a 4-bit weight: ``x`` is bf16 ``[..., in_features]`` or ``MX8Rows`` of that shape, ``bias``
     bf16 ``[out_features]``; returns bf16 ``[..., out_features]``: exact products, fp32 sums in a fixed order, rounded
-    once.  In calls of many 8-bit rows the products are added eight columns at a time in the matrix instruction's fixed
-    point, which keeps 13 bits below the largest, before they are added in fp32.  ``out`` must not reach into the memory from
-    ``x``'s first row to its last, that of its scales, the weight or ``bias``."""
+    once.  The order goes by the call's sizes: a row's last bit may change with the number of rows beside it.
 
+    More than 16 8-bit rows, where the products are enough work, go to the scaled matrix instruction: it adds the
+    products of eight columns in fixed point, which keeps 13 bits below the largest, before they are added in fp32
+    (about one output in a hundred rounds the other way).  ``exact`` takes such rows at their bf16 values instead
+    (``mx8_unpack``), with products and sums as above at any number of rows, in about 1.7 times the time for thousands of
+    them.  Elsewhere 8-bit rows count at their bf16 values too: those past bf16's range as infinities.
+
+    ``out`` must not reach into the memory from ``x``'s first row to its last, that of its scales, the weight or
+    ``bias``."""
+
+    if exact and isinstance(x, MX8Rows):
+        x = mx8_unpack(x)
     if _host_bound or _bind_host():
         done = _host.mx4_linear(x, weight, bias, out)
         if done is not None:
