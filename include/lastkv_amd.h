@@ -600,7 +600,8 @@ int32_t lkv_silu_mul(const void *gate, int64_t gate_stride, const void *up, int6
  *     scales [n, k / 32], and lkv_mx4_quantize of bf16 rows; lkv_mx4_unpack gives the values in bf16 (exact
  *     above bf16's least normal value).
  * A quantized block's scale is the smallest power of two (at least 2^-127) with max|y| <= 448 * scale (MX4: 6 *
- * scale), and its values are the nearest ones, ties to even; a block with an infinity or NaN has scale 255.
+ * scale), and its values are the nearest ones, ties to even; a block with an infinity or NaN, or one
+ * that no scale up to 2^127 holds, has scale 255.
  * Strides are in elements (bytes of 8-bit rows); one row's stride is not read by lkv_mx4_linear.  Outputs must not
  * overlap inputs, except that x may be residual.
  * ------------------------------------------------------------------------------------- */
@@ -637,6 +638,7 @@ int32_t lkv_silu_mul_mx8(const void *gate, int64_t gate_stride, const void *up, 
 int32_t lkv_mx8_unpack(const void *data, int64_t data_stride, const void *scales, int64_t scale_stride, void *out,
                        int64_t out_stride, int32_t rows, int32_t width, lkv_stream_t stream);
 
+/* Bytes of an MX4 weight of 1 to 2^24 rows and up to 2^20 columns; 0 for other sizes. */
 int64_t lkv_mx4_weight_bytes(int32_t n, int32_t k);
 
 int32_t lkv_mx4_pack(const void *codes, int64_t code_stride, const void *scales, int64_t scale_stride, int32_t n,

@@ -774,7 +774,7 @@ uintptr_t bits(const void* p) { return reinterpret_cast<uintptr_t>(p); }
               "an MX4 weight has 1 to 2^24 rows and a positive multiple of 32 columns up to 2^20, got %d x %d", n, k)
 
 extern "C" int64_t lkv_mx4_weight_bytes(int32_t n, int32_t k) {
-  if (n <= 0 || k <= 0) return 0;
+  if (n <= 0 || n > (1 << 24) || k <= 0 || k > (1 << 20)) return 0;
   return static_cast<int64_t>((n + 15) / 16) * lkv::mx4_tile_stride(lkv::mx4_units(k));
 }
 

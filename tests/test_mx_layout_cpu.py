@@ -8,6 +8,8 @@ import subprocess
 
 import pytest
 
+from lastkv_amd import _lib
+
 CSRC = pathlib.Path(__file__).resolve().parents[1] / "lastkv_amd" / "csrc"
 
 # The loads of one workgroup, as mx4_tile_kernel forms them from the layout's functions: kbn row tiles from nt0 on, all
@@ -62,3 +64,10 @@ def test_tile_loads_stay_inside_the_weight(tmp_path):
                    check=True)
     run = subprocess.run([str(tmp_path / "loads"), *(str(v) for shape in SHAPES for v in shape)], capture_output=True, text=True)
     assert run.returncode == 0, run.stdout
+
+
+def test_sizes_that_no_weight_has_need_no_bytes():
+    size = _lib.load().lkv_mx4_weight_bytes
+    assert size(1 << 24, 1 << 20) == (1 << 20) * (((1 << 11) * 17) | 1) * 256
+    for n, k in ((0, 32), (16, 0), (-1, 64), ((1 << 24) + 1, 32), (16, (1 << 20) + 32), (16, (1 << 31) - 32), ((1 << 31) - 1, (1 << 31) - 32)):
+        assert size(n, k) == 0, (n, k)
