@@ -324,11 +324,12 @@ __global__ __launch_bounds__(kWaves * 64, MT == 1 && NT == 1 ? 4 : 2) void mx4_r
 // tiles of 16 x 16.  Tiles of 128 columns go to LDS by direct loads, kBufs buffers in turn, one barrier a tile; two
 // or three workgroups share a CU where there are that many, so that one's products cover the other's reads of LDS.
 // MX8 rows: both operands and both scales go to the scaled matrix instruction as they are (a code is converted nowhere).
-// Bound by the matrix pipe, of which 4096 rows of 28672 x 4096 reach 2.57 PFLOP/s (375 us; bf16 weights in the library's
-// GEMM 641 us); independent products in registers reach 3.83 PFLOP/s on this card, this loop without its loads 3.4.  With
+// Bound by the waits for the next tile: 4096 rows of 28672 x 4096 reach 2.47-2.57 PFLOP/s (375-389 us; bf16 weights in the
+// library's GEMM 641 us), the matrix pipes 56 % busy; independent products in registers reach 3.83 PFLOP/s on this card, this
+// loop without its loads 3.4.  With
 // the tile staged through registers the same took 30-50 us more, with the outputs stored from registers 28.
 // bf16 rows: the codes are converted in registers as they are used, by waves side by side over the weight (WM = 1), so that
-// each is converted once and goes to its wave's registers only.  1000 rows of 6144 x 4096 take 43-45 us, 1.15 PFLOP/s, 4096 rows
+// each is converted once and goes to its wave's registers only.  1000 rows of 6144 x 4096 take 44-47 us, 1.07-1.14 PFLOP/s, 4096 rows
 // 151 us, 1.36 PFLOP/s (library, bf16 weights, 1000 rows: 52 us); bf16 products in registers reach 1.92 PFLOP/s.
 template <bool kMx8, int WN, int WM, int TN, int TM, int kBufs>
 __global__ __launch_bounds__(WN * WM * 64, 2) void mx4_tile_kernel(const LinearParams p, int mtiles, int grid) {

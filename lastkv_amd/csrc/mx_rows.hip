@@ -46,7 +46,7 @@ __device__ inline uint4 pack8(const float (&f)[8]) {
 // bits (no order of the sum then shows in a row's output, and no row's squares leave the range).
 // Bound by HBM: every load is issued before the first use, with no branch between them (a chunk past the row rereads the
 // last one); x and the residual are read once and take non-temporal accesses, as in lkv_rmsnorm.  4096 rows of 4096 with a
-// residual: 21.7 us, 5.4 TB/s (lkv_rmsnorm, bf16 out, 22.7; the outputs all in 64 bits 32); one row 3.0.
+// residual: 21.8 us, 5.4 TB/s (lkv_rmsnorm, bf16 out, 22.7; the outputs all in 64 bits 32); one row 2.9.
 template <bool kAdd, int kChunks>
 __global__ __launch_bounds__(kThreads) void rmsnorm_mx8_kernel(const NormParams p) {
   __shared__ double part[kThreads / 64];

@@ -582,7 +582,9 @@ class LastKVServingModel:
     power-of-two scale per 32 columns; embeddings, norms and lm_head stay bf16) and runs them as ``ops.mx4_linear``.
     ``activations="mxfp8"`` then also hands q / k / v, gate / up and down 8-bit rows, which the norms and the SwiGLU
     product write (``ops.rmsnorm_mx8``, ``ops.silu_mul_mx8``); the output projection reads the attention's bf16 rows.
-    The model passed in keeps its bf16 weights."""
+    This makes prompts faster; a decode step reads the same weights either way.  In calls of many rows the products of 8-bit
+    rows are added eight at a time in fixed point (``ops.mx4_linear``).
+    The model passed in keeps its bf16 weights, which the 4-bit copy comes on top of."""
 
     def __init__(self, model, *, max_batch: int, max_tokens_per_slot: int, source_pages: int | None = None,
                  num_splits: int | None = None, device=None, contract: str = "hf", weights: str = "bf16",
