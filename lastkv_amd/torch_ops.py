@@ -251,7 +251,7 @@ def _(x, weight, out_features, bias=None):
 @torch.library.custom_op("lastkv::mx4_linear_mx8", mutates_args=())
 def mx4_linear_mx8(data: Tensor, scales: Tensor, weight: Tensor, out_features: int,
                    bias: Optional[Tensor] = None) -> Tensor:
-    """``lkv_mx4_linear`` of MX8 rows."""
+    """``lkv_mx4_linear`` of MX8 rows (``mx4_linear`` of their ``mx8_unpack`` has fp32 sums at any number of rows)."""
 
     return ops.mx4_linear(ops.MX8Rows(data, scales), ops.MX4Weight(weight, out_features, data.shape[-1]), bias)
 
