@@ -34,7 +34,7 @@ typedef enum lkv_status {
 #define LKV_HEAD_DIM 128
 #define LKV_BLOCK_TOKENS 32
 #define LKV_BLOCK_ELEMS 4096
-#define LKV_ABI_VERSION 12
+#define LKV_ABI_VERSION 13
 
 /* Version of this ABI (LKV_ABI_VERSION). */
 int32_t lkv_abi_version(void);
@@ -677,6 +677,139 @@ typedef struct lkv_mx4_linear_args {
 } lkv_mx4_linear_args;
 
 int32_t lkv_mx4_linear(const lkv_mx4_linear_args *args, lkv_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * The shared cache in 8 bits.  No counterpart in the reference, whose cache is bf16.
+ * A page holds, per kv head, 32 tokens of K and of V as e4m3 codes (4096 bytes each, in the layout the attention
+ * kernels read: lastkv_amd/csrc/kv8.h) and one scale byte e each, which stands for 2^(e - 127) (255: the whole block is NaN).
+ * Codes of a quantized block are e4m3(x * 2^(127 - e)) to nearest even, with 2^(e - 127) the smallest power of
+ * two, at least 2^-127, that satisfies max|x| <= 448 * 2^(e - 127); a block with an infinity or NaN has e = 255.  So
+ * a code's value is exact in bf16 (above bf16's least subnormal value) and nothing saturates.
+ * Strides are in bytes; page p of head h is at h * head_stride + p * page_stride, its scale at h * scale_head_stride + p.
+ * ------------------------------------------------------------------------------------- */
+typedef struct lkv_kv8_pool {
+  int32_t struct_size; /* sizeof(lkv_kv8_pool) */
+  int32_t num_pages;
+  int32_t heads;
+  int32_t reserved;
+  void *k; /* 16-byte aligned, as are both strides */
+  void *v;
+  int64_t page_stride; /* at least 4096 */
+  int64_t head_stride;
+  void *k_scales;
+  void *v_scales;
+  int64_t scale_head_stride;
+} lkv_kv8_pool;
+
+/* Blocks [first_block, first_block + blocks) of every sequence's bf16 pages into 8-bit pages: block j of sequence b is page
+ * src_table[b * src_table_stride + j] of the bf16 pool and becomes page dst_table[b * dst_table_stride + j] of dst (ids
+ * clamped to the pools).  Only its first min(32, tokens - 32 j) tokens count; the others are stored as 0, and a block past
+ * the sequence's tokens is left as it is.  A destination page must not occur twice in a call. */
+typedef struct lkv_kv8_quantize_args {
+  int32_t struct_size; /* sizeof(lkv_kv8_quantize_args) */
+  int32_t batch;
+  int32_t heads;
+  int32_t head_dim; /* 128 */
+  int32_t first_block;
+  int32_t blocks;
+  int32_t tokens_const;
+  int32_t src_num_pages;
+  const int32_t *tokens; /* device [B] or NULL -> tokens_const */
+  const void *src_k;     /* bf16 pool, strides in elements */
+  const void *src_v;
+  int64_t src_page_stride;
+  int64_t src_head_stride;
+  const int32_t *src_table;
+  int64_t src_table_stride;
+  const int32_t *dst_table;
+  int64_t dst_table_stride;
+  int32_t src_table_width;
+  int32_t dst_table_width;
+} lkv_kv8_quantize_args;
+
+int32_t lkv_kv8_quantize(const lkv_kv8_quantize_args *args, const lkv_kv8_pool *dst, lkv_stream_t stream);
+
+/* Tokens [token0, token0 + tokens) of every sequence's 8-bit pages as bf16 rows [B, H, tokens, 128] (16-byte aligned,
+ * strides in elements). */
+int32_t lkv_kv8_unpack(const lkv_kv8_pool *src, const int32_t *table, int64_t table_stride, int32_t table_width,
+                       int32_t batch, int32_t token0, int32_t tokens, void *k, int64_t k_stride_b, int64_t k_stride_h,
+                       int64_t k_stride_t, void *v, int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_t,
+                       lkv_stream_t stream);
+
+/* lkv_decode_attn and lkv_prefill_attn whose older segment is in `older`, an 8-bit pool: args->older_k and older_v are
+ * NULL, older_block_table (with older_table_stride, older_capacity_tokens and the lengths) names pages of `older`, and the
+ * other older fields are not read.  The result is the attention over the codes' values: with older_vscale_mode 1
+ * V is bf16(value * vscale[h]).  Scores, softmax and sums are those of the bf16 calls; a sequence that sees a token of a NaN
+ * block has NaN outputs.  Codes past a sequence's length do not count, whatever they hold. */
+int32_t lkv_decode_attn_kv8(const lkv_decode_args *args, const lkv_kv8_pool *older, lkv_stream_t stream);
+
+int64_t lkv_prefill_kv8_workspace_bytes(const lkv_prefill_args *args);
+
+int32_t lkv_prefill_attn_kv8(const lkv_prefill_args *args, const lkv_kv8_pool *older, lkv_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Copies of pages inside one pool, K and V of every kv head: page dst[i] := page src[i] for i < count.  src and dst are
+ * HOST arrays, read before the call returns (a captured call keeps its pairs).  No page may be a destination twice or
+ * both a source and a destination; such lists, and ids outside [0, num_pages), are rejected.  For forking a sequence and for
+ * moving pages together (the reference clones whole caches: llm/src/lastkv/llm/modeling.py:59-67 reorder_cache).
+ * ------------------------------------------------------------------------------------- */
+typedef struct lkv_copy_pages_args {
+  int32_t struct_size; /* sizeof(lkv_copy_pages_args) */
+  int32_t count;
+  int32_t heads;
+  int32_t num_pages;
+  int32_t page_bytes; /* 8192: bf16 pages, 4096: 8-bit pages */
+  int32_t reserved;
+  const int32_t *src; /* host [count] */
+  const int32_t *dst; /* host [count] */
+  void *k;            /* page p of head h at h * head_stride + p * page_stride (bytes, multiples of 16) */
+  void *v;
+  int64_t page_stride;
+  int64_t head_stride;
+  void *k_scales; /* 8-bit pools: one byte a (page, head) at h * scale_head_stride + p; else NULL */
+  void *v_scales;
+  int64_t scale_head_stride;
+} lkv_copy_pages_args;
+
+int32_t lkv_copy_pages(const lkv_copy_pages_args *args, lkv_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Beam search's selection.  For each of `batch` prompts, of the beams * vocab candidates
+ *   total[k][v] = scores[b][k] + logits[b][k][v] - log sum_u exp(logits[b][k][u])
+ * the `count` greatest, in descending order: out_scores (fp32), out_beams (k) and out_tokens (v), each [batch, count].
+ * Totals are formed in 64 bits from sums of fp32 exponentials; equal ones go to the lowest beam, then to the greatest logit,
+ * then to the lowest token, so that one beam's candidates stand in the exact order of their logits.  A total that is NaN or
+ * infinite is no candidate (a beam of score -inf, a masked logit of -inf, a row with a NaN or +inf); where fewer than
+ * `count` are left the last entries are -inf, -1, -1.
+ * logits is bf16 or fp32, rows of `vocab` contiguous values at any alignment (strides in elements); the workspace holds
+ * lkv_beam_workspace_bytes(...) bytes and is the call's alone while it runs.  The reference's drop-in cache
+ * offers reorder_cache for such a search (modeling.py:59-67).
+ * ------------------------------------------------------------------------------------- */
+#define LKV_BEAM_MAX_COUNT 64
+#define LKV_BEAM_MAX_BEAMS 64
+
+typedef struct lkv_beam_select_args {
+  int32_t struct_size; /* sizeof(lkv_beam_select_args) */
+  int32_t batch;
+  int32_t beams; /* 1 to 64 */
+  int32_t vocab; /* 1 to 2^20 */
+  int32_t count; /* 1 to 64 */
+  int32_t logits_fp32; /* 0: bf16, 1: fp32 */
+  const void *logits;
+  int64_t logits_stride_b;
+  int64_t logits_stride_k;
+  const float *scores; /* [batch, beams] */
+  int64_t scores_stride_b;
+  float *out_scores; /* [batch, count] each, contiguous */
+  int32_t *out_beams;
+  int32_t *out_tokens;
+  void *workspace;
+  int64_t workspace_bytes;
+} lkv_beam_select_args;
+
+int64_t lkv_beam_workspace_bytes(int32_t batch, int32_t beams, int32_t vocab, int32_t count);
+
+int32_t lkv_beam_select(const lkv_beam_select_args *args, lkv_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------
  * Achievable-peak probes.  No counterpart in the reference: measurement support for the bench,

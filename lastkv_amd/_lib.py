@@ -11,7 +11,7 @@ import pathlib
 import threading
 
 LIB_PATH = pathlib.Path(__file__).resolve().parent / "liblastkv_amd.so"
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 
 class LastKVNativeError(RuntimeError):
@@ -366,6 +366,95 @@ class Mx4LinearArgs(ctypes.Structure):
     ]
 
 
+class Kv8Pool(ctypes.Structure):
+    """Mirror of ``lkv_kv8_pool``."""
+
+    _fields_ = [
+        ("struct_size", c_i32),
+        ("num_pages", c_i32),
+        ("heads", c_i32),
+        ("reserved", c_i32),
+        ("k", c_ptr),
+        ("v", c_ptr),
+        ("page_stride", c_i64),
+        ("head_stride", c_i64),
+        ("k_scales", c_ptr),
+        ("v_scales", c_ptr),
+        ("scale_head_stride", c_i64),
+    ]
+
+
+class Kv8QuantizeArgs(ctypes.Structure):
+    """Mirror of ``lkv_kv8_quantize_args``."""
+
+    _fields_ = [
+        ("struct_size", c_i32),
+        ("batch", c_i32),
+        ("heads", c_i32),
+        ("head_dim", c_i32),
+        ("first_block", c_i32),
+        ("blocks", c_i32),
+        ("tokens_const", c_i32),
+        ("src_num_pages", c_i32),
+        ("tokens", c_ptr),
+        ("src_k", c_ptr),
+        ("src_v", c_ptr),
+        ("src_page_stride", c_i64),
+        ("src_head_stride", c_i64),
+        ("src_table", c_ptr),
+        ("src_table_stride", c_i64),
+        ("dst_table", c_ptr),
+        ("dst_table_stride", c_i64),
+        ("src_table_width", c_i32),
+        ("dst_table_width", c_i32),
+    ]
+
+
+class CopyPagesArgs(ctypes.Structure):
+    """Mirror of ``lkv_copy_pages_args``."""
+
+    _fields_ = [
+        ("struct_size", c_i32),
+        ("count", c_i32),
+        ("heads", c_i32),
+        ("num_pages", c_i32),
+        ("page_bytes", c_i32),
+        ("reserved", c_i32),
+        ("src", c_ptr),
+        ("dst", c_ptr),
+        ("k", c_ptr),
+        ("v", c_ptr),
+        ("page_stride", c_i64),
+        ("head_stride", c_i64),
+        ("k_scales", c_ptr),
+        ("v_scales", c_ptr),
+        ("scale_head_stride", c_i64),
+    ]
+
+
+class BeamSelectArgs(ctypes.Structure):
+    """Mirror of ``lkv_beam_select_args``."""
+
+    _fields_ = [
+        ("struct_size", c_i32),
+        ("batch", c_i32),
+        ("beams", c_i32),
+        ("vocab", c_i32),
+        ("count", c_i32),
+        ("logits_fp32", c_i32),
+        ("logits", c_ptr),
+        ("logits_stride_b", c_i64),
+        ("logits_stride_k", c_i64),
+        ("scores", c_ptr),
+        ("scores_stride_b", c_i64),
+        ("out_scores", c_ptr),
+        ("out_beams", c_ptr),
+        ("out_tokens", c_ptr),
+        ("workspace", c_ptr),
+        ("workspace_bytes", c_i64),
+    ]
+
+
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lkv_abi_version": (c_i32, []),
     "lkv_last_error": (ctypes.c_char_p, []),
@@ -398,6 +487,18 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lkv_mx4_quantize": (c_i32, [c_ptr, c_i64, c_i32, c_i32, c_ptr, c_ptr]),
     "lkv_mx4_unpack": (c_i32, [c_ptr, c_i32, c_i32, c_ptr, c_i64, c_ptr]),
     "lkv_mx4_linear": (c_i32, [ctypes.POINTER(Mx4LinearArgs), c_ptr]),
+    "lkv_kv8_quantize": (c_i32, [ctypes.POINTER(Kv8QuantizeArgs), ctypes.POINTER(Kv8Pool), c_ptr]),
+    "lkv_kv8_unpack": (
+        c_i32,
+        [ctypes.POINTER(Kv8Pool), c_ptr, c_i64, c_i32, c_i32, c_i32, c_i32, c_ptr, c_i64, c_i64, c_i64, c_ptr, c_i64, c_i64,
+         c_i64, c_ptr],
+    ),
+    "lkv_decode_attn_kv8": (c_i32, [ctypes.POINTER(DecodeArgs), ctypes.POINTER(Kv8Pool), c_ptr]),
+    "lkv_prefill_kv8_workspace_bytes": (c_i64, [ctypes.POINTER(PrefillArgs)]),
+    "lkv_prefill_attn_kv8": (c_i32, [ctypes.POINTER(PrefillArgs), ctypes.POINTER(Kv8Pool), c_ptr]),
+    "lkv_copy_pages": (c_i32, [ctypes.POINTER(CopyPagesArgs), c_ptr]),
+    "lkv_beam_workspace_bytes": (c_i64, [c_i32, c_i32, c_i32, c_i32]),
+    "lkv_beam_select": (c_i32, [ctypes.POINTER(BeamSelectArgs), c_ptr]),
     "lkv_probe_read": (c_i32, [c_ptr, c_i64, c_ptr, c_i32, c_ptr]),
     "lkv_probe_mfma": (c_i32, [c_ptr, c_i32, c_i32, ctypes.c_uint32, c_ptr]),
 }

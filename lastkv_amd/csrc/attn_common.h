@@ -9,6 +9,7 @@
 // Blocks are numbered over the concatenation: older blocks first, then local blocks.
 #pragma once
 #include "common.h"
+#include "kv8.h"
 #include "runtime.h"
 
 namespace lkv {
@@ -240,8 +241,34 @@ __device__ inline uint4 scale_frag(uint4 v, float s) {
 // one score column per (query token, head) (decode.hip).  The arguments have passed
 // lkv_prefill_attn's checks; seg was filled from them.  class_n: the number of the ragged call's
 // sequences in the class when the host knows it (from cu_seqlens_q_host), else -1.
+// older8: the 8-bit pool that holds the older segment, or null.
 int32_t prefill_on_decode_kernel(const lkv_prefill_args* a, const SegParams& seg, int32_t group, int32_t col_lo,
-                                 int32_t col_hi, int32_t class_n, hipStream_t s);
+                                 int32_t col_hi, int32_t class_n, hipStream_t s, const Kv8Pool* older8 = nullptr);
+
+// Writes the bf16 copies of a prefill call's 8-bit older blocks, in the tiled layout, `blocks` per (sequence, kv head) at k16 / v16
+// (kv8.hip); sequences of at most `skip_rows` query rows per kv head, and blocks past a sequence's length, are left out.
+int32_t kv8_copy_blocks(const lkv_prefill_args* a, const Kv8Pool& o, int32_t group, int32_t skip_rows, int32_t blocks,
+                        uint16_t* k16, uint16_t* v16, hipStream_t s);
+
+// Checks the older segment of a call over an 8-bit pool and gives the arguments whose older fields name its pages (older_k is
+// then not null, so that the lengths count, but no bf16 kernel may read through it).
+template <class Args>
+inline int32_t kv8_segment(const Args* a, const lkv_kv8_pool* older, Args& b, Kv8Pool& pool) {
+  if (const int32_t st = kv8_pool(older, "older", pool)) return st;
+  LKV_REQUIRE(a->older_k == nullptr && a->older_v == nullptr, "older_k and older_v must be NULL in a call over an 8-bit pool");
+  LKV_REQUIRE(a->older_block_table != nullptr, "a call over an 8-bit pool needs older_block_table");
+  LKV_REQUIRE(older->heads == a->num_kv_heads, "the 8-bit pool has %d kv heads, the call %d", older->heads, a->num_kv_heads);
+  b = *a;
+  b.older_k = older->k;
+  b.older_v = older->v;
+  b.older_seq_stride = 0;
+  b.older_head_stride = older->head_stride;
+  b.older_slot = nullptr;
+  b.older_num_slots = 0;
+  b.older_page_stride = older->page_stride;
+  b.older_num_pages = older->num_pages;
+  return LKV_OK;
+}
 
 // The largest split count a ragged call's decode-kernel classes take (a lone sequence of the class
 // then spreads over 32 workgroups per kv head: 256 at Hkv 8).

@@ -77,8 +77,9 @@ __device__ inline void combine_row(const DecodeParams& p, const float* ml, const
   }
   for (; s < S; ++s) O[0] += sm_w[s] * o[s * kHeadDim + d];
   const float Ot = (O[0] + O[1]) + (O[2] + O[3]);
-  out_row[d] = out_bits(L > 0.f ? Ot / L : 0.f, p.out_scale, kvh);
-  if (lse != nullptr && d == 0) *lse = L > 0.f ? (M + __log2f(L)) * kLn2 : kNegInf;
+  const bool some = p.keep_nan ? L != 0.f : L > 0.f;
+  out_row[d] = out_bits(some ? Ot / L : 0.f, p.out_scale, kvh);
+  if (lse != nullptr && d == 0) *lse = some ? (M + __log2f(L)) * kLn2 : kNegInf;
   __syncthreads();  // (sm_w and sm_red are reused by the caller's next row)
 }
 
@@ -136,8 +137,10 @@ int32_t launch_combine(const DecodeParams& p, int rows, hipStream_t s, const cha
 
 // cg: 0 for decode calls (one column per head), else the 16-column groups of a short prefill call
 int32_t launch_decode(const DecodeParams& p, dim3 grid, bool vscale, bool nt, int cg, int rows, hipStream_t s,
-                      const char* what) {
-  if (cg == 1) {
+                      const char* what, const Kv8Pool* older8) {
+  if (older8 != nullptr) {
+    launch_decode_kv8(p, *older8, grid, vscale, cg, s);
+  } else if (cg == 1) {
     launch_multi<1>(p, grid, vscale, nt, s);
   } else if (cg == 2) {
     launch_multi<2>(p, grid, vscale, nt, s);
@@ -239,6 +242,7 @@ int32_t plan_short_rows(const lkv_prefill_args* a, const SegParams& seg, int32_t
   plan.items = class_n > 0 ? int64_t{class_n} * a->num_kv_heads * p.splits : 0;
   plan.vscale = a->older_vscale_mode == 1;
   plan.nt = use_nontemporal(0, pairs * tokens * kHeadDim * 2 * 2);
+  p.keep_nan = 0;
   p.interleave = seg.o_tab == nullptr && seg.l_tab == nullptr;
   // the instance holds the class's widest sequence: 16, 32 or 64 columns
   const int64_t cols = std::min<int64_t>(col_hi, static_cast<int64_t>(group) * p.L);
@@ -257,13 +261,14 @@ int32_t combine_short_rows(const ShortRowsPlan& plan, hipStream_t s, const char*
 }
 
 int32_t prefill_on_decode_kernel(const lkv_prefill_args* a, const SegParams& seg, int32_t group, int32_t col_lo,
-                                 int32_t col_hi, int32_t class_n, hipStream_t s) {
+                                 int32_t col_hi, int32_t class_n, hipStream_t s, const Kv8Pool* older8) {
   ShortRowsPlan plan;
   if (const int32_t st = plan_short_rows(a, seg, group, col_lo, col_hi, class_n, a->workspace, a->workspace_bytes, plan))
     return st;
   if (plan.empty) return LKV_OK;
+  plan.p.keep_nan = older8 != nullptr;
   return launch_decode(plan.p, plan.grid, plan.vscale, plan.nt, plan.cg, plan.out_rows, s,
-                       "lkv_prefill_attn (short call on the decode kernel)");
+                       "lkv_prefill_attn (short call on the decode kernel)", older8);
 }
 
 }  // namespace lkv
@@ -297,7 +302,7 @@ int32_t check_decode_args(const lkv_decode_args* a) {
 }
 
 // The decode call of checked args with the split partials in `ws` (ws_bytes bytes).
-int32_t run_decode(const lkv_decode_args* a, void* ws, int64_t ws_bytes, hipStream_t stream) {
+int32_t run_decode(const lkv_decode_args* a, void* ws, int64_t ws_bytes, hipStream_t stream, const Kv8Pool* older8 = nullptr) {
   DecodeParams p;
   if (const int32_t st = fill_segments(a, p.seg)) return st;
   if (a->batch == 0) return LKV_OK;
@@ -335,12 +340,13 @@ int32_t run_decode(const lkv_decode_args* a, void* ws, int64_t ws_bytes, hipStre
   p.splits = a->num_splits;
   p.scale_log2 = a->sm_scale * kLog2e;
   const int64_t kv_bytes = static_cast<int64_t>(a->batch) * a->num_kv_heads * call_key_tokens(a) * kHeadDim * 2 * 2;
+  p.keep_nan = older8 != nullptr;
   p.interleave = p.seg.o_tab == nullptr && p.seg.l_tab == nullptr;
   // groups above 16 query heads per kv head take the multi-column instances (columns = heads)
   const int cg = group <= 16 ? 0 : group <= 32 ? 2 : 4;
   return launch_decode(p, dim3(a->num_splits, a->num_kv_heads, a->batch), a->older_vscale_mode == 1,
                        use_nontemporal(a->kv_cache_hint, kv_bytes), cg, a->batch * a->num_q_heads, stream,
-                       "lkv_decode_attn");
+                       "lkv_decode_attn", older8);
 }
 
 // Scratch of the allocation-free entry point: the split partials of one call, in a static device
@@ -376,6 +382,15 @@ extern "C" int32_t lkv_decode_attn(const lkv_decode_args* a, lkv_stream_t stream
   using namespace lkv;
   if (const int32_t st = check_decode_args(a)) return st;
   return run_decode(a, a->workspace, a->workspace_bytes, as_stream(stream));
+}
+
+extern "C" int32_t lkv_decode_attn_kv8(const lkv_decode_args* a, const lkv_kv8_pool* older, lkv_stream_t stream) {
+  using namespace lkv;
+  if (const int32_t st = check_decode_args(a)) return st;
+  lkv_decode_args b;
+  Kv8Pool pool;
+  if (const int32_t st = kv8_segment(a, older, b, pool)) return st;
+  return run_decode(&b, a->workspace, a->workspace_bytes, as_stream(stream), &pool);
 }
 
 extern "C" int32_t lkv_decode_attn_noalloc(const lkv_decode_args* a, lkv_stream_t stream) {

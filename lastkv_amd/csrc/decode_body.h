@@ -5,6 +5,7 @@
 
 #include "attn_common.h"
 #include "common.h"
+#include "kv8.h"
 #include "runtime.h"
 
 namespace lkv {
@@ -37,6 +38,7 @@ struct DecodeParams {
   const int32_t* cu;
   int32_t rows, col_lo, col_hi;
   int32_t dyn_splits, cus, lmax;
+  int32_t keep_nan;    // rows of a NaN sum become NaN (calls over an 8-bit pool), else 0
   int32_t interleave;  // tiled caches: sequences of more than kInterleaveBlocks key blocks interleave their splits
 };
 
@@ -283,6 +285,72 @@ __device__ inline bool decode_item(const DecodeParams& p, int wg, DecodeItem& it
   return true;
 }
 
+// Joins the waves' states of one work item and writes its output rows (one split) or its split's state.  kKeepNaN: a
+// row whose sum is NaN becomes NaN (else 0, as a row without keys).
+template <bool kMulti, int CG, bool kPairs, bool kKeepNaN = false>
+__device__ __attribute__((always_inline)) inline void decode_merge_waves(const DecodeParams& p, const DecodeItem& it,
+                                                                         const SoftmaxState (&st)[CG], DecodeShared<CG>& sm) {
+  constexpr int kWaveCols = 16 * CG;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n16 = lane & 15, g4 = lane >> 4;
+  const int G = p.group, kvh = it.kvh, b = it.b, split = it.split, S = it.S;
+  const int64_t ws_row0 = it.ws_row0;
+  const MultiRows mr = it.mr;
+  const int cols = kMulti ? G * mr.L : G;
+  const int cg0 = kPairs ? (wave >> 1) * CG : 0;
+  const auto some = [](float L) { return kKeepNaN ? L != 0.f : L > 0.f; };
+  // merge the four waves' states
+#pragma unroll
+  for (int cg = 0; cg < CG; ++cg) {
+    if (g4 == 0 && 16 * (cg0 + cg) + n16 < cols) {
+      sm.m[wave][16 * cg + n16] = st[cg].m;
+      sm.l[wave][16 * cg + n16] = st[cg].l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int hl = 16 * cg + 4 * g4 + i;  // column 16 * cg0 + hl
+      if (16 * cg0 + hl < cols) {
+#pragma unroll
+        for (int nb = 0; nb < 8; ++nb) sm.o[wave][hl][16 * nb + n16] = st[cg].o[nb][i];
+      }
+    }
+  }
+  __syncthreads();
+  for (int idx = threadIdx.x; idx < cols * kHeadDim; idx += 256) {
+    const int h = idx >> 7, d = idx & (kHeadDim - 1);  // column h = (token tq, head hh)
+    const int tq = kMulti ? h / G : 0, hh = h - tq * G;
+    const int64_t row_q = (mr.row0 + tq) * p.hq + kvh * G + hh;  // [rows, Hq] row
+    // the waves that hold column h: all four, or the pair of its column group
+    const int pair = kPairs ? h / kWaveCols : 0;
+    const int w0 = 2 * pair, hl = h - pair * kWaveCols;  // its waves and its column inside their range
+    constexpr int kMergeWaves = kPairs ? 2 : kDecodeWaves;
+    float M = sm.m[w0][hl];
+#pragma unroll
+    for (int w = w0 + 1; w < w0 + kMergeWaves; ++w) M = fmaxf(M, sm.m[w][hl]);
+    float L = 0.f, O = 0.f;
+#pragma unroll
+    for (int w = w0; w < w0 + kMergeWaves; ++w) {
+      const float f = sm.m[w][hl] == kDecodeNegInf ? 0.f : fast_exp2(sm.m[w][hl] - M);
+      L += f * sm.l[w][hl];
+      O += f * sm.o[w][hl][d];
+    }
+    if (S == 1) {
+      p.out[(kMulti && p.cu ? mr.row0 * p.out_st : b * p.out_sb) + (kMulti ? tq * p.out_st : 0) +
+            static_cast<int64_t>(kvh * G + hh) * kHeadDim + d] =
+          out_bits(some(L) ? O / L : 0.f, p.out_scale, kvh);
+      if (p.lse != nullptr && d == 0) p.lse[row_q] = some(L) ? (M + __log2f(L)) * kLn2 : kDecodeNegInf;
+    } else {
+      const int64_t row = ((ws_row0 + tq) * p.hq + kvh * G + hh) * S + split;
+      p.ws_o[row * kHeadDim + d] = O;
+      if (d == 0) {
+        p.ws_ml[row * 2] = M;
+        p.ws_ml[row * 2 + 1] = L;
+      }
+    }
+  }
+}
+
 // kMulti: L > 1 query tokens per sequence, column c = (token c / G, head c % G) for c < G * L <=
 // 16 * CG (CG <= 2 per wave: four groups spill), in CG groups of 16 columns that share each block's K/V fragments (short prefill calls);
 // otherwise column c = head c (L = 1, CG = 1).
@@ -293,13 +361,11 @@ __device__ inline bool decode_item(const DecodeParams& p, int wg, DecodeItem& it
 template <bool kVScale, bool kNT, bool kMulti, int CG, bool kPairs, bool kFold>
 __device__ __attribute__((always_inline)) inline void decode_split_body(const DecodeParams& p, const DecodeItem& it,
                                                                         DecodeShared<CG>& sm) {
-  constexpr int kWaveCols = 16 * CG;  // columns one wave holds (a pair's share with kPairs)
   constexpr int kStride = kPairs ? 2 : kDecodeWaves;  // block stride of one wave
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n16 = lane & 15, g4 = lane >> 4;
   const int G = p.group, kvh = it.kvh, b = it.b, split = it.split, S = it.S;
-  const int64_t ws_row0 = it.ws_row0;
   const MultiRows mr = it.mr;
   const int Lq = mr.L;
 
@@ -397,55 +463,7 @@ __device__ __attribute__((always_inline)) inline void decode_split_body(const De
     if (fold) compute(fc, rc);
   }
 
-  // merge the four waves' states
-#pragma unroll
-  for (int cg = 0; cg < CG; ++cg) {
-    if (g4 == 0 && 16 * (cg0 + cg) + n16 < cols) {
-      sm.m[wave][16 * cg + n16] = st[cg].m;
-      sm.l[wave][16 * cg + n16] = st[cg].l;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int hl = 16 * cg + 4 * g4 + i;  // column 16 * cg0 + hl
-      if (16 * cg0 + hl < cols) {
-#pragma unroll
-        for (int nb = 0; nb < 8; ++nb) sm.o[wave][hl][16 * nb + n16] = st[cg].o[nb][i];
-      }
-    }
-  }
-  __syncthreads();
-  for (int idx = threadIdx.x; idx < cols * kHeadDim; idx += 256) {
-    const int h = idx >> 7, d = idx & (kHeadDim - 1);  // column h = (token tq, head hh)
-    const int tq = kMulti ? h / G : 0, hh = h - tq * G;
-    const int64_t row_q = (mr.row0 + tq) * p.hq + kvh * G + hh;  // [rows, Hq] row
-    // the waves that hold column h: all four, or the pair of its column group
-    const int pair = kPairs ? h / kWaveCols : 0;
-    const int w0 = 2 * pair, hl = h - pair * kWaveCols;  // its waves and its column inside their range
-    constexpr int kMergeWaves = kPairs ? 2 : kDecodeWaves;
-    float M = sm.m[w0][hl];
-#pragma unroll
-    for (int w = w0 + 1; w < w0 + kMergeWaves; ++w) M = fmaxf(M, sm.m[w][hl]);
-    float L = 0.f, O = 0.f;
-#pragma unroll
-    for (int w = w0; w < w0 + kMergeWaves; ++w) {
-      const float f = sm.m[w][hl] == kDecodeNegInf ? 0.f : fast_exp2(sm.m[w][hl] - M);
-      L += f * sm.l[w][hl];
-      O += f * sm.o[w][hl][d];
-    }
-    if (S == 1) {
-      p.out[(kMulti && p.cu ? mr.row0 * p.out_st : b * p.out_sb) + (kMulti ? tq * p.out_st : 0) +
-            static_cast<int64_t>(kvh * G + hh) * kHeadDim + d] =
-          out_bits(L > 0.f ? O / L : 0.f, p.out_scale, kvh);
-      if (p.lse != nullptr && d == 0) p.lse[row_q] = L > 0.f ? (M + __log2f(L)) * kLn2 : kDecodeNegInf;
-    } else {
-      const int64_t row = ((ws_row0 + tq) * p.hq + kvh * G + hh) * S + split;
-      p.ws_o[row * kHeadDim + d] = O;
-      if (d == 0) {
-        p.ws_ml[row * 2] = M;
-        p.ws_ml[row * 2 + 1] = L;
-      }
-    }
-  }
+  decode_merge_waves<kMulti, CG, kPairs>(p, it, st, sm);
 }
 
 // Key tokens a call can read per sequence (lengths read from device memory bounded by the
@@ -479,6 +497,10 @@ struct ShortRowsPlan {
 // sequences in the class when the host knows it, else -1.
 int32_t plan_short_rows(const lkv_prefill_args* a, const SegParams& seg, int32_t group, int32_t col_lo, int32_t col_hi,
                         int32_t class_n, void* ws, int64_t ws_bytes, ShortRowsPlan& plan);
+
+// Launches the kernel whose older segment is the 8-bit pool `older` (its page table and lengths in p.seg); cg as in ShortRowsPlan,
+// 0: one column a head.
+void launch_decode_kv8(const DecodeParams& p, const Kv8Pool& older, dim3 grid, bool vscale, int cg, hipStream_t s);
 
 // Merges the key splits of a launched plan (nothing to do for one split).
 int32_t combine_short_rows(const ShortRowsPlan& plan, hipStream_t s, const char* what);

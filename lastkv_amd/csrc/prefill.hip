@@ -1520,13 +1520,37 @@ extern "C" int32_t lkv_prefill_plan(const lkv_prefill_args* a, lkv_prefill_plan_
   return LKV_OK;
 }
 
-extern "C" int32_t lkv_prefill_attn(const lkv_prefill_args* a, lkv_stream_t stream) {
+namespace {
+
+// Key blocks of the older segment per (sequence, kv head): exact for a host-constant length, else the capacity's.
+int64_t older_blocks(const lkv_prefill_args* a) {
+  const int64_t n = a->older_len != nullptr ? a->older_capacity_tokens
+                                            : std::min(std::max(a->older_len_const, 0), std::max(a->older_capacity_tokens, 0));
+  return (n + lkv::kBlockTokens - 1) / lkv::kBlockTokens;
+}
+
+// Whether the tile kernel may run, which reads 8-bit older pages through bf16 copies.
+bool tiles_possible(const lkv_prefill_args* a) {
+  const int64_t seq_tokens = a->cu_seqlens_q ? std::min(a->max_seqlen_q, a->tokens) : a->tokens;
+  return a->tile_waves != 0 || seq_tokens * (a->num_q_heads / a->num_kv_heads) > 64;
+}
+
+// Bytes of the bf16 copies of the older segment's blocks.
+int64_t kv8_copy_bytes(const lkv_prefill_args* a) {
+  if (!tiles_possible(a)) return 0;
+  return static_cast<int64_t>(a->batch) * a->num_kv_heads * older_blocks(a) * (2 * lkv::kBlockElems * 2);
+}
+
+// The call of an lkv_prefill_args; older8: the 8-bit pool that its older segment's table names, whose bf16 copies take `copies`
+// (kv8_copy_bytes of it, 16-byte aligned), or null.
+int32_t run_prefill(const lkv_prefill_args* a, const lkv::Kv8Pool* older8, void* copies, lkv_stream_t stream) {
   using namespace lkv;
   PrefillParams p;
   if (const int32_t st = check_prefill_args(a, p.seg)) return st;
   if (a->batch == 0 || a->tokens == 0) return LKV_OK;
   CallPlan c;
   if (const int32_t st = plan_call(a, p.seg, c)) return st;
+  if (older8 != nullptr) c.mixed = false;  // (the joint launch has no instance over 8-bit pages)
   const bool ragged = a->cu_seqlens_q != nullptr;
   const int group = a->num_q_heads / a->num_kv_heads;
   // query tokens per sequence (ragged: an upper bound)
@@ -1542,11 +1566,29 @@ extern "C" int32_t lkv_prefill_attn(const lkv_prefill_args* a, lkv_stream_t stre
       if (!ragged && max_cols > bounds[i + 1]) continue;
       if (c.host.known && c.host.class_n[i] == 0) continue;
       if (const int32_t st = prefill_on_decode_kernel(a, p.seg, group, bounds[i], bounds[i + 1],
-                                                      c.host.known ? c.host.class_n[i] : -1, s))
+                                                      c.host.known ? c.host.class_n[i] : -1, s, older8))
         return st;
     }
   }
   if (!c.runs_tiles) return LKV_OK;
+  const bool older_paged = older8 == nullptr && a->older_block_table != nullptr;
+  if (older8 != nullptr) {  // from here on the older segment is its bf16 copies, one run per (sequence, kv head)
+    const int64_t blocks = older_blocks(a), run = blocks * kBlockElems;
+    uint16_t* k16 = static_cast<uint16_t*>(copies);
+    uint16_t* v16 = k16 + static_cast<int64_t>(a->batch) * a->num_kv_heads * run;
+    if (const int32_t st = kv8_copy_blocks(a, *older8, group, c.short_on_decode && ragged ? 64 : 0, static_cast<int32_t>(blocks), k16,
+                                           v16, s))
+      return st;
+    p.seg.ok = k16;
+    p.seg.ov = v16;
+    p.seg.o_ss = a->num_kv_heads * run;
+    p.seg.o_hs = run;
+    p.seg.o_cap = static_cast<int32_t>(blocks * kBlockTokens);
+    p.seg.o_nslots = a->batch;
+    p.seg.o_tab = nullptr;
+    p.seg.o_page = kBlockElems;
+    p.seg.o_npages = 1;
+  }
   const int64_t vblocks = c.vblocks;
   p.q = static_cast<const uint16_t*>(a->q);
   p.q_sb = a->q_stride_b;
@@ -1580,7 +1622,7 @@ extern "C" int32_t lkv_prefill_attn(const lkv_prefill_args* a, lkv_stream_t stre
   p.tiles = static_cast<int32_t>(c.tile.tiles);
   p.hkv = a->num_kv_heads;
   p.batch = a->batch;
-  const bool paged = a->older_block_table != nullptr || a->local_block_table != nullptr;
+  const bool paged = older_paged || a->local_block_table != nullptr;
   if (vblocks > 0) {  // (no keys at all: every row's output is zero; the main kernel skips its loop)
     const int per_wg = ragged ? 8 : 1;
     const dim3 vgrid(static_cast<unsigned>((vblocks + per_wg - 1) / per_wg), a->num_kv_heads,
@@ -1616,4 +1658,36 @@ extern "C" int32_t lkv_prefill_attn(const lkv_prefill_args* a, lkv_stream_t stre
   LKV_REQUIRE((items + 3) / 4 < (1LL << 31), "too many query rows");
   prefill_split_combine_kernel<<<static_cast<unsigned>((items + 3) / 4), 256, 0, s>>>(p, c.tile.rows_all);
   return check_launch("lkv_prefill_attn (key-split merge)");
+}
+
+}  // namespace
+
+extern "C" int32_t lkv_prefill_attn(const lkv_prefill_args* a, lkv_stream_t stream) {
+  return run_prefill(a, nullptr, nullptr, stream);
+}
+
+extern "C" int64_t lkv_prefill_kv8_workspace_bytes(const lkv_prefill_args* a) {
+  if (a == nullptr || a->batch <= 0 || a->num_kv_heads <= 0 || a->num_q_heads <= 0) return 0;
+  lkv_prefill_args b = *a;
+  b.older_k = b.older_v = a;  // (not null: the older segment's blocks count)
+  return kv8_copy_bytes(&b) + lkv_prefill_workspace_bytes(&b);
+}
+
+extern "C" int32_t lkv_prefill_attn_kv8(const lkv_prefill_args* a, const lkv_kv8_pool* older, lkv_stream_t stream) {
+  using namespace lkv;
+  LKV_REQUIRE(a != nullptr, "null args");
+  LKV_REQUIRE(a->struct_size == static_cast<int32_t>(sizeof(lkv_prefill_args)),
+              "lkv_prefill_args size mismatch (caller %d, library %d)", a->struct_size,
+              static_cast<int32_t>(sizeof(lkv_prefill_args)));
+  LKV_REQUIRE(a->batch >= 0 && a->tokens >= 0 && a->num_kv_heads > 0 && a->num_q_heads > 0, "bad sizes");
+  lkv_prefill_args b;
+  Kv8Pool pool;
+  if (const int32_t st = kv8_segment(a, older, b, pool)) return st;
+  const int64_t copies = kv8_copy_bytes(&b);
+  LKV_REQUIRE(copies == 0 || (a->workspace != nullptr && a->workspace_bytes > copies),
+              "prefill over an 8-bit pool needs a workspace of %lld bytes (lkv_prefill_kv8_workspace_bytes), got %lld",
+              static_cast<long long>(lkv_prefill_kv8_workspace_bytes(a)), static_cast<long long>(a->workspace_bytes));
+  b.workspace = a->workspace == nullptr ? nullptr : static_cast<uint8_t*>(a->workspace) + copies;
+  b.workspace_bytes = a->workspace_bytes - copies;
+  return run_prefill(&b, &pool, a->workspace, stream);
 }

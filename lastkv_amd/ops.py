@@ -161,6 +161,67 @@ class PagedKV:
         return self.k.device
 
 
+@dataclass
+class PagedKV8:
+    """K and V page pools in 8 bits: e4m3 codes ``[heads, pages, 4096]`` (float8_e4m3fn, in the layout that the attention
+    kernels read) and one scale byte for each page of each head, ``[heads, pages]`` uint8; byte e stands for
+    2^(e - 127), 255 for NaN.  Pages are addressed by block tables as those of a ``PagedKV``; ``kv8_quantize`` fills them
+    from bf16 pages, ``decode_attention`` and ``prefill_attention`` read them as their older segment."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scales: torch.Tensor
+    v_scales: torch.Tensor
+
+    def __post_init__(self) -> None:
+        for name in ("k", "v", "k_scales", "v_scales"):
+            t = getattr(self, name)
+            _require(isinstance(t, torch.Tensor), f"PagedKV8.{name} must be a tensor")
+            _require(t.is_cuda and t.device == self.k.device, f"PagedKV8.{name} must be on the pool's GPU (the kernels have no CPU path)")
+            _require(t.is_contiguous(), f"PagedKV8.{name} must be contiguous")
+            codes = name in ("k", "v")
+            _require(t.dtype == (torch.float8_e4m3fn if codes else torch.uint8),
+                     f"PagedKV8.{name} must be {'float8_e4m3fn' if codes else 'uint8'}, got {t.dtype}")
+            _require(t.dim() == (3 if codes else 2) and t.shape[:2] == self.k.shape[:2] and (not codes or t.shape[2] == BLOCK_ELEMS),
+                     f"PagedKV8.{name} must be [heads, pages{', 4096' if codes else ''}], as k")
+
+    @classmethod
+    def zeros(cls, pages: int, heads: int, device: torch.device | str) -> "PagedKV8":
+        codes, scales = (heads, pages, BLOCK_ELEMS), (heads, pages)
+        return cls(*(torch.zeros(codes, dtype=torch.float8_e4m3fn, device=device) for _ in range(2)),
+                   *(torch.zeros(scales, dtype=torch.uint8, device=device) for _ in range(2)))
+
+    @property
+    def pages(self) -> int:
+        return int(self.k.shape[1])
+
+    @property
+    def heads(self) -> int:
+        return int(self.k.shape[0])
+
+    @property
+    def page_stride(self) -> int:
+        return BLOCK_ELEMS
+
+    @property
+    def head_stride(self) -> int:
+        return self.pages * BLOCK_ELEMS
+
+    @property
+    def device(self) -> torch.device:
+        return self.k.device
+
+
+def _kv8_pool(pool: PagedKV8) -> "_lib.Kv8Pool":
+    pool.__post_init__()  # (its fields can be assigned)
+    a = _lib.Kv8Pool()
+    a.struct_size = ctypes.sizeof(_lib.Kv8Pool)
+    a.num_pages, a.heads = pool.pages, pool.heads
+    a.k, a.v, a.k_scales, a.v_scales = (t.data_ptr() for t in (pool.k, pool.v, pool.k_scales, pool.v_scales))
+    a.page_stride, a.head_stride, a.scale_head_stride = pool.page_stride, pool.head_stride, pool.pages
+    return a
+
+
 _host_bound = False
 
 
@@ -276,7 +337,7 @@ def _fill_segments(a, B: int, device: torch.device, older, older_len, older_slot
                    local_start, local_slot, older_table=None, local_table=None, local_ring_blocks=None) -> int:
     """Fill the older/local segment fields shared by DecodeArgs and PrefillArgs; returns Hkv.
 
-    ``older`` / ``local`` are a TiledKV (contiguous per slot) or a PagedKV with a block table
+    ``older`` / ``local`` are a TiledKV (contiguous per slot) or a PagedKV (``older`` also a PagedKV8) with a block table
     (``older_table`` [B, W]: older block j of sequence b is page ``older_table[b, j]``;
     ``local_table`` [B, >= ring blocks]: ring block rb is page ``local_table[b, rb]``)."""
 
@@ -295,10 +356,11 @@ def _fill_segments(a, B: int, device: torch.device, older, older_len, older_slot
                      f"{name} must be a contiguous int32 tensor of {B} entries on {device}")
     if older is not None:
         _require(older.device == device, "older cache on another device")
-        a.older_k, a.older_v = older.k.data_ptr(), older.v.data_ptr()
+        if not isinstance(older, PagedKV8):  # (an 8-bit pool goes to the library by itself)
+            a.older_k, a.older_v = older.k.data_ptr(), older.v.data_ptr()
         a.older_head_stride = older.head_stride
         a.older_len, a.older_len_const = _len_arg(older_len, B, "older_len", device)
-        if isinstance(older, PagedKV):
+        if isinstance(older, (PagedKV, PagedKV8)):
             _table_arg(older_table, B, "older", device)
             _require(older_slot is None, "older_slot does not apply to a paged segment")
             a.older_block_table, a.older_table_stride = older_table.data_ptr(), older_table.stride(0)
@@ -315,6 +377,7 @@ def _fill_segments(a, B: int, device: torch.device, older, older_len, older_slot
         if not isinstance(older_len, torch.Tensor):
             _require(0 <= older_len <= a.older_capacity_tokens, "older_len exceeds the cache capacity")
     if local is not None:
+        _require(not isinstance(local, PagedKV8), "the local segment is bf16 (a TiledKV or PagedKV)")
         _require(local.device == device, "local cache on another device")
         a.local_k, a.local_v = local.k.data_ptr(), local.v.data_ptr()
         a.local_head_stride = local.head_stride
@@ -353,7 +416,7 @@ def _out_scale_arg(a, out_scale: torch.Tensor | None, Hkv: int, device: torch.de
 def decode_attention(
     q: torch.Tensor,
     *,
-    older: TiledKV | PagedKV | None = None,
+    older: TiledKV | PagedKV | PagedKV8 | None = None,
     older_len: int | torch.Tensor = 0,
     older_slot: torch.Tensor | None = None,
     vscale: torch.Tensor | None = None,
@@ -384,6 +447,9 @@ def decode_attention(
     ``lkv_decode_attn_noalloc``: the split states go to the library's static per-GPU scratch
     (LKV_NOALLOC_SCRATCH_BYTES) instead of a workspace (pass ``out`` too for a call that allocates
     nothing); calls overlapping on one GPU then race.
+
+    With a ``PagedKV8`` as ``older`` (and ``older_table``) the result is the attention over the values of its codes;
+    a sequence that sees a token of a NaN block has NaN outputs, and ``kv_cache_hint`` has no effect.
     """
 
     if not no_alloc and (_host_bound or _bind_host()):
@@ -440,7 +506,12 @@ def decode_attention(
     a.lse = _ptr(lse)
     a.workspace = _ptr(workspace)
     a.workspace_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    if no_alloc:
+    if isinstance(older, PagedKV8):
+        _require(not no_alloc, "no_alloc calls read a bf16 cache")
+        pool = _kv8_pool(older)
+        with _on_device(device):
+            _lib.check(lib.lkv_decode_attn_kv8(ctypes.byref(a), ctypes.byref(pool), _stream(device)), "lkv_decode_attn_kv8")
+    elif no_alloc:
         _lib.check(lib.lkv_decode_attn_noalloc(ctypes.byref(a), _stream(device)), "lkv_decode_attn_noalloc")
     else:
         _lib.check(lib.lkv_decode_attn(ctypes.byref(a), _stream(device)), "lkv_decode_attn")
@@ -450,7 +521,7 @@ def decode_attention(
 def prefill_attention(
     q: torch.Tensor,
     *,
-    older: TiledKV | PagedKV | None = None,
+    older: TiledKV | PagedKV | PagedKV8 | None = None,
     older_len: int | torch.Tensor = 0,
     older_slot: torch.Tensor | None = None,
     vscale: torch.Tensor | None = None,
@@ -493,7 +564,9 @@ def prefill_attention(
     choose from the grid size and the device's CU count.  4 or 8 put a uniform call on the tile
     kernel at any size; in a ragged call they apply to its sequences above 64 query rows per kv
     head, and its shorter ones stay on the decode kernel unless all of its sequences are short.
-    ``out_scale`` as in ``decode_attention``."""
+    ``out_scale`` as in ``decode_attention``.  With a ``PagedKV8`` as ``older`` the values of its codes
+    are attended to; the workspace (``prefill_kv8_workspace_bytes``) then also holds bf16 copies of its blocks for
+    sequences above 64 query rows per kv head."""
 
     if _host_bound or _bind_host():
         done = _host.prefill_attention(q, older, older_len, older_slot, vscale, local, local_len, local_start, local_slot,
@@ -555,12 +628,18 @@ def prefill_attention(
     a.out, a.out_stride_b, a.out_stride_t = out.data_ptr(), out.stride(0), out.stride(1)
     a.lse = _ptr(lse)
     lib = _lib.load()
+    kv8 = isinstance(older, PagedKV8)
     if workspace is None:  # room for the tile kernel's key splits too
-        workspace = torch.empty(max(int(lib.lkv_prefill_workspace_bytes(ctypes.byref(a))), 16), dtype=torch.uint8,
-                                device=device)
+        size = lib.lkv_prefill_kv8_workspace_bytes if kv8 else lib.lkv_prefill_workspace_bytes
+        workspace = torch.empty(max(int(size(ctypes.byref(a))), 16), dtype=torch.uint8, device=device)
     _require(workspace.device == device and workspace.is_contiguous(), "workspace must be a contiguous tensor on the query's device")
     a.workspace = workspace.data_ptr()
     a.workspace_bytes = workspace.numel() * workspace.element_size()
+    if kv8:
+        pool = _kv8_pool(older)
+        with _on_device(device):
+            _lib.check(lib.lkv_prefill_attn_kv8(ctypes.byref(a), ctypes.byref(pool), _stream(device)), "lkv_prefill_attn_kv8")
+        return out[0] if ragged else out
     need = int(lib.lkv_prefill_workspace_min_bytes(ctypes.byref(a)))
     _require(a.workspace_bytes >= need, f"prefill workspace too small: {a.workspace_bytes} < {need} bytes")
     _lib.check(lib.lkv_prefill_attn(ctypes.byref(a), _stream(device)), "lkv_prefill_attn")
@@ -1007,6 +1086,154 @@ def silu_mul(gate: torch.Tensor, up: torch.Tensor, out: torch.Tensor | None = No
     _lib.check(_lib.load().lkv_silu_mul(gate.data_ptr(), gs, up.data_ptr(), us, out.data_ptr(), os_, rows, width,
                                         _stream(gate.device)), "lkv_silu_mul")
     return out
+
+
+def kv8_quantize(src: PagedKV, dst: PagedKV8, *, src_table: torch.Tensor, dst_table: torch.Tensor,
+                 tokens: int | torch.Tensor, first_block: int = 0, blocks: int | None = None) -> None:
+    """Blocks ``[first_block, first_block + blocks)`` of every sequence from bf16 pages into 8-bit pages: block j of
+    sequence b, page ``src_table[b, j]`` of ``src``, becomes page ``dst_table[b, j]`` of ``dst`` (both tables int32
+    ``[B, W]``; ``blocks`` defaults to the rest of the narrower one).
+
+    ``tokens`` (an int, or int32 ``[B]`` on the device) says how many tokens a sequence has: a block's scale is the smallest
+    power of two whose multiple by 448 reaches its greatest |value| among them, its codes the nearest e4m3 values, ties to even;
+    tokens past the end are stored as 0, and blocks past it left as they are.  A block that holds an infinity or NaN is NaN
+    (scale byte 255).  A destination page must not occur twice in one call."""
+
+    _require(isinstance(src, PagedKV) and isinstance(dst, PagedKV8), "kv8_quantize takes a PagedKV to a PagedKV8")
+    device = src.device
+    _require(dst.device == device, "the pools are on different devices")
+    _require(src.heads == dst.heads, f"the pools have {src.heads} and {dst.heads} kv heads")
+    _require(isinstance(src_table, torch.Tensor) and src_table.dim() == 2, "src_table must be an int32 [B, W] tensor")
+    B = src_table.shape[0]
+    _table_arg(src_table, B, "src", device)
+    _table_arg(dst_table, B, "dst", device)
+    width = min(src_table.shape[1], dst_table.shape[1])
+    blocks = width - int(first_block) if blocks is None else int(blocks)
+    _require(0 <= first_block and 0 <= blocks and first_block + blocks <= width,
+             f"blocks [{first_block}, {first_block + blocks}) exceed the tables' {width}")
+    src.__post_init__()
+    a = _lib.Kv8QuantizeArgs()
+    a.struct_size = ctypes.sizeof(_lib.Kv8QuantizeArgs)
+    a.batch, a.heads, a.head_dim, a.first_block, a.blocks = B, src.heads, HEAD_DIM, int(first_block), blocks
+    a.tokens, a.tokens_const = _len_arg(tokens, B, "tokens", device)
+    _require(isinstance(tokens, torch.Tensor) or (tokens is not None and a.tokens_const >= 0), "tokens must not be negative")
+    a.src_num_pages, a.src_page_stride, a.src_head_stride = src.pages, src.page_stride, src.head_stride
+    a.src_k, a.src_v = src.k.data_ptr(), src.v.data_ptr()
+    a.src_table, a.src_table_stride, a.src_table_width = src_table.data_ptr(), src_table.stride(0), src_table.shape[1]
+    a.dst_table, a.dst_table_stride, a.dst_table_width = dst_table.data_ptr(), dst_table.stride(0), dst_table.shape[1]
+    pool = _kv8_pool(dst)
+    with _on_device(device):
+        _lib.check(_lib.load().lkv_kv8_quantize(ctypes.byref(a), ctypes.byref(pool), _stream(device)), "lkv_kv8_quantize")
+
+
+def kv8_unpack(pool: PagedKV8, table: torch.Tensor, token0: int, tokens: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """K and V of tokens ``[token0, token0 + tokens)`` of every sequence, ``[B, H, tokens, 128]`` bf16 each (the codes' values
+    are exact in bf16)."""
+
+    _require(isinstance(pool, PagedKV8), "kv8_unpack takes a PagedKV8")
+    device = pool.device
+    _require(isinstance(table, torch.Tensor) and table.dim() == 2, "the table must be an int32 [B, W] tensor")
+    B = table.shape[0]
+    _table_arg(table, B, "unpack", device)
+    _require(token0 >= 0 and tokens >= 0 and token0 + tokens <= table.shape[1] * BLOCK_TOKENS,
+             f"tokens [{token0}, {token0 + tokens}) exceed the table's {table.shape[1]} blocks")
+    k, v = (torch.empty((B, pool.heads, tokens, HEAD_DIM), dtype=torch.bfloat16, device=device) for _ in range(2))
+    a = _kv8_pool(pool)
+    with _on_device(device):
+        _lib.check(_lib.load().lkv_kv8_unpack(
+            ctypes.byref(a), table.data_ptr(), table.stride(0), table.shape[1], B, int(token0), int(tokens), k.data_ptr(),
+            k.stride(0), k.stride(1), k.stride(2), v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), _stream(device)),
+            "lkv_kv8_unpack")
+    return k, v
+
+
+def prefill_kv8_workspace_bytes(batch: int, kv_heads: int, older_tokens: int, local_tokens: int, **kwargs) -> int:
+    """``prefill_workspace_bytes`` of a call whose older segment is a ``PagedKV8``: with room for bf16 copies of its
+    blocks."""
+
+    return (prefill_workspace_bytes(batch, kv_heads, older_tokens, local_tokens, **kwargs)
+            + batch * kv_heads * -(-older_tokens // BLOCK_TOKENS) * 2 * BLOCK_ELEMS * 2)
+
+
+def _page_list(name: str, ids) -> np.ndarray:
+    _require(not (isinstance(ids, torch.Tensor) and ids.is_cuda), f"{name} must be in host memory (a sequence of ints or an array)")
+    a = np.asarray(ids)
+    if a.size == 0:
+        a = a.astype(np.int32).reshape(-1)
+    _require(a.ndim == 1 and np.issubdtype(a.dtype, np.integer), f"{name} must be a list of page ids")
+    _require(a.dtype == np.int32 or a.size == 0 or (int(a.min()) >= 0 and int(a.max()) < 1 << 31), f"{name} holds ids outside the pool")
+    return np.ascontiguousarray(a, dtype=np.int32)
+
+
+def copy_pages(pool: PagedKV | PagedKV8, src, dst) -> None:
+    """Page ``dst[i]`` := page ``src[i]`` of the pool, every head's K and V (and scales), for all i at once.  ``src`` and
+    ``dst`` are host lists or integer arrays of one length: no page may be a destination twice or both a source and a
+    destination.  The lists are read during the call (a captured call keeps its pairs) and the copies run on the
+    current stream, without a wait."""
+
+    _require(isinstance(pool, (PagedKV, PagedKV8)), "copy_pages takes a PagedKV or a PagedKV8")
+    s, d = _page_list("src", src), _page_list("dst", dst)
+    _require(s.size == d.size, f"src and dst name {s.size} and {d.size} pages")
+    a = _lib.CopyPagesArgs()
+    a.struct_size = ctypes.sizeof(_lib.CopyPagesArgs)
+    a.count, a.heads, a.num_pages = s.size, pool.heads, pool.pages
+    a.src, a.dst = s.ctypes.data, d.ctypes.data
+    pool.__post_init__()
+    size = pool.k.element_size()
+    a.k, a.v = pool.k.data_ptr(), pool.v.data_ptr()
+    a.page_bytes, a.page_stride, a.head_stride = BLOCK_ELEMS * size, pool.page_stride * size, pool.head_stride * size
+    if isinstance(pool, PagedKV8):
+        a.k_scales, a.v_scales, a.scale_head_stride = pool.k_scales.data_ptr(), pool.v_scales.data_ptr(), pool.pages
+    with _on_device(pool.device):
+        _lib.check(_lib.load().lkv_copy_pages(ctypes.byref(a), _stream(pool.device)), "lkv_copy_pages")
+
+
+def beam_workspace_bytes(batch: int, beams: int, vocab: int, count: int) -> int:
+    """Bytes of the workspace ``beam_select`` needs."""
+
+    return int(_lib.load().lkv_beam_workspace_bytes(batch, beams, vocab, count))
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int, *, workspace: torch.Tensor | None = None
+                ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The ``count`` best candidates of each prompt's beams: ``logits`` ``[B, K, V]`` (bf16 or fp32, contiguous rows) and
+    ``scores`` fp32 ``[B, K]`` (the beams' log-probabilities so far, -inf for none) give the greatest of
+    ``scores[b, k] + log_softmax(logits[b, k])[v]`` in descending order, equal ones by lowest beam, then greatest
+    logit (one beam's candidates stand in the exact order of their logits), then lowest token.
+
+    Returns (scores fp32, beams int32, tokens int32), ``[B, count]`` each.  Totals that are NaN or infinite are no candidates;
+    entries without one are (-inf, -1, -1).  ``workspace`` (uint8, ``beam_workspace_bytes``) is the call's alone while it
+    runs; without it one is allocated."""
+
+    _require(isinstance(logits, torch.Tensor) and logits.is_cuda, "logits must be on a GPU (the kernels have no CPU path)")
+    _require(logits.dtype in (torch.bfloat16, torch.float32), f"logits must be bfloat16 or float32, got {logits.dtype}")
+    _require(logits.dim() == 3 and logits.shape[1] >= 1 and logits.shape[2] >= 1 and (logits.stride(2) == 1 or logits.shape[2] == 1),
+             "logits must be [B, K, V] with contiguous rows")
+    B, K, V = logits.shape
+    device = logits.device
+    _require(isinstance(scores, torch.Tensor) and scores.dtype == torch.float32 and scores.device == device
+             and tuple(scores.shape) == (B, K) and (scores.stride(1) == 1 or K == 1),
+             "scores must be fp32 [B, K] with contiguous rows on the logits' device")
+    _require(isinstance(count, int) and 1 <= count <= 64, f"count must be in [1, 64], got {count}")
+    _require(K <= 64 and V <= 1 << 20 and B * K <= 65535, "beam_select takes up to 64 beams, 2^20 tokens and 65535 rows")
+    need = beam_workspace_bytes(B, K, V, count)
+    if workspace is None:
+        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+    _require(workspace.device == device and workspace.is_contiguous() and workspace.numel() * workspace.element_size() >= need,
+             f"workspace too small: {need} bytes are needed on {device}")
+    out = torch.empty((B, count), dtype=torch.float32, device=device)
+    beams, tokens = (torch.empty((B, count), dtype=torch.int32, device=device) for _ in range(2))
+    a = _lib.BeamSelectArgs()
+    a.struct_size = ctypes.sizeof(_lib.BeamSelectArgs)
+    a.batch, a.beams, a.vocab, a.count = B, K, V, count
+    a.logits_fp32 = 1 if logits.dtype == torch.float32 else 0
+    a.logits, a.logits_stride_b, a.logits_stride_k = logits.data_ptr(), logits.stride(0), logits.stride(1)
+    a.scores, a.scores_stride_b = scores.data_ptr(), scores.stride(0)
+    a.out_scores, a.out_beams, a.out_tokens = out.data_ptr(), beams.data_ptr(), tokens.data_ptr()
+    a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    with _on_device(device):
+        _lib.check(_lib.load().lkv_beam_select(ctypes.byref(a), _stream(device)), "lkv_beam_select")
+    return out, beams, tokens
 
 
 MX_BLOCK = 32  # values that share one scale
