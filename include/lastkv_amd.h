@@ -696,9 +696,9 @@ typedef struct lkv_kv8_pool {
   void *v;
   int64_t page_stride; /* at least 4096 */
   int64_t head_stride;
-  void *k_scales;
+  void *k_scales; /* 4-byte aligned; heads * scale_head_stride bytes are read, by words */
   void *v_scales;
-  int64_t scale_head_stride;
+  int64_t scale_head_stride; /* a multiple of 4, at least num_pages */
 } lkv_kv8_pool;
 
 /* Blocks [first_block, first_block + blocks) of every sequence's bf16 pages into 8-bit pages: block j of sequence b is page

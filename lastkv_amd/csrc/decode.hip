@@ -139,7 +139,7 @@ int32_t launch_combine(const DecodeParams& p, int rows, hipStream_t s, const cha
 int32_t launch_decode(const DecodeParams& p, dim3 grid, bool vscale, bool nt, int cg, int rows, hipStream_t s,
                       const char* what, const Kv8Pool* older8) {
   if (older8 != nullptr) {
-    launch_decode_kv8(p, *older8, grid, vscale, cg, s);
+    launch_decode_kv8(p, *older8, grid, vscale, nt, cg, s);
   } else if (cg == 1) {
     launch_multi<1>(p, grid, vscale, nt, s);
   } else if (cg == 2) {
@@ -267,6 +267,8 @@ int32_t prefill_on_decode_kernel(const lkv_prefill_args* a, const SegParams& seg
     return st;
   if (plan.empty) return LKV_OK;
   plan.p.keep_nan = older8 != nullptr;
+  if (older8 != nullptr)
+    plan.nt = use_nontemporal(0, static_cast<int64_t>(a->batch) * a->num_kv_heads * call_key_bytes(a, true));
   return launch_decode(plan.p, plan.grid, plan.vscale, plan.nt, plan.cg, plan.out_rows, s,
                        "lkv_prefill_attn (short call on the decode kernel)", older8);
 }
@@ -339,7 +341,7 @@ int32_t run_decode(const lkv_decode_args* a, void* ws, int64_t ws_bytes, hipStre
   p.group = group;
   p.splits = a->num_splits;
   p.scale_log2 = a->sm_scale * kLog2e;
-  const int64_t kv_bytes = static_cast<int64_t>(a->batch) * a->num_kv_heads * call_key_tokens(a) * kHeadDim * 2 * 2;
+  const int64_t kv_bytes = static_cast<int64_t>(a->batch) * a->num_kv_heads * call_key_bytes(a, older8 != nullptr);
   p.keep_nan = older8 != nullptr;
   p.interleave = p.seg.o_tab == nullptr && p.seg.l_tab == nullptr;
   // groups above 16 query heads per kv head take the multi-column instances (columns = heads)

@@ -235,11 +235,11 @@ __device__ inline void compute_block(const BlockFrags& f, const BlockRef& r, con
 // LDS of one decode workgroup: the waves' states of the columns each holds, indexed by the column inside
 // the wave's own range (with kPairs each wave pair stages only its half of the columns, so the staging
 // takes 64 KiB at most and two workgroups fit on a CU).
-template <int CG>
+template <int CG, int kWaves = kDecodeWaves>
 struct DecodeShared {
-  float m[kDecodeWaves][16 * CG];
-  float l[kDecodeWaves][16 * CG];
-  float o[kDecodeWaves][16 * CG][kHeadDim];
+  float m[kWaves][16 * CG];
+  float l[kWaves][16 * CG];
+  float o[kWaves][16 * CG][kHeadDim];
 };
 
 // One (sequence, kv head, key split): its workgroup's share of the call.
@@ -287,9 +287,10 @@ __device__ inline bool decode_item(const DecodeParams& p, int wg, DecodeItem& it
 
 // Joins the waves' states of one work item and writes its output rows (one split) or its split's state.  kKeepNaN: a
 // row whose sum is NaN becomes NaN (else 0, as a row without keys).
-template <bool kMulti, int CG, bool kPairs, bool kKeepNaN = false>
+template <bool kMulti, int CG, bool kPairs, bool kKeepNaN = false, int kWaves = kDecodeWaves>
 __device__ __attribute__((always_inline)) inline void decode_merge_waves(const DecodeParams& p, const DecodeItem& it,
-                                                                         const SoftmaxState (&st)[CG], DecodeShared<CG>& sm) {
+                                                                         const SoftmaxState (&st)[CG],
+                                                                         DecodeShared<CG, kWaves>& sm) {
   constexpr int kWaveCols = 16 * CG;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -298,9 +299,9 @@ __device__ __attribute__((always_inline)) inline void decode_merge_waves(const D
   const int64_t ws_row0 = it.ws_row0;
   const MultiRows mr = it.mr;
   const int cols = kMulti ? G * mr.L : G;
-  const int cg0 = kPairs ? (wave >> 1) * CG : 0;
+  const int cg0 = kPairs ? wave / (kWaves / 2) * CG : 0;
   const auto some = [](float L) { return kKeepNaN ? L != 0.f : L > 0.f; };
-  // merge the four waves' states
+  // merge the waves' states
 #pragma unroll
   for (int cg = 0; cg < CG; ++cg) {
     if (g4 == 0 && 16 * (cg0 + cg) + n16 < cols) {
@@ -317,14 +318,14 @@ __device__ __attribute__((always_inline)) inline void decode_merge_waves(const D
     }
   }
   __syncthreads();
-  for (int idx = threadIdx.x; idx < cols * kHeadDim; idx += 256) {
+  for (int idx = threadIdx.x; idx < cols * kHeadDim; idx += 64 * kWaves) {
     const int h = idx >> 7, d = idx & (kHeadDim - 1);  // column h = (token tq, head hh)
     const int tq = kMulti ? h / G : 0, hh = h - tq * G;
     const int64_t row_q = (mr.row0 + tq) * p.hq + kvh * G + hh;  // [rows, Hq] row
-    // the waves that hold column h: all four, or the pair of its column group
+    // the waves that hold column h: all of them, or the half of its column group
     const int pair = kPairs ? h / kWaveCols : 0;
-    const int w0 = 2 * pair, hl = h - pair * kWaveCols;  // its waves and its column inside their range
-    constexpr int kMergeWaves = kPairs ? 2 : kDecodeWaves;
+    constexpr int kMergeWaves = kPairs ? kWaves / 2 : kWaves;
+    const int w0 = kMergeWaves * pair, hl = h - pair * kWaveCols;  // its waves and its column inside their range
     float M = sm.m[w0][hl];
 #pragma unroll
     for (int w = w0 + 1; w < w0 + kMergeWaves; ++w) M = fmaxf(M, sm.m[w][hl]);
@@ -469,15 +470,26 @@ __device__ __attribute__((always_inline)) inline void decode_split_body(const De
 // Key tokens a call can read per sequence (lengths read from device memory bounded by the
 // capacities); Args is lkv_decode_args or lkv_prefill_args (same segment fields).
 template <typename Args>
-inline int64_t call_key_tokens(const Args* a) {
-  const int64_t ring_tokens = static_cast<int64_t>(a->local_ring_blocks) * kBlockTokens;
+inline int64_t call_older_tokens(const Args* a) {
   const int64_t older = a->older_k == nullptr ? 0
                                               : (a->older_len != nullptr ? a->older_capacity_tokens
                                                                          : std::min(a->older_len_const, a->older_capacity_tokens));
+  return std::max<int64_t>(older, 0);
+}
+
+template <typename Args>
+inline int64_t call_key_tokens(const Args* a) {
+  const int64_t ring_tokens = static_cast<int64_t>(a->local_ring_blocks) * kBlockTokens;
   const int64_t local = a->local_k == nullptr
                             ? 0
                             : (a->local_len != nullptr ? ring_tokens : std::min<int64_t>(a->local_len_const, ring_tokens));
-  return std::max<int64_t>(older, 0) + std::max<int64_t>(local, 0);
+  return call_older_tokens(a) + std::max<int64_t>(local, 0);
+}
+
+// Bytes of K and V that a (sequence, kv head) of the call can read.
+template <typename Args>
+inline int64_t call_key_bytes(const Args* a, bool older8) {
+  return (call_key_tokens(a) * 2 - (older8 ? call_older_tokens(a) : 0)) * kHeadDim * 2;
 }
 
 // The launch of a ragged or short prefill call's sequences of one column class (col_lo < group * tokens <=
@@ -500,7 +512,7 @@ int32_t plan_short_rows(const lkv_prefill_args* a, const SegParams& seg, int32_t
 
 // Launches the kernel whose older segment is the 8-bit pool `older` (its page table and lengths in p.seg); cg as in ShortRowsPlan,
 // 0: one column a head.
-void launch_decode_kv8(const DecodeParams& p, const Kv8Pool& older, dim3 grid, bool vscale, int cg, hipStream_t s);
+void launch_decode_kv8(const DecodeParams& p, const Kv8Pool& older, dim3 grid, bool vscale, bool nt, int cg, hipStream_t s);
 
 // Merges the key splits of a launched plan (nothing to do for one split).
 int32_t combine_short_rows(const ShortRowsPlan& plan, hipStream_t s, const char* what);

@@ -1,10 +1,10 @@
 // Split-K decode attention over [8-bit shared pages | bf16 ring], also of a few query tokens a sequence.
 //
-// The scheme is the bf16 kernel's (decode.hip): a workgroup of 4 waves takes one (sequence, kv head, key split), a
+// The scheme is the bf16 kernel's (decode.hip): a workgroup takes one (sequence, kv head, key split), a
 // wave streams 32-token blocks from HBM to registers and keeps a running maximum, sum and O of its columns.  An older
 // block is 8 KiB (K and V codes, 8 loads of 1 KiB) and two scale bytes; its codes become the exact bf16 operands of the bf16
 // kernel (one conversion instruction for two values, the block's power of two applied by it), so that scores, softmax and
-// sums are that kernel's, and with equal splits of an older segment alone the outputs are equal bit for bit.
+// sums are that kernel's.
 #include "attn_common.h"
 #include "common.h"
 #include "decode_body.h"
@@ -14,19 +14,50 @@
 namespace lkv {
 namespace {
 
+// Waves of a workgroup: two a SIMD, one for two column groups (whose state takes more than half of a SIMD's registers).
+constexpr int waves8(int cg) { return cg == 1 ? 8 : 4; }
+
+typedef const __attribute__((address_space(4))) uint32_t* ConstWords;
+
+// Words of constant memory: what is the same for a wave is then read with scalar loads, whose waits leave the blocks' vector
+// loads in flight.
+__device__ inline ConstWords const_words(const void* p) { return (ConstWords)p; }
+
 struct Block8 {
   uint4 k[4], v[4];
-  uint32_t ks, vs;  // scale bytes
+  uint32_t ks, vs, page;  // the words that hold the page's scale bytes
+
+  __device__ uint32_t byte(uint32_t w) const { return (w >> (8 * (page & 3))) & 0xffu; }
 };
 
-__device__ inline void load_block8(Block8& f, const Kv8Pool& o, int64_t base, int64_t sbase, int page, int lane) {
-  const int64_t at = base + page * o.page + lane * 16;
+template <bool kNT>
+__device__ inline uint4 load16(const uint8_t* p) {
+  return kNT ? load_nt(p) : *reinterpret_cast<const uint4*>(p);
+}
+
+// The pool's part of one kv head.
+struct HeadPool {
+  const uint8_t* k;
+  const uint8_t* v;
+  ConstWords ks, vs;
+  int64_t page;
+  int32_t pages;
+};
+
+__device__ inline HeadPool head_pool(const Kv8Pool& o, int kvh) {
+  return HeadPool{o.k + kvh * o.hs, o.v + kvh * o.hs, const_words(o.ks + kvh * o.s_hs), const_words(o.vs + kvh * o.s_hs), o.page, o.pages};
+}
+
+template <bool kNT>
+__device__ inline void load_block8(Block8& f, const HeadPool& o, int page, int lane) {
+  const int64_t at = page * o.page + lane * 16;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) f.k[i] = *reinterpret_cast<const uint4*>(o.k + at + i * 1024);
+  for (int i = 0; i < 4; ++i) f.k[i] = load16<kNT>(o.k + at + i * 1024);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) f.v[i] = *reinterpret_cast<const uint4*>(o.v + at + i * 1024);
-  f.ks = o.ks[sbase + page];
-  f.vs = o.vs[sbase + page];
+  for (int i = 0; i < 4; ++i) f.v[i] = load16<kNT>(o.v + at + i * 1024);
+  f.ks = o.ks[page >> 2];
+  f.vs = o.vs[page >> 2];
+  f.page = page;
 }
 
 // Bytes of the first n (of four) tokens of a word.
@@ -36,7 +67,7 @@ __device__ inline uint32_t keep_bytes(uint32_t w, int n) {
 
 // The bf16 operands of a block whose first `hi` tokens count (V codes of the others become 0: they may be anything, and 0 * NaN is NaN).
 __device__ inline void expand_block8(const Block8& f, int hi, int g4, BlockFrags& x) {
-  const float ks = kv8_scale(f.ks), vs = kv8_scale(f.vs);
+  const float ks = kv8_scale(f.byte(f.ks)), vs = kv8_scale(f.byte(f.vs));
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     x.k[i >> 1][2 * (i & 1)] = kv8_to_bf16(f.k[i].x, f.k[i].y, ks);
@@ -54,30 +85,48 @@ __device__ inline void expand_block8(const Block8& f, int hi, int g4, BlockFrags
   }
 }
 
-template <bool kVScale, bool kMulti, int CG, bool kPairs>
-__global__ __launch_bounds__(256) void decode_kv8_kernel(const DecodeParams p, const Kv8Pool o) {
-  __shared__ DecodeShared<CG> sm;
+// The kernel's arguments, read again where they are needed: held from its start, with those of the other segment and of
+// the merge, they take more scalar registers than there are.
+struct Arguments {
+  DecodeParams p;
+  Kv8Pool o;
+};
+
+__device__ inline const Arguments& reread() {
+  uint32_t zero;
+  asm volatile("s_mov_b32 %0, 0" : "=s"(zero));
+  typedef const __attribute__((address_space(4))) uint8_t* Kernarg;
+  return *reinterpret_cast<const Arguments*>((const uint8_t*)((Kernarg)__builtin_amdgcn_kernarg_segment_ptr() + zero));
+}
+
+template <bool kVScale, bool kNT, bool kMulti, int CG, bool kPairs>
+__global__ __launch_bounds__(waves8(CG) * 64, waves8(CG) / 4) void decode_kv8_kernel(const Arguments args) {
+  const DecodeParams& p = args.p;
+  constexpr int kWaves = waves8(CG);
+  constexpr int kStride = kPairs ? kWaves / 2 : kWaves;  // waves that share the blocks of a workgroup
+  __shared__ DecodeShared<CG, kWaves> sm;
   DecodeItem it;
   if (!decode_item<kMulti>(p, blockIdx.x, it)) return;  // (workgroup-uniform)
-  constexpr int kStride = kPairs ? 2 : kDecodeWaves;    // block stride of one wave
+  if (p.cu == nullptr) {  // the splits of one (sequence, kv head) side by side on one XCD
+    const int id = blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z);
+    const int at = xcd_logical_index(id, gridDim.x * gridDim.y * gridDim.z);
+    it.split = at % it.S;
+    it.kvh = at / it.S % gridDim.y;
+    it.b = at / (it.S * gridDim.y);
+    it.mr = kMulti ? multi_rows(p, it.b) : MultiRows{1, it.b};
+    it.ws_row0 = it.mr.row0;
+  }
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n16 = lane & 15, g4 = lane >> 4;
   const int G = p.group, kvh = it.kvh, b = it.b;
   const int Lq = it.mr.L;
-  const SeqView sv = make_seq_view(p.seg, b, kvh);
-  const int nbl = local_blocks(sv, sv.n1);
-  // The split's share in bytes: an older block counts 1, a ring block 2.
-  const int units = sv.nb0 + 2 * nbl, per = (units + it.S - 1) / it.S;
-  const int u0 = min(it.split * per, units), u1 = min(u0 + per, units);
-  const int ob = min(u0, sv.nb0), oe = min(u1, sv.nb0);
-  const int lb = sv.nb0 + ((max(u0 - sv.nb0, 0) + 1) >> 1), le = sv.nb0 + ((max(u1 - sv.nb0, 0) + 1) >> 1);
-
   const int cols = kMulti ? G * Lq : G;
+  const SeqView sv = make_seq_view(p.seg, b, kvh);
   uint4 qf[CG][4];
   int lim[CG], lim_min = 0;  // causal limits (local token index) of this lane's columns and of column 0
   if (kMulti) lim_min = p.causal ? sv.n1 - Lq : sv.n1 - 1;
-  const int cg0 = kPairs ? (wave >> 1) * CG : 0;
+  const int cg0 = kPairs ? wave / kStride * CG : 0;
 #pragma unroll
   for (int cg = 0; cg < CG; ++cg) {
     const int c = 16 * (cg0 + cg) + n16;
@@ -89,7 +138,7 @@ __global__ __launch_bounds__(256) void decode_kv8_kernel(const DecodeParams p, c
       qf[cg][kb] = c < cols ? *reinterpret_cast<const uint4*>(qrow + 32 * kb + 8 * g4) : make_uint4(0, 0, 0, 0);
     lim[cg] = kMulti && p.causal ? lim_min + t : lim_min;
   }
-  const float vs = kVScale ? p.vscale[kvh] : 1.f;
+  const float vs = kVScale ? p.vscale[kvh] : 1.f, scale_log2 = p.scale_log2;
   SoftmaxState st[CG];
 #pragma unroll
   for (int cg = 0; cg < CG; ++cg) {
@@ -101,83 +150,124 @@ __global__ __launch_bounds__(256) void decode_kv8_kernel(const DecodeParams p, c
   auto compute = [&](const BlockFrags& f, const BlockRef& r) __attribute__((always_inline)) {
 #pragma unroll
     for (int cg = 0; cg < CG; ++cg)
-      compute_block<kVScale, kMulti>(f, r, qf[cg], vs, p.scale_log2, n16, g4, lim[cg], lim_min, st[cg]);
+      compute_block<kVScale, kMulti>(f, r, qf[cg], vs, scale_log2, n16, g4, lim[cg], lim_min, st[cg]);
   };
-  const int w = kPairs ? (wave & 1) : wave;
 
-  // older blocks: ob + w, + kStride, ...
-  const int64_t base = kvh * o.hs, sbase = kvh * o.s_hs;
+  // The blocks of a segment are dealt one by one to all waves of all splits, so that the workgroups of a (sequence, kv head)
+  // walk one window of its K and V together; the waves that got one ring block less have the first older ones.
+  const int me = it.split * kStride + (kPairs ? wave % kStride : wave), step = it.S * kStride;
+  const int nbl = local_blocks(sv, sv.n1), nb0 = sv.nb0, n0 = sv.n0;
+  int first = me - nbl % step;
+  if (first < 0) first += step;
+  const int n = first < nb0 ? (nb0 - 1 - first) / step + 1 : 0;
   uint32_t nan = 0;  // a NaN block was among them
-  auto page = [&](int blk) { return min(max(sv.otab[blk], 0), o.pages - 1); };
-  auto compute8 = [&](const Block8& f, int blk) __attribute__((always_inline)) {
+  const ConstWords table = const_words(sv.otab);
+  HeadPool o;
+  Block8 f0, f1, f2;
+  int pg = 0;
+  auto at = [&](int t) { return first + step * t; };
+  auto look = [&](int t) { pg = min(max(static_cast<int>(table[at(min(t, n - 1))]), 0), o.pages - 1); };
+  auto load = [&](Block8& f) __attribute__((always_inline)) { load_block8<kNT>(f, o, pg, lane); };
+  auto compute8 = [&](const Block8& f, int t) __attribute__((always_inline)) {
     BlockRef r;
     r.lo = 0;
-    r.hi = min(kBlockTokens, sv.n0 - blk * kBlockTokens);
+    r.hi = min(kBlockTokens, n0 - at(t) * kBlockTokens);
     r.seg_tok = -1;
     r.older = true;
-    nan |= (f.ks == 255u) | (f.vs == 255u);
+    nan |= static_cast<uint32_t>(f.byte(f.ks) == 255u || f.byte(f.vs) == 255u);
     BlockFrags x;
     expand_block8(f, r.hi, g4, x);
     compute(x, r);
   };
-  int blk = ob + w;
-  if (blk < oe) {
-    Block8 fa, fb;
-    load_block8(fa, o, base, sbase, page(blk), lane);
-    while (blk + kStride < oe) {
-      load_block8(fb, o, base, sbase, page(blk + kStride), lane);
-      __builtin_amdgcn_sched_barrier(0);
-      compute8(fa, blk);
-      blk += kStride;
-      fa = fb;
-    }
-    compute8(fa, blk);
-  }
-  // ring blocks: lb + w, + kStride, ...
-  blk = lb + w;
-  if (blk < le) {
-    BlockFrags fa, fb;
-    BlockRef ra = block_ref(sv, blk), rb;
-    load_block<false>(fa, ra, n16, g4);
-    while (blk + kStride < le) {
-      rb = block_ref(sv, blk + kStride);
-      load_block<false>(fb, rb, n16, g4);
+  // The first two older blocks are on their way while the last ring block is computed.
+  auto begin = [&]() __attribute__((always_inline)) {
+    if (n == 0) return;
+    o = head_pool(reread().o, kvh);
+    look(0);
+    load(f0);
+    if (n == 1) return;
+    look(1);
+    load(f1);
+    look(2);
+  };
+  int blk = nb0 + me;
+  const int le = nb0 + nbl;
+  BlockFrags fa, fb;
+  BlockRef ra, rb;
+  const bool ring = blk < le;
+  if (ring) {
+    ra = block_ref(sv, blk);
+    load_block<kNT>(fa, ra, n16, g4);
+    while (blk + step < le) {
+      rb = block_ref(sv, blk + step);
+      load_block<kNT>(fb, rb, n16, g4);
       __builtin_amdgcn_sched_barrier(0);
       compute(fa, ra);
-      blk += kStride;
+      blk += step;
       fa = fb;
       ra = rb;
     }
-    compute(fa, ra);
+  }
+  begin();
+  __builtin_amdgcn_sched_barrier(0);
+  if (ring) compute(fa, ra);
+  if (n > 0) {
+    // Two blocks are on their way while one is computed.  In the loop the loads are unconditional (the compiler
+    // then counts them exactly for its waits), and the page of the next one is looked up a step ahead.
+    int t = 0;
+    auto pass = [&](Block8& in, const Block8& now, int i) __attribute__((always_inline)) {
+      load(in);
+      look(t + i + 3);
+      __builtin_amdgcn_sched_barrier(0);
+      compute8(now, t + i);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    for (; t + 4 < n; t += 3) {
+      pass(f2, f0, 0);
+      pass(f0, f1, 1);
+      pass(f1, f2, 2);
+    }
+    // one to four are left, two of them loaded
+    if (t + 2 < n) load(f2);
+    compute8(f0, t);
+    if (t + 3 < n) {
+      look(t + 3);
+      load(f0);
+    }
+    if (t + 1 < n) compute8(f1, t + 1);
+    if (t + 2 < n) compute8(f2, t + 2);
+    if (t + 3 < n) compute8(f0, t + 3);
   }
   if (nan) {
 #pragma unroll
     for (int cg = 0; cg < CG; ++cg) st[cg].l = __builtin_nanf("");
   }
-  decode_merge_waves<kMulti, CG, kPairs, true>(p, it, st, sm);
+  decode_merge_waves<kMulti, CG, kPairs, true, kWaves>(reread().p, it, st, sm);
 }
 
-template <int CG, bool kPairs>
-void launch_multi8(const DecodeParams& p, const Kv8Pool& o, dim3 grid, bool vscale, hipStream_t s) {
-  if (vscale)
-    decode_kv8_kernel<true, true, CG, kPairs><<<grid, 256, 0, s>>>(p, o);
+template <bool kMulti, int CG, bool kPairs>
+void launch8(const DecodeParams& p, const Kv8Pool& o, dim3 grid, bool vscale, bool nt, hipStream_t s) {
+  if (vscale && nt)
+    decode_kv8_kernel<true, true, kMulti, CG, kPairs><<<grid, waves8(CG) * 64, 0, s>>>(Arguments{p, o});
+  else if (vscale)
+    decode_kv8_kernel<true, false, kMulti, CG, kPairs><<<grid, waves8(CG) * 64, 0, s>>>(Arguments{p, o});
+  else if (nt)
+    decode_kv8_kernel<false, true, kMulti, CG, kPairs><<<grid, waves8(CG) * 64, 0, s>>>(Arguments{p, o});
   else
-    decode_kv8_kernel<false, true, CG, kPairs><<<grid, 256, 0, s>>>(p, o);
+    decode_kv8_kernel<false, false, kMulti, CG, kPairs><<<grid, waves8(CG) * 64, 0, s>>>(Arguments{p, o});
 }
 
 }  // namespace
 
-void launch_decode_kv8(const DecodeParams& p, const Kv8Pool& older, dim3 grid, bool vscale, int cg, hipStream_t s) {
+void launch_decode_kv8(const DecodeParams& p, const Kv8Pool& older, dim3 grid, bool vscale, bool nt, int cg, hipStream_t s) {
   if (cg == 1)
-    launch_multi8<1, false>(p, older, grid, vscale, s);
+    launch8<true, 1, false>(p, older, grid, vscale, nt, s);
   else if (cg == 2)
-    launch_multi8<2, false>(p, older, grid, vscale, s);
+    launch8<true, 2, false>(p, older, grid, vscale, nt, s);
   else if (cg == 4)
-    launch_multi8<2, true>(p, older, grid, vscale, s);
-  else if (vscale)
-    decode_kv8_kernel<true, false, 1, false><<<grid, 256, 0, s>>>(p, older);
+    launch8<true, 2, true>(p, older, grid, vscale, nt, s);
   else
-    decode_kv8_kernel<false, false, 1, false><<<grid, 256, 0, s>>>(p, older);
+    launch8<false, 1, false>(p, older, grid, vscale, nt, s);
 }
 
 }  // namespace lkv

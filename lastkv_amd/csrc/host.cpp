@@ -44,6 +44,14 @@ struct Library {
   decltype(&lkv_mx8_unpack) mx8_unpack;
   decltype(&lkv_mx4_linear) mx4_linear;
   decltype(&lkv_mx4_weight_bytes) mx4_weight_bytes;
+  decltype(&lkv_decode_attn_kv8) decode_attn_kv8;
+  decltype(&lkv_prefill_attn_kv8) prefill_attn_kv8;
+  decltype(&lkv_prefill_kv8_workspace_bytes) prefill_kv8_workspace_bytes;
+  decltype(&lkv_kv8_quantize) kv8_quantize;
+  decltype(&lkv_kv8_unpack) kv8_unpack;
+  decltype(&lkv_copy_pages) copy_pages;
+  decltype(&lkv_beam_workspace_bytes) beam_workspace_bytes;
+  decltype(&lkv_beam_select) beam_select;
 };
 
 Library g_lib;
@@ -51,6 +59,9 @@ PyTypeObject* g_tiled = nullptr;
 PyTypeObject* g_paged = nullptr;
 PyTypeObject* g_mx8 = nullptr;
 PyTypeObject* g_mx4 = nullptr;
+PyTypeObject* g_paged8 = nullptr;
+PyObject* g_str_k_scales = nullptr;
+PyObject* g_str_v_scales = nullptr;
 PyObject* g_error = nullptr;  // LastKVNativeError
 PyObject* g_str_k = nullptr;
 PyObject* g_str_v = nullptr;
@@ -147,6 +158,59 @@ bool segment(PyObject* o, Kv& s) {
   return ok;
 }
 
+// An attribute's tensor as the kernels may address it (empty otherwise).
+at::Tensor tensor_attr(PyObject* o, PyObject* name) {
+  PyObject* a = PyObject_GetAttr(o, name);
+  if (a == nullptr) {
+    PyErr_Clear();
+    return at::Tensor();
+  }
+  const at::Tensor* t = tensor(a);
+  at::Tensor r = t != nullptr ? *t : at::Tensor();
+  Py_DECREF(a);
+  return r;
+}
+
+// Kernels are launched on the current device.
+bool on_current_device(const at::Tensor& t) { return t.device().index() == c10::hip::current_device(); }
+
+// A PagedKV8 with the forms ops.PagedKV8 checks, on the current device.
+struct Kv8 {
+  at::Tensor k, v, ks, vs;
+  lkv_kv8_pool pool;
+};
+
+bool pool8(PyObject* o, Kv8& s) {
+  if (Py_TYPE(o) != g_paged8) return false;
+  s.k = tensor_attr(o, g_str_k);
+  s.v = tensor_attr(o, g_str_v);
+  s.ks = tensor_attr(o, g_str_k_scales);
+  s.vs = tensor_attr(o, g_str_v_scales);
+  if (!s.k.defined() || s.k.dim() != 3 || s.k.size(2) != LKV_BLOCK_ELEMS || !on_current_device(s.k)) return false;
+  const int64_t heads = s.k.size(0), pages = s.k.size(1), scale_pages = (pages + 3) / 4 * 4;
+  for (const at::Tensor* t : {&s.k, &s.v})
+    if (!t->defined() || t->scalar_type() != at::kFloat8_e4m3fn || !t->is_contiguous() || t->device() != s.k.device() ||
+        t->sizes() != s.k.sizes())
+      return false;
+  for (const at::Tensor* t : {&s.ks, &s.vs})
+    if (!t->defined() || t->scalar_type() != at::kByte || !t->is_contiguous() || t->device() != s.k.device() || t->dim() != 2 ||
+        t->size(0) != heads || t->size(1) != scale_pages)
+      return false;
+  if (pages > INT32_MAX || heads > INT32_MAX) return false;
+  std::memset(&s.pool, 0, sizeof(s.pool));
+  s.pool.struct_size = sizeof(s.pool);
+  s.pool.num_pages = static_cast<int32_t>(pages);
+  s.pool.heads = static_cast<int32_t>(heads);
+  s.pool.k = ptr(s.k);
+  s.pool.v = ptr(s.v);
+  s.pool.page_stride = LKV_BLOCK_ELEMS;
+  s.pool.head_stride = pages * LKV_BLOCK_ELEMS;
+  s.pool.k_scales = ptr(s.ks);
+  s.pool.v_scales = ptr(s.vs);
+  s.pool.scale_head_stride = scale_pages;
+  return true;
+}
+
 // A block table: int32 [batch, W] with contiguous rows.
 const at::Tensor* table(PyObject* o, int64_t batch, const at::Device& dev) {
   const at::Tensor* t = tensor(o);
@@ -161,13 +225,20 @@ struct SegmentArgs {
       *local_table, *local_ring_blocks;
 };
 
-// The older / local fields of the decode and prefill structs (ops._fill_segments).
+// The older / local fields of the decode and prefill structs (ops._fill_segments).  older8: set (its k defined) for a PagedKV8,
+// whose pointers are not in the struct.
 template <class A>
-bool fill_segments(A& a, int64_t B, const at::Device& dev, const SegmentArgs& s, int64_t& hkv) {
+bool fill_segments(A& a, int64_t B, const at::Device& dev, const SegmentArgs& s, int64_t& hkv, Kv8& older8) {
   Kv older, local;
   const bool has_older = s.older != Py_None, has_local = s.local != Py_None;
   if (!has_older && !has_local) return false;
-  if (has_older && !segment(s.older, older)) return false;
+  const bool eight = has_older && Py_TYPE(s.older) == g_paged8;
+  if (eight ? !pool8(s.older, older8) : has_older && !segment(s.older, older)) return false;
+  if (eight) {  // (its codes stand for the bf16 pools: the same shape and device)
+    older.paged = true;
+    older.k = older8.k;
+    older.v = older8.v;
+  }
   if (has_local && !segment(s.local, local)) return false;
   hkv = has_older ? older.heads() : local.heads();
   if (has_older && has_local && older.heads() != local.heads()) return false;
@@ -179,8 +250,10 @@ bool fill_segments(A& a, int64_t B, const at::Device& dev, const SegmentArgs& s,
   a.vscale = vs ? ptr<const float>(*vs) : nullptr;
   if (has_older) {
     if (older.k.device() != dev) return false;
-    a.older_k = ptr(older.k);
-    a.older_v = ptr(older.v);
+    if (!eight) {
+      a.older_k = ptr(older.k);
+      a.older_v = ptr(older.v);
+    }
     a.older_head_stride = older.head_stride();
     if (!length(s.older_len, B, dev, a.older_len, a.older_len_const)) return false;
     if (older.paged) {
@@ -309,8 +382,10 @@ PyObject* decode_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
     std::memset(&a, 0, sizeof(a));
     a.struct_size = sizeof(a);
     int64_t hkv = 0;
+    Kv8 older8;
     const SegmentArgs seg{v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8], v[9], v[10], v[11]};
-    if (!fill_segments(a, B, dev, seg, hkv) || hkv < 1 || hq % hkv != 0 || hq / hkv > 64) return not_handled();
+    if (!fill_segments(a, B, dev, seg, hkv, older8) || hkv < 1 || hq % hkv != 0 || hq / hkv > 64) return not_handled();
+    const bool eight = older8.k.defined();
     at::Tensor out;
     if (v[14] != Py_None) {
       const at::Tensor* o = tensor(v[14]);
@@ -329,7 +404,7 @@ PyObject* decode_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
       const int cus = dev.index() >= 0 && dev.index() < kMaxDevices ? g_cus[dev.index()] : 0;
       if (cus == 0) return not_handled();
       int64_t keys = 0;
-      if (a.older_k != nullptr) keys += a.older_len != nullptr ? a.older_capacity_tokens : a.older_len_const;
+      if (a.older_k != nullptr || eight) keys += a.older_len != nullptr ? a.older_capacity_tokens : a.older_len_const;
       if (a.local_k != nullptr)
         keys += a.local_len != nullptr ? int64_t{a.local_ring_blocks} * LKV_BLOCK_TOKENS : a.local_len_const;
       const int64_t pairs = std::max<int64_t>(1, B * hkv);
@@ -363,6 +438,7 @@ PyObject* decode_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
     a.workspace = ws.defined() ? ptr(ws) : nullptr;
     a.workspace_bytes = ws.defined() ? static_cast<int64_t>(ws.nbytes()) : 0;
     const lkv_stream_t s = stream_of(*q);
+    if (eight) return issue("lkv_decode_attn_kv8", v[14], out, [&] { return g_lib.decode_attn_kv8(&a, &older8.pool, s); });
     return issue("lkv_decode_attn", v[14], out, [&] { return g_lib.decode_attn(&a, s); });
   });
 }
@@ -404,7 +480,9 @@ PyObject* prefill_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
     }
     int64_t hkv = 0;
     const SegmentArgs seg{v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8], v[9], v[10], v[11]};
-    if (!fill_segments(a, B, dev, seg, hkv) || hkv < 1 || hq % hkv != 0) return not_handled();
+    Kv8 older8;
+    if (!fill_segments(a, B, dev, seg, hkv, older8) || hkv < 1 || hq % hkv != 0) return not_handled();
+    const bool eight = older8.k.defined();
     at::Tensor out;
     if (v[14] != Py_None) {
       const at::Tensor* o = tensor(v[14]);
@@ -456,11 +534,12 @@ PyObject* prefill_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
       if (w == nullptr || w->device() != dev || !w->is_contiguous()) return not_handled();
       ws = *w;
     } else {
-      ws = new_bytes(std::max<int64_t>(16, g_lib.prefill_workspace_bytes(&a)), dev);
+      ws = new_bytes(std::max<int64_t>(16, eight ? g_lib.prefill_kv8_workspace_bytes(&a) : g_lib.prefill_workspace_bytes(&a)), dev);
     }
     a.workspace = ptr(ws);
     a.workspace_bytes = static_cast<int64_t>(ws.nbytes());
     const lkv_stream_t s = stream_of(*q);
+    if (eight) return issue("lkv_prefill_attn_kv8", v[14], out, [&] { return g_lib.prefill_attn_kv8(&a, &older8.pool, s); });
     return issue("lkv_prefill_attn", v[14], out, [&] { return g_lib.prefill_attn(&a, s); });
   });
 }
@@ -688,22 +767,6 @@ PyObject* silu_mul(PyObject*, PyObject* const* v, Py_ssize_t n) {
 }
 
 // ---- MX8 rows and MX4 weights ----
-
-// An attribute's tensor as the kernels may address it (empty otherwise).
-at::Tensor tensor_attr(PyObject* o, PyObject* name) {
-  PyObject* a = PyObject_GetAttr(o, name);
-  if (a == nullptr) {
-    PyErr_Clear();
-    return at::Tensor();
-  }
-  const at::Tensor* t = tensor(a);
-  at::Tensor r = t != nullptr ? *t : at::Tensor();
-  Py_DECREF(a);
-  return r;
-}
-
-// Kernels are launched on the current device.
-bool on_current_device(const at::Tensor& t) { return t.device().index() == c10::hip::current_device(); }
 
 // The shape of up to three dims as rows of `width` with one stride (rows2d without the type).
 bool rows_of(const at::Tensor& t, int64_t& n, int64_t& width, int64_t& stride) {
@@ -954,11 +1017,205 @@ PyObject* mx4_linear(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
-// bind(addresses: the entry points in Library's order, TiledKV, PagedKV, LastKVNativeError, MX8Rows, MX4Weight)
+// ---- the 8-bit cache, page copies, beam selection ----
+
+// (src, dst, src_table, dst_table, tokens, first_block, blocks or None) -> True
+PyObject* kv8_quantize(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  if (n != 7 || !plain_mode()) return not_handled();
+  return guarded([&]() -> PyObject* {
+    Kv src;
+    Kv8 dst;
+    if (!segment(v[0], src) || !src.paged || !pool8(v[1], dst) || src.k.device() != dst.k.device()) return not_handled();
+    const at::Device dev = src.k.device();
+    const at::Tensor* st = tensor(v[2]);
+    if (st == nullptr || st->dim() != 2) return not_handled();
+    const int64_t B = st->size(0);
+    st = table(v[2], B, dev);
+    const at::Tensor* dt = table(v[3], B, dev);
+    lkv_kv8_quantize_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.struct_size = sizeof(a);
+    if (st == nullptr || dt == nullptr || !length(v[4], B, dev, a.tokens, a.tokens_const) || a.tokens_const < 0 ||
+        !as_i32(v[5], a.first_block))
+      return not_handled();
+    const int64_t width = std::min(st->size(1), dt->size(1));
+    int64_t blocks = width - a.first_block;
+    if (v[6] != Py_None && !as_int(v[6], blocks)) return not_handled();
+    if (a.first_block < 0 || blocks < 0 || a.first_block + blocks > width || width > INT32_MAX || B > INT32_MAX) return not_handled();
+    a.batch = static_cast<int32_t>(B);
+    a.heads = static_cast<int32_t>(src.heads());
+    a.head_dim = LKV_HEAD_DIM;
+    a.blocks = static_cast<int32_t>(blocks);
+    a.src_num_pages = static_cast<int32_t>(src.pages());
+    a.src_k = ptr(src.k);
+    a.src_v = ptr(src.v);
+    a.src_page_stride = LKV_BLOCK_ELEMS;
+    a.src_head_stride = src.head_stride();
+    a.src_table = ptr<const int32_t>(*st);
+    a.src_table_stride = st->stride(0);
+    a.dst_table = ptr<const int32_t>(*dt);
+    a.dst_table_stride = dt->stride(0);
+    a.src_table_width = static_cast<int32_t>(st->size(1));
+    a.dst_table_width = static_cast<int32_t>(dt->size(1));
+    const lkv_stream_t s = stream_of(src.k);
+    return issue("lkv_kv8_quantize", Py_True, at::Tensor(), [&] { return g_lib.kv8_quantize(&a, &dst.pool, s); });
+  });
+}
+
+// A tuple of tensors (new references), made before the launch so that nothing can fail after it; null with the error set.
+PyObject* tuple_of(std::initializer_list<at::Tensor> ts) {
+  PyObject* r = PyTuple_New(static_cast<Py_ssize_t>(ts.size()));
+  if (r == nullptr) return nullptr;
+  Py_ssize_t i = 0;
+  for (const at::Tensor& t : ts) {
+    PyObject* o = THPVariable_Wrap(t);
+    if (o == nullptr) {
+      Py_DECREF(r);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(r, i++, o);
+  }
+  return r;
+}
+
+template <class F>
+PyObject* issue_tuple(const char* what, std::initializer_list<at::Tensor> outs, F&& call) {
+  PyObject* r = tuple_of(outs);
+  if (r == nullptr) return nullptr;
+  PyObject* done = issue(what, r, at::Tensor(), call);
+  Py_DECREF(r);
+  return done;
+}
+
+// (pool, table, token0, tokens)
+PyObject* kv8_unpack(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  if (n != 4 || !plain_mode()) return not_handled();
+  return guarded([&]() -> PyObject* {
+    Kv8 src;
+    if (!pool8(v[0], src)) return not_handled();
+    const at::Device dev = src.k.device();
+    const at::Tensor* t = tensor(v[1]);
+    if (t == nullptr || t->dim() != 2) return not_handled();
+    const int64_t B = t->size(0);
+    t = table(v[1], B, dev);
+    int32_t token0, tokens;
+    if (t == nullptr || !as_i32(v[2], token0) || !as_i32(v[3], tokens) || token0 < 0 || tokens < 0 || B > INT32_MAX ||
+        t->size(1) > INT32_MAX || int64_t{token0} + tokens > t->size(1) * LKV_BLOCK_TOKENS)
+      return not_handled();
+    const int64_t H = src.pool.heads;
+    const at::Tensor k = new_bf16({B, H, tokens, LKV_HEAD_DIM}, dev), o = new_bf16({B, H, tokens, LKV_HEAD_DIM}, dev);
+    const lkv_stream_t s = stream_of(src.k);
+    return issue_tuple("lkv_kv8_unpack", {k, o}, [&] {
+      return g_lib.kv8_unpack(&src.pool, ptr<const int32_t>(*t), t->stride(0), static_cast<int32_t>(t->size(1)),
+                              static_cast<int32_t>(B), token0, tokens, ptr(k), k.stride(0), k.stride(1), k.stride(2), ptr(o),
+                              o.stride(0), o.stride(1), o.stride(2), s);
+    });
+  });
+}
+
+// A host array of int32 (as numpy makes it).
+bool host_ids(PyObject* o, Buffer& b, const int32_t*& ids, int64_t& n) {
+  if (!PyObject_CheckBuffer(o) || PyObject_GetBuffer(o, &b.view, PyBUF_FORMAT | PyBUF_ND | PyBUF_C_CONTIGUOUS) != 0) {
+    PyErr_Clear();
+    return false;
+  }
+  ids = static_cast<const int32_t*>(b.view.buf);
+  n = b.view.len / 4;
+  return b.view.ndim == 1 && b.view.itemsize == 4 && b.view.format != nullptr && std::strcmp(b.view.format, "i") == 0;
+}
+
+// (pool, src, dst) -> True
+PyObject* copy_pages(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  if (n != 3 || !plain_mode()) return not_handled();
+  return guarded([&]() -> PyObject* {
+    lkv_copy_pages_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.struct_size = sizeof(a);
+    Buffer sb, db;
+    int64_t ns, nd;
+    if (!host_ids(v[1], sb, a.src, ns) || !host_ids(v[2], db, a.dst, nd) || ns != nd || ns > INT32_MAX) return not_handled();
+    Kv kv;
+    Kv8 e;
+    at::Tensor k;
+    if (pool8(v[0], e)) {
+      k = e.k;
+      a.k = e.pool.k;
+      a.v = e.pool.v;
+      a.k_scales = e.pool.k_scales;
+      a.v_scales = e.pool.v_scales;
+      a.scale_head_stride = e.pool.scale_head_stride;
+    } else if (segment(v[0], kv) && kv.paged && kv.pages() <= INT32_MAX) {
+      k = kv.k;
+      a.k = ptr(kv.k);
+      a.v = ptr(kv.v);
+    } else {
+      return not_handled();
+    }
+    if (!on_current_device(k)) return not_handled();
+    a.count = static_cast<int32_t>(ns);
+    a.heads = static_cast<int32_t>(k.size(0));
+    a.num_pages = static_cast<int32_t>(k.size(1));
+    a.page_bytes = static_cast<int32_t>(LKV_BLOCK_ELEMS * k.element_size());
+    a.page_stride = a.page_bytes;
+    a.head_stride = a.num_pages * a.page_stride;
+    const lkv_stream_t s = stream_of(k);
+    return issue("lkv_copy_pages", Py_True, at::Tensor(), [&] { return g_lib.copy_pages(&a, s); });
+  });
+}
+
+// (logits, scores, count, workspace)
+PyObject* beam_select(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  if (n != 4 || !plain_mode()) return not_handled();
+  return guarded([&]() -> PyObject* {
+    const at::Tensor *x = tensor(v[0]), *sc = tensor(v[1]);
+    lkv_beam_select_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.struct_size = sizeof(a);
+    if (x == nullptr || sc == nullptr || x->dim() != 3 || !(bf16(x) || x->scalar_type() == at::kFloat) || !as_i32(v[2], a.count) ||
+        a.count < 1 || a.count > LKV_BEAM_MAX_COUNT || !on_current_device(*x))
+      return not_handled();
+    const int64_t B = x->size(0), K = x->size(1), V = x->size(2);
+    const at::Device dev = x->device();
+    if (K < 1 || K > LKV_BEAM_MAX_BEAMS || V < 1 || V > (1 << 20) || B * K > 65535 || (V > 1 && x->stride(2) != 1) ||
+        sc->scalar_type() != at::kFloat || sc->device() != dev || sc->dim() != 2 || sc->size(0) != B || sc->size(1) != K ||
+        (K > 1 && sc->stride(1) != 1))
+      return not_handled();
+    a.batch = static_cast<int32_t>(B);
+    a.beams = static_cast<int32_t>(K);
+    a.vocab = static_cast<int32_t>(V);
+    const int64_t need = g_lib.beam_workspace_bytes(a.batch, a.beams, a.vocab, a.count);
+    at::Tensor ws;
+    if (v[3] != Py_None) {
+      const at::Tensor* w = tensor(v[3]);
+      if (w == nullptr || w->device() != dev || !w->is_contiguous() || static_cast<int64_t>(w->nbytes()) < need) return not_handled();
+      ws = *w;
+    } else {
+      ws = new_bytes(std::max<int64_t>(16, need), dev);
+    }
+    const auto i32 = at::TensorOptions().dtype(at::kInt).device(dev);
+    const at::Tensor out = at::empty({B, a.count}, at::TensorOptions().dtype(at::kFloat).device(dev));
+    const at::Tensor beams = at::empty({B, a.count}, i32), tokens = at::empty({B, a.count}, i32);
+    a.logits_fp32 = x->scalar_type() == at::kFloat;
+    a.logits = ptr(*x);
+    a.logits_stride_b = x->stride(0);
+    a.logits_stride_k = x->stride(1);
+    a.scores = ptr<const float>(*sc);
+    a.scores_stride_b = sc->stride(0);
+    a.out_scores = ptr<float>(out);
+    a.out_beams = ptr<int32_t>(beams);
+    a.out_tokens = ptr<int32_t>(tokens);
+    a.workspace = ptr(ws);
+    a.workspace_bytes = static_cast<int64_t>(ws.nbytes());
+    const lkv_stream_t s = stream_of(*x);
+    return issue_tuple("lkv_beam_select", {out, beams, tokens}, [&] { return g_lib.beam_select(&a, s); });
+  });
+}
+
+// bind(addresses: the entry points in Library's order, TiledKV, PagedKV, LastKVNativeError, MX8Rows, MX4Weight, PagedKV8)
 PyObject* bind(PyObject*, PyObject* args) {
-  PyObject *addresses, *tiled, *paged, *error, *mx8, *mx4;
-  if (!PyArg_ParseTuple(args, "O!O!O!O!O!O!", &PyTuple_Type, &addresses, &PyType_Type, &tiled, &PyType_Type, &paged,
-                        &PyType_Type, &error, &PyType_Type, &mx8, &PyType_Type, &mx4))
+  PyObject *addresses, *tiled, *paged, *error, *mx8, *mx4, *paged8;
+  if (!PyArg_ParseTuple(args, "O!O!O!O!O!O!O!", &PyTuple_Type, &addresses, &PyType_Type, &tiled, &PyType_Type, &paged,
+                        &PyType_Type, &error, &PyType_Type, &mx8, &PyType_Type, &mx4, &PyType_Type, &paged8))
     return nullptr;
   constexpr Py_ssize_t kEntries = sizeof(Library) / sizeof(void*);
   if (PyTuple_GET_SIZE(addresses) != kEntries) {
@@ -979,6 +1236,8 @@ PyObject* bind(PyObject*, PyObject* args) {
   Py_INCREF(error);
   Py_INCREF(mx8);
   Py_INCREF(mx4);
+  Py_INCREF(paged8);
+  g_paged8 = reinterpret_cast<PyTypeObject*>(paged8);
   g_error = error;
   g_mx8 = reinterpret_cast<PyTypeObject*>(mx8);
   g_mx4 = reinterpret_cast<PyTypeObject*>(mx4);
@@ -1012,6 +1271,10 @@ PyMethodDef kMethods[] = {
     {"silu_mul_mx8", fast(silu_mul_mx8), METH_FASTCALL, nullptr},
     {"mx8_unpack", fast(mx8_unpack), METH_FASTCALL, nullptr},
     {"mx4_linear", fast(mx4_linear), METH_FASTCALL, nullptr},
+    {"kv8_quantize", fast(kv8_quantize), METH_FASTCALL, nullptr},
+    {"kv8_unpack", fast(kv8_unpack), METH_FASTCALL, nullptr},
+    {"copy_pages", fast(copy_pages), METH_FASTCALL, nullptr},
+    {"beam_select", fast(beam_select), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 
@@ -1023,6 +1286,8 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", "Native launch path of th
 PyMODINIT_FUNC PyInit__host() {
   g_str_k = PyUnicode_InternFromString("k");
   g_str_v = PyUnicode_InternFromString("v");
+  g_str_k_scales = PyUnicode_InternFromString("k_scales");
+  g_str_v_scales = PyUnicode_InternFromString("v_scales");
   g_str_data = PyUnicode_InternFromString("data");
   g_str_scales = PyUnicode_InternFromString("scales");
   g_str_out_features = PyUnicode_InternFromString("out_features");

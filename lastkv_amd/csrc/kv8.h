@@ -28,8 +28,8 @@ struct Kv8Pool {
 // Checks an lkv_kv8_pool (no device calls) and copies it.
 int32_t kv8_pool(const lkv_kv8_pool* a, const char* name, Kv8Pool& p);
 
-__device__ inline float kv8_scale(int byte) {  // (byte 0 is subnormal, 255 NaN)
-  return __uint_as_float(byte == 0 ? 0x400000u : byte == 255 ? 0x7fc00000u : static_cast<uint32_t>(byte) << 23);
+__device__ inline float kv8_scale(uint32_t byte) {  // (0 and 255 set the mantissa's top bit: 2^-127 and NaN)
+  return __uint_as_float(byte << 23 | (((byte + 1) & 0xfeu) == 0 ? 0x400000u : 0u));
 }
 
 // Eight e4m3 codes times a power of two as eight bf16 values.

@@ -19,9 +19,12 @@ int32_t kv8_pool(const lkv_kv8_pool* a, const char* name, Kv8Pool& p) {
   LKV_REQUIRE(a->num_pages > 0 && a->heads > 0, "%s: an 8-bit pool needs pages and heads", name);
   LKV_REQUIRE(((reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v)) & 15) == 0,
               "%s: 8-bit pools must be 16-byte aligned", name);
-  LKV_REQUIRE(a->page_stride >= kKv8Block && a->page_stride % 16 == 0 && a->head_stride >= 0 && a->head_stride % 16 == 0 &&
-                  a->scale_head_stride >= 0,
+  LKV_REQUIRE(a->page_stride >= kKv8Block && a->page_stride % 16 == 0 && a->head_stride >= 0 && a->head_stride % 16 == 0,
               "%s: strides of an 8-bit pool must be multiples of 16 bytes, a page at least 4096", name);
+  // (the attention reads scales by words)
+  LKV_REQUIRE(((reinterpret_cast<uintptr_t>(a->k_scales) | reinterpret_cast<uintptr_t>(a->v_scales)) & 3) == 0 &&
+                  a->scale_head_stride % 4 == 0 && a->scale_head_stride >= a->num_pages,
+              "%s: scales of an 8-bit pool must be 4-byte aligned, scale_head_stride a multiple of 4 that holds the pages", name);
   p.k = static_cast<const uint8_t*>(a->k);
   p.v = static_cast<const uint8_t*>(a->v);
   p.ks = static_cast<const uint8_t*>(a->k_scales);

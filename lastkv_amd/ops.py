@@ -164,8 +164,8 @@ class PagedKV:
 @dataclass
 class PagedKV8:
     """K and V page pools in 8 bits: e4m3 codes ``[heads, pages, 4096]`` (float8_e4m3fn, in the layout that the attention
-    kernels read) and one scale byte for each page of each head, ``[heads, pages]`` uint8; byte e stands for
-    2^(e - 127), 255 for NaN.  Pages are addressed by block tables as those of a ``PagedKV``; ``kv8_quantize`` fills them
+    kernels read) and one scale byte for each page of each head, ``[heads, pages]`` uint8 with the pages rounded up to a
+    multiple of four; byte e stands for 2^(e - 127), 255 for NaN.  Pages are addressed by block tables as those of a ``PagedKV``; ``kv8_quantize`` fills them
     from bf16 pages, ``decode_attention`` and ``prefill_attention`` read them as their older segment."""
 
     k: torch.Tensor
@@ -182,12 +182,16 @@ class PagedKV8:
             codes = name in ("k", "v")
             _require(t.dtype == (torch.float8_e4m3fn if codes else torch.uint8),
                      f"PagedKV8.{name} must be {'float8_e4m3fn' if codes else 'uint8'}, got {t.dtype}")
-            _require(t.dim() == (3 if codes else 2) and t.shape[:2] == self.k.shape[:2] and (not codes or t.shape[2] == BLOCK_ELEMS),
-                     f"PagedKV8.{name} must be [heads, pages{', 4096' if codes else ''}], as k")
+            want = tuple(self.k.shape[:2]) + (BLOCK_ELEMS,) if codes else (self.k.shape[0], self._scale_pages(self.k.shape[1]))
+            _require(self.k.dim() == 3 and tuple(t.shape) == want, f"PagedKV8.{name} must be {list(want)} beside k's pages")
+
+    @staticmethod
+    def _scale_pages(pages: int) -> int:
+        return -(-pages // 4) * 4  # (the kernels read scales by words)
 
     @classmethod
     def zeros(cls, pages: int, heads: int, device: torch.device | str) -> "PagedKV8":
-        codes, scales = (heads, pages, BLOCK_ELEMS), (heads, pages)
+        codes, scales = (heads, pages, BLOCK_ELEMS), (heads, cls._scale_pages(pages))
         return cls(*(torch.zeros(codes, dtype=torch.float8_e4m3fn, device=device) for _ in range(2)),
                    *(torch.zeros(scales, dtype=torch.uint8, device=device) for _ in range(2)))
 
@@ -218,7 +222,7 @@ def _kv8_pool(pool: PagedKV8) -> "_lib.Kv8Pool":
     a.struct_size = ctypes.sizeof(_lib.Kv8Pool)
     a.num_pages, a.heads = pool.pages, pool.heads
     a.k, a.v, a.k_scales, a.v_scales = (t.data_ptr() for t in (pool.k, pool.v, pool.k_scales, pool.v_scales))
-    a.page_stride, a.head_stride, a.scale_head_stride = pool.page_stride, pool.head_stride, pool.pages
+    a.page_stride, a.head_stride, a.scale_head_stride = pool.page_stride, pool.head_stride, pool.k_scales.shape[1]
     return a
 
 
@@ -238,9 +242,11 @@ def _bind_host() -> bool:
         return False
     names = ("lkv_decode_attn", "lkv_decode_workspace_bytes", "lkv_prefill_attn", "lkv_prefill_workspace_bytes",
              "lkv_qkv_epilogue", "lkv_rmsnorm", "lkv_silu_mul", "lkv_last_error", "lkv_rmsnorm_mx8", "lkv_silu_mul_mx8",
-             "lkv_mx8_unpack", "lkv_mx4_linear", "lkv_mx4_weight_bytes")
+             "lkv_mx8_unpack", "lkv_mx4_linear", "lkv_mx4_weight_bytes", "lkv_decode_attn_kv8", "lkv_prefill_attn_kv8",
+             "lkv_prefill_kv8_workspace_bytes", "lkv_kv8_quantize", "lkv_kv8_unpack", "lkv_copy_pages",
+             "lkv_beam_workspace_bytes", "lkv_beam_select")
     _host.bind(tuple(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names), TiledKV, PagedKV,
-               _lib.LastKVNativeError, MX8Rows, MX4Weight)
+               _lib.LastKVNativeError, MX8Rows, MX4Weight, PagedKV8)
     _host_bound = True
     return True
 
@@ -449,7 +455,7 @@ def decode_attention(
     nothing); calls overlapping on one GPU then race.
 
     With a ``PagedKV8`` as ``older`` (and ``older_table``) the result is the attention over the values of its codes;
-    a sequence that sees a token of a NaN block has NaN outputs, and ``kv_cache_hint`` has no effect.
+    a sequence that sees a token of a NaN block has NaN outputs.
     """
 
     if not no_alloc and (_host_bound or _bind_host()):
@@ -1099,6 +1105,9 @@ def kv8_quantize(src: PagedKV, dst: PagedKV8, *, src_table: torch.Tensor, dst_ta
     tokens past the end are stored as 0, and blocks past it left as they are.  A block that holds an infinity or NaN is NaN
     (scale byte 255).  A destination page must not occur twice in one call."""
 
+    if _host_bound or _bind_host():
+        if _host.kv8_quantize(src, dst, src_table, dst_table, tokens, first_block, blocks) is not None:
+            return
     _require(isinstance(src, PagedKV) and isinstance(dst, PagedKV8), "kv8_quantize takes a PagedKV to a PagedKV8")
     device = src.device
     _require(dst.device == device, "the pools are on different devices")
@@ -1130,6 +1139,10 @@ def kv8_unpack(pool: PagedKV8, table: torch.Tensor, token0: int, tokens: int) ->
     """K and V of tokens ``[token0, token0 + tokens)`` of every sequence, ``[B, H, tokens, 128]`` bf16 each (the codes' values
     are exact in bf16)."""
 
+    if _host_bound or _bind_host():
+        done = _host.kv8_unpack(pool, table, token0, tokens)
+        if done is not None:
+            return done
     _require(isinstance(pool, PagedKV8), "kv8_unpack takes a PagedKV8")
     device = pool.device
     _require(isinstance(table, torch.Tensor) and table.dim() == 2, "the table must be an int32 [B, W] tensor")
@@ -1171,6 +1184,9 @@ def copy_pages(pool: PagedKV | PagedKV8, src, dst) -> None:
     destination.  The lists are read during the call (a captured call keeps its pairs) and the copies run on the
     current stream, without a wait."""
 
+    if _host_bound or _bind_host():
+        if _host.copy_pages(pool, src, dst) is not None:
+            return
     _require(isinstance(pool, (PagedKV, PagedKV8)), "copy_pages takes a PagedKV or a PagedKV8")
     s, d = _page_list("src", src), _page_list("dst", dst)
     _require(s.size == d.size, f"src and dst name {s.size} and {d.size} pages")
@@ -1183,7 +1199,7 @@ def copy_pages(pool: PagedKV | PagedKV8, src, dst) -> None:
     a.k, a.v = pool.k.data_ptr(), pool.v.data_ptr()
     a.page_bytes, a.page_stride, a.head_stride = BLOCK_ELEMS * size, pool.page_stride * size, pool.head_stride * size
     if isinstance(pool, PagedKV8):
-        a.k_scales, a.v_scales, a.scale_head_stride = pool.k_scales.data_ptr(), pool.v_scales.data_ptr(), pool.pages
+        a.k_scales, a.v_scales, a.scale_head_stride = pool.k_scales.data_ptr(), pool.v_scales.data_ptr(), pool.k_scales.shape[1]
     with _on_device(pool.device):
         _lib.check(_lib.load().lkv_copy_pages(ctypes.byref(a), _stream(pool.device)), "lkv_copy_pages")
 
@@ -1205,6 +1221,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int, *, works
     entries without one are (-inf, -1, -1).  ``workspace`` (uint8, ``beam_workspace_bytes``) is the call's alone while it
     runs; without it one is allocated."""
 
+    if _host_bound or _bind_host():
+        done = _host.beam_select(logits, scores, count, workspace)
+        if done is not None:
+            return done
     _require(isinstance(logits, torch.Tensor) and logits.is_cuda, "logits must be on a GPU (the kernels have no CPU path)")
     _require(logits.dtype in (torch.bfloat16, torch.float32), f"logits must be bfloat16 or float32, got {logits.dtype}")
     _require(logits.dim() == 3 and logits.shape[1] >= 1 and logits.shape[2] >= 1 and (logits.stride(2) == 1 or logits.shape[2] == 1),

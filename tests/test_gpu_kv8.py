@@ -252,9 +252,9 @@ def test_decode_against_64_bits(Hq, Hkv, older, local, vscale, splits):
 
 @pytest.mark.parametrize("splits", [1, 2, 5])
 @pytest.mark.parametrize("vscale", [False, True])
-@pytest.mark.parametrize("T", [1, 32, 100, 1000])
+@pytest.mark.parametrize("T", [1, 32, 100])
 def test_decode_over_a_history_alone_is_the_bf16_call_over_its_values(T, vscale, splits):
-    """The same blocks in the same order: equal in every bit."""
+    """A block a wave, joined in the same order: equal in every bit."""
 
     pool, table, k, v = history(T, 3, 4, T)
     twin = paged(k.transpose(1, 2), v.transpose(1, 2), table)
@@ -339,16 +339,17 @@ def test_prefill_bidirectional_without_a_ring_and_fixed_lengths():
                 check(out[b], want, mean, err, 2.0 ** -10, (L, n, b))
 
 
+@pytest.mark.parametrize("splits", [0, 3])
 @pytest.mark.parametrize("host", [False, True])
 @pytest.mark.parametrize("counts", [[1, 1, 1], [1, 7, 1, 40], [20, 1, 33, 2, 16], [5]])
-def test_ragged_prefill_against_64_bits(counts, host):
+def test_ragged_prefill_against_64_bits(counts, host, splits):
     older = [97 * i % 400 for i in range(len(counts))]
     local = [n + 11 * i % 60 for i, n in enumerate(counts)]
     seg, keys = segments(61, 8, 2, older, local, True)
     cu = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
     q = rand(62, int(cu[-1]), 8, 128, gain=False)
     out = ops.prefill_attention(q.to(DEV), causal=True, cu_seqlens_q=torch.from_numpy(cu).to(DEV), max_seqlen_q=max(counts),
-                                cu_seqlens_q_host=cu if host else None, **seg)
+                                cu_seqlens_q_host=cu if host else None, num_splits=splits, **seg)
     for b, (k, v) in enumerate(keys):
         want, mean, err, _ = attention64(q[cu[b]:cu[b + 1]], k, v, counts[b])
         check(out[cu[b]:cu[b + 1]], want, mean, err, 2.0 ** -10, (b, host))
