@@ -245,11 +245,6 @@ __device__ inline uint4 scale_frag(uint4 v, float s) {
 int32_t prefill_on_decode_kernel(const lkv_prefill_args* a, const SegParams& seg, int32_t group, int32_t col_lo,
                                  int32_t col_hi, int32_t class_n, hipStream_t s, const Kv8Pool* older8 = nullptr);
 
-// Writes the bf16 copies of a prefill call's 8-bit older blocks, in the tiled layout, `blocks` per (sequence, kv head) at k16 / v16
-// (kv8.hip); sequences of at most `skip_rows` query rows per kv head, and blocks past a sequence's length, are left out.
-int32_t kv8_copy_blocks(const lkv_prefill_args* a, const Kv8Pool& o, int32_t group, int32_t skip_rows, int32_t blocks,
-                        uint16_t* k16, uint16_t* v16, hipStream_t s);
-
 // Checks the older segment of a call over an 8-bit pool and gives the arguments whose older fields name its pages (older_k is
 // then not null, so that the lengths count, but no bf16 kernel may read through it).
 template <class Args>

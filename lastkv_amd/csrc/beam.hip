@@ -138,20 +138,29 @@ __global__ __launch_bounds__(kBeamThreads) void beam_slice_kernel(const BeamPara
 #pragma unroll
   for (int c = 0; c < kChunks; ++c) load_values<kF32, kVec>(row, e0 + c * kStep, V, x[c]);
   if (t == 0) sm_n = 0;
-  float best = kNegInf;
+  float best = kNegInf;  // (NaN where one is: its row then has no candidate, whatever the slices hold)
 #pragma unroll
   for (int c = 0; c < kChunks; ++c) {
-    top[c] = x[c][0] > kNegInf ? x[c][0] : kNegInf;  // (fmaxf drops NaN)
+    top[c] = x[c][0];
 #pragma unroll
-    for (int j = 1; j < kVec; ++j) top[c] = fmaxf(top[c], x[c][j]);
-    best = fmaxf(best, top[c]);
+    for (int j = 1; j + 1 < kVec; j += 2) top[c] = fmax3_nan(top[c], x[c][j], x[c][j + 1]);
+    top[c] = fmax_nan(top[c], x[c][kVec - 1]);
+    best = fmax_nan(best, top[c]);
   }
   float m = best;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  for (int o = 32; o > 0; o >>= 1) m = fmax_nan(m, __shfl_xor(m, o));
   if (lane == 0) sm_max[wave] = m;
   const float floor = nth_floor(best, n, sm_floor);  // (its barriers publish sm_max and sm_n)
-  m = fmaxf(fmaxf(sm_max[0], sm_max[1]), fmaxf(sm_max[2], sm_max[3]));
+  m = fmax_nan(fmax_nan(sm_max[0], sm_max[1]), fmax_nan(sm_max[2], sm_max[3]));
+  const int64_t out = (static_cast<int64_t>(row_id) * p.slices + slice);
+  float* val = p.val + out * n;
+  int32_t* idx = p.idx + out * n;
+  if (m != m) {
+    if (t == 0) p.sums[out] = SliceSum{__builtin_nan(""), kNegInf, 0};
+    for (int r = t; r < n; r += kBeamThreads) idx[r] = -1;
+    return;
+  }
   // the values that reach the floor, as (order, lowest index first)
   auto key = [&](float v, int e) {
     return (static_cast<uint64_t>(order_bits(v)) << 32) | static_cast<uint32_t>(~static_cast<uint32_t>(e));
@@ -166,21 +175,18 @@ __global__ __launch_bounds__(kBeamThreads) void beam_slice_kernel(const BeamPara
         if (at < kBeamCap) sm_cand[at] = key(x[c][j], e0 + c * kStep + j);
       }
   }
-  const float ref = m == kNegInf ? 0.f : m;
+  const float ref = m == kNegInf ? 0.f : m;  // (x - ref is 0 for the greatest, whose term is then exactly 1)
   float part = 0.f;
 #pragma unroll
   for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) part += fast_exp2((x[c][j] - ref) * kLog2e);  // (a NaN or +inf of the row makes its sum NaN)
+    for (int j = 0; j < kVec; ++j) part += fast_exp2((x[c][j] - ref) * kLog2e);  // (a +inf makes it NaN)
   double sum = part;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
   if (lane == 0) sm_sum[wave] = sum;
   __syncthreads();
-  const int64_t out = (static_cast<int64_t>(row_id) * p.slices + slice);
   if (t == 0) p.sums[out] = SliceSum{(sm_sum[0] + sm_sum[1]) + (sm_sum[2] + sm_sum[3]), m, 0};
-  float* val = p.val + out * n;
-  int32_t* idx = p.idx + out * n;
   auto put = [&](int r, uint64_t c) {
     val[r] = from_order(static_cast<uint32_t>(c >> 32));
     idx[r] = static_cast<int32_t>(~static_cast<uint32_t>(c));

@@ -65,8 +65,18 @@ __device__ inline uint32_t keep_bytes(uint32_t w, int n) {
   return n >= 4 ? w : n <= 0 ? 0u : w & ((1u << (8 * n)) - 1u);
 }
 
-// The bf16 operands of a block whose first `hi` tokens count (V codes of the others become 0: they may be anything, and 0 * NaN is NaN).
-__device__ inline void expand_block8(const Block8& f, int hi, int g4, BlockFrags& x) {
+// Eight codes times a power of two and s, rounded to bf16 (the product with s is exact in fp32 for a bf16 s: the same bits as bf16(value * s)).
+__device__ inline uint4 scaled_to_bf16(uint32_t lo, uint32_t hi, float s) {
+  const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(lo, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(lo, true);
+  const auto c = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), d = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
+  return make_uint4(pack_bf16x2(a[0] * s, a[1] * s), pack_bf16x2(b[0] * s, b[1] * s), pack_bf16x2(c[0] * s, c[1] * s),
+                    pack_bf16x2(d[0] * s, d[1] * s));
+}
+
+// The bf16 operands of a block whose first `hi` tokens count (V codes of the others become 0: they may be anything, and 0 * NaN is
+// NaN); kVScale: V times s.
+template <bool kVScale>
+__device__ inline void expand_block8(const Block8& f, int hi, int g4, float s, BlockFrags& x) {
   const float ks = kv8_scale(f.byte(f.ks)), vs = kv8_scale(f.byte(f.vs));
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -80,8 +90,8 @@ __device__ inline void expand_block8(const Block8& f, int hi, int g4, BlockFrags
       const int n = hi - 8 * g4;
       c = make_uint4(keep_bytes(c.x, n), keep_bytes(c.y, n - 4), keep_bytes(c.z, n), keep_bytes(c.w, n - 4));
     }
-    x.v[2 * i] = kv8_to_bf16(c.x, c.y, vs);
-    x.v[2 * i + 1] = kv8_to_bf16(c.z, c.w, vs);
+    x.v[2 * i] = kVScale ? scaled_to_bf16(c.x, c.y, vs * s) : kv8_to_bf16(c.x, c.y, vs);
+    x.v[2 * i + 1] = kVScale ? scaled_to_bf16(c.z, c.w, vs * s) : kv8_to_bf16(c.z, c.w, vs);
   }
 }
 
@@ -150,7 +160,7 @@ __global__ __launch_bounds__(waves8(CG) * 64, waves8(CG) / 4) void decode_kv8_ke
   auto compute = [&](const BlockFrags& f, const BlockRef& r) __attribute__((always_inline)) {
 #pragma unroll
     for (int cg = 0; cg < CG; ++cg)
-      compute_block<kVScale, kMulti>(f, r, qf[cg], vs, scale_log2, n16, g4, lim[cg], lim_min, st[cg]);
+      compute_block<false, kMulti>(f, r, qf[cg], 1.f, scale_log2, n16, g4, lim[cg], lim_min, st[cg]);
   };
 
   // The blocks of a segment are dealt one by one to all waves of all splits, so that the workgroups of a (sequence, kv head)
@@ -176,7 +186,7 @@ __global__ __launch_bounds__(waves8(CG) * 64, waves8(CG) / 4) void decode_kv8_ke
     r.older = true;
     nan |= static_cast<uint32_t>(f.byte(f.ks) == 255u || f.byte(f.vs) == 255u);
     BlockFrags x;
-    expand_block8(f, r.hi, g4, x);
+    expand_block8<kVScale>(f, r.hi, g4, vs, x);
     compute(x, r);
   };
   // The first two older blocks are on their way while the last ring block is computed.

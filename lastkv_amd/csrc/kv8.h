@@ -32,6 +32,12 @@ __device__ inline float kv8_scale(uint32_t byte) {  // (0 and 255 set the mantis
   return __uint_as_float(byte << 23 | (((byte + 1) & 0xfeu) == 0 ? 0x400000u : 0u));
 }
 
+// The first n of eight bf16 values, the others 0.
+__device__ inline uint4 keep_tokens(uint4 x, int n) {
+  const auto mask = [n](int i) { return n >= 2 * i + 2 ? 0xffffffffu : n == 2 * i + 1 ? 0xffffu : 0u; };
+  return make_uint4(x.x & mask(0), x.y & mask(1), x.z & mask(2), x.w & mask(3));
+}
+
 // Eight e4m3 codes times a power of two as eight bf16 values.
 __device__ inline uint4 kv8_to_bf16(uint32_t lo, uint32_t hi, float scale) {
   return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false)),

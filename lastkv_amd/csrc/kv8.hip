@@ -4,9 +4,6 @@
 // e4m3(x * 2^-E) rounded to nearest even.  Bound by memory: 2 bytes read and 1 written a value.  One workgroup a (block, kv head,
 // sequence) takes K and V: a thread holds 16 values of each (two bf16 operands of its lane, 16 bytes of the 8-bit
 // block), so every load and store is 16 bytes a lane and nothing but the two maxima passes through LDS.
-#include <algorithm>
-
-#include "attn_common.h"
 #include "kv8.h"
 
 namespace lkv {
@@ -71,11 +68,6 @@ __device__ inline uint2 codes8(uint4 x, float f) {
 __device__ inline int scale_byte(uint32_t bits) {
   const int ex = static_cast<int>(bits >> 7);
   return ex == 255 ? 255 : max(0, ex - 8 + ((bits & 0x7fu) > 0x60u));
-}
-
-__device__ inline uint4 keep_tokens(uint4 x, int n) {  // the first n of eight values, the others 0
-  const auto mask = [n](int i) { return n >= 2 * i + 2 ? 0xffffffffu : n == 2 * i + 1 ? 0xffffu : 0u; };
-  return make_uint4(x.x & mask(0), x.y & mask(1), x.z & mask(2), x.w & mask(3));
 }
 
 __global__ __launch_bounds__(256) void kv8_quantize_kernel(const QuantizeParams p) {
@@ -175,73 +167,7 @@ __global__ __launch_bounds__(256) void kv8_unpack_kernel(const UnpackParams p) {
   }
 }
 
-struct CopyBlocksParams {
-  Kv8Pool src;
-  const int32_t* table;
-  int64_t ts;
-  const int32_t* len;
-  int32_t len_c, cap;
-  const int32_t* cu;
-  int32_t rows, max_rows, group, skip_rows, heads, blocks;
-  uint16_t* k;
-  uint16_t* v;
-};
-
-// One workgroup a (block, kv head, sequence): its codes as bf16 in the tiled layout.  V codes past the sequence's length become 0 (the
-// tile kernel multiplies them by 0).
-__global__ __launch_bounds__(256) void kv8_copy_blocks_kernel(const CopyBlocksParams p) {
-  const int j = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-  const int n = min(max(p.len ? p.len[b] : p.len_c, 0), p.cap) - j * kBlockTokens;
-  if (n <= 0) return;
-  if (p.cu != nullptr) {  // (as multi_rows counts them)
-    const int s0 = min(max(p.cu[b], 0), p.rows);
-    const int L = min(min(max(p.cu[b + 1], s0), p.rows) - s0, p.max_rows);
-    if (L <= 0 || static_cast<int64_t>(L) * p.group <= p.skip_rows) return;
-  }
-  const int lane = threadIdx.x & 63, piece = threadIdx.x >> 6, n16 = lane & 15, g4 = lane >> 4;
-  const int page = min(max(p.table[b * p.ts + j], 0), p.src.pages - 1);
-  const int64_t at = page * p.src.page + h * p.src.hs + threadIdx.x * 16;
-  const uint4 k = *reinterpret_cast<const uint4*>(p.src.k + at), v = *reinterpret_cast<const uint4*>(p.src.v + at);
-  const float sk = kv8_scale(p.src.ks[h * p.src.s_hs + page]), sv = kv8_scale(p.src.vs[h * p.src.s_hs + page]);
-  const int64_t to = ((static_cast<int64_t>(b) * p.heads + h) * p.blocks + j) * kBlockElems;
-  uint16_t* kd = p.k + to + (((piece >> 1) * 4 + (piece & 1) * 2) * 16 + n16) * 32 + 8 * g4;
-  *reinterpret_cast<uint4*>(kd) = kv8_to_bf16(k.x, k.y, sk);
-  *reinterpret_cast<uint4*>(kd + 16 * 32) = kv8_to_bf16(k.z, k.w, sk);
-  uint16_t* vd = p.v + to + (32 * piece + n16) * 32 + 8 * g4;
-  uint4 v0 = kv8_to_bf16(v.x, v.y, sv), v1 = kv8_to_bf16(v.z, v.w, sv);
-  if (n < kBlockTokens) {
-    v0 = keep_tokens(v0, n - 8 * g4);
-    v1 = keep_tokens(v1, n - 8 * g4);
-  }
-  *reinterpret_cast<uint4*>(vd) = v0;
-  *reinterpret_cast<uint4*>(vd + 16 * 32) = v1;
-}
-
 }  // namespace
-
-int32_t kv8_copy_blocks(const lkv_prefill_args* a, const Kv8Pool& o, int32_t group, int32_t skip_rows, int32_t blocks,
-                        uint16_t* k16, uint16_t* v16, hipStream_t s) {
-  if (blocks == 0) return LKV_OK;
-  CopyBlocksParams p;
-  p.src = o;
-  p.table = a->older_block_table;
-  p.ts = a->older_table_stride;
-  p.len = a->older_len;
-  p.len_c = a->older_len_const;
-  p.cap = a->older_capacity_tokens;
-  p.cu = a->cu_seqlens_q;
-  p.rows = a->tokens;
-  p.max_rows = a->cu_seqlens_q ? std::min(a->max_seqlen_q, a->tokens) : a->tokens;
-  p.group = group;
-  p.skip_rows = skip_rows;
-  p.heads = a->num_kv_heads;
-  p.blocks = blocks;
-  p.k = k16;
-  p.v = v16;
-  kv8_copy_blocks_kernel<<<dim3(blocks, a->num_kv_heads, a->batch), 256, 0, s>>>(p);
-  return check_launch("lkv_prefill_attn_kv8 (copies of 8-bit blocks)");
-}
-
 }  // namespace lkv
 
 extern "C" int32_t lkv_kv8_quantize(const lkv_kv8_quantize_args* a, const lkv_kv8_pool* dst, lkv_stream_t stream) {

@@ -28,31 +28,39 @@ struct CopyParams {
 };
 
 // kChunks: 16-byte pieces a thread copies of one page (page_bytes / 4096).  Workgroup x: pages [4 x, 4 x + 4) of the runs, of
-// one head's K or V; all of its loads come before its stores.
+// one head's K or V; all of its loads come before its stores.  The run of its first page is searched once.  Sources are read
+// with the non-temporal hint (2048 pages of 8 heads in 32 runs: 146 us with a search a page and without the hint, 97 us; hipMemcpy of the same bytes 90).
 template <int kChunks>
 __global__ __launch_bounds__(256) void copy_pages_kernel(const CopyParams p, const CopyRuns r) {
   const int h = blockIdx.y, kv = blockIdx.z;
   uint8_t* pool = p.pool[kv] + h * p.head;
   const int i0 = blockIdx.x * kPagesPerItem;
-  int64_t from[kPagesPerItem], to[kPagesPerItem];
+  int run = 0;
+  for (int hi = r.n - 1; run < hi;) {  // the first run whose end is past i0
+    const int mid = (run + hi) >> 1;
+    if (r.end[mid] > i0)
+      hi = mid;
+    else
+      run = mid + 1;
+  }
+  int end = r.end[run], start = run > 0 ? r.end[run - 1] : 0;
+  int src = r.src[run] - start, dst = r.dst[run] - start;
+  int from[kPagesPerItem], to[kPagesPerItem];
   uint4 x[kPagesPerItem][kChunks];
 #pragma unroll
   for (int q = 0; q < kPagesPerItem; ++q) {
     const int i = min(i0 + q, p.total - 1);
-    int lo = 0, hi = r.n - 1;  // the first run whose end is past i
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (r.end[mid] > i)
-        hi = mid;
-      else
-        lo = mid + 1;
+    if (i >= end) {  // (runs are not empty: the next one holds it)
+      start = end;
+      ++run;
+      end = r.end[run];
+      src = r.src[run] - start;
+      dst = r.dst[run] - start;
     }
-    const int in = i - (lo > 0 ? r.end[lo - 1] : 0);
-    from[q] = r.src[lo] + in;
-    to[q] = r.dst[lo] + in;
+    from[q] = src + i;
+    to[q] = dst + i;
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c)
-      x[q][c] = *reinterpret_cast<const uint4*>(pool + from[q] * p.page + (c * 256 + threadIdx.x) * 16);
+    for (int c = 0; c < kChunks; ++c) x[q][c] = load_nt(pool + from[q] * p.page + (c * 256 + threadIdx.x) * 16);
   }
 #pragma unroll
   for (int q = 0; q < kPagesPerItem; ++q) {

@@ -378,6 +378,113 @@ __device__ __attribute__((always_inline)) inline void v16_stage_blocks(const Pre
   __syncthreads();  // (sm_over is reused by the next sequence's call)
 }
 
+// The pre-pass of a call whose older segment is in 8-bit pages: as above, and the older blocks' K and V as bf16 copies in the
+// tiled layout (k16 / v16b, `blocks` per (sequence, kv head)), which the tile kernels read as a contiguous older segment.  A
+// thread holds 16 K and 16 V codes of a block; V codes past the sequence's length become 0 (the tiles multiply them by 0).
+struct Kv8Stage {
+  Kv8Pool src;
+  const int32_t* table;
+  int64_t ts;
+  uint16_t* k16;
+  uint16_t* v16b;
+  int32_t blocks;
+};
+
+template <bool kPaged, int kBlocks>
+__device__ __attribute__((always_inline)) inline void kv8_stage_blocks(const PrefillParams& p, const Kv8Stage& e, int b, int kvh, int x) {
+  const SeqView sv = make_seq_view(p.seg, b, kvh);
+  const int nb = sv.nb0 + local_blocks(sv, sv.n1);
+  const float vs = p.vscale_mode ? p.vscale[kvh] : 1.f;
+  const int blk0 = x * kBlocks;
+  const int n = min(kBlocks, nb - blk0);  // (workgroup-uniform)
+  if (n <= 0) return;
+  const int t = threadIdx.x, n16 = t & 15, g4 = (t >> 4) & 3, piece = t >> 6;
+  uint4 raw[kBlocks][2];  // older: K and V codes; local: 16 bf16 V values
+  float sk[kBlocks], sq[kBlocks];
+#pragma unroll
+  for (int k = 0; k < kBlocks; ++k) {
+    if (k >= n) break;
+    const int blk = blk0 + k;
+    if (blk < sv.nb0) {
+      const int page = min(max(e.table[b * e.ts + blk], 0), e.src.pages - 1);
+      const int64_t at = page * e.src.page + kvh * e.src.hs + t * 16;
+      sk[k] = kv8_scale(e.src.ks[kvh * e.src.s_hs + page]);
+      sq[k] = kv8_scale(e.src.vs[kvh * e.src.s_hs + page]);
+      raw[k][0] = *reinterpret_cast<const uint4*>(e.src.k + at);
+      raw[k][1] = *reinterpret_cast<const uint4*>(e.src.v + at);
+    } else {
+      const uint16_t* src = sv.lv + block_offset<kPaged>(sv, blk);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) raw[k][j] = *reinterpret_cast<const uint4*>(src + (t + j * 256) * 8);
+    }
+  }
+  uint32_t over = 0;  // bit k: block k holds a value fp16 cannot
+#pragma unroll
+  for (int k = 0; k < kBlocks; ++k) {
+    if (k >= n) break;
+    const int blk = blk0 + k;
+    const bool older = blk < sv.nb0;
+    uint4 v[2] = {raw[k][0], raw[k][1]};
+    int at = t * 8, step = 256 * 8;  // where v[j] stands in the block: at + j * step
+    if (older) {
+      const uint4 kc = raw[k][0], vc = raw[k][1];
+      const int valid = sv.n0 - blk * kBlockTokens - 8 * g4;
+      v[0] = keep_tokens(kv8_to_bf16(vc.x, vc.y, sq[k]), valid);
+      v[1] = keep_tokens(kv8_to_bf16(vc.z, vc.w, sq[k]), valid);
+      at = (32 * piece + n16) * 32 + 8 * g4;
+      step = 16 * 32;
+      const int64_t to = ((static_cast<int64_t>(b) * p.hkv + kvh) * e.blocks + blk) * kBlockElems;
+      uint16_t* kd = e.k16 + to + (((piece >> 1) * 4 + (piece & 1) * 2) * 16 + n16) * 32 + 8 * g4;
+      *reinterpret_cast<uint4*>(kd) = kv8_to_bf16(kc.x, kc.y, sk[k]);
+      *reinterpret_cast<uint4*>(kd + 16 * 32) = kv8_to_bf16(kc.z, kc.w, sk[k]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) *reinterpret_cast<uint4*>(e.v16b + to + at + j * step) = v[j];
+    }
+    uint16_t* dst = p.v16 + ((static_cast<int64_t>(b) * p.hkv + kvh) * p.v16_blocks + blk) * kBlockElems;
+    const float s = older ? vs : 1.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint4 y = scale_frag(v[j], s);
+      if (f16_overflow(y.x) || f16_overflow(y.y) || f16_overflow(y.z) || f16_overflow(y.w)) over |= 1u << k;
+      *reinterpret_cast<uint4*>(dst + at + j * step) =
+          make_uint4(f16x2_bits(bf16_lo(y.x), bf16_hi(y.x)), f16x2_bits(bf16_lo(y.y), bf16_hi(y.y)),
+                     f16x2_bits(bf16_lo(y.z), bf16_hi(y.z)), f16x2_bits(bf16_lo(y.w), bf16_hi(y.w)));
+    }
+  }
+  __shared__ uint32_t sm_over;
+  if (threadIdx.x == 0) sm_over = 0;
+  __syncthreads();
+  if (over != 0) atomicOr(&sm_over, over);
+  __syncthreads();
+  if (threadIdx.x < n)
+    p.vflags[(static_cast<int64_t>(b) * p.hkv + kvh) * p.vflag_stride + blk0 + threadIdx.x] =
+        (sm_over >> threadIdx.x) & 1u;
+  __syncthreads();  // (sm_over is reused by the next sequence's call)
+}
+
+// The grid is v16_stage_kernel's.
+template <bool kPaged, int kBlocks>
+__global__ __launch_bounds__(256) void kv8_stage_kernel(const PrefillParams p, const Kv8Stage e) {
+  const int kvh = blockIdx.y;
+  if ((blockIdx.x | blockIdx.y | blockIdx.z) == 0 && threadIdx.x == 0) *p.any_wide = 0.f;
+  if constexpr (kBlocks == 1) {
+    if (on_tile_path(p, seq_rows(p, blockIdx.z))) kv8_stage_blocks<kPaged, kBlocks>(p, e, blockIdx.z, kvh, blockIdx.x);
+    return;
+  }
+  const int lane = threadIdx.x & 63;
+  int rank = 0;
+  for (int i0 = 0; i0 < p.batch; i0 += 64) {
+    const int i = i0 + lane;
+    uint64_t m = __builtin_amdgcn_ballot_w64(i < p.batch && on_tile_path(p, seq_rows(p, i)));
+    while (m != 0) {  // (wave-uniform)
+      const int l = __builtin_ctzll(m);
+      m &= m - 1;
+      if (rank++ % static_cast<int>(gridDim.z) == static_cast<int>(blockIdx.z))
+        kv8_stage_blocks<kPaged, kBlocks>(p, e, i0 + l, kvh, blockIdx.x);
+    }
+  }
+}
+
 // Whether some block in [0, nbt) of (b, kvh) holds a V value fp16 cannot (the pre-pass's flags),
 // read 16 flags per load over the wave.
 // The flags of blocks [i, i + 16) of a flag row, those at or past nbt cleared (by masks, not by an
@@ -1572,15 +1679,17 @@ int32_t run_prefill(const lkv_prefill_args* a, const lkv::Kv8Pool* older8, void*
   }
   if (!c.runs_tiles) return LKV_OK;
   const bool older_paged = older8 == nullptr && a->older_block_table != nullptr;
-  if (older8 != nullptr) {  // from here on the older segment is its bf16 copies, one run per (sequence, kv head)
+  Kv8Stage stage8{};
+  if (older8 != nullptr) {  // for the tiles the older segment is its bf16 copies, one run per (sequence, kv head)
     const int64_t blocks = older_blocks(a), run = blocks * kBlockElems;
-    uint16_t* k16 = static_cast<uint16_t*>(copies);
-    uint16_t* v16 = k16 + static_cast<int64_t>(a->batch) * a->num_kv_heads * run;
-    if (const int32_t st = kv8_copy_blocks(a, *older8, group, c.short_on_decode && ragged ? 64 : 0, static_cast<int32_t>(blocks), k16,
-                                           v16, s))
-      return st;
-    p.seg.ok = k16;
-    p.seg.ov = v16;
+    stage8.src = *older8;
+    stage8.table = a->older_block_table;
+    stage8.ts = a->older_table_stride;
+    stage8.k16 = static_cast<uint16_t*>(copies);
+    stage8.v16b = stage8.k16 + static_cast<int64_t>(a->batch) * a->num_kv_heads * run;
+    stage8.blocks = static_cast<int32_t>(blocks);
+    p.seg.ok = stage8.k16;
+    p.seg.ov = stage8.v16b;
     p.seg.o_ss = a->num_kv_heads * run;
     p.seg.o_hs = run;
     p.seg.o_cap = static_cast<int32_t>(blocks * kBlockTokens);
@@ -1624,10 +1733,18 @@ int32_t run_prefill(const lkv_prefill_args* a, const lkv::Kv8Pool* older8, void*
   p.batch = a->batch;
   const bool paged = older_paged || a->local_block_table != nullptr;
   if (vblocks > 0) {  // (no keys at all: every row's output is zero; the main kernel skips its loop)
-    const int per_wg = ragged ? 8 : 1;
+    const int per_wg = !ragged ? 1 : older8 != nullptr ? 2 : 8;
     const dim3 vgrid(static_cast<unsigned>((vblocks + per_wg - 1) / per_wg), a->num_kv_heads,
                      ragged ? std::min(a->batch, 4) : a->batch);
-    if (paged && ragged)
+    if (older8 != nullptr && paged && ragged)
+      kv8_stage_kernel<true, 2><<<vgrid, 256, 0, s>>>(p, stage8);
+    else if (older8 != nullptr && paged)
+      kv8_stage_kernel<true, 1><<<vgrid, 256, 0, s>>>(p, stage8);
+    else if (older8 != nullptr && ragged)
+      kv8_stage_kernel<false, 2><<<vgrid, 256, 0, s>>>(p, stage8);
+    else if (older8 != nullptr)
+      kv8_stage_kernel<false, 1><<<vgrid, 256, 0, s>>>(p, stage8);
+    else if (paged && ragged)
       v16_stage_kernel<true, 8><<<vgrid, 256, 0, s>>>(p);
     else if (paged)
       v16_stage_kernel<true, 1><<<vgrid, 256, 0, s>>>(p);
