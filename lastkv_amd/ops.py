@@ -1160,12 +1160,18 @@ def kv8_unpack(pool: PagedKV8, table: torch.Tensor, token0: int, tokens: int) ->
     return k, v
 
 
+def kv8_copy_bytes(batch: int, kv_heads: int, older_tokens: int) -> int:
+    """Workspace of the bf16 copies that a prefill call over a ``PagedKV8`` makes for sequences above 64 query rows per kv
+    head, on top of ``prefill_workspace_bytes`` of the same arguments."""
+
+    return batch * kv_heads * -(-older_tokens // BLOCK_TOKENS) * 2 * BLOCK_ELEMS * 2
+
+
 def prefill_kv8_workspace_bytes(batch: int, kv_heads: int, older_tokens: int, local_tokens: int, **kwargs) -> int:
-    """``prefill_workspace_bytes`` of a call whose older segment is a ``PagedKV8``: with room for bf16 copies of its
-    blocks."""
+    """``prefill_workspace_bytes`` of a call whose older segment is a ``PagedKV8``."""
 
     return (prefill_workspace_bytes(batch, kv_heads, older_tokens, local_tokens, **kwargs)
-            + batch * kv_heads * -(-older_tokens // BLOCK_TOKENS) * 2 * BLOCK_ELEMS * 2)
+            + kv8_copy_bytes(batch, kv_heads, older_tokens))
 
 
 def _page_list(name: str, ids) -> np.ndarray:

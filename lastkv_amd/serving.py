@@ -103,12 +103,14 @@ class PinnedStager:
 class PageAllocator:
     """Host bookkeeping of sequence slots and shared-cache pages: per slot a table row of page ids
     (unused entries name ``scratch``), pages handed out in order as a sequence grows and returned
-    when its slot closes."""
+    when its slot closes.  A forked slot shares pages with its parent (``refs`` counts a page's slots); a shared page goes
+    back when the last of them closes."""
 
     def __init__(self, *, max_slots: int, pages: int, width: int, scratch: int):
         self.width, self.scratch = width, scratch
         self.table = np.full((max_slots, width), scratch, dtype=np.int32)
         self.used = np.zeros(max_slots, dtype=np.int64)
+        self.refs = np.zeros(pages, dtype=np.int64)
         self._free_pages = list(range(pages - 1, -1, -1))
         self._free_slots = list(range(max_slots - 1, -1, -1))
 
@@ -123,7 +125,10 @@ class PageAllocator:
 
     def close_slot(self, slot: int) -> None:
         n = int(self.used[slot])
-        self._free_pages.extend(int(p) for p in self.table[slot, :n][::-1])
+        for p in self.table[slot, :n][::-1]:
+            self.refs[p] -= 1
+            if self.refs[p] == 0:
+                self._free_pages.append(int(p))
         self.table[slot, :] = self.scratch
         self.used[slot] = 0
         self._free_slots.append(slot)
@@ -140,18 +145,92 @@ class PageAllocator:
         if need - have > len(self._free_pages):
             raise RuntimeError("the page pool is out of shared-cache pages")
         for j in range(have, need):
-            self.table[slot, j] = self._free_pages.pop()
+            self.table[slot, j] = self._take()
         self.used[slot] = need
         return have, need
+
+    def _take(self) -> int:
+        p = self._free_pages.pop()
+        self.refs[p] = 1
+        return p
+
+    def fork(self, slot: int, shared: int) -> int:
+        """A new slot whose first ``shared`` blocks are ``slot``'s pages and whose other blocks, as many as ``slot`` has, are
+        pages of its own (to be filled by the caller)."""
+
+        n = int(self.used[slot])
+        shared = min(shared, n)
+        if n - shared > len(self._free_pages):
+            raise RuntimeError("the page pool is out of shared-cache pages")
+        new = self.open_slot()
+        self.table[new, :shared] = self.table[slot, :shared]
+        self.refs[self.table[slot, :shared]] += 1
+        for j in range(shared, n):
+            self.table[new, j] = self._take()
+        self.used[new] = n
+        return new
+
+    def compact(self) -> list[tuple[list[int], list[int]]]:
+        """Renumber the pages in use so that every slot's stand in order from page 0 on (a shared page where its first
+        slot has it), and return the copies this takes: rounds of (sources, destinations), to be made one
+        after another, no page in both lists of a round.  Without a free page to move through, pages whose places are
+        taken stay where they are."""
+
+        order = dict.fromkeys(int(p) for slot in range(self.table.shape[0]) for p in self.table[slot, :int(self.used[slot])])
+        at = {p: p for p in order}  # where each page in use is now
+        holds = dict(at)            # and which one a place holds
+        empty = dict.fromkeys(p for p in range(len(self.refs) - 1, -1, -1) if p not in holds)  # the longest empty first
+        rounds: list[tuple[list[int], list[int]]] = []
+        src, dst, busy = [], [], set()
+
+        def move(page: int, to: int) -> None:
+            nonlocal src, dst, busy
+            here = at[page]
+            if here in busy or to in busy:  # (a place of this round: the next one goes on)
+                rounds.append((src, dst))
+                src, dst, busy = [], [], set()
+            src.append(here)
+            dst.append(to)
+            busy |= {here, to}
+            del holds[here], empty[to]
+            holds[to], at[page] = page, to
+            empty[here] = None
+
+        for target, page in enumerate(order):
+            if at[page] == target:
+                continue
+            if target in holds:  # the place is taken: its page makes room
+                spare = next(iter(empty), None)
+                if spare is None:
+                    continue
+                move(holds[target], spare)
+            move(page, target)
+        if src:
+            rounds.append((src, dst))
+        refs = {at[p]: int(self.refs[p]) for p in order}
+        for slot in range(self.table.shape[0]):
+            n = int(self.used[slot])
+            self.table[slot, :n] = [at[int(p)] for p in self.table[slot, :n]]
+        self.refs[:] = 0
+        for p, count in refs.items():
+            self.refs[p] = count
+        self._free_pages = [p for p in range(len(self.refs) - 1, -1, -1) if p not in refs]
+        return rounds
 
 
 class LastKVPagePool:
     """One head-major ``[Hkv, pages, 4096]`` K/V pool: shared last-layer pages (handed out per slot on demand)
     and per-layer ring pages (fixed per slot), plus one scratch page that padded rows and unused
-    table entries name.  Device copies of the page tables sit beside the host bookkeeping."""
+    table entries name.  Device copies of the page tables sit beside the host bookkeeping.
+
+    ``shared_cache="kv8"`` holds the shared pages in 8 bits, in a pool of their own (``shared``, an ``ops.PagedKV8``).  The
+    final layer's K/V are then written to a bf16 ring per slot (``stage_table``), long enough to keep every 32-token block
+    until all of it is history, and become 8-bit pages when their chunk does (``LastKVFastPath``): one rounding a value."""
 
     def __init__(self, *, num_layers: int, kv_heads: int, chunk_size: int, max_slots: int, source_pages: int,
-                 max_tokens_per_slot: int, device: torch.device | str):
+                 max_tokens_per_slot: int, device: torch.device | str, shared_cache: str = "bf16"):
+        if shared_cache not in ("bf16", "kv8"):
+            raise ValueError(f"shared_cache must be 'bf16' or 'kv8', got {shared_cache!r}")
         if min(num_layers, kv_heads, chunk_size, max_slots, source_pages, max_tokens_per_slot) < 1:
             raise ValueError("pool sizes must be positive")
         self.num_layers, self.kv_heads, self.chunk_size, self.max_slots = num_layers, kv_heads, chunk_size, max_slots
@@ -160,13 +239,26 @@ class LastKVPagePool:
         self.ring_blocks = self.ring_tokens // BLOCK
         self.src_width = -(-max_tokens_per_slot // BLOCK)
         self.source_pages = source_pages
+        self.kv8 = shared_cache == "kv8"
         ring_pages = num_layers * max_slots * self.ring_blocks
-        self.scratch_page = source_pages + ring_pages
+        first_ring = 0 if self.kv8 else source_pages
+        # a chunk becomes history as the next one ends: 2 C tokens, and what its first block holds of the chunk before
+        self.stage_blocks = -(-(2 * chunk_size + BLOCK - 1) // BLOCK) if self.kv8 else 0
+        self.first_stage = first_ring + ring_pages
+        self.scratch_page = self.first_stage + max_slots * self.stage_blocks
         self.pool = ops.PagedKV.zeros(self.scratch_page + 1, kv_heads, self.device)
         # ring pages: static table [L, slots, ring_blocks] behind the shared pages
-        ring = source_pages + np.arange(ring_pages, dtype=np.int64).reshape(num_layers, max_slots, self.ring_blocks)
-        self.ring_table = torch.from_numpy(ring.astype(np.int32)).to(self.device)
-        self.pages = PageAllocator(max_slots=max_slots, pages=source_pages, width=self.src_width, scratch=self.scratch_page)
+        self.ring_pages = first_ring + np.arange(ring_pages, dtype=np.int64).reshape(num_layers, max_slots, self.ring_blocks)
+        self.ring_table = torch.from_numpy(self.ring_pages.astype(np.int32)).to(self.device)
+        if self.kv8:
+            self.shared = ops.PagedKV8.zeros(source_pages + 1, kv_heads, self.device)
+            self.shared_scratch = source_pages
+            stage = (self.first_stage + np.arange(max_slots)[:, None] * self.stage_blocks
+                     + np.arange(self.src_width)[None, :] % self.stage_blocks)
+            self.stage_table = torch.from_numpy(stage.astype(np.int32)).to(self.device)
+        else:
+            self.shared, self.shared_scratch, self.stage_table = self.pool, self.scratch_page, None
+        self.pages = PageAllocator(max_slots=max_slots, pages=source_pages, width=self.src_width, scratch=self.shared_scratch)
         self.src_table = torch.from_numpy(self.pages.table.copy()).to(self.device)
         self.stager = PinnedStager(self.device)
         self._dirty_lo, self._dirty_hi = max_slots, 0  # table rows changed since the last flush
@@ -180,7 +272,7 @@ class LastKVPagePool:
 
     def close_slot(self, slot: int) -> None:
         self.pages.close_slot(slot)
-        self.src_table[slot].fill_(self.scratch_page)
+        self.src_table[slot].fill_(self.shared_scratch)
 
     def reserve(self, slot: int, tokens: int) -> None:
         """Give ``slot`` shared pages for positions ``[0, tokens)`` (host table; ``flush`` copies
@@ -188,8 +280,42 @@ class LastKVPagePool:
 
         lo, hi = self.pages.reserve(slot, tokens)
         if hi > lo:
-            self._dirty_lo = min(self._dirty_lo, slot)
-            self._dirty_hi = max(self._dirty_hi, slot + 1)
+            self._dirty(slot, slot + 1)
+
+    def _dirty(self, lo: int, hi: int) -> None:
+        self._dirty_lo, self._dirty_hi = min(self._dirty_lo, lo), max(self._dirty_hi, hi)
+
+    def fork_slot(self, slot: int, tokens: int, history: int) -> int:
+        """A new slot that continues as ``slot``, which holds ``tokens`` tokens: it shares the pages that are full and not
+        written again, and gets copies of the others and of the rings.  ``history``: the tokens that 8-bit pages hold."""
+
+        kept = history if self.kv8 else tokens
+        new = self.pages.fork(slot, kept // BLOCK)
+        if kept % BLOCK:
+            j = kept // BLOCK
+            ops.copy_pages(self.shared, self.pages.table[slot, j:j + 1], self.pages.table[new, j:j + 1])
+        blocks = -(-tokens // BLOCK)
+        src, dst = ([self.ring_pages[:, s, :blocks].reshape(-1)] for s in (slot, new))
+        if self.kv8:
+            stage = np.arange(min(self.stage_blocks, blocks))
+            for ids, s in ((src, slot), (dst, new)):
+                ids.append(self.first_stage + s * self.stage_blocks + stage)
+        ops.copy_pages(self.pool, *(np.concatenate(ids).astype(np.int32) for ids in (src, dst)))
+        self._dirty(new, new + 1)
+        return new
+
+    def compact(self) -> int:
+        """Move the shared pages in use together, every slot's in order (attention then streams them from one run
+        per kv head), and return how many copies that took.  Between steps only; captured decode graphs stay valid."""
+
+        moved = 0
+        for src, dst in self.pages.compact():
+            ops.copy_pages(self.shared, np.array(src, dtype=np.int32), np.array(dst, dtype=np.int32))
+            moved += len(src)
+        if moved:
+            self._dirty(0, self.max_slots)
+            self.flush()
+        return moved
 
     def flush(self) -> None:
         """One host-to-device copy of the table rows changed since the last flush."""
@@ -254,7 +380,9 @@ class LastKVFastPath:
         self._cu = torch.zeros(max_batch + 1, **i32)  # row offsets of a ragged step (cu_seqlens)
         self._cu_host = None  # the same offsets on the host
         self._slots = torch.zeros(max_batch, dtype=torch.long, device=dev)
-        self._older_table = torch.full((max_batch, pool.src_width), pool.scratch_page, **i32)
+        self._older_table = torch.full((max_batch, pool.src_width), pool.shared_scratch, **i32)
+        # where the final layer's K/V go: the shared pages, or with an 8-bit cache their bf16 ring
+        self._deep_table = torch.full((max_batch, pool.src_width), pool.scratch_page, **i32) if pool.kv8 else self._older_table
         self._ring_table = torch.full((pool.num_layers, max_batch, pool.ring_blocks), pool.scratch_page, **i32)
         self._cos1 = torch.zeros((max_batch, 1, ops.HEAD_DIM), dtype=torch.bfloat16, device=dev)
         self._sin1 = torch.zeros_like(self._cos1)
@@ -312,6 +440,17 @@ class LastKVFastPath:
         self._open[slot] = False
         self.pool.close_slot(slot)
 
+    def fork_sequence(self, slot: int) -> int:
+        """A new sequence that continues as ``slot`` from here on (between steps): it shares the full pages of their history
+        and has copies of what either will write."""
+
+        if not (0 <= slot < self.pool.max_slots) or not self._open[slot]:
+            raise ValueError(f"slot {slot} is not in use")
+        new = self.pool.fork_slot(slot, int(self._seen[slot]), max(0, int(self._committed[slot]) - self.pool.chunk_size))
+        self._seen[new], self._committed[new] = self._seen[slot], self._committed[slot]
+        self._open[new] = True
+        return new
+
     def seen(self, slot: int) -> int:
         return int(self._seen[slot])
 
@@ -362,8 +501,11 @@ class LastKVFastPath:
         P.stager.copy(slots, np.array([r.slot for r in parsed], dtype=np.int64))
         self._older_table[:B].copy_(P.src_table.index_select(0, slots))
         self._ring_table[:, :B].copy_(P.ring_table.index_select(1, slots))
+        if P.kv8:
+            self._deep_table[:B].copy_(P.stage_table.index_select(0, slots))
+            self._deep_table[B:Bp].fill_(P.scratch_page)
         if Bp > B:
-            self._older_table[B:Bp].fill_(P.scratch_page)
+            self._older_table[B:Bp].fill_(P.shared_scratch)
             self._ring_table[:, B:Bp].fill_(P.scratch_page)
         Hq = self.num_q_heads
         self.tokens = sum(r.tokens for r in parsed) + (Bp - B)
@@ -401,6 +543,8 @@ class LastKVFastPath:
             else:
                 need = max(need, ops.ragged_split_state_bytes(B, Hq, P.kv_heads, max(r.tokens for r in parsed),
                                                               self.num_splits or 0, ops._cu_count(P.device)))
+            if P.kv8:
+                need += ops.kv8_copy_bytes(B, P.kv_heads, width * BLOCK)
             if self._prefill_ws.numel() < need:
                 self._prefill_ws = torch.empty(need, dtype=torch.uint8, device=P.device)
         if self._q_out.shape[0] < self.tokens:
@@ -417,9 +561,15 @@ class LastKVFastPath:
         alpha, om, s = self.blend
         if self.contract == "vllm":  # rings hold V / s: blend with the unscaled shared V
             s = None
+        deep = P.stage_table if P.kv8 else P.src_table
         ops.blend_chunk(P.pool.k, P.pool.v, P.pool, batch=1, chunk_start=boundary - P.chunk_size, chunk_len=P.chunk_size,
                         alpha=alpha, one_minus_alpha=om, vscale=s, ring_table=P.ring_table[:, slot:slot + 1],
-                        ring_tokens=P.ring_tokens, deep_table=P.src_table[slot:slot + 1])
+                        ring_tokens=P.ring_tokens, deep_table=deep[slot:slot + 1])
+        history = boundary - P.chunk_size
+        if P.kv8 and history > 0:  # the chunk before becomes history: its 8-bit blocks, the one it starts in again as a whole
+            first = (history - P.chunk_size) // BLOCK
+            ops.kv8_quantize(P.pool, P.shared, src_table=P.stage_table[slot:slot + 1], dst_table=P.src_table[slot:slot + 1],
+                             tokens=history, first_block=first, blocks=-(-history // BLOCK) - first)
         self._committed[slot] = boundary
 
     # -------------------------------------------------------------- per-layer op sequence
@@ -452,9 +602,9 @@ class LastKVFastPath:
                 query[:T].reshape(B, n, Hq * 128), key[:T].reshape(B, n, Hkv * 128), value[:T].reshape(B, n, Hkv * 128),
                 cos, sin, num_q_heads=Hq, num_kv_heads=Hkv, q_norm_weight=qn_w, k_norm_weight=kn_w, eps=eps,
                 positions=pos[:B], ring=P.pool, ring_table=ring_tab[:B], ring_tokens=P.ring_tokens,
-                deep=P.pool if top else None, deep_table=self._older_table[:B] if top else None,
+                deep=P.pool if top else None, deep_table=self._deep_table[:B] if top else None,
                 q_out=self._q_out[:T].view(B, n, Hq, 128), **epi)
-            seg = dict(older=P.pool, older_table=self._older_table[:B], older_len=older_len[:B], vscale=vs, local=P.pool,
+            seg = dict(older=P.shared, older_table=self._older_table[:B], older_len=older_len[:B], vscale=vs, local=P.pool,
                        local_table=ring_tab[:B], local_ring_blocks=P.ring_blocks, local_len=local_len[:B],
                        local_start=local_start[:B], out_scale=out_scale)
             if n == 1:
@@ -477,10 +627,10 @@ class LastKVFastPath:
             query[:T].reshape(T, Hq * 128), key[:T].reshape(T, Hkv * 128), value[:T].reshape(T, Hkv * 128),
             cos, sin, num_q_heads=Hq, num_kv_heads=Hkv, q_norm_weight=qn_w, k_norm_weight=kn_w, eps=eps,
             positions=pos[:B], ring=P.pool, ring_table=ring_tab[:B], ring_tokens=P.ring_tokens,
-            deep=P.pool if top else None, deep_table=self._older_table[:B] if top else None,
+            deep=P.pool if top else None, deep_table=self._deep_table[:B] if top else None,
             q_out=self._q_out[:T], cu_seqlens=cu, max_seqlen=self.max_rows, **epi)
         width = max(1, -(-max(r.older for r in self.rows) // BLOCK))
-        seg = dict(older=P.pool, older_table=self._older_table[:B, :width], older_len=older_len[:B], vscale=vs,
+        seg = dict(older=P.shared, older_table=self._older_table[:B, :width], older_len=older_len[:B], vscale=vs,
                    local=P.pool, local_table=ring_tab[:B], local_ring_blocks=P.ring_blocks, local_len=local_len[:B],
                    local_start=local_start[:B], out_scale=out_scale)
         ops.prefill_attention(q_out, causal=True, out=output[:T].view(T, Hq, 128), workspace=self._prefill_ws,
@@ -584,11 +734,15 @@ class LastKVServingModel:
     product write (``ops.rmsnorm_mx8``, ``ops.silu_mul_mx8``); the output projection reads the attention's bf16 rows.
     This makes prompts faster; a decode step reads the same weights either way.  In calls of many rows the products of 8-bit
     rows are added eight at a time in fixed point (``ops.mx4_linear``).
-    The model passed in keeps its bf16 weights, which the 4-bit copy comes on top of."""
+    The model passed in keeps its bf16 weights, which the 4-bit copy comes on top of.
+
+    ``shared_cache="kv8"`` holds the shared history in 8 bits (``ops.PagedKV8``: e4m3 with a power-of-two scale per 32 tokens
+    of a kv head), half of its memory and of the bytes that every layer's attention reads of it; the recent and current
+    chunk stay bf16.  ``fork_sequence`` and ``beam_search`` work over either."""
 
     def __init__(self, model, *, max_batch: int, max_tokens_per_slot: int, source_pages: int | None = None,
                  num_splits: int | None = None, device=None, contract: str = "hf", weights: str = "bf16",
-                 activations: str = "bf16"):
+                 activations: str = "bf16", shared_cache: str = "bf16"):
         if weights not in ("bf16", "mxfp4"):
             raise ValueError(f"weights must be 'bf16' or 'mxfp4', got {weights!r}")
         if activations not in ("bf16", "mxfp8"):
@@ -605,7 +759,7 @@ class LastKVServingModel:
         self.pool = LastKVPagePool(num_layers=cfg.num_hidden_layers, kv_heads=cfg.num_key_value_heads,
                                    chunk_size=cfg.chunk_size, max_slots=max_batch,
                                    source_pages=source_pages or max_batch * per_slot,
-                                   max_tokens_per_slot=max_tokens_per_slot, device=device)
+                                   max_tokens_per_slot=max_tokens_per_slot, device=device, shared_cache=shared_cache)
         self.fast = LastKVFastPath.from_model(model, self.pool, max_batch=max_batch, num_splits=num_splits,
                                               contract=contract)
         self.config = cfg
@@ -624,6 +778,11 @@ class LastKVServingModel:
 
     def free_sequence(self, slot: int) -> None:
         self.fast.free_sequence(slot)
+
+    def fork_sequence(self, slot: int) -> int:
+        """A new sequence that continues as ``slot`` from here on (``LastKVFastPath.fork_sequence``)."""
+
+        return self.fast.fork_sequence(slot)
 
     @torch.no_grad()
     def step(self, rows: list[tuple[int, torch.Tensor]], pad_to: int | None = None) -> torch.Tensor:
@@ -736,6 +895,96 @@ class LastKVServingModel:
             for slot in slots:
                 self.free_sequence(slot)
         return [torch.cat([p.reshape(-1).cpu(), torch.tensor(g, dtype=p.dtype)]) for p, g in zip(prompts, gen)]
+
+
+    @torch.no_grad()
+    def beam_search(self, prompts: list[torch.Tensor], num_beams: int, max_new_tokens: int, *, eos_token_id: int | None = None,
+                    length_penalty: float = 1.0, prefill_chunk: int | None = None) -> list[list[tuple[torch.Tensor, float]]]:
+        """Beam search over every prompt with ``num_beams`` sequences each, all of them in one step: the best candidates of
+        a prompt's beams are selected (``ops.beam_select``) and beams that go on more than once are forked.
+
+        Returns per prompt its ``num_beams`` best hypotheses as (prompt and new ids, score), best first; a score is the sum of
+        the new tokens' log-probabilities divided by their number to the power of ``length_penalty``.  A beam that chooses
+        ``eos_token_id`` is a finished hypothesis, and a prompt with ``num_beams`` of them is done; without one
+        every hypothesis has ``max_new_tokens`` new ids."""
+
+        K = num_beams
+        count = K if eos_token_id is None else 2 * K
+        if K < 1 or count > min(64, self.model.lm_head.weight.shape[0]) or max_new_tokens < 1:
+            raise ValueError(f"{count} candidates of {K} beams: 1 to 64 and no more than the vocabulary, and max_new_tokens >= 1")
+        if len(prompts) * K > self.pool.max_slots - int(self.fast._open.sum()):
+            raise ValueError(f"{len(prompts)} prompts of {K} beams need that many free sequences")
+        flats = [p.reshape(-1) for p in prompts]
+        if any(f.numel() == 0 for f in flats):
+            raise ValueError("prompts must not be empty")
+        slots: list[list[int]] = []  # per prompt: the alive beams' slots, best first
+        new: list[list[list[int]]] = [[[]] for _ in flats]  # their new ids
+        scores: list[list[float]] = [[0.0] for _ in flats]
+        done: list[list[tuple[float, list[int]]]] = [[] for _ in flats]
+
+        def choose(live: list[int], logits: torch.Tensor) -> list[int]:
+            """One selection for the prompts ``live``, whose beams' logits follow each other; returns those that go on."""
+
+            at = torch.tensor([scores[i] for i in live], dtype=torch.float32, device=logits.device)
+            picks = ops.beam_select(logits.view(len(live), -1, logits.shape[-1]), at, count)
+            on = []
+            for i, *rows in zip(live, *(t.tolist() for t in picks)):
+                kids = []  # (score, beam, token)
+                for rank, (score, k, tok) in enumerate(zip(*rows)):
+                    if tok < 0:
+                        raise RuntimeError("the logits leave fewer candidates than beams")
+                    if tok == eos_token_id:
+                        if rank < K:
+                            done[i].append((score, new[i][k] + [tok]))
+                    elif len(kids) < K:
+                        kids.append((score, k, tok))
+                last = len(new[i][0]) + 1 >= max_new_tokens
+                if last and len(done[i]) < K:
+                    done[i] += [(score, new[i][k] + [tok]) for score, k, tok in kids]
+                old, goes_on = slots[i], {} if last or len(done[i]) >= K else dict.fromkeys(k for _, k, _ in kids)
+                for k, slot in enumerate(old):
+                    if k not in goes_on:
+                        self.free_sequence(slot)
+                slots[i] = [old[k] for k in goes_on]
+                if not goes_on:
+                    continue
+                mine = []
+                for _, k, _ in kids:  # a beam's first successor goes on in its slot
+                    if goes_on[k] is None:
+                        goes_on[k] = old[k]
+                        mine.append(old[k])
+                    else:
+                        slots[i].append(self.fork_sequence(old[k]))
+                        mine.append(slots[i][-1])
+                slots[i] = mine
+                new[i] = [new[i][k] + [tok] for _, k, tok in kids]
+                scores[i] = [score for score, _, _ in kids]
+                on.append(i)
+            return on
+
+        C = self.config.chunk_size
+        try:
+            live = []
+            for i, flat in enumerate(flats):
+                slots.append([self.add_sequence()])
+                fed = 0
+                while fed < flat.numel():
+                    take = min(flat.numel() - fed, C - self.fast.seen(slots[i][0]) % C, prefill_chunk or flat.numel())
+                    logits = self.step([(slots[i][0], flat[fed:fed + take])])
+                    fed += take
+                live += choose([i], logits)
+            while live:
+                rows = [(slot, torch.tensor(new[i][k][-1:], dtype=flats[i].dtype)) for i in live for k, slot in enumerate(slots[i])]
+                live = choose(live, self.step(rows))
+        finally:
+            for mine in slots:
+                for slot in mine:
+                    self.free_sequence(slot)
+        out = []
+        for flat, hyps in zip(flats, done):
+            ranked = sorted(((s / len(t) ** length_penalty, t) for s, t in hyps), key=lambda h: -h[0])[:K]
+            out.append([(torch.cat([flat.cpu(), torch.tensor(t, dtype=flat.dtype)]), s) for s, t in ranked])
+        return out
 
 
 class DecodeGraph:
