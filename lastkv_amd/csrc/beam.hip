@@ -48,31 +48,39 @@ __device__ inline uint32_t order_bits(float x) {
 __device__ inline float from_order(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 template <int kCtrl>
-__device__ inline float quad_swap(float x) {
+__device__ inline float dpp_move(float x) {
   return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), kCtrl, 0xf, 0xf, true));
 }
 
-// A floor that at least n (<= kQuads) of the values reach of which each of the 4 * kQuads threads gives the greatest: the
-// n-th greatest of the quads' maxima, found by counting for each how many stand before it (a quarter of them a thread).
-template <int kQuads>
+// A floor that at least n (<= 64) of the values reach of which each of the kThreads threads gives the greatest: the n-th
+// greatest of the maxima of 64 groups of neighbours, found by counting for each how many stand before it (a wave counts a
+// part of them).  64 groups are the fewest that do, and their counting the least: with groups of four the choice below,
+// of 1024 threads, took 9.5 us in place of @@.
+template <int kThreads>
 struct FloorShared {
-  float top[kQuads];
-  int32_t before[kQuads];
+  float top[64];
+  int32_t before[64];
   float result;
 };
 
-template <int kQuads>
-__device__ inline float nth_floor(float x, int n, FloorShared<kQuads>& sm) {
-  const int t = threadIdx.x, i = t % kQuads, part = t / kQuads;
-  x = fmaxf(x, quad_swap<0xb1>(x));
-  x = fmaxf(x, quad_swap<0x4e>(x));
-  if ((t & 3) == 0) sm.top[t >> 2] = x;
+template <int kThreads>
+__device__ inline float nth_floor(float x, int n, FloorShared<kThreads>& sm) {
+  constexpr int kGroup = kThreads / 64, kWaves = kThreads / 64, kPart = 64 / kWaves;
+  static_assert(kGroup == 4 || kGroup == 16, "groups are quads or rows of 16 lanes");
+  const int t = threadIdx.x, i = t & 63, part = t >> 6;
+  x = fmaxf(x, dpp_move<0xb1>(x));
+  x = fmaxf(x, dpp_move<0x4e>(x));
+  if (kGroup == 16) {
+    x = fmaxf(x, dpp_move<0x141>(x));  // (the row's halves mirrored, then the row)
+    x = fmaxf(x, dpp_move<0x140>(x));
+  }
+  if (t % kGroup == 0) sm.top[t / kGroup] = x;
   if (part == 0) sm.before[i] = 0;
   __syncthreads();
   const float mine = sm.top[i];
   int before = 0;
-#pragma unroll 4
-  for (int j = part * (kQuads / 4); j < (part + 1) * (kQuads / 4); j += 4) {
+#pragma unroll
+  for (int j = part * kPart; j < (part + 1) * kPart; j += 4) {
     const float4 k = *reinterpret_cast<const float4*>(&sm.top[j]);
     before += (k.x > mine) || (k.x == mine && j < i);
     before += (k.y > mine) || (k.y == mine && j + 1 < i);
@@ -119,7 +127,7 @@ __device__ inline void load_values(const void* row, int64_t e0, int V, float (&x
 template <bool kF32, int kChunks>
 __global__ __launch_bounds__(kBeamThreads) void beam_slice_kernel(const BeamParams p) {
   constexpr int kVec = kF32 ? 4 : 8;
-  __shared__ __align__(16) FloorShared<kBeamThreads / 4> sm_floor;
+  __shared__ __align__(16) FloorShared<kBeamThreads> sm_floor;
   __shared__ uint64_t sm_cand[kBeamCap];
   __shared__ double sm_sum[4];
   __shared__ float sm_max[4];
@@ -244,7 +252,7 @@ __device__ inline bool ahead(const Candidate& a, const Candidate& b) {
 constexpr int kChooseThreads = 1024, kChooseWaves = kChooseThreads / 64, kHeld = 4;
 
 __global__ __launch_bounds__(kChooseThreads) void beam_choose_kernel(const BeamParams p) {
-  __shared__ __align__(16) FloorShared<kChooseThreads / 4> sm_floor;
+  __shared__ __align__(16) FloorShared<kChooseThreads> sm_floor;
   __shared__ double sm_lse[LKV_BEAM_MAX_BEAMS], sm_score[LKV_BEAM_MAX_BEAMS], sm_total[kBeamCap], sm_wtotal[kChooseWaves];
   __shared__ uint64_t sm_tie[kBeamCap], sm_wtie[kChooseWaves];
   __shared__ uint32_t sm_n;
@@ -398,11 +406,11 @@ extern "C" int32_t lkv_beam_select(const lkv_beam_select_args* a, lkv_stream_t s
   LKV_REQUIRE(a->vocab >= 1 && a->vocab <= (1 << 20), "vocab must be in [1, 2^20], got %d", a->vocab);
   LKV_REQUIRE(a->count >= 1 && a->count <= LKV_BEAM_MAX_COUNT, "count must be in [1, %d], got %d", LKV_BEAM_MAX_COUNT, a->count);
   LKV_REQUIRE(a->logits_fp32 == 0 || a->logits_fp32 == 1, "logits_fp32 must be 0 or 1");
+  if (a->batch == 0) return LKV_OK;  // (empty tensors have no address)
   LKV_REQUIRE(a->logits && a->scores && a->out_scores && a->out_beams && a->out_tokens, "null tensor");
   const int64_t rows = static_cast<int64_t>(a->batch) * a->beams;
   LKV_REQUIRE(rows <= 65535, "batch * beams must be <= 65535");
   LKV_REQUIRE((reinterpret_cast<uintptr_t>(a->logits) & (a->logits_fp32 ? 3 : 1)) == 0, "logits must be aligned to their type");
-  if (a->batch == 0) return LKV_OK;
   const int64_t need = lkv_beam_workspace_bytes(a->batch, a->beams, a->vocab, a->count);
   if (a->workspace == nullptr || a->workspace_bytes < need)
     return fail(LKV_ERR_WORKSPACE, "beam selection needs %lld bytes of workspace, got %lld", static_cast<long long>(need),

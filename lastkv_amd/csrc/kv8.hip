@@ -181,6 +181,7 @@ extern "C" int32_t lkv_kv8_quantize(const lkv_kv8_quantize_args* a, const lkv_kv
   LKV_REQUIRE(a->head_dim == kHeadDim, "head_dim must be 128, got %d", a->head_dim);
   LKV_REQUIRE(a->batch >= 0 && a->blocks >= 0 && a->first_block >= 0, "bad sizes");
   LKV_REQUIRE(a->heads == dst->heads, "the pools have %d and %d kv heads", a->heads, dst->heads);
+  if (a->batch == 0 || a->blocks == 0) return LKV_OK;  // (empty tensors have no address)
   LKV_REQUIRE(a->src_k && a->src_v && a->src_table && a->dst_table, "null tensor");
   LKV_REQUIRE(a->src_num_pages > 0, "src_num_pages must be positive");
   LKV_REQUIRE(((reinterpret_cast<uintptr_t>(a->src_k) | reinterpret_cast<uintptr_t>(a->src_v)) & 15) == 0 &&
@@ -192,7 +193,6 @@ extern "C" int32_t lkv_kv8_quantize(const lkv_kv8_quantize_args* a, const lkv_kv
               "blocks [%d, %lld) exceed the tables' %d and %d", a->first_block, static_cast<long long>(end),
               a->src_table_width, a->dst_table_width);
   LKV_REQUIRE(a->batch <= 65535 && a->heads <= 65535 && end < (1 << 26), "batch and heads must be <= 65535, blocks < 2^26");
-  if (a->batch == 0 || a->blocks == 0) return LKV_OK;
   p.k = static_cast<const uint16_t*>(a->src_k);
   p.v = static_cast<const uint16_t*>(a->src_v);
   p.page = a->src_page_stride;
@@ -216,7 +216,6 @@ extern "C" int32_t lkv_kv8_unpack(const lkv_kv8_pool* src, const int32_t* table,
   using namespace lkv;
   UnpackParams p;
   if (const int32_t st = kv8_pool(src, "src", p.src)) return st;
-  LKV_REQUIRE(table && k && v, "null tensor");
   LKV_REQUIRE(batch >= 0 && token0 >= 0 && tokens >= 0, "bad sizes");
   const int64_t end = (static_cast<int64_t>(token0) + tokens + kBlockTokens - 1) / kBlockTokens;
   LKV_REQUIRE(end <= table_width, "tokens [%d, %lld) exceed the table's %d blocks", token0,
@@ -225,7 +224,8 @@ extern "C" int32_t lkv_kv8_unpack(const lkv_kv8_pool* src, const int32_t* table,
                   ((k_stride_b | k_stride_h | k_stride_t | v_stride_b | v_stride_h | v_stride_t) & 7) == 0,
               "rows must be 16-byte aligned");
   LKV_REQUIRE(batch <= 65535 && src->heads <= 65535, "batch and heads must be <= 65535");
-  if (batch == 0 || tokens == 0) return LKV_OK;
+  if (batch == 0 || tokens == 0) return LKV_OK;  // (empty tensors have no address)
+  LKV_REQUIRE(table && k && v, "null tensor");
   p.table = table;
   p.ts = table_stride;
   p.k = static_cast<uint16_t*>(k);

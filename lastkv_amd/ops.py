@@ -164,9 +164,10 @@ class PagedKV:
 @dataclass
 class PagedKV8:
     """K and V page pools in 8 bits: e4m3 codes ``[heads, pages, 4096]`` (float8_e4m3fn, in the layout that the attention
-    kernels read) and one scale byte for each page of each head, ``[heads, pages]`` uint8 with the pages rounded up to a
-    multiple of four; byte e stands for 2^(e - 127), 255 for NaN.  Pages are addressed by block tables as those of a ``PagedKV``; ``kv8_quantize`` fills them
-    from bf16 pages, ``decode_attention`` and ``prefill_attention`` read them as their older segment."""
+    kernels read) and one scale byte for each page of each head, ``[heads, pages]`` uint8 with the pages rounded up to
+    a multiple of four; byte e stands for 2^(e - 127), 255 for NaN.  Pages are addressed by block tables as those of a
+    ``PagedKV``; ``kv8_quantize`` fills them from bf16 pages, ``decode_attention`` and ``prefill_attention`` read them
+    as their older segment."""
 
     k: torch.Tensor
     v: torch.Tensor

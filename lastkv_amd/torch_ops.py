@@ -16,7 +16,7 @@ library default.
 
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 from torch import Tensor
@@ -24,7 +24,8 @@ from torch import Tensor
 from . import ops
 
 __all__ = ["decode_attention", "prefill_attention", "merge_states", "qkv_epilogue", "blend_chunk", "rmsnorm",
-           "silu_mul", "rmsnorm_mx8", "add_rmsnorm_mx8", "silu_mul_mx8", "mx8_unpack", "mx4_linear", "mx4_linear_mx8"]
+           "silu_mul", "rmsnorm_mx8", "add_rmsnorm_mx8", "silu_mul_mx8", "mx8_unpack", "mx4_linear", "mx4_linear_mx8",
+           "kv8_quantize", "kv8_unpack", "decode_attention_kv8", "prefill_attention_kv8", "copy_pages", "beam_select"]
 
 
 def _seg(k: Optional[Tensor], v: Optional[Tensor], table: Optional[Tensor]):
@@ -259,3 +260,114 @@ def mx4_linear_mx8(data: Tensor, scales: Tensor, weight: Tensor, out_features: i
 @mx4_linear_mx8.register_fake
 def _(data, scales, weight, out_features, bias=None):
     return data.new_empty((*data.shape[:-1], out_features), dtype=torch.bfloat16)
+
+
+# An 8-bit pool (ops.PagedKV8) enters as its four tensors: the codes of K and V and their scale bytes.
+@torch.library.custom_op("lastkv::kv8_quantize", mutates_args=("dst_k", "dst_v", "dst_k_scales", "dst_v_scales"))
+def kv8_quantize(src_k: Tensor, src_v: Tensor, dst_k: Tensor, dst_v: Tensor, dst_k_scales: Tensor,
+                 dst_v_scales: Tensor, src_table: Tensor, dst_table: Tensor, tokens: Optional[Tensor],
+                 tokens_const: int, first_block: int = 0, blocks: int = -1) -> None:
+    """``lkv_kv8_quantize``: blocks of bf16 pages into 8-bit pages (``blocks`` -1: the rest of the narrower table)."""
+
+    ops.kv8_quantize(ops.PagedKV(src_k, src_v), ops.PagedKV8(dst_k, dst_v, dst_k_scales, dst_v_scales),
+                     src_table=src_table, dst_table=dst_table, tokens=_len(tokens, tokens_const),
+                     first_block=first_block, blocks=None if blocks == -1 else blocks)
+
+
+@kv8_quantize.register_fake
+def _(src_k, src_v, dst_k, dst_v, dst_k_scales, dst_v_scales, src_table, dst_table, tokens, tokens_const,
+      first_block=0, blocks=-1):
+    return None
+
+
+@torch.library.custom_op("lastkv::kv8_unpack", mutates_args=())
+def kv8_unpack(k: Tensor, v: Tensor, k_scales: Tensor, v_scales: Tensor, table: Tensor, token0: int,
+               tokens: int) -> tuple[Tensor, Tensor]:
+    """``lkv_kv8_unpack``: K and V of a token range, ``[B, H, tokens, 128]`` bf16."""
+
+    return ops.kv8_unpack(ops.PagedKV8(k, v, k_scales, v_scales), table, token0, tokens)
+
+
+@kv8_unpack.register_fake
+def _(k, v, k_scales, v_scales, table, token0, tokens):
+    shape = (table.shape[0], k.shape[0], tokens, ops.HEAD_DIM)
+    return k.new_empty(shape, dtype=torch.bfloat16), k.new_empty(shape, dtype=torch.bfloat16)
+
+
+@torch.library.custom_op("lastkv::decode_attention_kv8", mutates_args=())
+def decode_attention_kv8(q: Tensor, older_k: Tensor, older_v: Tensor, older_k_scales: Tensor, older_v_scales: Tensor,
+                         older_len: Optional[Tensor], older_len_const: int, older_table: Tensor,
+                         vscale: Optional[Tensor], local_k: Optional[Tensor], local_v: Optional[Tensor],
+                         local_len: Optional[Tensor], local_len_const: int, local_start: Optional[Tensor],
+                         local_start_const: int, local_table: Optional[Tensor], local_ring_blocks: int,
+                         sm_scale: float, num_splits: int, out_scale: Optional[Tensor] = None) -> Tensor:
+    """``lkv_decode_attn_kv8``: ``decode_attention`` whose older segment is an 8-bit pool."""
+
+    return ops.decode_attention(
+        q, older=ops.PagedKV8(older_k, older_v, older_k_scales, older_v_scales),
+        older_len=_len(older_len, older_len_const), vscale=vscale, local=_seg(local_k, local_v, local_table),
+        local_len=_len(local_len, local_len_const), local_start=_len(local_start, local_start_const),
+        older_table=older_table, local_table=local_table, local_ring_blocks=local_ring_blocks or None,
+        sm_scale=sm_scale or None, num_splits=num_splits or None, out_scale=out_scale)
+
+
+@decode_attention_kv8.register_fake
+def _(q, older_k, older_v, older_k_scales, older_v_scales, older_len, older_len_const, older_table, vscale, local_k,
+      local_v, local_len, local_len_const, local_start, local_start_const, local_table, local_ring_blocks, sm_scale,
+      num_splits, out_scale=None):
+    return q.new_empty((q.shape[0], q.shape[1], ops.HEAD_DIM))
+
+
+@torch.library.custom_op("lastkv::prefill_attention_kv8", mutates_args=())
+def prefill_attention_kv8(q: Tensor, older_k: Tensor, older_v: Tensor, older_k_scales: Tensor, older_v_scales: Tensor,
+                          older_len: Optional[Tensor], older_len_const: int, older_table: Tensor,
+                          vscale: Optional[Tensor], local_k: Optional[Tensor], local_v: Optional[Tensor],
+                          local_len: Optional[Tensor], local_len_const: int, local_start: Optional[Tensor],
+                          local_start_const: int, local_table: Optional[Tensor], local_ring_blocks: int, causal: bool,
+                          sm_scale: float, out_scale: Optional[Tensor] = None, cu_seqlens_q: Optional[Tensor] = None,
+                          max_seqlen_q: int = 0, num_splits: int = 0,
+                          cu_seqlens_q_host: Optional[Tensor] = None) -> Tensor:
+    """``lkv_prefill_attn_kv8``: ``prefill_attention`` whose older segment is an 8-bit pool."""
+
+    return ops.prefill_attention(
+        q, older=ops.PagedKV8(older_k, older_v, older_k_scales, older_v_scales),
+        older_len=_len(older_len, older_len_const), vscale=vscale, local=_seg(local_k, local_v, local_table),
+        local_len=_len(local_len, local_len_const), local_start=_len(local_start, local_start_const),
+        older_table=older_table, local_table=local_table, local_ring_blocks=local_ring_blocks or None, causal=causal,
+        sm_scale=sm_scale or None, out_scale=out_scale, cu_seqlens_q=cu_seqlens_q,
+        max_seqlen_q=max_seqlen_q if cu_seqlens_q is not None else None, num_splits=num_splits,
+        cu_seqlens_q_host=None if cu_seqlens_q_host is None else cu_seqlens_q_host.numpy())
+
+
+@prefill_attention_kv8.register_fake
+def _(q, older_k, older_v, older_k_scales, older_v_scales, older_len, older_len_const, older_table, vscale, local_k,
+      local_v, local_len, local_len_const, local_start, local_start_const, local_table, local_ring_blocks, causal,
+      sm_scale, out_scale=None, cu_seqlens_q=None, max_seqlen_q=0, num_splits=0, cu_seqlens_q_host=None):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("lastkv::copy_pages", mutates_args=("k", "v", "k_scales", "v_scales"))
+def copy_pages(k: Tensor, v: Tensor, k_scales: Optional[Tensor], v_scales: Optional[Tensor], src: Sequence[int],
+               dst: Sequence[int]) -> None:
+    """``lkv_copy_pages`` of a bf16 pool (no scales) or an 8-bit one: page ``dst[i]`` := page ``src[i]``."""
+
+    ops.copy_pages(ops.PagedKV(k, v) if k_scales is None else ops.PagedKV8(k, v, k_scales, v_scales), src, dst)
+
+
+@copy_pages.register_fake
+def _(k, v, k_scales, v_scales, src, dst):
+    return None
+
+
+@torch.library.custom_op("lastkv::beam_select", mutates_args=())
+def beam_select(logits: Tensor, scores: Tensor, count: int) -> tuple[Tensor, Tensor, Tensor]:
+    """``lkv_beam_select``: (scores fp32, beams int32, tokens int32), ``[B, count]`` each."""
+
+    return ops.beam_select(logits, scores, count)
+
+
+@beam_select.register_fake
+def _(logits, scores, count):
+    shape = (logits.shape[0], count)
+    return (logits.new_empty(shape, dtype=torch.float32), logits.new_empty(shape, dtype=torch.int32),
+            logits.new_empty(shape, dtype=torch.int32))
