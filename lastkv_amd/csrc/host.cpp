@@ -409,7 +409,13 @@ PyObject* decode_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
         keys += a.local_len != nullptr ? int64_t{a.local_ring_blocks} * LKV_BLOCK_TOKENS : a.local_len_const;
       const int64_t pairs = std::max<int64_t>(1, B * hkv);
       const int64_t blocks = std::max<int64_t>(1, (keys + LKV_BLOCK_TOKENS - 1) / LKV_BLOCK_TOKENS);
-      splits = std::max<int64_t>(1, std::min<int64_t>({std::max<int64_t>(1, cus / pairs), (blocks + 3) / 4, 1024}));
+      splits = std::max<int64_t>(1, cus / pairs);
+      if (eight && pairs > cus && pairs % cus > 0 && pairs % cus <= cus / 2) {
+        auto rounds = [&](int64_t n) { return static_cast<double>((pairs * n + cus - 1) / cus) / static_cast<double>(n); };
+        for (int64_t n = 2; n <= std::min<int64_t>(8, blocks / 64); ++n)
+          if (rounds(n) < rounds(splits)) splits = n;
+      }
+      splits = std::max<int64_t>(1, std::min<int64_t>({splits, (blocks + 3) / 4, 1024}));
     } else if (!as_int(v[13], splits) || splits < 1 || splits > 1024) {
       return not_handled();
     }

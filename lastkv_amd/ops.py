@@ -312,15 +312,23 @@ def _cu_count(device: torch.device) -> int:
     return _CU_COUNT[index]
 
 
-def default_decode_splits(batch: int, kv_heads: int, max_tokens: int, cu_count: int) -> int:
+def default_decode_splits(batch: int, kv_heads: int, max_tokens: int, cu_count: int, older8: bool = False) -> int:
     """Key splits per (sequence, kv head): as many as fit one round of workgroups (one 4-wave
     workgroup runs per CU).  A second round costs more than the CUs one round leaves idle: at 8K
     keys and 8 kv heads, B = 20 takes 99 us with one split (160 workgroups) against 124 us with two,
-    B = 12 71 us with two (192) against 93 us with three."""
+    B = 12 71 us with two (192) against 93 us with three.
+
+    With an 8-bit older segment (``older8``, 8-wave workgroups) more pairs than CUs whose last round is at most half full
+    are split into up to 8 parts of 64 blocks or more, as many as give the fewest rounds a part: at 8 kv heads and 9.3K
+    keys B = 34 takes 137 us with four against 162 with one, B = 40 146 against 165, B = 72 247 with three against 271, and
+    B = 40 at 30K 400 against 479; with fuller last rounds one is best (B = 56 190 against 198, B = 32 105 against 116)."""
 
     pairs = max(1, batch * kv_heads)
     blocks = max(1, math.ceil(max_tokens / BLOCK_TOKENS))
     splits = max(1, cu_count // pairs)
+    if older8 and pairs > cu_count and 0 < pairs % cu_count <= cu_count // 2:
+        rounds = lambda n: math.ceil(pairs * n / cu_count) / n
+        splits = min(range(1, min(8, max(1, blocks // 64)) + 1), key=rounds)
     return int(max(1, min(splits, math.ceil(blocks / 4), 1024)))
 
 
@@ -494,7 +502,7 @@ def decode_attention(
     if local is not None:
         max_tokens += a.local_ring_blocks * BLOCK_TOKENS if isinstance(local_len, torch.Tensor) else int(local_len)
     if num_splits is None:
-        num_splits = default_decode_splits(B, Hkv, max_tokens, _cu_count(device))
+        num_splits = default_decode_splits(B, Hkv, max_tokens, _cu_count(device), isinstance(older, PagedKV8))
     lib = _lib.load()
     need = lib.lkv_decode_workspace_bytes(B, Hq, num_splits)
     if no_alloc:

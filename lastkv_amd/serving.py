@@ -514,8 +514,8 @@ class LastKVFastPath:
             self._cos1[:Bp].copy_(cos)
             self._sin1[:Bp].copy_(sin)
             keys = max(r.older + r.local for r in parsed)
-            self.splits = num_splits or self.num_splits or ops.default_decode_splits(Bp, P.kv_heads, keys,
-                                                                                      ops._cu_count(P.device))
+            self.splits = num_splits or self.num_splits or ops.default_decode_splits(
+                Bp, P.kv_heads, keys, ops._cu_count(P.device), P.kv8)
             need = ops.decode_workspace_bytes(Bp, Hq, self.splits)
             if self._decode_ws.numel() < need:
                 self._decode_ws = torch.empty(need, dtype=torch.uint8, device=P.device)
@@ -1010,7 +1010,7 @@ class DecodeGraph:
             raise ValueError(f"{B} slots exceed max_batch {fast.max_batch}")
         max_keys = pool.src_width * BLOCK + pool.ring_tokens
         self.num_splits = num_splits or fast.num_splits or ops.default_decode_splits(
-            B, pool.kv_heads, max_keys, ops._cu_count(pool.device))
+            B, pool.kv_heads, max_keys, ops._cu_count(pool.device), pool.kv8)
         self.ids = torch.zeros(B, dtype=torch.long, device=pool.device)
         self.graph: torch.cuda.CUDAGraph | None = None
         self.logits: torch.Tensor | None = None

@@ -48,6 +48,19 @@ def test_decode_native_and_python(call, monkeypatch):
     _both(monkeypatch, make)
 
 
+@pytest.mark.parametrize("B", [32, 34, 40, 64])
+def test_default_splits_of_many_sequences(B, monkeypatch):
+    """More (sequence, kv head) pairs than CUs: both ways choose the splits that ``default_decode_splits`` names."""
+
+    pool, table, _, _ = history(28, 1, 8, 4200)
+    rows = table.expand(B, -1).contiguous()
+    q = rand(29, B, 8, 128).to(DEV)
+    splits = ops.default_decode_splits(B, 8, 4200, ops._cu_count(q.device), True)
+    call = lambda **kw: (ops.decode_attention(q, older=pool, older_table=rows, older_len=4200, **kw),)
+    _both(monkeypatch, call)
+    assert torch.equal(call()[0], call(num_splits=splits)[0])
+
+
 @pytest.mark.parametrize("call", ["plain", "ragged", "ragged_host", "both"])
 @pytest.mark.parametrize("tokens", [3, 40])
 def test_prefill_native_and_python(call, tokens, monkeypatch):

@@ -1,11 +1,12 @@
 """The custom operators of the 8-bit cache, page copies and beam selection without a GPU: the tensors their schemas say they
-write, and the shapes their fake forms give."""
+write, the shapes their fake forms give, and the key splits of a decode call."""
 
 from __future__ import annotations
 
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
+from lastkv_amd import ops
 import lastkv_amd.torch_ops  # noqa: F401
 
 L = torch.ops.lastkv
@@ -44,3 +45,11 @@ def test_fake_shapes():
         assert L.copy_pages(codes, codes, scales, scales, [0], [1]) is None
         pool = torch.empty((8, 12, 4096), dtype=torch.bfloat16)
         assert L.kv8_quantize(pool, pool, codes, codes, scales, scales, table, table, None, 64) is None
+
+
+def test_default_decode_splits():
+    splits = lambda B, tokens, older8: ops.default_decode_splits(B, 8, tokens, 256, older8)
+    for B, tokens in ((1, 500), (7, 9300), (20, 9300), (32, 9300), (56, 9300), (64, 9300), (40, 2000)):
+        assert splits(B, tokens, True) == splits(B, tokens, False), (B, tokens)
+    for B, tokens, want in ((34, 9300, 4), (40, 9300, 4), (48, 9300, 2), (72, 9300, 4), (33, 40000, 8)):
+        assert splits(B, tokens, True) == want and splits(B, tokens, False) == 1, (B, tokens)
