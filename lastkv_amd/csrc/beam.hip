@@ -1,13 +1,15 @@
 // Beam search's selection: the `count` best of a prompt's beams x vocab candidates score + (logit - lse(beam's logits)).
 //
 // Inside one beam the order of the totals is the order of the logits, so one pass over the logits does all of the reading:
-//   slice kernel: a workgroup holds a slice of one beam's row in registers (8 to 32 values a thread), takes its maximum,
+//   slice kernel: a workgroup holds a slice of one beam's row in registers (8 or 32 values a thread), takes its maximum,
 //     the sum of its exponentials and its `count` greatest logits;
 //   choose kernel: a workgroup a prompt joins the slices' sums in 64 bits and chooses among the slices' candidates.
 // Choosing the n greatest of many values needs no sort: the n-th greatest of the threads' own maxima is a floor that at
 // least n values reach and few others do; those go to LDS and each counts the ones before it.  Where too many values reach
 // the floor for LDS (equal logits), n rounds take the next one each; both give the same set.
-// Bound by the read of the logits; small calls by two dependent launches.
+// 16 prompts of 8 beams of 128256 bf16 logits, 16 of each: slices 11.3 us (2.9 TB/s; the loads and the maximum alone 5.9, with
+// the exponentials 8.2, so that half is the choice and its barriers), choosing 7.6; one prompt of 4 beams 4.4 and 4.8, which
+// are two dependent launches.
 #include "common.h"
 #include "runtime.h"
 
@@ -37,6 +39,7 @@ struct BeamParams {
   float* val;       // [B * K, slices, count]: logits
   int32_t* idx;     // tokens, -1: none
   int32_t beams, vocab, count, slices;
+  float per_tile;   // beams in one tile of the choose kernel: 1 over a beam's tiles
 };
 
 // Monotone in x for every x but NaN; above 0.
@@ -54,12 +57,13 @@ __device__ inline float dpp_move(float x) {
 
 // A floor that at least n (<= 64) of the values reach of which each of the kThreads threads gives the greatest: the n-th
 // greatest of the maxima of 64 groups of neighbours, found by counting for each how many stand before it (a wave counts a
-// part of them).  64 groups are the fewest that do, and their counting the least: with groups of four the choice below,
-// of 1024 threads, took 9.5 us in place of @@.
+// part of them).  A group's number takes the place of its maximum's lowest six bits, so that one comparison decides; the
+// floor is the n-th with those bits clear, at or below it.  64 groups are the fewest that do, and their counting the least
+// (256 groups of four made the choice below 6.5 us where it takes 4.8, for one prompt of 4 beams).
 template <int kThreads>
 struct FloorShared {
-  float top[64];
-  int32_t before[64];
+  uint32_t top[64];
+  uint32_t before[64];
   float result;
 };
 
@@ -74,54 +78,59 @@ __device__ inline float nth_floor(float x, int n, FloorShared<kThreads>& sm) {
     x = fmaxf(x, dpp_move<0x141>(x));  // (the row's halves mirrored, then the row)
     x = fmaxf(x, dpp_move<0x140>(x));
   }
-  if (t % kGroup == 0) sm.top[t / kGroup] = x;
+  if (t % kGroup == 0) sm.top[t / kGroup] = (order_bits(x) & ~63u) | static_cast<uint32_t>(t / kGroup);
   if (part == 0) sm.before[i] = 0;
   __syncthreads();
-  const float mine = sm.top[i];
-  int before = 0;
+  const uint32_t mine = sm.top[i];
+  uint32_t before = 0;
 #pragma unroll
   for (int j = part * kPart; j < (part + 1) * kPart; j += 4) {
-    const float4 k = *reinterpret_cast<const float4*>(&sm.top[j]);
-    before += (k.x > mine) || (k.x == mine && j < i);
-    before += (k.y > mine) || (k.y == mine && j + 1 < i);
-    before += (k.z > mine) || (k.z == mine && j + 2 < i);
-    before += (k.w > mine) || (k.w == mine && j + 3 < i);
+    const uint4 k = *reinterpret_cast<const uint4*>(&sm.top[j]);
+    before += k.x > mine;
+    before += k.y > mine;
+    before += k.z > mine;
+    before += k.w > mine;
   }
   atomicAdd(&sm.before[i], before);
   __syncthreads();
-  if (part == 0 && sm.before[i] == n - 1) sm.result = mine;
+  if (part == 0 && sm.before[i] == static_cast<uint32_t>(n - 1)) sm.result = from_order(max(mine & ~63u, 0x007fffffu));  // (-inf's place: those below are NaN)
   __syncthreads();
   return sm.result;
 }
 
-// Eight bf16 or four fp32 values of a row from element e0 on; elements outside [0, V) are not read and become -inf.
-template <bool kF32, int kVec>
-__device__ inline void load_values(const void* row, int64_t e0, int V, float (&x)[kVec]) {
-  if (e0 >= 0 && e0 + kVec <= V) {
+// Takes n places of a list in LDS.  (The 0 from the asm keeps the counter's address a vector register: seeing one address for
+// the wave the compiler adds the lanes' shares up one lane after the other first; the slices of 128 rows took 12.0 us so,
+// 11.4 this way.)
+__device__ inline uint32_t take_places(uint32_t* counter, uint32_t n) {
+  uint32_t zero;
+  asm("v_mov_b32 %0, 0" : "=v"(zero));
+  return atomicAdd(counter + zero, n);
+}
+
+// Sixteen bytes of a row, eight bf16 or four fp32 values from element e0 on, where the row begins or ends among them or lies
+// elsewhere: elements outside [0, V) are not read and are -inf.
+template <bool kF32>
+__device__ inline uint4 border_piece(const void* row, int e0, int V) {
+  uint32_t u[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
     if constexpr (kF32) {
-      const float4 f = *reinterpret_cast<const float4*>(static_cast<const float*>(row) + e0);
-      x[0] = f.x;
-      x[1] = f.y;
-      x[2] = f.z;
-      x[3] = f.w;
+      const int e = e0 + j;
+      u[j] = e >= 0 && e < V ? static_cast<const uint32_t*>(row)[e] : 0xff800000u;
     } else {
-      const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + e0);
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[2 * j] = bf16_lo(u[j]);
-        x[2 * j + 1] = bf16_hi(u[j]);
-      }
+      const int e = e0 + 2 * j;
+      const uint32_t lo = e >= 0 && e < V ? static_cast<const uint16_t*>(row)[e] : 0xff80u;
+      const uint32_t hi = e + 1 >= 0 && e + 1 < V ? static_cast<const uint16_t*>(row)[e + 1] : 0xff80u;
+      u[j] = lo | hi << 16;
     }
-    return;
   }
-#pragma unroll
-  for (int j = 0; j < kVec; ++j) {
-    const int64_t e = e0 + j;
-    x[j] = kNegInf;
-    if (e >= 0 && e < V)
-      x[j] = kF32 ? static_cast<const float*>(row)[e] : bf16_bits_to_f32(static_cast<const uint16_t*>(row)[e]);
-  }
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+
+template <bool kF32>
+__device__ inline float value_of(const uint4& w, int j) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+  return kF32 ? __uint_as_float(u[j & 3]) : j & 1 ? bf16_hi(u[j >> 1]) : bf16_lo(u[j >> 1]);
 }
 
 template <bool kF32, int kChunks>
@@ -142,17 +151,31 @@ __global__ __launch_bounds__(kBeamThreads) void beam_slice_kernel(const BeamPara
   const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / (kF32 ? 4 : 2));
   const int e0 = (slice * kChunks * kBeamThreads + t) * kVec - shift;  // this thread's first element
   constexpr int kStep = kBeamThreads * kVec;
-  float x[kChunks][kVec], top[kChunks];
+  // Every thread's loads are issued before the first is waited for: pieces that are not the row's read one that is, and the
+  // row's ends are put right after that (with a branch at each load the loads followed one another, and 128 rows of 128256
+  // took 1 us of 15 longer).
+  const int head = (kVec - shift) % kVec, tail = head + ((V - head) / kVec - 1) * kVec;  // the row's whole pieces
+  uint4 raw[kChunks];
+  if (V >= head + kVec) {
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c) load_values<kF32, kVec>(row, e0 + c * kStep, V, x[c]);
+    for (int c = 0; c < kChunks; ++c) {
+      const int e = min(max(e0 + c * kStep, head), tail);
+      raw[c] = *reinterpret_cast<const uint4*>(static_cast<const char*>(row) + static_cast<int64_t>(e) * (kF32 ? 4 : 2));
+    }
+  }
+  const int begin = slice * kChunks * kStep - shift;
+  if (begin < 0 || begin + kChunks * kStep > V) {
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c)
+      if (e0 + c * kStep < head || e0 + c * kStep > tail) raw[c] = border_piece<kF32>(row, e0 + c * kStep, V);
+  }
   if (t == 0) sm_n = 0;
-  float best = kNegInf;  // (NaN where one is: its row then has no candidate, whatever the slices hold)
+  float best = kNegInf, top[kChunks];  // (NaN where one is: its row then has no candidate, whatever the slices hold)
 #pragma unroll
   for (int c = 0; c < kChunks; ++c) {
-    top[c] = x[c][0];
+    top[c] = kNegInf;
 #pragma unroll
-    for (int j = 1; j + 1 < kVec; j += 2) top[c] = fmax3_nan(top[c], x[c][j], x[c][j + 1]);
-    top[c] = fmax_nan(top[c], x[c][kVec - 1]);
+    for (int j = 0; j < kVec; j += 2) top[c] = fmax3_nan(top[c], value_of<kF32>(raw[c], j), value_of<kF32>(raw[c], j + 1));
     best = fmax_nan(best, top[c]);
   }
   float m = best;
@@ -169,26 +192,47 @@ __global__ __launch_bounds__(kBeamThreads) void beam_slice_kernel(const BeamPara
     for (int r = t; r < n; r += kBeamThreads) idx[r] = -1;
     return;
   }
-  // the values that reach the floor, as (order, lowest index first)
+  // the values that reach the floor, as (order, lowest index first).  Few do: a thread looks into the pieces whose maximum
+  // does, one after the other, and takes their values out by selects (a test of every value in every wave was 3 us of 14)
   auto key = [&](float v, int e) {
     return (static_cast<uint64_t>(order_bits(v)) << 32) | static_cast<uint32_t>(~static_cast<uint32_t>(e));
   };
+  const float cut = fmaxf(floor, -3.402823466e38f);
+  uint32_t pieces = 0;
 #pragma unroll
-  for (int c = 0; c < kChunks; ++c) {
-    if (!(top[c] >= floor && top[c] > kNegInf)) continue;
+  for (int c = 0; c < kChunks; ++c) pieces |= top[c] >= cut ? 1u << c : 0u;
+  while (pieces != 0) {
+    const int c = __builtin_ctz(pieces);
+    pieces &= pieces - 1;
+    uint32_t x = raw[0].x, y = raw[0].y, z = raw[0].z, o = raw[0].w;
 #pragma unroll
-    for (int j = 0; j < kVec; ++j)
-      if (x[c][j] >= floor && x[c][j] > kNegInf) {
-        const uint32_t at = atomicAdd(&sm_n, 1u);
-        if (at < kBeamCap) sm_cand[at] = key(x[c][j], e0 + c * kStep + j);
-      }
+    for (int k = 1; k < kChunks; ++k) {
+      x = c == k ? raw[k].x : x;
+      y = c == k ? raw[k].y : y;
+      z = c == k ? raw[k].z : z;
+      o = c == k ? raw[k].w : o;
+    }
+    const uint4 w = make_uint4(x, y, z, o);
+    uint32_t hits = 0;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) hits |= value_of<kF32>(w, j) >= cut ? 1u << j : 0u;
+    uint32_t at = take_places(&sm_n, static_cast<uint32_t>(__builtin_popcount(hits)));
+    while (hits != 0) {
+      const int j = __builtin_ctz(hits);
+      hits &= hits - 1;
+      const int word = kF32 ? j : j >> 1;
+      const uint32_t u = word & 2 ? (word & 1 ? o : z) : (word & 1 ? y : x);
+      const float v = kF32 ? __uint_as_float(u) : j & 1 ? bf16_hi(u) : bf16_lo(u);
+      if (at < kBeamCap) sm_cand[at] = key(v, e0 + c * kStep + j);
+      ++at;
+    }
   }
   const float ref = m == kNegInf ? 0.f : m;  // (x - ref is 0 for the greatest, whose term is then exactly 1)
   float part = 0.f;
 #pragma unroll
   for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) part += fast_exp2((x[c][j] - ref) * kLog2e);  // (a +inf makes it NaN)
+    for (int j = 0; j < kVec; ++j) part += fast_exp2((value_of<kF32>(raw[c], j) - ref) * kLog2e);  // (a +inf makes it NaN)
   double sum = part;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
@@ -205,6 +249,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_slice_kernel(const BeamPara
     for (int i = t; i < found; i += kBeamThreads) {
       const uint64_t mine = sm_cand[i];
       int before = 0;
+#pragma unroll 8
       for (int k = 0; k < found; ++k) before += sm_cand[k] > mine;
       if (before < n) put(before, mine);
     }
@@ -217,8 +262,9 @@ __global__ __launch_bounds__(kBeamThreads) void beam_slice_kernel(const BeamPara
     for (int c = 0; c < kChunks; ++c)
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
-        if (!(x[c][j] > kNegInf)) continue;
-        const uint64_t k = key(x[c][j], e0 + c * kStep + j);
+        const float x = value_of<kF32>(raw[c], j);
+        if (!(x > kNegInf)) continue;
+        const uint64_t k = key(x, e0 + c * kStep + j);
         if (k < last && k > next) next = k;
       }
 #pragma unroll
@@ -262,11 +308,14 @@ __global__ __launch_bounds__(kChooseThreads) void beam_choose_kernel(const BeamP
   const int tiles = (per + 63) / 64, all = K * tiles;
   const int64_t base = static_cast<int64_t>(b) * K * per;
   if (t == 0) sm_n = 0;
+  // (there are at most 64 * 513 tiles, so that the product is closer to the quotient than that is to the next integer; an
+  // integer division for every tile in every pass was 1 us of the kernel)
+  auto beam_of = [&](int tile) { return static_cast<int>((static_cast<float>(tile) + 0.5f) * p.per_tile); };
   // the held tiles' tokens and logits are on their way while the sums are joined
   int token[kHeld];
   float logit[kHeld];
   auto fetch = [&](int tile, int& tk, float& x) {
-    const int k = tile / tiles, i = (tile - k * tiles) * 64 + lane;
+    const int k = beam_of(tile), i = (tile - k * tiles) * 64 + lane;
     tk = -1;
     x = 0.f;
     if (i < per) {
@@ -286,7 +335,7 @@ __global__ __launch_bounds__(kChooseThreads) void beam_choose_kernel(const BeamP
     for (int i = lane; i < S; i += 64) {
       const SliceSum v = ss[i];  // (an empty slice's sum is 0, or NaN)
       const float to = fmaxf(m, v.m);
-      if (m != to) s *= exp(static_cast<double>(m) - static_cast<double>(to));
+      if (m != to && m != kNegInf) s *= exp(static_cast<double>(m) - static_cast<double>(to));
       s += v.m == to || v.m == kNegInf ? v.s : v.s * exp(static_cast<double>(v.m) - static_cast<double>(to));
       m = to;
     }
@@ -303,7 +352,7 @@ __global__ __launch_bounds__(kChooseThreads) void beam_choose_kernel(const BeamP
   }
   __syncthreads();
   auto candidate = [&](int tile, int tk, float x) {
-    const int k = tile / tiles;
+    const int k = beam_of(tile);
     const double total = sm_score[k] + (static_cast<double>(x) - sm_lse[k]);
     return tk >= 0 && fabs(total) < __builtin_inf() ? make_candidate(total, k, x, tk) : Candidate{0, 0};
   };
@@ -326,7 +375,7 @@ __global__ __launch_bounds__(kChooseThreads) void beam_choose_kernel(const BeamP
   const float floor = nth_floor(top, n, sm_floor);
   each([&](const Candidate& c) {
     if (c.tie != 0 && __double2float_rd(c.total) >= floor) {
-      const uint32_t at = atomicAdd(&sm_n, 1u);
+      const uint32_t at = take_places(&sm_n, 1);
       if (at < kBeamCap) {
         sm_total[at] = c.total;
         sm_tie[at] = c.tie;
@@ -346,6 +395,7 @@ __global__ __launch_bounds__(kChooseThreads) void beam_choose_kernel(const BeamP
     if (t < found) {
       const Candidate mine{sm_total[t], sm_tie[t]};
       int before = 0;
+#pragma unroll 4
       for (int k = 0; k < found; ++k) before += ahead(Candidate{sm_total[k], sm_tie[k]}, mine);
       if (before < n) put(before, mine);
     }
@@ -429,6 +479,7 @@ extern "C" int32_t lkv_beam_select(const lkv_beam_select_args* a, lkv_stream_t s
   p.vocab = a->vocab;
   p.count = a->count;
   p.slices = slice_count(rows, a->vocab);
+  p.per_tile = 1.f / static_cast<float>((static_cast<int64_t>(p.slices) * a->count + 63) / 64);
   p.sums = static_cast<SliceSum*>(a->workspace);
   p.val = reinterpret_cast<float*>(p.sums + rows * p.slices);
   p.idx = reinterpret_cast<int32_t*>(p.val + rows * p.slices * a->count);
