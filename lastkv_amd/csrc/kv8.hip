@@ -35,6 +35,10 @@ int32_t kv8_pool(const lkv_kv8_pool* a, const char* name, Kv8Pool& p) {
 
 namespace {
 
+// A call that reads more than this does so non-temporally: 16 sequences of 8192 tokens (512 MiB) take 130 us (6.2 TB/s of
+// reads and writes) so and 157 with plain loads, but 1024 tokens each, which the caches hold, 19.2 and 16.8.
+constexpr int64_t kQuantizeNtBytes = int64_t{384} << 20;
+
 struct QuantizeParams {
   const uint16_t* k;
   const uint16_t* v;
@@ -54,6 +58,25 @@ __device__ inline uint32_t max_bits(uint4 x, uint32_t m) {
   return m;
 }
 
+template <int kCtrl>
+__device__ inline uint32_t max_dpp(uint32_t x) {
+  return max(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, x, kCtrl, 0xf, 0xf, true)));
+}
+
+// The greatest of the wave's, without LDS: within quads, the halves of a row, the row, then across rows.
+__device__ inline uint32_t wave_max_bits(uint32_t x) {
+  x = max_dpp<0x140>(max_dpp<0x141>(max_dpp<0x4e>(max_dpp<0xb1>(x))));
+  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = max(a[0], a[1]);
+  const auto c = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return max(c[0], c[1]);
+}
+
+template <bool kNt>
+__device__ inline uint4 load16(const void* p) {
+  return kNt ? load_nt(p) : *reinterpret_cast<const uint4*>(p);
+}
+
 // Two e4m3 codes of a packed bf16 pair times f, in the low or high half.
 template <bool kHigh>
 __device__ inline int code_pair(int old, uint32_t w, float f) {
@@ -70,6 +93,7 @@ __device__ inline int scale_byte(uint32_t bits) {
   return ex == 255 ? 255 : max(0, ex - 8 + ((bits & 0x7fu) > 0x60u));
 }
 
+template <bool kNt>
 __global__ __launch_bounds__(256) void kv8_quantize_kernel(const QuantizeParams p) {
   __shared__ uint32_t sm_max[2][4];
   const int b = blockIdx.z, h = blockIdx.y, j = p.first + blockIdx.x;
@@ -84,8 +108,8 @@ __global__ __launch_bounds__(256) void kv8_quantize_kernel(const QuantizeParams 
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     // K: piece = u * 2 + kp, operand kb = 2 kp + i; V: operand nb = 2 piece + i
-    k[i] = *reinterpret_cast<const uint4*>(p.k + so + (((piece >> 1) * 4 + (piece & 1) * 2 + i) * 16 + n16) * 32 + 8 * g4);
-    v[i] = *reinterpret_cast<const uint4*>(p.v + so + (16 * (2 * piece + i) + n16) * 32 + 8 * g4);
+    k[i] = load16<kNt>(p.k + so + (((piece >> 1) * 4 + (piece & 1) * 2 + i) * 16 + n16) * 32 + 8 * g4);
+    v[i] = load16<kNt>(p.v + so + (16 * (2 * piece + i) + n16) * 32 + 8 * g4);
   }
   if (valid < kBlockTokens) {  // what lies past the sequence's end does not count and is stored as 0
     const int w = ((n16 >> 2) << 3) | ((piece >> 1) << 2) | (n16 & 3);  // this thread's K token
@@ -96,11 +120,8 @@ __global__ __launch_bounds__(256) void kv8_quantize_kernel(const QuantizeParams 
     }
   }
   uint32_t mk = max_bits(k[1], max_bits(k[0], 0)), mv = max_bits(v[1], max_bits(v[0], 0));
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    mk = max(mk, __shfl_xor(mk, off));
-    mv = max(mv, __shfl_xor(mv, off));
-  }
+  mk = wave_max_bits(mk);
+  mv = wave_max_bits(mv);
   if (lane == 0) {
     sm_max[0][piece] = mk;
     sm_max[1][piece] = mv;
@@ -205,7 +226,11 @@ extern "C" int32_t lkv_kv8_quantize(const lkv_kv8_quantize_args* a, const lkv_kv
   p.tokens = a->tokens;
   p.tokens_c = a->tokens_const;
   p.first = a->first_block;
-  kv8_quantize_kernel<<<dim3(a->blocks, a->heads, a->batch), 256, 0, as_stream(stream)>>>(p);
+  const dim3 grid(a->blocks, a->heads, a->batch);
+  if (static_cast<int64_t>(a->batch) * a->heads * a->blocks * kBlockElems * 4 > kQuantizeNtBytes)
+    kv8_quantize_kernel<true><<<grid, 256, 0, as_stream(stream)>>>(p);
+  else
+    kv8_quantize_kernel<false><<<grid, 256, 0, as_stream(stream)>>>(p);
   return check_launch("lkv_kv8_quantize");
 }
 
