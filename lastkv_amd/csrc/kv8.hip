@@ -35,9 +35,10 @@ int32_t kv8_pool(const lkv_kv8_pool* a, const char* name, Kv8Pool& p) {
 
 namespace {
 
-// A call that reads more than this does so non-temporally: 16 sequences of 8192 tokens (512 MiB) take 130 us (6.2 TB/s of
-// reads and writes) so and 157 with plain loads, but 1024 tokens each, which the caches hold, 19.2 and 16.8.
-constexpr int64_t kQuantizeNtBytes = int64_t{384} << 20;
+// Calls over more bf16 values than this read non-temporally: 16 sequences of 8192 tokens (512 MiB) are quantised in 130 us
+// (6.2 TB/s of reads and writes) so and in 157 with plain loads, unpacked in 141 and 148; 1024 tokens each, which the caches
+// hold, in 19.2 and 16.8, 20.0 and 17.0.
+constexpr int64_t kNtBytes = int64_t{384} << 20;
 
 struct QuantizeParams {
   const uint16_t* k;
@@ -157,13 +158,14 @@ struct UnpackParams {
 
 // One workgroup a (block, kv head, sequence).  A thread's 16 K codes are 8 + 8 dims of one token, stored as they are; V
 // (16 codes of two dims) turns through LDS into 16 dims of one token.
+template <bool kNt>
 __global__ __launch_bounds__(256) void kv8_unpack_kernel(const UnpackParams p) {
   __shared__ __align__(16) uint8_t sm[kBlockTokens][kHeadDim];
   const int b = blockIdx.z, h = blockIdx.y, j = (p.token0 >> 5) + blockIdx.x;
   const int lane = threadIdx.x & 63, piece = threadIdx.x >> 6, n16 = lane & 15, g4 = lane >> 4;
   const int page = min(max(p.table[b * p.ts + j], 0), p.src.pages - 1);
   const int64_t at = page * p.src.page + h * p.src.hs + threadIdx.x * 16;
-  const uint4 k = *reinterpret_cast<const uint4*>(p.src.k + at), v = *reinterpret_cast<const uint4*>(p.src.v + at);
+  const uint4 k = load16<kNt>(p.src.k + at), v = load16<kNt>(p.src.v + at);
   const float sk = kv8_scale(p.src.ks[h * p.src.s_hs + page]), sv = kv8_scale(p.src.vs[h * p.src.s_hs + page]);
   const int t0 = j * kBlockTokens - p.token0;  // row of the block's token 0
   {
@@ -227,7 +229,7 @@ extern "C" int32_t lkv_kv8_quantize(const lkv_kv8_quantize_args* a, const lkv_kv
   p.tokens_c = a->tokens_const;
   p.first = a->first_block;
   const dim3 grid(a->blocks, a->heads, a->batch);
-  if (static_cast<int64_t>(a->batch) * a->heads * a->blocks * kBlockElems * 4 > kQuantizeNtBytes)
+  if (static_cast<int64_t>(a->batch) * a->heads * a->blocks * kBlockElems * 4 > kNtBytes)
     kv8_quantize_kernel<true><<<grid, 256, 0, as_stream(stream)>>>(p);
   else
     kv8_quantize_kernel<false><<<grid, 256, 0, as_stream(stream)>>>(p);
@@ -263,6 +265,10 @@ extern "C" int32_t lkv_kv8_unpack(const lkv_kv8_pool* src, const int32_t* table,
   p.vst = v_stride_t;
   p.token0 = token0;
   p.tokens = tokens;
-  kv8_unpack_kernel<<<dim3(static_cast<unsigned>(end - (token0 >> 5)), src->heads, batch), 256, 0, as_stream(stream)>>>(p);
+  const dim3 grid(static_cast<unsigned>(end - (token0 >> 5)), src->heads, batch);
+  if (static_cast<int64_t>(batch) * src->heads * grid.x * kBlockElems * 4 > kNtBytes)
+    kv8_unpack_kernel<true><<<grid, 256, 0, as_stream(stream)>>>(p);
+  else
+    kv8_unpack_kernel<false><<<grid, 256, 0, as_stream(stream)>>>(p);
   return check_launch("lkv_kv8_unpack");
 }
