@@ -175,7 +175,14 @@ __global__ __launch_bounds__(waves8(CG) * 64, waves8(CG) / 4) void decode_kv8_ke
   HeadPool o;
   Block8 f0, f1, f2;
   int pg = 0;
-  auto at = [&](int t) { return first + step * t; };
+  // Few pairs start their walks apart: sequences whose pages lie a power of two from each other would be read at the same
+  // place of all of them, and so from the same memory channels (4 sequences of 131072 tokens 197 us, so 172; other lengths
+  // and more pairs keep their times).
+  const int rot = it.S >= 4 && nb0 >= 256 ? ((kvh + b * static_cast<int>(gridDim.y)) * 101) & 255 : 0;
+  auto at = [&](int t) {
+    const int i = first + step * t + rot;
+    return i >= nb0 ? i - nb0 : i;
+  };
   auto look = [&](int t) { pg = min(max(static_cast<int>(table[at(min(t, n - 1))]), 0), o.pages - 1); };
   auto load = [&](Block8& f) __attribute__((always_inline)) { load_block8<kNT>(f, o, pg, lane); };
   auto compute8 = [&](const Block8& f, int t) __attribute__((always_inline)) {

@@ -269,6 +269,19 @@ def test_offsets_past_32_bits():
         torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("splits", [None, 1, 4, 7, 64])
+@pytest.mark.parametrize("older", [[8192, 8191], [8193, 255 * 32], [12345, 33]])
+def test_long_decode_rows(older, splits):
+    """Histories of 255 blocks and more, which the splits of a call begin to read at different places."""
+
+    seg, keys = segments(30, 8, 2, older, [9, 64], True)
+    q = rand(31, 2, 8, 128).to(DEV)
+    got = ops.decode_attention(q, num_splits=splits, **seg)
+    for b in range(2):
+        want, mean, err, _ = attention64(q[b:b + 1].cpu(), *keys[b], 0)
+        check(got[b:b + 1], want, mean, err, 2.0 ** -8, b)  # (weights rounded to bf16: 2^-8 at most)
+
+
 @pytest.mark.parametrize("T", [4000, 9001])
 def test_long_ragged_batches(T):
     """Ragged rows over long histories: a prompt's chunk, a few tokens, one token, and none."""
