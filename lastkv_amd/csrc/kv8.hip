@@ -215,7 +215,7 @@ extern "C" int32_t lkv_kv8_quantize(const lkv_kv8_quantize_args* a, const lkv_kv
   LKV_REQUIRE(end <= a->src_table_width && end <= a->dst_table_width,
               "blocks [%d, %lld) exceed the tables' %d and %d", a->first_block, static_cast<long long>(end),
               a->src_table_width, a->dst_table_width);
-  LKV_REQUIRE(a->batch <= 65535 && a->heads <= 65535 && end < (1 << 26), "batch and heads must be <= 65535, blocks < 2^26");
+  LKV_REQUIRE(a->batch <= 65535 && a->heads <= 65535 && end < (1 << 24), "batch and heads must be <= 65535, blocks < 2^24");
   p.k = static_cast<const uint16_t*>(a->src_k);
   p.v = static_cast<const uint16_t*>(a->src_v);
   p.page = a->src_page_stride;
@@ -250,7 +250,7 @@ extern "C" int32_t lkv_kv8_unpack(const lkv_kv8_pool* src, const int32_t* table,
   LKV_REQUIRE(((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0 &&
                   ((k_stride_b | k_stride_h | k_stride_t | v_stride_b | v_stride_h | v_stride_t) & 7) == 0,
               "rows must be 16-byte aligned");
-  LKV_REQUIRE(batch <= 65535 && src->heads <= 65535, "batch and heads must be <= 65535");
+  LKV_REQUIRE(batch <= 65535 && src->heads <= 65535 && end < (1 << 24), "batch and heads must be <= 65535, blocks < 2^24");
   if (batch == 0 || tokens == 0) return LKV_OK;  // (empty tensors have no address)
   LKV_REQUIRE(table && k && v, "null tensor");
   p.table = table;

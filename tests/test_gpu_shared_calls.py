@@ -298,3 +298,79 @@ def test_long_ragged_batches(T):
                 want, mean, err, _ = attention64(q[rows].cpu(), *keys[b], n)
                 # weights rounded to bf16 (2^-8 at most) or V to fp16 (2^-11): the larger
                 check(got[rows], want, mean, err, 2.0 ** -8, (T, b))
+
+
+# ---------------------------------------------------------------------------------------- calls at their edges
+@pytest.mark.parametrize("host", [False, True])
+@pytest.mark.parametrize("counts", [[3, 1], [70, 1, 9], [1, 1]])
+def test_rows_behind_the_last_sequence_stay(counts, host):
+    """A padded ragged batch: rows past the last offset are neither read nor written, nor are their LSEs."""
+
+    seg, _ = segments(32, 8, 2, [200, 64, 33][:len(counts)], [n + 5 for n in counts], True)
+    T = sum(counts)
+    q = rand(33, T + 11, 8, 128).to(DEV)
+    cu = np.concatenate(([0], np.cumsum(counts))).astype(np.int32)
+    kw = dict(cu_seqlens_q=torch.from_numpy(cu).to(DEV), max_seqlen_q=max(counts), **(dict(cu_seqlens_q_host=cu) if host else {}), **seg)
+    want = ops.prefill_attention(q[:T].contiguous(), **kw)
+    out, lse = torch.full_like(q, 7.0), torch.full((T + 11, 8), 7.0, device=DEV)
+    q[T:] = float("nan")
+    ops.prefill_attention(q, out=out, lse=lse, **kw)
+    assert torch.equal(out[:T], want) and bool((out[T:] == 7).all()) and bool((lse[T:] == 7).all())
+
+
+def test_table_entries_past_a_length_are_not_followed():
+    pool, table, _, _ = history(34, 2, 2, 300)
+    wide = torch.full((2, 40), -5, dtype=torch.int32, device=DEV)
+    wide[:, ::2] = 1 << 30
+    wide[:, :10] = table
+    q = rand(35, 2, 40, 8, 128).to(DEV)
+    lens = i32(300, 33)
+    for n in (1, 3, 40):
+        rows = q[:, :n].contiguous()
+        a, b = (ops.prefill_attention(rows, older=pool, older_table=t, older_len=lens, num_splits=1) for t in (table, wide))
+        assert torch.equal(a, b)
+    a, b = (ops.decode_attention(q[:, 0].contiguous(), older=pool, older_table=t, older_len=lens, num_splits=3) for t in (table, wide))
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("T", [0, 1, 31, 32])
+def test_shortest_histories(T):
+    seg, keys = segments(36, 16, 1, [T, 0], [1, 1], True)
+    for L in (1, 2, 5):
+        q = rand(37, 2, L, 16, 128).to(DEV)
+        local = [L, L]
+        seg, keys = segments(36, 16, 1, [T, 0], local, True)
+        got = ops.prefill_attention(q, **seg) if L > 1 else ops.decode_attention(q[:, 0].contiguous(), **seg)[:, None]
+        for b in range(2):
+            want, mean, err, _ = attention64(q[b].cpu(), *keys[b], L)
+            check(got[b], want, mean, err, 2.0 ** -8, (T, L, b))  # (weights rounded to bf16: 2^-8 at most)
+
+
+def test_strided_logits_and_scores():
+    logits = torch.randn(4, 6, 3000, device=DEV)[::2, 1::2, 7:2900]
+    scores = -torch.rand(4, 9, device=DEV)[::2, 3:6]
+    got = ops.beam_select(logits, scores, 6)
+    assert all(torch.equal(a, b) for a, b in zip(got, ops.beam_select(logits.contiguous(), scores.contiguous(), 6)))
+    for bad in (torch.randn(2, 3000, 3, device=DEV).transpose(1, 2), logits.double(), logits[0], logits.cpu()):
+        with pytest.raises((ValueError, _lib.LastKVNativeError)):
+            ops.beam_select(bad, scores, 6)
+
+
+def test_calls_on_two_streams():
+    """Two calls in flight at once, each with its own workspace, give what they give alone."""
+
+    segs = [segments(38 + i, 8, 2, [5000 + i, 77], [9, 30], True)[0] for i in range(2)]
+    qs = [rand(40 + i, 2, 8, 128).to(DEV) for i in range(2)]
+    logits = [torch.randn(2, 4, 50000, device=DEV) for _ in range(2)]
+    scores = torch.zeros(2, 4, device=DEV)
+    alone = [(ops.decode_attention(q, num_splits=8, **s), *ops.beam_select(x, scores, 8)) for q, s, x in zip(qs, segs, logits)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        got = []
+        for st, q, s, x in zip(streams, qs, segs, logits):
+            with torch.cuda.stream(st):
+                got.append((ops.decode_attention(q, num_splits=8, **s), *ops.beam_select(x, scores, 8)))
+        torch.cuda.synchronize()
+        for a, b in zip(alone, got):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
