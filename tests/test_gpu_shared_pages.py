@@ -298,3 +298,63 @@ def test_beam_search_of_one_beam_is_greedy_and_prompts_share_steps():
         assert [s for _, s in hyps] == sorted((s for _, s in hyps), reverse=True)
         assert len({tuple(ids.tolist()) for ids, _ in hyps}) == 3
     assert r.pool.free_pages == r.pool.source_pages
+
+
+@pytest.mark.parametrize("shared_cache", ["bf16", "kv8"])
+@pytest.mark.parametrize("contract", ["hf", "vllm"])
+def test_forks_at_and_around_boundaries(shared_cache, contract):
+    """Forks of prompts that end before, at and behind a chunk's or page's end, and forks of forks, beside sequences prefilled by
+    themselves; then a captured step over all of them."""
+
+    _, model = _tiny(chunk=24)
+    lengths = [1, 23, 24, 25, 31, 32, 48, 72, 96, 97]
+    logits = []
+    for fork in (True, False):
+        r = LastKVServingModel(model, max_batch=3, max_tokens_per_slot=256, num_splits=2, shared_cache=shared_cache, contract=contract)
+        seen = []
+        for n in lengths:
+            ids = _ids(n, n)
+            s = [_prefill(r, ids)[0]]
+            for i in range(2):
+                s.append(r.fork_sequence(s[i]) if fork else _prefill(r, ids)[0])
+            tok = _ids(n + 1, 60 * 3).view(60, 3)
+            for t in range(50):
+                seen.append(r.step([(x, tok[t, i:i + 1]) for i, x in enumerate(s)]).clone())
+            graph = r.decode_graph(s, num_splits=2)
+            for t in range(50, 60):
+                seen.append(graph.step(tok[t].to(DEV))[0].clone())
+            torch.cuda.synchronize()
+            del graph
+            for x in s:
+                r.free_sequence(x)
+        assert r.pool.free_pages == r.pool.source_pages
+        logits.append(seen)
+    for t, (a, b) in enumerate(zip(*logits)):
+        assert torch.equal(a, b), (lengths[t // 60], t % 60)
+
+
+def test_fork_of_an_empty_sequence():
+    _, model = _tiny(chunk=24)
+    r = LastKVServingModel(model, max_batch=2, max_tokens_per_slot=128, shared_cache="kv8")
+    a = r.add_sequence()
+    b = r.fork_sequence(a)
+    tok = _ids(3, 60)
+    for t in range(60):
+        got = r.step([(a, tok[t:t + 1]), (b, tok[t:t + 1])])
+        assert torch.equal(got[0], got[1])
+
+
+@pytest.mark.parametrize("contract", ["hf", "vllm"])
+def test_the_runtime_self_check_covers_8_bits(contract, monkeypatch, capsys):
+    """Every layer's call next to its two passes (history alone, ring alone, merged): each of the passes, their merge and the call
+    round to bf16, 2^-8 of a value each, and the vLLM contract rounds the first three twice."""
+
+    monkeypatch.setenv("LASTKV_MERGED_CHECK", "1")
+    _, model = _tiny(chunk=24)
+    r = LastKVServingModel(model, max_batch=2, max_tokens_per_slot=256, contract=contract, shared_cache="kv8")
+    slots = [_prefill(r, _ids(i, 75 + 40 * i))[0] for i in range(2)]
+    for t in range(3):
+        r.step([(slots[0], _ids(t, 1)), (slots[1], _ids(t + 9, 1 + 3 * (t == 1)))])
+    lines = [line for line in capsys.readouterr().out.splitlines() if "lastkv_merged_check" in line]
+    rels = [float(line.split("'rel': ")[1].split(",")[0]) for line in lines]
+    assert len(rels) > 20 and any("'older': [48" in line for line in lines) and max(rels) <= 7 * 2.0 ** -8
