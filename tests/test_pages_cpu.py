@@ -109,6 +109,25 @@ def test_copy_pages_refuses_bad_arguments(kw, message):
     assert lib.lkv_copy_pages(ctypes.byref(a), None) == 1 and message in lib.lkv_last_error()
 
 
+@pytest.mark.parametrize("pages", [64, 4096, 1 << 20])
+@pytest.mark.parametrize("n", [2, 9, 40, 64])
+def test_copy_pages_finds_a_wrong_pair_anywhere(n, pages):
+    """Lists of few and many pairs, of small and large pools, with one page that is a destination twice or on both sides."""
+
+    lib = _lib.load()
+    rng = np.random.default_rng(n + pages)
+    for _ in range(20):
+        ids = rng.permutation(min(pages, 500))[:2 * n] if 2 * n <= min(pages, 500) else rng.permutation(pages)
+        n = min(n, len(ids) // 2)
+        src, dst = ids[:n].tolist(), ids[n:2 * n].tolist()
+        i, j = (int(x) for x in rng.choice(n, 2, replace=False))
+        for lists, message in ((([*src], [dst[j] if k == i else d for k, d in enumerate(dst)]), b"destination twice"),
+                               (([dst[j] if k == i else x for k, x in enumerate(src)], dst), b"source and a destination"),
+                               ((src, [pages if k == i else d for k, d in enumerate(dst)]), b"outside")):
+            a, keep = _copy_args(*lists, num_pages=pages, head_stride=pages * 8192)
+            assert lib.lkv_copy_pages(ctypes.byref(a), None) == 1 and message in lib.lkv_last_error()
+
+
 def test_copy_pages_of_nothing_launches_nothing():
     lib = _lib.load()
     a, keep = _copy_args([], [])
