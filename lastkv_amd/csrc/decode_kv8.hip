@@ -186,9 +186,10 @@ __global__ __launch_bounds__(waves8(CG) * 64, waves8(CG) / 4) void decode_kv8_ke
   Block8 f0, f1, f2;
   int pg = 0;
   // Few pairs start their walks apart: sequences whose pages lie a power of two from each other would be read at the same
-  // place of all of them, and so from the same memory channels (4 sequences of 131072 tokens 197 us, so 172; other lengths
-  // and more pairs keep their times).
-  const int rot = it.S >= 4 && nb0 >= 256 ? ((kvh + b * static_cast<int>(gridDim.y)) * 101) & 255 : 0;
+  // place of all of them, and so from the same memory channels (4 sequences of 131072 tokens 197 us, so 171, up to 255 blocks
+  // apart 177; other lengths and more pairs keep their times).
+  const int apart = it.S < 4 ? 0 : nb0 >= 1024 ? 1023 : nb0 >= 256 ? 255 : 0;
+  const int rot = ((kvh + b * static_cast<int>(gridDim.y)) * 101) & apart;
   auto at = [&](int t) {
     const int i = first + step * t + rot;
     return i >= nb0 ? i - nb0 : i;

@@ -271,7 +271,7 @@ def test_offsets_past_32_bits():
 
 
 @pytest.mark.parametrize("splits", [None, 1, 4, 7, 64])
-@pytest.mark.parametrize("older", [[8192, 8191], [8193, 255 * 32], [12345, 33]])
+@pytest.mark.parametrize("older", [[8192, 8191], [8193, 255 * 32], [12345, 33], [32768, 32 * 1024 - 31], [34000, 32 * 1023]])
 def test_long_decode_rows(older, splits):
     """Histories of 255 blocks and more, which the splits of a call begin to read at different places."""
 
