@@ -125,14 +125,15 @@ __global__ __launch_bounds__(waves8(CG) * 64, waves8(CG) / 4) void decode_kv8_ke
   DecodeItem it;
   if (!decode_item<kMulti>(p, blockIdx.x, it)) return;  // (workgroup-uniform)
   // The splits of one (sequence, kv head) side by side on one XCD, the heads of one sequence apart: a long sequence among short
-  // ones keeps all XCDs busy (8 sequences, one of 9000 tokens and the others below 1000: 22.5 us, with its heads side by side 28.9;
-  // equal lengths the same).
+  // ones keeps all XCDs busy (8 sequences, one of 9000 tokens and the others below 1000: 22.7 us, with its heads side by side 28.9;
+  // equal lengths as before, 24 of 9300 77 where it was 84).  An XCD takes another head of each sequence: with the same one
+  // of all 64 of 9300 tokens took 219 us, so 210.
   if (p.cu == nullptr) {
     const int id = blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z);
     const int at = xcd_logical_index(id, gridDim.x * gridDim.y * gridDim.z);
     it.split = at % it.S;
     it.b = at / it.S % gridDim.z;
-    it.kvh = at / (it.S * gridDim.z);
+    it.kvh = (at / (it.S * gridDim.z) + it.b) % gridDim.y;
     it.mr = kMulti ? multi_rows(p, it.b) : MultiRows{1, it.b};
     it.ws_row0 = it.mr.row0;
   }
