@@ -320,8 +320,8 @@ def default_decode_splits(batch: int, kv_heads: int, max_tokens: int, cu_count: 
 
     With an 8-bit older segment (``older8``, 8-wave workgroups) more pairs than CUs whose last round is at most half full
     are split into up to 8 parts of 64 blocks or more, as many as give the fewest rounds a part: at 8 kv heads and 9.3K
-    keys B = 34 takes 137 us with four against 162 with one, B = 40 146 against 165, B = 72 247 with three against 271, and
-    B = 40 at 30K 400 against 479; with fuller last rounds one is best (B = 56 190 against 198, B = 32 105 against 116)."""
+    keys B = 34 takes 138 us with four against 162 with one, B = 40 148 against 170, B = 72 256 against 269, and B = 40 at
+    30K 412 against 480; with fuller last rounds one is best (B = 56 186 against 201, B = 32 106 against 113)."""
 
     pairs = max(1, batch * kv_heads)
     blocks = max(1, math.ceil(max_tokens / BLOCK_TOKENS))
