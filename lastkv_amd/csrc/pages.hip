@@ -29,7 +29,8 @@ struct CopyParams {
 
 // kChunks: 16-byte pieces a thread copies of one page (page_bytes / 4096).  Workgroup x: pages [4 x, 4 x + 4) of the runs, of
 // one head's K or V; all of its loads come before its stores.  The run of its first page is searched once.  Sources are read
-// with the non-temporal hint (2048 pages of 8 heads in 32 runs: 146 us with a search a page and without the hint, 97 us; hipMemcpy of the same bytes 90).
+// with the non-temporal hint (2048 pages of 8 heads in 32 runs: 146 us with a search a page and without the hint, so 97;
+// hipMemcpy of the same bytes 90).
 template <int kChunks>
 __global__ __launch_bounds__(256) void copy_pages_kernel(const CopyParams p, const CopyRuns r) {
   const int h = blockIdx.y, kv = blockIdx.z;
