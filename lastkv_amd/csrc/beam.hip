@@ -93,7 +93,8 @@ __device__ inline float nth_floor(float x, int n, FloorShared<kThreads>& sm) {
   }
   atomicAdd(&sm.before[i], before);
   __syncthreads();
-  if (part == 0 && sm.before[i] == static_cast<uint32_t>(n - 1)) sm.result = from_order(max(mine & ~63u, 0x007fffffu));  // (-inf's place: those below are NaN)
+  if (part == 0 && sm.before[i] == static_cast<uint32_t>(n - 1))
+    sm.result = from_order(max(mine & ~63u, 0x007fffffu));  // (-inf's place: those below are NaN)
   __syncthreads();
   return sm.result;
 }
