@@ -108,24 +108,35 @@ __device__ inline uint32_t take_places(uint32_t* counter, uint32_t n) {
   return atomicAdd(counter + zero, n);
 }
 
-// Sixteen bytes of a row, eight bf16 or four fp32 values from element e0 on, where the row begins or ends among them or lies
-// elsewhere: elements outside [0, V) are not read and are -inf.
+// Sixteen bytes of a row, eight bf16 or four fp32 values from element e0 >= 0 on, where the row ends among or before them:
+// elements from V on are not read and are -inf.
 template <bool kF32>
-__device__ inline uint4 border_piece(const void* row, int e0, int V) {
+__device__ inline uint4 last_piece(const void* row, int e0, int V) {
   uint32_t u[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if constexpr (kF32) {
       const int e = e0 + j;
-      u[j] = e >= 0 && e < V ? static_cast<const uint32_t*>(row)[e] : 0xff800000u;
+      u[j] = e < V ? static_cast<const uint32_t*>(row)[e] : 0xff800000u;
     } else {
       const int e = e0 + 2 * j;
-      const uint32_t lo = e >= 0 && e < V ? static_cast<const uint16_t*>(row)[e] : 0xff80u;
-      const uint32_t hi = e + 1 >= 0 && e + 1 < V ? static_cast<const uint16_t*>(row)[e + 1] : 0xff80u;
+      const uint32_t lo = e < V ? static_cast<const uint16_t*>(row)[e] : 0xff80u;
+      const uint32_t hi = e + 1 < V ? static_cast<const uint16_t*>(row)[e + 1] : 0xff80u;
       u[j] = lo | hi << 16;
     }
   }
   return make_uint4(u[0], u[1], u[2], u[3]);
+}
+
+// Sixteen bytes at the alignment of a row's values (the card loads dwords from any address).
+template <bool kF32>
+__device__ inline uint4 load_piece(const void* row, int e) {
+  uint4 w;
+  if constexpr (kF32)
+    __builtin_memcpy(&w, static_cast<const float*>(row) + e, 16);
+  else
+    __builtin_memcpy(&w, static_cast<const uint16_t*>(row) + e, 16);
+  return w;
 }
 
 template <bool kF32>
@@ -148,27 +159,24 @@ __global__ __launch_bounds__(kBeamThreads) void beam_slice_kernel(const BeamPara
   const int64_t off = (row_id / p.beams) * p.sb + (row_id % p.beams) * p.sk;
   const void* row = kF32 ? static_cast<const void*>(static_cast<const float*>(p.logits) + off)
                          : static_cast<const void*>(static_cast<const uint16_t*>(p.logits) + off);
-  // 16-byte pieces start at addresses that are multiples of 16: the row's first piece may begin before it
-  const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / (kF32 ? 4 : 2));
-  const int e0 = (slice * kChunks * kBeamThreads + t) * kVec - shift;  // this thread's first element
+  // Pieces are counted from the row's first value, whatever its address: which values a thread adds in fp32, and so every bit of
+  // a row's sum, then goes by the row's values alone, and equal beams tie exactly.  (With pieces at multiples of 16 bytes the
+  // logarithms of equal rows at different alignments differed by 1e-8, which put a later beam first.)
+  const int e0 = (slice * kChunks * kBeamThreads + t) * kVec;  // this thread's first element
   constexpr int kStep = kBeamThreads * kVec;
   // Every thread's loads are issued before the first is waited for: pieces that are not the row's read one that is, and the
-  // row's ends are put right after that (with a branch at each load the loads followed one another, and 128 rows of 128256
+  // row's end is put right after that (with a branch at each load the loads followed one another, and 128 rows of 128256
   // took 1 us of 15 longer).
-  const int head = (kVec - shift) % kVec, tail = head + ((V - head) / kVec - 1) * kVec;  // the row's whole pieces
+  const int tail = V / kVec * kVec - kVec;  // the row's last whole piece
   uint4 raw[kChunks];
-  if (V >= head + kVec) {
+  if (tail >= 0) {
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-      const int e = min(max(e0 + c * kStep, head), tail);
-      raw[c] = *reinterpret_cast<const uint4*>(static_cast<const char*>(row) + static_cast<int64_t>(e) * (kF32 ? 4 : 2));
-    }
+    for (int c = 0; c < kChunks; ++c) raw[c] = load_piece<kF32>(row, min(e0 + c * kStep, tail));
   }
-  const int begin = slice * kChunks * kStep - shift;
-  if (begin < 0 || begin + kChunks * kStep > V) {
+  if ((slice + 1) * kChunks * kStep > V) {
 #pragma unroll
     for (int c = 0; c < kChunks; ++c)
-      if (e0 + c * kStep < head || e0 + c * kStep > tail) raw[c] = border_piece<kF32>(row, e0 + c * kStep, V);
+      if (e0 + c * kStep > tail) raw[c] = last_piece<kF32>(row, e0 + c * kStep, V);
   }
   if (t == 0) sm_n = 0;
   float best = kNegInf, top[kChunks];  // (NaN where one is: its row then has no candidate, whatever the slices hold)
@@ -430,10 +438,9 @@ int slice_values(int64_t rows, int32_t vocab) {
   return rows * ((vocab + kWideSlice - 1) / kWideSlice) >= 256 ? kWideSlice : kNarrowSlice;
 }
 
-// Slices of a row: its first 16-byte piece may hold up to 7 values that lie before the row.
 int32_t slice_count(int64_t rows, int32_t vocab) {
   const int n = slice_values(rows, vocab);
-  return (vocab + 7 + n - 1) / n;
+  return (vocab + n - 1) / n;
 }
 
 }  // namespace
@@ -443,7 +450,9 @@ extern "C" int64_t lkv_beam_workspace_bytes(int32_t batch, int32_t beams, int32_
   using namespace lkv;
   if (batch <= 0 || beams <= 0 || vocab <= 0 || count <= 0) return 0;
   const int64_t rows = static_cast<int64_t>(batch) * beams;
-  return rows * slice_count(rows, vocab) * (static_cast<int64_t>(sizeof(SliceSum)) + count * 8);
+  // (of up to 7 values more than the row has: the size that callers of this ABI version know)
+  const int n = slice_values(rows, vocab);
+  return rows * ((vocab + 7 + n - 1) / n) * (static_cast<int64_t>(sizeof(SliceSum)) + count * 8);
 }
 
 extern "C" int32_t lkv_beam_select(const lkv_beam_select_args* a, lkv_stream_t stream) {
