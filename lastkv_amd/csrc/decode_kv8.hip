@@ -186,11 +186,13 @@ __global__ __launch_bounds__(waves8(CG) * 64, waves8(CG) / 4) void decode_kv8_ke
   HeadPool o;
   Block8 f0, f1, f2;
   int pg = 0;
-  // Few pairs start their walks apart: sequences whose pages lie a power of two from each other would be read at the same
-  // place of all of them, and so from the same memory channels (4 sequences of 131072 tokens 197 us, so 171, up to 255 blocks
-  // apart 177; other lengths and more pairs keep their times).
+  // With few pairs the heads start their walks apart: heads and sequences whose pages lie a power of two from each other would be read at
+  // the same place of all of them, and so from the same memory channels (replayed calls over 4 sequences of 131072 tokens: 205 us
+  // where all start at 0, 186 so; 2 sequences 115 and 104; other lengths and more pairs within 3 %).  The start goes by the
+  // head and the sequence's own length alone, so that with a fixed split count a sequence's bits do not depend on its place in
+  // the batch (starts that differ by sequence too: 183).
   const int apart = it.S < 4 ? 0 : nb0 >= 1024 ? 1023 : nb0 >= 256 ? 255 : 0;
-  const int rot = ((kvh + b * static_cast<int>(gridDim.y)) * 101) & apart;
+  const int rot = (kvh * 101) & apart;
   auto at = [&](int t) {
     const int i = first + step * t + rot;
     return i >= nb0 ? i - nb0 : i;
