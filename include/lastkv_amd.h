@@ -740,7 +740,7 @@ int32_t lkv_kv8_unpack(const lkv_kv8_pool *src, const int32_t *table, int64_t ta
  * NULL, older_block_table (with older_table_stride, older_capacity_tokens and the lengths) names pages of `older`, and the
  * other older fields are not read.  The result is the attention over the codes' values: with older_vscale_mode 1
  * V is bf16(value * vscale[h]).  Scores, softmax and sums are those of the bf16 calls; a sequence that sees a token of a NaN
- * block has NaN outputs.  Codes past a sequence's length do not count, whatever they hold. */
+ * block has NaN outputs and LSEs for that kv head.  Codes past a sequence's length do not count, whatever they hold. */
 int32_t lkv_decode_attn_kv8(const lkv_decode_args *args, const lkv_kv8_pool *older, lkv_stream_t stream);
 
 int64_t lkv_prefill_kv8_workspace_bytes(const lkv_prefill_args *args);

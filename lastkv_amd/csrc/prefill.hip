@@ -47,6 +47,7 @@ struct PrefillParams {
   int32_t batch;
   float scale_log2;
   int32_t vscale_mode;
+  int32_t keep_nan;    // the LSE of a NaN sum is NaN (calls over an 8-bit pool, as on the decode kernel), else -inf
   uint16_t* v16;       // fp16 V of every key block, [B, Hkv, v16_blocks, 4096]
   int32_t v16_blocks;  // blocks per (sequence, kv head) in v16
   // per key block of v16: 1 when some V value (older: bf16(V * s)) is finite with magnitude >= 65536,
@@ -92,6 +93,11 @@ __device__ inline SeqRows seq_rows(const PrefillParams& p, int b) {
   r.o0 = s0 * p.out_st;
   r.lse0 = s0;
   return r;
+}
+
+// The natural-log LSE of a row whose weights add up to l in units of 2^m.
+__device__ inline float row_lse(float l, float m, int keep_nan) {
+  return l > 0.f || (keep_nan != 0 && l != l) ? (m + __log2f(l)) * kLn2 : kNegInf;
 }
 
 // Whether sequence b's queries run in this kernel (ragged calls hand short sequences to the decode
@@ -411,8 +417,9 @@ __device__ __attribute__((always_inline)) inline void kv8_stage_blocks(const Pre
     if (blk < sv.nb0) {
       const int page = min(max(e.table[b * e.ts + blk], 0), e.src.pages - 1);
       const int64_t at = page * e.src.page + kvh * e.src.hs + t * 16;
-      sk[k] = kv8_scale(e.src.ks[kvh * e.src.s_hs + page]);
-      sq[k] = kv8_scale(e.src.vs[kvh * e.src.s_hs + page]);
+      const uint8_t ek = e.src.ks[kvh * e.src.s_hs + page], ev = e.src.vs[kvh * e.src.s_hs + page];
+      sk[k] = kv8_scale(ev == 255 ? 255 : ek);  // (a block whose V is NaN is NaN: so are its rows' sums and LSE)
+      sq[k] = kv8_scale(ev);
       raw[k][0] = *reinterpret_cast<const uint4*>(e.src.k + at);
       raw[k][1] = *reinterpret_cast<const uint4*>(e.src.v + at);
     } else {
@@ -975,8 +982,7 @@ __device__ __attribute__((always_inline)) inline void prefill_tile(const Prefill
         *reinterpret_cast<uint2*>(orow + 16 * nb + 4 * g4) = make_uint2(w01, w23);
       }
       if (p.lse != nullptr && g4 == 0)
-        p.lse[(sr.lse0 + tok) * p.hq + kvh * G + h] =
-            lt > 0.f ? (rs[cg].mc + __log2f(lt)) * kLn2 : kNegInf;
+        p.lse[(sr.lse0 + tok) * p.hq + kvh * G + h] = row_lse(lt, rs[cg].mc, p.keep_nan);
     }
   }
 }
@@ -1158,7 +1164,7 @@ __global__ __launch_bounds__(256) void prefill_split_combine_kernel(const Prefil
   if (p.out_scale != nullptr) w01 = pack_bf16x2(bf16_lo(w01) * p.out_scale[kvh], bf16_hi(w01) * p.out_scale[kvh]);
   uint16_t* orow = p.out + sr.o0 + tok * p.out_st + static_cast<int64_t>(h) * kHeadDim;
   *reinterpret_cast<uint32_t*>(orow + 2 * lane) = w01;
-  if (p.lse != nullptr && lane == 0) p.lse[row * p.hq + h] = l > 0.f ? (m + __log2f(l)) * kLn2 : kNegInf;
+  if (p.lse != nullptr && lane == 0) p.lse[row * p.hq + h] = row_lse(l, m, p.keep_nan);
 }
 
 // The wide instance: one workgroup per (sequence, kv head) pair at a time, min(pairs, CUs) of them.
@@ -1660,6 +1666,7 @@ int32_t run_prefill(const lkv_prefill_args* a, const lkv::Kv8Pool* older8, void*
   if (a->batch == 0 || a->tokens == 0) return LKV_OK;
   CallPlan c;
   if (const int32_t st = plan_call(a, p.seg, c)) return st;
+  p.keep_nan = older8 != nullptr;
   if (older8 != nullptr) c.mixed = false;  // (the joint launch has no instance over 8-bit pages)
   const bool ragged = a->cu_seqlens_q != nullptr;
   const int group = a->num_q_heads / a->num_kv_heads;

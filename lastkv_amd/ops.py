@@ -464,7 +464,7 @@ def decode_attention(
     nothing); calls overlapping on one GPU then race.
 
     With a ``PagedKV8`` as ``older`` (and ``older_table``) the result is the attention over the values of its codes;
-    a sequence that sees a token of a NaN block has NaN outputs.
+    a sequence that sees a token of a NaN block has NaN outputs and LSEs for that kv head.
     """
 
     if not no_alloc and (_host_bound or _bind_host()):
