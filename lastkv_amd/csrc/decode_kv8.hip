@@ -72,10 +72,11 @@ __device__ inline uint32_t keep_bytes(uint32_t w, int n) {
   return n >= 4 ? w : n <= 0 ? 0u : w & ((1u << (8 * n)) - 1u);
 }
 
-// Eight codes times a power of two and s, rounded to bf16 (the product with s is exact in fp32 for a bf16 s: the same bits as bf16(value * s)).
-__device__ inline uint4 scaled_to_bf16(uint32_t lo, uint32_t hi, float s) {
-  const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(lo, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(lo, true);
-  const auto c = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), d = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
+// Eight codes times a power of two, in fp32 exactly, and then times s, rounded to bf16: bf16(value * s).  (The power of two times s first
+// may lie beyond fp32 where no value does, and would turn the block's zeros into NaN.)
+__device__ inline uint4 scaled_to_bf16(uint32_t lo, uint32_t hi, float scale, float s) {
+  const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(lo, scale, true);
+  const auto c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(hi, scale, true);
   return make_uint4(pack_bf16x2(a[0] * s, a[1] * s), pack_bf16x2(b[0] * s, b[1] * s), pack_bf16x2(c[0] * s, c[1] * s),
                     pack_bf16x2(d[0] * s, d[1] * s));
 }
@@ -97,8 +98,8 @@ __device__ inline void expand_block8(const Block8& f, int hi, int g4, float s, B
       const int n = hi - 8 * g4;
       c = make_uint4(keep_bytes(c.x, n), keep_bytes(c.y, n - 4), keep_bytes(c.z, n), keep_bytes(c.w, n - 4));
     }
-    x.v[2 * i] = kVScale ? scaled_to_bf16(c.x, c.y, vs * s) : kv8_to_bf16(c.x, c.y, vs);
-    x.v[2 * i + 1] = kVScale ? scaled_to_bf16(c.z, c.w, vs * s) : kv8_to_bf16(c.z, c.w, vs);
+    x.v[2 * i] = kVScale ? scaled_to_bf16(c.x, c.y, vs, s) : kv8_to_bf16(c.x, c.y, vs);
+    x.v[2 * i + 1] = kVScale ? scaled_to_bf16(c.z, c.w, vs, s) : kv8_to_bf16(c.z, c.w, vs);
   }
 }
 

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from lastkv_amd import ops
-from test_gpu_kv8 import DEV, attention64, history, rand, segments
+from test_gpu_kv8 import DEV, attention64, history, paged, rand, segments, table_of
 
 pytestmark = pytest.mark.gpu
 
@@ -129,3 +129,42 @@ def test_the_lse_of_prefill_against_64_bits(Hq, Hkv, L, older, local, kw, causal
         off = (lse[b].double().cpu() - want).abs()
         room = err + 2.0 ** -11 + k.shape[1] * 2.0 ** -25 + 2.0 ** -20 * (1 + float(want.abs().max()))
         assert float(off.max()) <= room, (b, float(off.max()), room)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_zeros_beside_a_large_value_stay_zeros_under_a_scale(name):
+    """V is bf16(value * vscale): where a block's power of two times vscale lies beyond fp32, the zeros of the block are 0 all the
+    same, and so are the outputs that only zeros go into."""
+
+    tokens, Hq, _, _ = CALLS[name]
+    k, v = rand(1, 1, 64, 2, 128), torch.zeros(1, 64, 2, 128).bfloat16()
+    v[0, 3, :, 5] = 3e38
+    v[0, 40:, :, 7] = 0.25
+    table = table_of(1, 2)
+    pool = ops.PagedKV8.zeros(2, 2, DEV)
+    ops.kv8_quantize(paged(k, v, table), pool, src_table=table, dst_table=table, tokens=64)
+    q = rand(2, 1, tokens, Hq, 128, gain=False).to(DEV)
+    lse = torch.zeros(1, tokens, Hq, device=DEV)
+    out = attend(name, q, lse, older=pool, older_table=table, older_len=i32(64), vscale=torch.tensor([512.0, 1024.0], device=DEV))
+    # (dim 5 holds an infinity, whose product with a weight's second, smaller half may be a NaN)
+    assert not bool(out[..., 5].isfinite().any()) and bool(out[..., 7].isfinite().all()) and bool((out[..., 7] > 0).all())
+    rest = [d for d in range(128) if d not in (5, 7)]
+    assert bool((out[..., rest] == 0).all())
+
+
+@pytest.mark.parametrize("factor,scales", [(2.0 ** -126, [2.0 ** 100, 1.375 * 2.0 ** 110]), (2.0 ** 118, [2.0 ** -100, 1.375 * 2.0 ** -115]),
+                                           (2.0 ** -10, [-0.8203125, 1.5])])
+@pytest.mark.parametrize("Hq,splits", [(8, 1), (8, 2), (64, 1)])
+def test_scaled_values_of_any_magnitude_are_the_bf16_calls(Hq, splits, factor, scales):
+    """Down to bf16's subnormal values and up to its largest: a block a wave, equal to the call over the same values in every bit."""
+
+    table = table_of(2, 4)
+    k = rand(5, 2, 128, 2, 128)
+    v = (rand(6, 2, 128, 2, 128).float() * factor).bfloat16()
+    pool = ops.PagedKV8.zeros(8, 2, DEV)
+    ops.kv8_quantize(paged(k, v, table), pool, src_table=table, dst_table=table, tokens=128)
+    k8, v8 = ops.kv8_unpack(pool, table, 0, 128)
+    twin = paged(k8.transpose(1, 2), v8.transpose(1, 2), table)
+    q = rand(7, 2, Hq, 128, gain=False).to(DEV)
+    kw = dict(older_table=table, older_len=i32(100, 128), vscale=torch.tensor(scales, device=DEV), num_splits=splits)
+    assert torch.equal(ops.decode_attention(q, older=pool, **kw), ops.decode_attention(q, older=twin, **kw))
