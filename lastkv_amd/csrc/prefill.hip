@@ -384,18 +384,16 @@ __device__ __attribute__((always_inline)) inline void v16_stage_blocks(const Pre
   __syncthreads();  // (sm_over is reused by the next sequence's call)
 }
 
-// The pre-pass of a call whose older segment is in 8-bit pages: as above, and the older blocks' K and V as bf16 copies in the
-// tiled layout (k16 / v16b, `blocks` per (sequence, kv head)), which the tile kernels read as a contiguous older segment.  A
+// The pre-pass of a call whose older segment is in 8-bit pages: as above, and the older blocks' K as bf16 copies in the
+// tiled layout (k16, `blocks` per (sequence, kv head)), which the tile kernels read as a contiguous older segment.  A
 // thread holds 16 K and 16 V codes of a block; V codes past the sequence's length become 0 (the tiles multiply them by 0).
 // One pass instead of codes read in the tiles: every tile of 64 query rows reads all keys, so 1024 tokens of 32 heads would
-// convert each block 64 times in the tiles' loops, which the matrix pipes already wait for; the pass takes 13 us of that call's
-// 150 over 7168 keys (59 MB written), the call over bf16 pages 147.
+// convert each block 64 times in the tiles' loops, which the matrix pipes already wait for.
 struct Kv8Stage {
   Kv8Pool src;
   const int32_t* table;
   int64_t ts;
   uint16_t* k16;
-  uint16_t* v16b;
   int32_t blocks;
 };
 
@@ -447,8 +445,6 @@ __device__ __attribute__((always_inline)) inline void kv8_stage_blocks(const Pre
       uint16_t* kd = e.k16 + to + (((piece >> 1) * 4 + (piece & 1) * 2) * 16 + n16) * 32 + 8 * g4;
       *reinterpret_cast<uint4*>(kd) = kv8_to_bf16(kc.x, kc.y, sk[k]);
       *reinterpret_cast<uint4*>(kd + 16 * 32) = kv8_to_bf16(kc.z, kc.w, sk[k]);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) *reinterpret_cast<uint4*>(e.v16b + to + at + j * step) = v[j];
     }
     uint16_t* dst = p.v16 + ((static_cast<int64_t>(b) * p.hkv + kvh) * p.v16_blocks + blk) * kBlockElems;
     const float s = older ? vs : 1.f;
@@ -573,6 +569,33 @@ __host__ __device__ inline int effective_splits(int S, int nbt, int nb0, int wav
   return se < 1 ? 1 : se;
 }
 
+// stage_load of the wide instance over 8-bit pages: K as there, an older block's V (bf16) from its codes.
+template <int NW>
+__device__ inline void stage_load_codes(Stage<NW>& st, const Kv8Stage& e, const SeqView& sv, const uint16_t* kblk,
+                                        const uint16_t* vblk, int blk, int b, int kvh, int wave, int lane, int lane_off) {
+#pragma unroll
+  for (int j = 0; j < 8 / NW; ++j)
+    st.r[j] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(make_rsrc(kblk, kBlockElems * 2), lane_off,
+                                                                              (wave + j * NW) * 1024, 0));
+  if (blk >= sv.nb0) {  // (wave-uniform)
+#pragma unroll
+    for (int j = 8 / NW; j < 16 / NW; ++j)
+      st.r[j] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(make_rsrc(vblk, kBlockElems * 2), lane_off,
+                                                                                (wave + j * NW - 8) * 1024, 0));
+    return;
+  }
+  const int page = min(max(e.table[b * e.ts + blk], 0), e.src.pages - 1);
+  const uint8_t* codes = e.src.v + page * e.src.page + kvh * e.src.hs + lane * 16;
+  const float scale = kv8_scale(e.src.vs[kvh * e.src.s_hs + page]);
+  const int valid = sv.n0 - blk * kBlockTokens - 8 * (lane >> 4);
+#pragma unroll
+  for (int j = 8 / NW; j < 16 / NW; ++j) {
+    const int nb = wave + j * NW - 8;
+    const uint2 c = *reinterpret_cast<const uint2*>(codes + (nb >> 1) * 1024 + (nb & 1) * 8);
+    st.r[j] = keep_tokens(kv8_to_bf16(c.x, c.y, scale), valid);
+  }
+}
+
 // Workgroup = NW waves x 16 * CG query rows (CG 16-column groups per wave).  K (bf16, from the caches)
 // and V (fp16, from the pre-pass) blocks go through a ring of kRing LDS buffers; two register
 // stage sets keep the global loads two steps ahead of their LDS store.  Step i (block i in
@@ -587,11 +610,14 @@ __host__ __device__ inline int effective_splits(int S, int nbt, int nb0, int wav
 // kWide: the instance for tiles whose V does not fit fp16 (the pre-pass flagged one of their blocks):
 // V staged as bf16 from the caches (older blocks as bf16(V * s)), P split into bf16 hi + lo, P V and
 // the row sums on bf16 MFMAs; the fp16 instance skips those tiles and this one runs only them.
+// kCodes: the wide instance over 8-bit pages `e` (the others read nothing through e).
 // KS = 2: the workgroup has NW waves for each half of the split's keys (2 NW in all, both on the same
 // query rows, each half with an LDS ring of its own); the halves' states are merged through LDS at the end.
-template <int NW, int CG, bool kPaged, bool kWide = false, int KS = 1>
+template <int NW, int CG, bool kPaged, bool kWide = false, int KS = 1, bool kCodes = false>
 __device__ __attribute__((always_inline)) inline void prefill_tile(const PrefillParams& p, const int b, const int kvh,
-                                                                   const int tile, const int split, uint4* lds) {
+                                                                   const int tile, const int split, uint4* lds,
+                                                                   const Kv8Stage* e = nullptr) {
+  static_assert(kWide || !kCodes, "the fp16 instance reads V from the workspace");
   constexpr bool kSplitP = NW == 2 || kWide;
   constexpr bool kAnyStart = NW == 4 && !kWide;  // key splits may start in the local segment
   constexpr float kUnsetMc = kAnyStart ? kUnset : 0.f;
@@ -716,15 +742,20 @@ __device__ __attribute__((always_inline)) inline void prefill_tile(const Prefill
     // (the V blocks of the wide instance; the fp16 instance reads V from the workspace)
     auto vb = [&](int blk) __attribute__((always_inline)) { return kWide ? v_block<kPaged>(sv, blk) : nullptr; };
     auto vs_of = [&](int blk) __attribute__((always_inline)) { return kWide && blk < sv.nb0 ? vs_older : 1.f; };
+    auto load = [&](Stage<NW>& st, const uint16_t* kblk, const uint16_t* vblk, int blk) __attribute__((always_inline)) {
+      if constexpr (kCodes)
+        stage_load_codes<NW>(st, *e, sv, kblk, vblk, blk, b, kvh, wave, lane, lane_off);
+      else
+        stage_load<NW, kWide>(st, rsrc, kblk, vblk, blk, wave, lane_off);
+    };
 #pragma unroll
     for (int j = 0; j < kStages; ++j)
-      stage_load<NW, kWide>(sets[j], rsrc, k_block<kPaged>(sv, min(kb0 + j, last)), vb(min(kb0 + j, last)),
-                            min(kb0 + j, last), wave, lane_off);
+      load(sets[j], k_block<kPaged>(sv, min(kb0 + j, last)), vb(min(kb0 + j, last)), min(kb0 + j, last));
 #pragma unroll
     for (int j = 0; j < kDist; ++j) {
       stage_store<NW, kWide>(sets[j % kStages], ring + j * kBuf, wave, lane, vs_of(min(kb0 + j, last)));
       const int lb = min(kb0 + j + kStages, last);
-      stage_load<NW, kWide>(sets[j % kStages], rsrc, k_block<kPaged>(sv, lb), vb(lb), lb, wave, lane_off);
+      load(sets[j % kStages], k_block<kPaged>(sv, lb), vb(lb), lb);
     }
     if (!kWide) needs_wide = flags_any(flag_peek, p, b, kvh, nbt);
     if (!kWide && needs_wide) {
@@ -892,7 +923,7 @@ __device__ __attribute__((always_inline)) inline void prefill_tile(const Prefill
         }
       }
       stage_store<NW, kWide>(st, wr, wave, lane, st_vs);
-      stage_load<NW, kWide>(st, rsrc, ld_k, ld_v, ld_blk, wave, lane_off);
+      load(st, ld_k, ld_v, ld_blk);
 #pragma unroll
       for (int i = 0; i < (kSplitP ? 18 : 9) * CG; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA (P V and P 1 of block i)
@@ -1173,19 +1204,35 @@ __global__ __launch_bounds__(256) void prefill_split_combine_kernel(const Prefil
 // Otherwise a pair none of whose V blocks the pre-pass flagged is skipped after one flag scan, and a
 // flagged pair's tiles run here one after another, each tile again checking whether its own blocks
 // reach a flagged one (the fp16 instance ran the others).
-template <int NW, int CG, int WPE, bool kPaged>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(WPE))) void prefill_wide_kernel(
-    const PrefillParams p) {
-  __shared__ uint4 lds[kTileRing * kTileBuf];
+template <int NW, int CG, bool kPaged, bool kCodes>
+__device__ __attribute__((always_inline)) inline void wide_workgroup(const PrefillParams& p, uint4* lds, const Kv8Stage* e) {
   if (*p.any_wide == 0.f) return;  // the fp16 instance ran every tile (workgroup-uniform)
   const int pairs = p.batch * p.hkv;
   for (int pair = blockIdx.x; pair < pairs; pair += gridDim.x) {
     if (!pair_needs_wide(p, pair / p.hkv, pair % p.hkv)) continue;  // (workgroup-uniform)
     for (int tile = 0; tile < p.tiles; ++tile) {
-      prefill_tile<NW, CG, kPaged, true>(p, pair / p.hkv, pair % p.hkv, tile, 0, lds);
+      prefill_tile<NW, CG, kPaged, true, 1, kCodes>(p, pair / p.hkv, pair % p.hkv, tile, 0, lds, e);
       __syncthreads();  // the next tile's staging reuses the LDS ring
     }
   }
+}
+
+template <int NW, int CG, int WPE, bool kPaged>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(WPE))) void prefill_wide_kernel(
+    const PrefillParams p) {
+  __shared__ uint4 lds[kTileRing * kTileBuf];
+  wide_workgroup<NW, CG, kPaged, false>(p, lds, nullptr);
+}
+
+// Over 8-bit pages: an older block's V is read from its codes and converted in every tile.  bf16 copies of V would be faster
+// (1024 tokens over 6144 of history, all of it beyond fp16: 8.65 ms, so 10.9), but every call would write them and
+// hold as much memory again as the K copies, for V that nearly no call has (without them four sequences of that size take 495 us
+// where they took 510).
+template <int NW, int CG, int WPE, bool kPaged>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(WPE))) void prefill_wide_kv8_kernel(
+    const PrefillParams p, const Kv8Stage e) {
+  __shared__ uint4 lds[kTileRing * kTileBuf];
+  wide_workgroup<NW, CG, kPaged, true>(p, lds, &e);
 }
 
 }  // namespace
@@ -1445,22 +1492,29 @@ void launch_mixed(bool paged, int64_t tile_wgs, const lkv::PrefillParams& p, con
 }
 
 // The wide-range V instance for the same wave count and addressing, over `pair_wgs` workgroups
-// (4-wave tiles at one wave per SIMD: the bf16 instance needs more than 256 registers).
-void launch_wide(int waves, bool paged, int pair_wgs, const lkv::PrefillParams& p, hipStream_t s) {
+// (4-wave tiles at one wave per SIMD: the bf16 instance needs more than 256 registers).  e: the 8-bit pages of the older
+// segment, or null.
+template <int NW, int WPE>
+void launch_wide(bool paged, int pair_wgs, const lkv::PrefillParams& p, const lkv::Kv8Stage* e, hipStream_t s) {
   using namespace lkv;
   const dim3 grid(static_cast<unsigned>(pair_wgs));
-  if (waves == 8 && paged)
-    prefill_wide_kernel<8, 2, 2, true><<<grid, 8 * 64, 0, s>>>(p);
-  else if (waves == 8)
-    prefill_wide_kernel<8, 2, 2, false><<<grid, 8 * 64, 0, s>>>(p);
-  else if (waves == 4 && paged)
-    prefill_wide_kernel<4, 2, 1, true><<<grid, 4 * 64, 0, s>>>(p);
-  else if (waves == 4)
-    prefill_wide_kernel<4, 2, 1, false><<<grid, 4 * 64, 0, s>>>(p);
+  if (e != nullptr && paged)
+    prefill_wide_kv8_kernel<NW, 2, WPE, true><<<grid, NW * 64, 0, s>>>(p, *e);
+  else if (e != nullptr)
+    prefill_wide_kv8_kernel<NW, 2, WPE, false><<<grid, NW * 64, 0, s>>>(p, *e);
   else if (paged)
-    prefill_wide_kernel<2, 2, 1, true><<<grid, 2 * 64, 0, s>>>(p);
+    prefill_wide_kernel<NW, 2, WPE, true><<<grid, NW * 64, 0, s>>>(p);
   else
-    prefill_wide_kernel<2, 2, 1, false><<<grid, 2 * 64, 0, s>>>(p);
+    prefill_wide_kernel<NW, 2, WPE, false><<<grid, NW * 64, 0, s>>>(p);
+}
+
+void launch_wide(int waves, bool paged, int pair_wgs, const lkv::PrefillParams& p, const lkv::Kv8Stage* e, hipStream_t s) {
+  if (waves == 8)
+    launch_wide<8, 2>(paged, pair_wgs, p, e, s);
+  else if (waves == 4)
+    launch_wide<4, 1>(paged, pair_wgs, p, e, s);
+  else
+    launch_wide<2, 1>(paged, pair_wgs, p, e, s);
 }
 
 namespace {
@@ -1651,10 +1705,10 @@ bool tiles_possible(const lkv_prefill_args* a) {
   return a->tile_waves != 0 || seq_tokens * (a->num_q_heads / a->num_kv_heads) > 64;
 }
 
-// Bytes of the bf16 copies of the older segment's blocks.
+// Bytes of the bf16 copies of the K of the older segment's blocks.
 int64_t kv8_copy_bytes(const lkv_prefill_args* a) {
   if (!tiles_possible(a)) return 0;
-  return static_cast<int64_t>(a->batch) * a->num_kv_heads * older_blocks(a) * (2 * lkv::kBlockElems * 2);
+  return static_cast<int64_t>(a->batch) * a->num_kv_heads * older_blocks(a) * (lkv::kBlockElems * 2);
 }
 
 // The call of an lkv_prefill_args; older8: the 8-bit pool that its older segment's table names, whose bf16 copies take `copies`
@@ -1690,16 +1744,15 @@ int32_t run_prefill(const lkv_prefill_args* a, const lkv::Kv8Pool* older8, void*
   if (!c.runs_tiles) return LKV_OK;
   const bool older_paged = older8 == nullptr && a->older_block_table != nullptr;
   Kv8Stage stage8{};
-  if (older8 != nullptr) {  // for the tiles the older segment is its bf16 copies, one run per (sequence, kv head)
+  if (older8 != nullptr) {  // for the tiles the older segment's K is its bf16 copies, one run per (sequence, kv head)
     const int64_t blocks = older_blocks(a), run = blocks * kBlockElems;
     stage8.src = *older8;
     stage8.table = a->older_block_table;
     stage8.ts = a->older_table_stride;
     stage8.k16 = static_cast<uint16_t*>(copies);
-    stage8.v16b = stage8.k16 + static_cast<int64_t>(a->batch) * a->num_kv_heads * run;
     stage8.blocks = static_cast<int32_t>(blocks);
     p.seg.ok = stage8.k16;
-    p.seg.ov = stage8.v16b;
+    p.seg.ov = nullptr;  // (the fp16 tiles read V from the workspace, the wide ones from the codes)
     p.seg.o_ss = a->num_kv_heads * run;
     p.seg.o_hs = run;
     p.seg.o_cap = static_cast<int32_t>(blocks * kBlockTokens);
@@ -1778,7 +1831,7 @@ int32_t run_prefill(const lkv_prefill_args* a, const lkv::Kv8Pool* older8, void*
   // flags at a time
   const int64_t heads = static_cast<int64_t>(a->num_kv_heads) * a->batch;
   const int64_t cus = device_cu_count() > 0 ? device_cu_count() : 256;
-  launch_wide(c.tile.waves, paged, static_cast<int>(std::min(heads, cus)), p, s);
+  launch_wide(c.tile.waves, paged, static_cast<int>(std::min(heads, cus)), p, older8 != nullptr ? &stage8 : nullptr, s);
   if (const int32_t e = check_launch("lkv_prefill_attn (wide-range V)")) return e;
   if (splits == 1) return LKV_OK;
   const int64_t items = c.tile.rows_all * a->num_q_heads;  // (row, query head) pairs, 4 per workgroup

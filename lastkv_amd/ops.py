@@ -580,7 +580,7 @@ def prefill_attention(
     kernel at any size; in a ragged call they apply to its sequences above 64 query rows per kv
     head, and its shorter ones stay on the decode kernel unless all of its sequences are short.
     ``out_scale`` as in ``decode_attention``.  With a ``PagedKV8`` as ``older`` the values of its codes
-    are attended to; the workspace (``prefill_kv8_workspace_bytes``) then also holds bf16 copies of its blocks for
+    are attended to; the workspace (``prefill_kv8_workspace_bytes``) then also holds bf16 copies of its blocks' K for
     sequences above 64 query rows per kv head."""
 
     if _host_bound or _bind_host():
@@ -1170,10 +1170,10 @@ def kv8_unpack(pool: PagedKV8, table: torch.Tensor, token0: int, tokens: int) ->
 
 
 def kv8_copy_bytes(batch: int, kv_heads: int, older_tokens: int) -> int:
-    """Workspace of the bf16 copies that a prefill call over a ``PagedKV8`` makes for sequences above 64 query rows per kv
+    """Workspace of the bf16 copies of K that a prefill call over a ``PagedKV8`` makes for sequences above 64 query rows per kv
     head, on top of ``prefill_workspace_bytes`` of the same arguments."""
 
-    return batch * kv_heads * -(-older_tokens // BLOCK_TOKENS) * 2 * BLOCK_ELEMS * 2
+    return batch * kv_heads * -(-older_tokens // BLOCK_TOKENS) * BLOCK_ELEMS * 2
 
 
 def prefill_kv8_workspace_bytes(batch: int, kv_heads: int, older_tokens: int, local_tokens: int, **kwargs) -> int:
