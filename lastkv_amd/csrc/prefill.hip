@@ -385,7 +385,9 @@ __device__ __attribute__((always_inline)) inline void v16_stage_blocks(const Pre
 }
 
 // The pre-pass of a call whose older segment is in 8-bit pages: as above, and the older blocks' K as bf16 copies in the
-// tiled layout (k16, `blocks` per (sequence, kv head)), which the tile kernels read as a contiguous older segment.  A
+// tiled layout (k16, `blocks` per (sequence, kv head)), which the tile kernels read as a contiguous older segment.  In a ragged
+// call only the sequences on the tile path have copies, in the order of their ranks, which go to `slots` for the tiles (-1 for
+// any past the `copies` that there is room for: it has an empty older segment).  A
 // thread holds 16 K and 16 V codes of a block; V codes past the sequence's length become 0 (the tiles multiply them by 0).
 // One pass instead of codes read in the tiles: every tile of 64 query rows reads all keys, so 1024 tokens of 32 heads would
 // convert each block 64 times in the tiles' loops, which the matrix pipes already wait for.
@@ -395,10 +397,12 @@ struct Kv8Stage {
   int64_t ts;
   uint16_t* k16;
   int32_t blocks;
+  int32_t* slots;  // [B] of a ragged call, else null: a sequence's copies are at its index
+  int32_t copies;  // sequences that k16 holds
 };
 
 template <bool kPaged, int kBlocks>
-__device__ __attribute__((always_inline)) inline void kv8_stage_blocks(const PrefillParams& p, const Kv8Stage& e, int b, int kvh, int x) {
+__device__ __attribute__((always_inline)) inline void kv8_stage_blocks(const PrefillParams& p, const Kv8Stage& e, int b, int slot, int kvh, int x) {
   const SeqView sv = make_seq_view(p.seg, b, kvh);
   const int nb = sv.nb0 + local_blocks(sv, sv.n1);
   const float vs = p.vscale_mode ? p.vscale[kvh] : 1.f;
@@ -441,10 +445,12 @@ __device__ __attribute__((always_inline)) inline void kv8_stage_blocks(const Pre
       v[1] = keep_tokens(kv8_to_bf16(vc.z, vc.w, sq[k]), valid);
       at = (32 * piece + n16) * 32 + 8 * g4;
       step = 16 * 32;
-      const int64_t to = ((static_cast<int64_t>(b) * p.hkv + kvh) * e.blocks + blk) * kBlockElems;
+      const int64_t to = ((static_cast<int64_t>(slot) * p.hkv + kvh) * e.blocks + blk) * kBlockElems;
       uint16_t* kd = e.k16 + to + (((piece >> 1) * 4 + (piece & 1) * 2) * 16 + n16) * 32 + 8 * g4;
-      *reinterpret_cast<uint4*>(kd) = kv8_to_bf16(kc.x, kc.y, sk[k]);
-      *reinterpret_cast<uint4*>(kd + 16 * 32) = kv8_to_bf16(kc.z, kc.w, sk[k]);
+      if (slot < e.copies) {
+        *reinterpret_cast<uint4*>(kd) = kv8_to_bf16(kc.x, kc.y, sk[k]);
+        *reinterpret_cast<uint4*>(kd + 16 * 32) = kv8_to_bf16(kc.z, kc.w, sk[k]);
+      }
     }
     uint16_t* dst = p.v16 + ((static_cast<int64_t>(b) * p.hkv + kvh) * p.v16_blocks + blk) * kBlockElems;
     const float s = older ? vs : 1.f;
@@ -474,7 +480,7 @@ __global__ __launch_bounds__(256) void kv8_stage_kernel(const PrefillParams p, c
   const int kvh = blockIdx.y;
   if ((blockIdx.x | blockIdx.y | blockIdx.z) == 0 && threadIdx.x == 0) *p.any_wide = 0.f;
   if constexpr (kBlocks == 1) {
-    if (on_tile_path(p, seq_rows(p, blockIdx.z))) kv8_stage_blocks<kPaged, kBlocks>(p, e, blockIdx.z, kvh, blockIdx.x);
+    if (on_tile_path(p, seq_rows(p, blockIdx.z))) kv8_stage_blocks<kPaged, kBlocks>(p, e, blockIdx.z, blockIdx.z, kvh, blockIdx.x);
     return;
   }
   const int lane = threadIdx.x & 63;
@@ -485,8 +491,10 @@ __global__ __launch_bounds__(256) void kv8_stage_kernel(const PrefillParams p, c
     while (m != 0) {  // (wave-uniform)
       const int l = __builtin_ctzll(m);
       m &= m - 1;
-      if (rank++ % static_cast<int>(gridDim.z) == static_cast<int>(blockIdx.z))
-        kv8_stage_blocks<kPaged, kBlocks>(p, e, i0 + l, kvh, blockIdx.x);
+      const int slot = rank++;
+      if (slot % static_cast<int>(gridDim.z) != static_cast<int>(blockIdx.z)) continue;
+      if ((blockIdx.x | blockIdx.y) == 0 && threadIdx.x == 0) e.slots[i0 + l] = slot < e.copies ? slot : -1;
+      kv8_stage_blocks<kPaged, kBlocks>(p, e, i0 + l, slot, kvh, blockIdx.x);
     }
   }
 }
@@ -1377,6 +1385,7 @@ struct HostPlan {
   bool known;
   int32_t class_n[3];
   bool any_tile;
+  int32_t tiles;      // the sequences with more than 64 query rows per kv head
   int64_t tile_rows;  // query rows per kv head of the sequences with more than 64
 };
 
@@ -1393,6 +1402,7 @@ HostPlan host_plan(const lkv_prefill_args* a, int64_t group) {
     const int64_t cols = L * group;
     if (cols > 64) {
       h.any_tile = true;
+      ++h.tiles;
       h.tile_rows += cols;
     } else {
       ++h.class_n[cols <= 16 ? 0 : cols <= 32 ? 1 : 2];
@@ -1699,16 +1709,26 @@ int64_t older_blocks(const lkv_prefill_args* a) {
   return (n + lkv::kBlockTokens - 1) / lkv::kBlockTokens;
 }
 
-// Whether the tile kernel may run, which reads 8-bit older pages through bf16 copies.
-bool tiles_possible(const lkv_prefill_args* a) {
-  const int64_t seq_tokens = a->cu_seqlens_q ? std::min(a->max_seqlen_q, a->tokens) : a->tokens;
-  return a->tile_waves != 0 || seq_tokens * (a->num_q_heads / a->num_kv_heads) > 64;
+// The sequences that may run on the tile kernel, which reads the K of 8-bit older pages through bf16 copies: those above 64 query
+// rows per kv head, counted in the host's offsets, without which as many as the call's tokens allow; all of them where
+// no sequence runs on the decode kernel.
+int64_t tile_sequences(const lkv_prefill_args* a) {
+  const int64_t group = a->num_q_heads / a->num_kv_heads, least = 64 / std::max<int64_t>(group, 1) + 1;
+  if (a->cu_seqlens_q == nullptr) return a->tile_waves != 0 || a->tokens >= least ? a->batch : 0;
+  if (std::min(a->max_seqlen_q, a->tokens) < least) return a->tile_waves != 0 ? a->batch : 0;
+  const int64_t most = std::min<int64_t>(a->batch, a->tokens / least);
+  const HostPlan h = host_plan(a, group);
+  return h.known ? std::min<int64_t>(h.tiles, most) : most;
 }
 
-// Bytes of the bf16 copies of the K of the older segment's blocks.
+int64_t kv8_slots_bytes(const lkv_prefill_args* a) {
+  return a->cu_seqlens_q == nullptr ? 0 : (static_cast<int64_t>(a->batch) * 4 + 15) / 16 * 16;
+}
+
+// Bytes of the bf16 copies of the K of the older segment's blocks, and of the sequences' places among them.
 int64_t kv8_copy_bytes(const lkv_prefill_args* a) {
-  if (!tiles_possible(a)) return 0;
-  return static_cast<int64_t>(a->batch) * a->num_kv_heads * older_blocks(a) * (lkv::kBlockElems * 2);
+  const int64_t n = tile_sequences(a);
+  return n == 0 ? 0 : n * a->num_kv_heads * older_blocks(a) * (lkv::kBlockElems * 2) + kv8_slots_bytes(a);
 }
 
 // The call of an lkv_prefill_args; older8: the 8-bit pool that its older segment's table names, whose bf16 copies take `copies`
@@ -1745,12 +1765,14 @@ int32_t run_prefill(const lkv_prefill_args* a, const lkv::Kv8Pool* older8, void*
   const bool older_paged = older8 == nullptr && a->older_block_table != nullptr;
   Kv8Stage stage8{};
   if (older8 != nullptr) {  // for the tiles the older segment's K is its bf16 copies, one run per (sequence, kv head)
-    const int64_t blocks = older_blocks(a), run = blocks * kBlockElems;
+    const int64_t blocks = older_blocks(a), run = blocks * kBlockElems, held = tile_sequences(a);
     stage8.src = *older8;
     stage8.table = a->older_block_table;
     stage8.ts = a->older_table_stride;
     stage8.k16 = static_cast<uint16_t*>(copies);
     stage8.blocks = static_cast<int32_t>(blocks);
+    stage8.copies = static_cast<int32_t>(held);
+    stage8.slots = ragged ? reinterpret_cast<int32_t*>(stage8.k16 + held * a->num_kv_heads * run) : nullptr;
     p.seg.ok = stage8.k16;
     p.seg.ov = nullptr;  // (the fp16 tiles read V from the workspace, the wide ones from the codes)
     p.seg.o_ss = a->num_kv_heads * run;
@@ -1816,6 +1838,10 @@ int32_t run_prefill(const lkv_prefill_args* a, const lkv::Kv8Pool* older8, void*
     else
       v16_stage_kernel<false, 1><<<vgrid, 256, 0, s>>>(p);
     if (const int32_t e = check_launch("lkv_prefill_attn (V pre-pass)")) return e;
+    if (stage8.slots != nullptr) {  // (written by the pre-pass)
+      p.seg.o_slot = stage8.slots;
+      p.seg.o_nslots = stage8.copies;
+    }
   }
   if (c.mixed) {
     launch_mixed(paged, wgs, p, c.rows16, s);

@@ -1169,18 +1169,23 @@ def kv8_unpack(pool: PagedKV8, table: torch.Tensor, token0: int, tokens: int) ->
     return k, v
 
 
-def kv8_copy_bytes(batch: int, kv_heads: int, older_tokens: int) -> int:
-    """Workspace of the bf16 copies of K that a prefill call over a ``PagedKV8`` makes for sequences above 64 query rows per kv
-    head, on top of ``prefill_workspace_bytes`` of the same arguments."""
+def kv8_copy_bytes(sequences: int, kv_heads: int, older_tokens: int, ragged_batch: int = 0) -> int:
+    """Workspace of the bf16 copies of K that a prefill call over a ``PagedKV8`` makes for its ``sequences`` above 64 query rows
+    per kv head (of all its sequences if a ``tile_waves`` puts a call of short ones on the tile kernel), on top of
+    ``prefill_workspace_bytes``; in a ragged call of ``ragged_batch`` sequences their places are held too.  A ragged call
+    counts those sequences in ``cu_seqlens_q_host``; without it room for as many as its rows allow is needed."""
 
-    return batch * kv_heads * -(-older_tokens // BLOCK_TOKENS) * BLOCK_ELEMS * 2
+    if sequences == 0:
+        return 0
+    return sequences * kv_heads * -(-older_tokens // BLOCK_TOKENS) * BLOCK_ELEMS * 2 + -(-4 * ragged_batch // 16) * 16
 
 
 def prefill_kv8_workspace_bytes(batch: int, kv_heads: int, older_tokens: int, local_tokens: int, **kwargs) -> int:
-    """``prefill_workspace_bytes`` of a call whose older segment is a ``PagedKV8``."""
+    """``prefill_workspace_bytes`` of a call whose older segment is a ``PagedKV8`` (any number of its sequences above 64 query
+    rows per kv head)."""
 
     return (prefill_workspace_bytes(batch, kv_heads, older_tokens, local_tokens, **kwargs)
-            + kv8_copy_bytes(batch, kv_heads, older_tokens))
+            + kv8_copy_bytes(batch, kv_heads, older_tokens, batch))
 
 
 def _page_list(name: str, ids) -> np.ndarray:

@@ -543,8 +543,9 @@ class LastKVFastPath:
             else:
                 need = max(need, ops.ragged_split_state_bytes(B, Hq, P.kv_heads, max(r.tokens for r in parsed),
                                                               self.num_splits or 0, ops._cu_count(P.device)))
-            if P.kv8:
-                need += ops.kv8_copy_bytes(B, P.kv_heads, width * BLOCK)
+            if P.kv8:  # (rows on the decode kernel read the 8-bit pages themselves)
+                tiles = sum(r.tokens * (Hq // P.kv_heads) > 64 for r in parsed)
+                need += ops.kv8_copy_bytes(tiles, P.kv_heads, width * BLOCK, 0 if uniform else B)
             if self._prefill_ws.numel() < need:
                 self._prefill_ws = torch.empty(need, dtype=torch.uint8, device=P.device)
         if self._q_out.shape[0] < self.tokens:
@@ -737,8 +738,11 @@ class LastKVServingModel:
     The model passed in keeps its bf16 weights, which the 4-bit copy comes on top of.
 
     ``shared_cache="kv8"`` holds the shared history in 8 bits (``ops.PagedKV8``: e4m3 with a power-of-two scale per 32 tokens
-    of a kv head), half of its memory and of the bytes that every layer's attention reads of it; the recent and current
-    chunk stay bf16.  ``fork_sequence`` and ``beam_search`` work over either."""
+    of a kv head): half of its pages' memory and of the bytes that every layer's attention reads of it; the recent and current
+    chunk stay bf16, in the final layer's staging pages too (two chunks a sequence, on top).  A step with rows above 64 query rows
+    per kv head keeps a bf16 copy of their K history in its workspace, as large as their 8-bit pages: prompts fed one after
+    another take one sequence's, all sequences' pieces in one step what the 8 bits save.  ``fork_sequence`` and ``beam_search`` work
+    over either."""
 
     def __init__(self, model, *, max_batch: int, max_tokens_per_slot: int, source_pages: int | None = None,
                  num_splits: int | None = None, device=None, contract: str = "hf", weights: str = "bf16",

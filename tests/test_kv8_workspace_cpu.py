@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes
 
+import numpy as np
 import pytest
 
 from lastkv_amd import _lib, ops
@@ -30,3 +31,24 @@ def test_tiles_take_the_bf16_call_s_and_one_copy_of_k(batch, tokens, older):
 def test_short_calls_take_nothing_more(tokens):
     eight, bf16 = sizes(tokens=tokens)
     assert eight == bf16
+
+
+def _ragged(counts, host=True, **kw):
+    cu = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    args = dict(batch=len(counts), tokens=int(cu[-1]), cu_seqlens_q=16, max_seqlen_q=max(counts), older_len=16, older_capacity_tokens=8192,
+                older_table_stride=256, **kw)
+    return sizes(**args, **(dict(cu_seqlens_q_host=cu.ctypes.data) if host else {}))
+
+
+@pytest.mark.parametrize("counts,tiles", [([1] * 31 + [512], 1), ([17, 16, 40, 1, 1, 16], 2), ([16] * 9, 0), ([17] * 5, 5)])
+def test_only_sequences_on_the_tiles_have_copies(counts, tiles):
+    """Groups of 4: those above 16 tokens, as the host's offsets say."""
+
+    eight, bf16 = _ragged(counts)
+    assert eight - bf16 == ops.kv8_copy_bytes(tiles, 2, 8192, len(counts))
+    eight, bf16 = _ragged(counts, host=False)  # (as many as the rows allow)
+    most = min(len(counts), sum(counts) // 17) if max(counts) > 16 else 0
+    assert eight - bf16 == ops.kv8_copy_bytes(most, 2, 8192, len(counts)) and most >= tiles
+    if max(counts) <= 16:  # (a call of short ones alone that is put on the tile kernel)
+        eight, bf16 = _ragged(counts, tile_waves=4)
+        assert eight - bf16 == ops.kv8_copy_bytes(len(counts), 2, 8192, len(counts))
