@@ -291,16 +291,20 @@ class LastKVPagePool:
 
         kept = history if self.kv8 else tokens
         new = self.pages.fork(slot, kept // BLOCK)
-        if kept % BLOCK:
-            j = kept // BLOCK
-            ops.copy_pages(self.shared, self.pages.table[slot, j:j + 1], self.pages.table[new, j:j + 1])
-        blocks = -(-tokens // BLOCK)
-        src, dst = ([self.ring_pages[:, s, :blocks].reshape(-1)] for s in (slot, new))
-        if self.kv8:
-            stage = np.arange(min(self.stage_blocks, blocks))
-            for ids, s in ((src, slot), (dst, new)):
-                ids.append(self.first_stage + s * self.stage_blocks + stage)
-        ops.copy_pages(self.pool, *(np.concatenate(ids).astype(np.int32) for ids in (src, dst)))
+        try:
+            if kept % BLOCK:
+                j = kept // BLOCK
+                ops.copy_pages(self.shared, self.pages.table[slot, j:j + 1], self.pages.table[new, j:j + 1])
+            blocks = -(-tokens // BLOCK)
+            src, dst = ([self.ring_pages[:, s, :blocks].reshape(-1)] for s in (slot, new))
+            if self.kv8:
+                stage = np.arange(min(self.stage_blocks, blocks))
+                for ids, s in ((src, slot), (dst, new)):
+                    ids.append(self.first_stage + s * self.stage_blocks + stage)
+            ops.copy_pages(self.pool, *(np.concatenate(ids).astype(np.int32) for ids in (src, dst)))
+        except BaseException:
+            self.pages.close_slot(new)  # (its pages go back; what a copy may have written there belongs to no one)
+            raise
         self._dirty(new, new + 1)
         return new
 
