@@ -914,7 +914,8 @@ class LastKVServingModel:
         Returns per prompt its ``num_beams`` best hypotheses as (prompt and new ids, score), best first; a score is the sum of
         the new tokens' log-probabilities divided by their number to the power of ``length_penalty``.  A beam that chooses
         ``eos_token_id`` is a finished hypothesis, and a prompt with ``num_beams`` of them is done; without one
-        every hypothesis has ``max_new_tokens`` new ids."""
+        every hypothesis has ``max_new_tokens`` new ids.  Logits that leave fewer than ``num_beams`` ways to go on (or end, at
+        the last token) raise."""
 
         K = num_beams
         count = K if eos_token_id is None else 2 * K
@@ -940,13 +941,15 @@ class LastKVServingModel:
                 kids = []  # (score, beam, token)
                 for rank, (score, k, tok) in enumerate(zip(*rows)):
                     if tok < 0:
-                        raise RuntimeError("the logits leave fewer candidates than beams")
+                        break  # (no more candidates: those behind are none either)
                     if tok == eos_token_id:
                         if rank < K:
                             done[i].append((score, new[i][k] + [tok]))
                     elif len(kids) < K:
                         kids.append((score, k, tok))
                 last = len(new[i][0]) + 1 >= max_new_tokens
+                if len(done[i]) < K and len(kids) + (len(done[i]) if last else 0) < K:
+                    raise RuntimeError("the logits leave fewer candidates than beams")
                 if last and len(done[i]) < K:
                     done[i] += [(score, new[i][k] + [tok]) for score, k, tok in kids]
                 old, goes_on = slots[i], {} if last or len(done[i]) >= K else dict.fromkeys(k for _, k, _ in kids)

@@ -1,4 +1,4 @@
-"""Forks that fail half way (gpu)."""
+"""Forks that fail half way and beam searches over few candidates (gpu)."""
 
 from __future__ import annotations
 
@@ -44,3 +44,44 @@ def test_a_fork_whose_copies_fail_takes_nothing(shared_cache, failing, monkeypat
     for x in (s, *twins):
         r.free_sequence(x)
     assert r.pool.free_pages == r.pool.source_pages
+
+
+def _masked(r, allowed, value):
+    """The runner's steps with every other token's logit at `value`."""
+
+    step = LastKVServingModel.step
+
+    def masked(rows, *args):
+        logits = step(r, rows, *args).clone()
+        keep = torch.zeros(logits.shape[-1], dtype=torch.bool, device=logits.device)
+        keep[allowed] = True
+        return logits.masked_fill(~keep, value)
+
+    return masked
+
+
+@pytest.mark.parametrize("K,eos,allowed,steps", [(3, 11, [11, 5, 17, 40], 9), (3, 11, [5, 17, 40], 4), (2, 11, [11, 5, 17], 1),
+                                                 (4, 11, [3, 4, 5, 6, 11], 6), (1, 11, [11, 7], 5)])
+def test_beam_search_over_few_tokens(K, eos, allowed, steps, monkeypatch):
+    """K successors are enough, where 2K candidates are looked for: the hypotheses are those of a search that gives all other tokens a
+    far lower, finite logit."""
+
+    _, model = _tiny(chunk=8, seed=23)
+    out = []
+    for value in (-torch.inf, -1e4):
+        r = LastKVServingModel(model, max_batch=K, max_tokens_per_slot=128, num_splits=2)
+        monkeypatch.setattr(r, "step", _masked(r, allowed, value))
+        out.append(r.beam_search([_ids(3, 21)], num_beams=K, max_new_tokens=steps, eos_token_id=eos)[0])
+        assert r.pool.free_pages == r.pool.source_pages and not r.fast._open.any()
+    assert [(ids.tolist(), s) for ids, s in out[0]] == [(ids.tolist(), s) for ids, s in out[1]]
+    assert len(out[0]) == K and {t for ids, _ in out[0] for t in ids[21:].tolist()} <= set(allowed)
+
+
+@pytest.mark.parametrize("K,eos,allowed,steps", [(3, 11, [5, 17], 4), (3, None, [5, 17], 4), (3, 11, [11, 5, 17], 4), (3, 11, [5, 17], 1)])
+def test_beam_search_over_fewer_tokens_than_beams(K, eos, allowed, steps, monkeypatch):
+    _, model = _tiny(chunk=8, seed=23)
+    r = LastKVServingModel(model, max_batch=K, max_tokens_per_slot=128, num_splits=2)
+    monkeypatch.setattr(r, "step", _masked(r, allowed, -torch.inf))
+    with pytest.raises(RuntimeError, match="fewer candidates than beams"):
+        r.beam_search([_ids(3, 21)], num_beams=K, max_new_tokens=steps, eos_token_id=eos)
+    assert r.pool.free_pages == r.pool.source_pages and not r.fast._open.any()
