@@ -103,3 +103,32 @@ def test_every_block_of_a_long_history_is_read_once(T, splits):
     want = v[0, :T, 0].double().mean(0)
     off = (out.double().cpu() - want).abs()
     assert bool((off <= want * (2.0 ** -8 + 2.0 ** -15)).all()), float((off / want.clamp(min=1e-9)).max())
+
+
+@pytest.mark.parametrize("host", [False, True])
+@pytest.mark.parametrize("counts", [[16, 5, 1, 0], [1, 1, 8, 2], [130, 5, 1, 16]])
+@pytest.mark.parametrize("T", [4000, 9001])
+def test_long_ragged_rows_to_the_weights_precision(T, counts, host):
+    """Rows on the decode kernel (16 tokens of a group of 4 and less) to 2^-15 of a weight, on the tiles to fp16's 2^-11 and the sum's."""
+
+    seg, keys = segments(26, 8, 2, [T, 33, T - 1, 64], [n + 7 for n in counts], True, ring_blocks=5)
+    q = rand(27, sum(counts), 8, 128).to(DEV)
+    cu = np.concatenate(([0], np.cumsum(counts))).astype(np.int32)
+    got = ops.prefill_attention(q, cu_seqlens_q=torch.from_numpy(cu).to(DEV), max_seqlen_q=max(counts),
+                                cu_seqlens_q_host=cu if host else None, **seg)
+    for b, n in enumerate(counts):
+        if n:
+            rows = slice(int(cu[b]), int(cu[b + 1]))
+            want, mean, err, _ = attention64(q[rows].cpu(), *keys[b], n)
+            check(got[rows], want, mean, err, 2.0 ** -15 if n <= 16 else 2.0 ** -10, (T, b))
+
+
+@pytest.mark.parametrize("T", [0, 1, 31, 32])
+@pytest.mark.parametrize("L", [1, 2, 4])
+def test_shortest_histories_to_the_weights_precision(T, L):
+    seg, keys = segments(36, 16, 1, [T, 0], [L, L], True)
+    q = rand(37, 2, L, 16, 128).to(DEV)
+    got = ops.prefill_attention(q, **seg) if L > 1 else ops.decode_attention(q[:, 0].contiguous(), **seg)[:, None]
+    for b in range(2):
+        want, mean, err, _ = attention64(q[b].cpu(), *keys[b], L)
+        check(got[b], want, mean, err, 2.0 ** -15, (T, L, b))
