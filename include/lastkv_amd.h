@@ -743,6 +743,10 @@ int32_t lkv_kv8_unpack(const lkv_kv8_pool *src, const int32_t *table, int64_t ta
  * block has NaN outputs and LSEs for that kv head.  Codes past a sequence's length do not count, whatever they hold. */
 int32_t lkv_decode_attn_kv8(const lkv_decode_args *args, const lkv_kv8_pool *older, lkv_stream_t stream);
 
+/* lkv_prefill_workspace_bytes of the call and, on top, 8192 bytes a (32-token block of the older segment, kv head) for every
+ * sequence of more than 64 query rows per kv head: a bf16 copy of its K.  A ragged call counts those sequences in
+ * cu_seqlens_q_host; without it as many as its rows allow are held room for.  Sequences beyond that number, which host offsets
+ * unlike the device's can leave, have no defined outputs. */
 int64_t lkv_prefill_kv8_workspace_bytes(const lkv_prefill_args *args);
 
 int32_t lkv_prefill_attn_kv8(const lkv_prefill_args *args, const lkv_kv8_pool *older, lkv_stream_t stream);

@@ -7,9 +7,9 @@
 // Choosing the n greatest of many values needs no sort: the n-th greatest of the threads' own maxima is a floor that at
 // least n values reach and few others do; those go to LDS and each counts the ones before it.  Where too many values reach
 // the floor for LDS (equal logits), n rounds take the next one each; both give the same set.
-// 16 prompts of 8 beams of 128256 bf16 logits, 16 of each: slices 11.3 us (2.9 TB/s; the loads and the maximum alone 5.9, with
-// the exponentials 8.2, so that half is the choice and its barriers), choosing 7.6; one prompt of 4 beams 4.4 and 4.8, which
-// are two dependent launches.
+// 16 prompts of 8 beams of 128256 bf16 logits, 16 of each: slices 12.0 us (2.7 TB/s; 13.0 on the mean; the loads and the maximum
+// alone 5.9, with the exponentials 8.2, so that a third is the choice and its barriers), choosing 6.9-7.6; one prompt of 4 beams of
+// 32000 3.8-4.5 and 3.2-5.0, which are two dependent launches.
 #include "common.h"
 #include "runtime.h"
 

@@ -6,9 +6,9 @@
 // kernel (one conversion instruction for two values, the block's power of two applied by it), so that scores, softmax and
 // sums are that kernel's.
 //
-// Bound by memory for many rows (32 sequences of 9.2K keys, 8 kv heads: 103-105 us, 6.5 TB/s; 4 of 128K 171 us, 6.3; the bf16 kernel's
+// Bound by memory for many rows (32 sequences of 9.2K keys, 8 kv heads: 105 us, 6.5 TB/s; 4 of 128K 175 us, 6.2; the bf16 kernel's
 // calls 178 and 328), for few by the blocks that follow each other in a wave (7 sequences of up to 12K keys, 4 kv heads, s per
-// head: 17-18 us where the bytes are 5).  Half the bytes a block ask for twice the blocks in flight: eight waves of three
+// head: 15-18 us where the bytes are 4).  Half the bytes a block ask for twice the blocks in flight: eight waves of three
 // buffers, so that two blocks are on their way while one is computed, and nothing but the blocks goes through vector loads (32
 // sequences 126 us with two buffers and page ids and scales by vector loads).  Dealing the blocks to all waves of all splits,
 // with a pair's splits on one XCD, reads one window at a time: 6.6-6.8 TB/s where a range a split reads 5.8.

@@ -35,9 +35,9 @@ int32_t kv8_pool(const lkv_kv8_pool* a, const char* name, Kv8Pool& p) {
 
 namespace {
 
-// Calls over more bf16 values than this read non-temporally: 16 sequences of 8192 tokens (512 MiB) are quantised in 130 us
-// (6.2 TB/s of reads and writes) so and in 157 with plain loads, unpacked in 141 and 148; 1024 tokens each, which the caches
-// hold, in 19.2 and 16.8, 20.0 and 17.0.
+// Calls over more bf16 values than this read non-temporally: 16 sequences of 8192 tokens (512 MiB), replayed, are quantised in 123 us
+// (6.5 TB/s of reads and writes) so and in 164 with plain loads, unpacked in 144 and 148; calls of 1024 tokens each, which the caches
+// hold, take plain loads (19.2 us quantised and 20.0 unpacked without, 16.8 and 17.0 with them).
 constexpr int64_t kNtBytes = int64_t{384} << 20;
 
 struct QuantizeParams {
