@@ -135,3 +135,40 @@ def test_offsets_that_the_call_has_no_room_for_stay_inside_it():
     ops.prefill_attention(q, cu_seqlens_q=i32(0, T, 0, T, 0, T, 0), workspace=ws[:need], **args)
     torch.cuda.synchronize()
     assert bool((ws[need:] == 0xa5).all())
+
+
+@pytest.mark.parametrize("length", ["device", "fixed"])
+@pytest.mark.parametrize("ring", ["tiled", "paged"])
+@pytest.mark.parametrize("counts,kw", [([40, 1, 17, 90], dict()), ([3, 16, 0, 9], dict(tile_waves=4)), ([1, 5], dict(tile_waves=8)),
+                                       ([3, 70, 16], dict(tile_waves=8))])
+def test_ragged_tiles_beside_rings_of_either_kind(counts, kw, ring, length):
+    """Rows on the tiles, short ones too where `tile_waves` puts a call of those alone there, equal the call over bf16 pages of the same
+    values in every bit; rings in slots of any order."""
+
+    B, H, T, W = len(counts), 2, 200, 4
+    pool, table, k, v = history(21, B, H, 224)
+    twin = ops.PagedKV.zeros(table.numel(), H, DEV)
+    ops.append_paged(k.transpose(1, 2).contiguous(), v.transpose(1, 2).contiguous(), twin, table, token0=0)
+    kl, vl = rand(22, B, 32 * W, H, 128).to(DEV), rand(23, B, 32 * W, H, 128).to(DEV)
+    order = np.random.default_rng(B).permutation(B).astype(np.int32)
+    local = [n + 5 for n in counts]
+    args = dict(local_len=i32(*local), local_start=i32(*[7 * b for b in range(B)]), causal=True, num_splits=1,
+                older_table=table, older_len=T if length == "fixed" else i32(*[T - 63 * b for b in range(B)]),
+                vscale=torch.tensor([0.8203125, -1.5], device=DEV))
+    if ring == "tiled":
+        cache = ops.TiledKV.zeros(B, H, 32 * W, DEV)
+        ops.pack_kv(kl.transpose(1, 2).contiguous(), vl.transpose(1, 2).contiguous(), cache)
+        args.update(local=cache, local_slot=torch.from_numpy(order).to(DEV))
+    else:
+        rtab = torch.from_numpy((order[:, None] * W + np.arange(W)).astype(np.int32)).to(DEV)
+        local_pool = ops.PagedKV.zeros(B * W, H, DEV)
+        ops.append_paged(kl, vl, local_pool, rtab, token0=0)
+        args.update(local=local_pool, local_table=rtab, local_ring_blocks=W)
+    cu = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    q = rand(24, int(cu[-1]), 8, 128, gain=False).to(DEV)
+    for host in (None, cu):
+        got, want = (ops.prefill_attention(q, older=p, cu_seqlens_q=torch.from_numpy(cu).to(DEV), max_seqlen_q=max(counts),
+                                           cu_seqlens_q_host=host, **args, **kw) for p in (pool, twin))
+        for b, n in enumerate(counts):
+            if n > 16 or max(counts) <= 16:
+                assert torch.equal(got[cu[b]:cu[b + 1]], want[cu[b]:cu[b + 1]]), b
